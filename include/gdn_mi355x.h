@@ -332,6 +332,119 @@ int64_t gdn_bwd_segment_workspace_size(const GdnBwdParams* params, int seg_chunk
 /* Enqueue the backward on `stream`; returns a GdnStatus / hipError_t. */
 int gdn_bwd_launch(const GdnBwdParams* params, void* stream);
 
+/* ------------------------------------------------------------------------
+ * The operators of a hybrid model beside the gated delta rule.  None has a
+ * counterpart in the reference.  Same launch contract: work is enqueued on
+ * `stream`, nothing is allocated or synchronised, workspaces are the
+ * caller's and need no initialisation.
+ * ------------------------------------------------------------------------ */
+
+/* Elementwise gated linear recurrence over T rows of D channels:
+ *     h_t = e^{g_t} h_{t-1} + x_t,    y_t = h_t,
+ * h in fp32.  Dense [B,T,D] (cu_seqlens NULL), or N sequences packed along t
+ * of batch 0 with offsets cu_seqlens as in GdnFwdParams (device memory, not
+ * read on the host, clamped to [0, T] by the kernels; rows that no sequence
+ * holds are not written).
+ *   - x, y (and dy, dx): x_dtype; g (and dg): g_dtype, x_dtype or fp32.  The
+ *     channel dimension is contiguous, (b, t) strides in elements are any;
+ *     with an even D, 4-byte aligned pointers (8-byte for fp32) and even
+ *     strides two channels are moved at a time.
+ *   - h0, dfinal (nullable: zero), final_state, dh0 (nullable): [N,D] fp32
+ *     with unit channel stride; h0_stride, dfinal_stride per sequence, the
+ *     outputs dense.
+ *   - states: fp32 [slots, D], the state at the start of every chunk of
+ *     gdn_scan_chunk() rows; slots = gdn_scan_slots().  The forward writes
+ *     it (nullable there: then it lies in the workspace); the backward reads
+ *     it (nullable: recomputed from x, g and h0).
+ *   - workspace: gdn_scan_workspace_size() / gdn_scan_bwd_workspace_size()
+ *     bytes, 256-byte aligned. */
+typedef struct GdnScanParams {
+  const void* x;
+  const void* g;
+  const float* h0;
+  void* y;                  /* forward only */
+  float* final_state;       /* forward only */
+  float* states;
+  const void* dy;           /* backward only, like the rest below */
+  const float* dfinal;
+  void* dx;
+  void* dg;
+  float* dh0;
+  const int64_t* cu_seqlens;
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t x_stride[2];
+  int64_t g_stride[2];
+  int64_t y_stride[2];
+  int64_t dy_stride[2];
+  int64_t dx_stride[2];
+  int64_t dg_stride[2];
+  int64_t h0_stride;
+  int64_t dfinal_stride;
+  int32_t B, T, D, N;       /* N = B without cu_seqlens */
+  int32_t x_dtype;
+  int32_t g_dtype;
+} GdnScanParams;
+
+int gdn_scan_chunk(void);
+int64_t gdn_scan_slots(int B, int T, int N, int packed);
+int64_t gdn_scan_workspace_size(const GdnScanParams* params);
+int64_t gdn_scan_bwd_workspace_size(const GdnScanParams* params);
+int gdn_scan_launch(const GdnScanParams* params, void* stream);
+int gdn_scan_bwd_launch(const GdnScanParams* params, void* stream);
+
+/* Root-mean-square norm of rows of D, with the residual's addition:
+ *     r = x + res,   y = r / sqrt(mean(r^2) + eps) * w
+ * (r in fp32; y is formed from it before r is rounded to r_dtype), and its
+ * gradient at the stored r:
+ *     dr = dr_in + rstd (w dy - n mean(w dy n)),  dw = sum_rows dy n,
+ *     n = r rstd.
+ * Rows are (n_outer, n_inner) with a stride for each; the columns are
+ * contiguous.
+ *   - res nullable: r = x, r_out is not written and r_dtype is x_dtype.
+ *   - y: x_dtype, or e4m3 bytes when `scale` is set: y / scale rounded to the
+ *     nearest, scale = max|y| / 448 over the row (group 0) or over each 128
+ *     columns (group 128, D a multiple of it); scale is dense
+ *     [rows, D / group] (or [rows]); a group of zeros has scale 0.
+ *   - backward: r, dy (x_dtype), dr_in (nullable, r_dtype); dr (r_dtype), dx
+ *     (nullable: the same in x_dtype), dw (w_dtype).
+ *   - w and dw: w_dtype (x_dtype or fp32), dense. */
+typedef struct GdnNormParams {
+  const void* x;            /* forward only */
+  const void* res;
+  const void* w;
+  void* y;
+  void* r_out;
+  float* scale;
+  const void* r;            /* backward only, like the rest below */
+  const void* dy;
+  const void* dr_in;
+  void* dr;
+  void* dx;
+  void* dw;
+  void* workspace;          /* gdn_norm_bwd_workspace_size() bytes */
+  int64_t workspace_bytes;
+  int64_t x_stride[2];      /* (outer, inner) rows, in elements */
+  int64_t res_stride[2];
+  int64_t y_stride[2];
+  int64_t r_out_stride[2];
+  int64_t r_stride[2];
+  int64_t dy_stride[2];
+  int64_t dr_in_stride[2];
+  int64_t dr_stride[2];
+  int64_t dx_stride[2];
+  int32_t n_outer, n_inner, D;
+  float eps;
+  int32_t group;            /* 0 or 128 */
+  int32_t x_dtype;
+  int32_t r_dtype;          /* of res, r_out, r, dr_in, dr */
+  int32_t w_dtype;
+} GdnNormParams;
+
+int gdn_norm_launch(const GdnNormParams* params, void* stream);
+int64_t gdn_norm_bwd_workspace_size(const GdnNormParams* params);
+int gdn_norm_bwd_launch(const GdnNormParams* params, void* stream);
+
 /* Human-readable text for a status code. */
 const char* gdn_fwd_status_string(int status);
 

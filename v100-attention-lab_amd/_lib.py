@@ -44,8 +44,18 @@ EXPORTED_SYMBOLS = (
     "gdn_bwd_launch",
     "gdn_fwd_launch_noalloc",
     "gdn_fwd_scratch_bytes",
+    "gdn_scan_chunk",
+    "gdn_scan_slots",
+    "gdn_scan_workspace_size",
+    "gdn_scan_bwd_workspace_size",
+    "gdn_scan_launch",
+    "gdn_scan_bwd_launch",
+    "gdn_norm_launch",
+    "gdn_norm_bwd_workspace_size",
+    "gdn_norm_bwd_launch",
 )
 
+_I64x2 = ctypes.c_int64 * 2
 _I64x3 = ctypes.c_int64 * 3
 _I64x4 = ctypes.c_int64 * 4
 
@@ -138,6 +148,34 @@ class GdnBwdParams(ctypes.Structure):
         [("cu_seqlens", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64)]
 
 
+def _fields(*groups):
+    """(name, type) pairs of groups of names with one type each."""
+    return [(n, t) for names, t in groups for n in names.split()]
+
+
+class GdnScanParams(ctypes.Structure):
+    """Mirror of ``GdnScanParams`` in include/gdn_mi355x.h."""
+
+    _fields_ = _fields(
+        ("x g h0 y final_state states dy dfinal dx dg dh0 cu_seqlens workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
+        ("x_stride g_stride y_stride dy_stride dx_stride dg_stride", _I64x2),
+        ("h0_stride dfinal_stride", ctypes.c_int64),
+        ("B T D N x_dtype g_dtype", ctypes.c_int32))
+
+
+class GdnNormParams(ctypes.Structure):
+    """Mirror of ``GdnNormParams`` in include/gdn_mi355x.h."""
+
+    _fields_ = _fields(
+        ("x res w y r_out scale r dy dr_in dr dx dw workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
+        ("x_stride res_stride y_stride r_out_stride r_stride dy_stride dr_in_stride dr_stride dx_stride", _I64x2),
+        ("n_outer n_inner D", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("group x_dtype r_dtype w_dtype", ctypes.c_int32))
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -179,6 +217,17 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
         lib.gdn_bwd_workspace_size_params.restype = ctypes.c_int64
         lib.gdn_bwd_segment_workspace_size.argtypes = [ctypes.POINTER(GdnBwdParams), ctypes.c_int]
         lib.gdn_bwd_segment_workspace_size.restype = ctypes.c_int64
+        for name, struct in (("scan", GdnScanParams), ("scan_bwd", GdnScanParams), ("norm", GdnNormParams),
+                             ("norm_bwd", GdnNormParams)):
+            if f"gdn_{name}_workspace_size" in EXPORTED_SYMBOLS:
+                size = getattr(lib, f"gdn_{name}_workspace_size")
+                size.argtypes, size.restype = [ctypes.POINTER(struct)], ctypes.c_int64
+            launch = getattr(lib, f"gdn_{name}_launch")
+            launch.argtypes, launch.restype = [ctypes.POINTER(struct), ctypes.c_void_p], ctypes.c_int
+        lib.gdn_scan_chunk.argtypes = []
+        lib.gdn_scan_chunk.restype = ctypes.c_int
+        lib.gdn_scan_slots.argtypes = [ctypes.c_int] * 4
+        lib.gdn_scan_slots.restype = ctypes.c_int64
         lib.gdn_fwd_abi_version.argtypes = []
         lib.gdn_fwd_abi_version.restype = ctypes.c_int
         ver = lib.gdn_fwd_abi_version()
@@ -190,3 +239,18 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
 
 def status_string(code: int) -> str:
     return load_library().gdn_fwd_status_string(int(code)).decode()
+
+
+_OP_STATUS = {
+    GDN_ERR_NULL_POINTER: "a required pointer is NULL",
+    GDN_ERR_BAD_SHAPE: "invalid sizes",
+    GDN_ERR_UNSUPPORTED: "unsupported configuration",
+    GDN_ERR_MISALIGNED: "rows must be 16-byte aligned with a contiguous last dimension",
+    GDN_ERR_BAD_DTYPE: "unsupported dtypes",
+    GDN_ERR_WORKSPACE: "workspace missing, misaligned or too small",
+}
+
+
+def op_status_string(code: int) -> str:
+    """Text of a status of the scan and norm calls."""
+    return _OP_STATUS.get(code) or status_string(code)

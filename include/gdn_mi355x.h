@@ -445,6 +445,80 @@ int gdn_norm_launch(const GdnNormParams* params, void* stream);
 int64_t gdn_norm_bwd_workspace_size(const GdnNormParams* params);
 int gdn_norm_bwd_launch(const GdnNormParams* params, void* stream);
 
+/* Softmax attention with a sliding window and first keys that stay visible.
+ * A sequence has Tq query rows and Tk key rows, the query rows being the last
+ * Tq positions: row i of the queries stands at position p = Tk - Tq + i and
+ * sees key j where j <= p and (j > p - window or j < sinks).  Hq query heads
+ * share Hk key heads (Hq a multiple of Hk), head h reads key head h / (Hq/Hk).
+ *     P = softmax(scale q k^T) over the visible keys, o = P v,
+ *     lse = log sum e^{scale q k^T}
+ * A row that sees no key has o = 0, lse = -inf and no gradients.
+ *   - q, o, dO, dq [B,Tq,Hq,D], k, v, dk, dv [B,Tk,Hk,D]: one 16-bit dtype;
+ *     D in {64, 128}, contiguous; pointers and (b, t, h) strides give
+ *     16-byte aligned rows.  lse [B,Tq,Hq] fp32, dense.
+ *   - cu_seqlens (nullable): N sequences packed along t of batch 0, the same
+ *     offsets for queries and keys (Tq = Tk), read by the kernels only and
+ *     clamped to [0, T].
+ *   - window >= 1 (INT32_MAX: every earlier key); sinks >= 0. */
+typedef struct GdnAttnParams {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* o;                  /* written by the forward, read by the backward */
+  float* lse;               /* the same; nullable in the forward */
+  const void* d_o;          /* backward only, like the rest below */
+  void* dq;
+  void* dk;
+  void* dv;
+  const int64_t* cu_seqlens;
+  void* workspace;          /* gdn_attn_bwd_workspace_size() bytes */
+  int64_t workspace_bytes;
+  int64_t q_stride[3];      /* (b, t, h), in elements */
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  int64_t o_stride[3];
+  int64_t do_stride[3];
+  int64_t dq_stride[3];
+  int64_t dk_stride[3];
+  int64_t dv_stride[3];
+  int32_t B, Tq, Tk, N;     /* N = B without cu_seqlens */
+  int32_t Hq, Hk, D;
+  int32_t window, sinks;
+  float scale;
+  int32_t dtype;
+} GdnAttnParams;
+
+int gdn_attn_launch(const GdnAttnParams* params, void* stream);
+int64_t gdn_attn_bwd_workspace_size(const GdnAttnParams* params);
+int gdn_attn_bwd_launch(const GdnAttnParams* params, void* stream);
+
+/* The same attention for the newest T tokens of each of B sequences over a
+ * cache: q, o [B,T,Hq,D]; k, v [B,S,Hk,D], of which the first
+ * cache_seqlens[b] rows are keys (the new tokens' own rows are the last T of
+ * them).  cache_seqlens: device int32, clamped to [0, S] by the kernel; cache
+ * rows from cache_seqlens[b] on are never read.  T in 1..16. */
+typedef struct GdnAttnDecodeParams {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* o;
+  const int32_t* cache_seqlens;
+  void* workspace;          /* gdn_attn_decode_workspace_size() bytes */
+  int64_t workspace_bytes;
+  int64_t q_stride[3];      /* (b, t, h), in elements */
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  int64_t o_stride[3];
+  int32_t B, T, S;
+  int32_t Hq, Hk, D;
+  int32_t window, sinks;
+  float scale;
+  int32_t dtype;
+} GdnAttnDecodeParams;
+
+int64_t gdn_attn_decode_workspace_size(const GdnAttnDecodeParams* params);
+int gdn_attn_decode_launch(const GdnAttnDecodeParams* params, void* stream);
+
 /* Human-readable text for a status code. */
 const char* gdn_fwd_status_string(int status);
 

@@ -53,6 +53,11 @@ EXPORTED_SYMBOLS = (
     "gdn_norm_launch",
     "gdn_norm_bwd_workspace_size",
     "gdn_norm_bwd_launch",
+    "gdn_attn_launch",
+    "gdn_attn_bwd_workspace_size",
+    "gdn_attn_bwd_launch",
+    "gdn_attn_decode_workspace_size",
+    "gdn_attn_decode_launch",
 )
 
 _I64x2 = ctypes.c_int64 * 2
@@ -176,6 +181,30 @@ class GdnNormParams(ctypes.Structure):
         ("group x_dtype r_dtype w_dtype", ctypes.c_int32))
 
 
+class GdnAttnParams(ctypes.Structure):
+    """Mirror of ``GdnAttnParams`` in include/gdn_mi355x.h."""
+
+    _fields_ = _fields(
+        ("q k v o lse d_o dq dk dv cu_seqlens workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
+        ("q_stride k_stride v_stride o_stride do_stride dq_stride dk_stride dv_stride", _I64x3),
+        ("B Tq Tk N Hq Hk D window sinks", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("dtype", ctypes.c_int32))
+
+
+class GdnAttnDecodeParams(ctypes.Structure):
+    """Mirror of ``GdnAttnDecodeParams`` in include/gdn_mi355x.h."""
+
+    _fields_ = _fields(
+        ("q k v o cache_seqlens workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
+        ("q_stride k_stride v_stride o_stride", _I64x3),
+        ("B T S Hq Hk D window sinks", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("dtype", ctypes.c_int32))
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -218,7 +247,8 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
         lib.gdn_bwd_segment_workspace_size.argtypes = [ctypes.POINTER(GdnBwdParams), ctypes.c_int]
         lib.gdn_bwd_segment_workspace_size.restype = ctypes.c_int64
         for name, struct in (("scan", GdnScanParams), ("scan_bwd", GdnScanParams), ("norm", GdnNormParams),
-                             ("norm_bwd", GdnNormParams)):
+                             ("norm_bwd", GdnNormParams), ("attn", GdnAttnParams), ("attn_bwd", GdnAttnParams),
+                             ("attn_decode", GdnAttnDecodeParams)):
             if f"gdn_{name}_workspace_size" in EXPORTED_SYMBOLS:
                 size = getattr(lib, f"gdn_{name}_workspace_size")
                 size.argtypes, size.restype = [ctypes.POINTER(struct)], ctypes.c_int64
@@ -252,5 +282,5 @@ _OP_STATUS = {
 
 
 def op_status_string(code: int) -> str:
-    """Text of a status of the scan and norm calls."""
+    """Text of a status of the scan, norm and attention calls."""
     return _OP_STATUS.get(code) or status_string(code)

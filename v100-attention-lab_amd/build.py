@@ -21,7 +21,7 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 # compiled in parallel.
 SOURCES = ["gdn_fwd_api.hip", "gdn_fwd_f16.hip", "gdn_fwd_bf16.hip", "gdn_fwd_f32.hip",
            "gdn_fwd_f32_batch.hip", "gdn_fwd_c64.hip", "gdn_fwd_scan32.hip", "gdn_prep.hip", "gdn_bwd.hip",
-           "gdn_scan.hip", "gdn_norm.hip"]
+           "gdn_scan.hip", "gdn_norm.hip", "gdn_attn_fwd.hip", "gdn_attn_bwd.hip", "gdn_attn_decode.hip"]
 OBJ_DIR = os.path.join(PKG_DIR, "_build")
 INCLUDE = os.path.join(REPO_DIR, "include")
 LIB_DIR = os.path.join(PKG_DIR, "lib")

@@ -1,0 +1,442 @@
+// Shared parts of the windowed attention kernels: operand types, the LDS tile
+// of key or query rows, the visible range of keys, and the map from workgroups
+// to sequences.
+//
+// Matrix products are v_mfma_f32_32x32x16: lane l supplies row (A) or column
+// (B) l % 32 and 8 contraction slots of half l / 32; accumulator register r
+// holds column l % 32, row 8 (r / 4) + 4 (l / 32) + r % 4.  Contraction order
+// is free, so a product P whose rows are the contraction of the next product
+// enters it straight from its accumulators: registers 8 s .. 8 s + 7 are the
+// slots of step s, contraction index 16 s + 8 (i / 4) + 4 (l / 32) + i % 4,
+// and the other operand is read in that order by two transposing LDS reads.
+#pragma once
+
+#include "gdn_row_io.h"
+
+namespace gdn {
+namespace attn {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef __attribute__((address_space(3))) void lds_void;
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// fp16 probabilities are kept times 2^7: with the running maximum at most 2^8
+// behind (kLazy) none overflows, and 2^-21 of the largest is still normal.
+template <typename T>
+struct Ops;
+template <>
+struct Ops<f16> {
+  typedef f16x8 Vec;
+  static constexpr float kShift = 7.f;
+  static constexpr uint32_t kExp = 0x7c00u;
+  static constexpr uint32_t kOne = 0x3c00u;
+  __device__ static __forceinline__ f32x16 mfma(Vec a, Vec b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+  __device__ static __forceinline__ uint32_t pack(float a, float b) {
+    typedef f16 f16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, f16x2{(f16)a, (f16)b});
+  }
+};
+template <>
+struct Ops<bf16_t> {
+  typedef bf16x8 Vec;
+  static constexpr float kShift = 0.f;
+  static constexpr uint32_t kExp = 0x7f80u;
+  static constexpr uint32_t kOne = 0x3f80u;
+  __device__ static __forceinline__ f32x16 mfma(Vec a, Vec b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  __device__ static __forceinline__ uint32_t pack(float a, float b) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
+  }
+};
+// How far (in powers of 2) the row maximum may rise before the accumulators
+// are rescaled.
+constexpr float kLazy = 8.f;
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float swap_halves(float x) { return __shfl_xor(x, 32, 64); }
+
+// Registers 8 s .. 8 s + 7 of a product as the operand of the next one.
+template <typename T>
+__device__ __forceinline__ typename Ops<T>::Vec acc_operand(const f32x16& p, int s) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = Ops<T>::pack(p[8 * s + 2 * i], p[8 * s + 2 * i + 1]);
+  typename Ops<T>::Vec v;
+  __builtin_memcpy(&v, w, 16);
+  return v;
+}
+
+// Accumulator row of register r.
+__device__ __forceinline__ int acc_row(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+
+// LDS byte address of a shared array.
+__device__ __forceinline__ uint32_t lds_addr(const void* p) { return (uint32_t)(uintptr_t)(lds_void*)p; }
+
+// 16 bytes per lane from global memory to LDS at `at` + 16 * lane (at
+// uniform).  Written out, so that the compiler does not take every LDS read
+// that follows for a reader of these bytes and wait for them there: a buffer
+// is read only after dma_wait() in every wave that filled it and a barrier.
+// (m0 holds nothing else: the compiler sets it right before each use.)
+// The instruction has no result registers, and a count of outstanding loads
+// that the compiler waits for is only met later for it, never earlier.
+__device__ __forceinline__ void dma16(const void* src, uint32_t at) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(at) : "memory");
+}
+// the same from a uniform base and a byte offset per lane
+__device__ __forceinline__ void dma16(const void* base, uint32_t ofs, uint32_t at) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(ofs), "s"(base), "s"(at)
+               : "memory");
+}
+// Every load of this wave so far, from memory and from LDS, is done.
+__device__ __forceinline__ void dma_wait() {
+  __builtin_amdgcn_s_waitcnt(7 << 4);   // vmcnt(0) lgkmcnt(0)
+  asm volatile("" ::: "memory");
+}
+// A pointer that is the same in every lane, in scalar registers.
+__device__ __forceinline__ const void* uniform_ptr(const void* p) {
+  const uint64_t u = (uint64_t)(uintptr_t)p;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)u), hi = __builtin_amdgcn_readfirstlane((uint32_t)(u >> 32));
+  return (const void*)(uintptr_t)(((uint64_t)hi << 32) | lo);
+}
+
+// ROWS rows of D 16-bit elements in LDS, in 16-byte pieces; piece c of row r
+// lies at piece c ^ swz(r) of the row.  16 rows at one piece (a product's
+// operand) and 4 rows at 64 neighbouring bytes (a transposing read) then each
+// cover all banks once.  swz depends on r % 16 only.
+template <int D>
+struct Tile {
+  static constexpr int kPieces = D / 8;
+  static constexpr int kRowBytes = 2 * D;
+  __device__ static __forceinline__ int swz(int row) {
+    return D == 128 ? ((row & 3) << 2) | ((row >> 2) & 3) : (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+  }
+  // Byte offset in a tile of this lane's operand rows: row l % 32, elements
+  // 8 (l / 32) ...  Step i is at offset ^ (32 i), 32 rows on at + 32 rows.
+  __device__ static __forceinline__ uint32_t row_ofs(int lane) {
+    const int r = lane & 31, h = lane >> 5;
+    return r * kRowBytes + ((h ^ swz(r)) << 4);
+  }
+  __device__ static __forceinline__ uint4 row8(uint32_t addr, int i, int imm) {
+    const u32x4 v = *(const lds_u32x4*)((addr ^ (uint32_t)(32 * i)) + imm);
+    return make_uint4(v[0], v[1], v[2], v[3]);
+  }
+  // Transposed operand: lane l receives element d0 + l % 32 of rows k0 + 4 h +
+  // {0..3} and k0 + 8 + 4 h + {0..3}, h = l / 32 (k0 a multiple of 16, d0 =
+  // 32 dt).  ds_read_b64_tr_b16: lane i of 16 receives halfword i % 4 of the 8
+  // bytes addressed by lanes 4 j + i / 4, j = 0..3.  The offsets of the two
+  // reads at k0 = 0, dt = 0; dt is at offset ^ (64 dt), k0 at + k0 rows.
+  __device__ static __forceinline__ uint32_t col_ofs(int lane, int which) {
+    const int a = lane & 15, h = lane >> 5, d = 16 * ((lane >> 4) & 1) + 4 * (a & 3);
+    const int r = 8 * which + 4 * h + (a >> 2);
+    return r * kRowBytes + (((d >> 3) ^ swz(r)) << 4) + 2 * (d & 7);
+  }
+  __device__ static __forceinline__ uint4 col8(uint32_t addr0, uint32_t addr1, int dt, int imm) {
+    union {
+      s16x4 h[2];
+      uint4 v;
+    } u;
+    u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)((addr0 ^ (uint32_t)(64 * dt)) + imm));
+    u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)((addr1 ^ (uint32_t)(64 * dt)) + imm));
+    return u.v;
+  }
+};
+
+// Copies rows row0 .. row0 + ROWS - 1 of a [rows, D] matrix (row stride ld
+// elements) into a tile by LDS-DMA, NT threads; rows past the last one are
+// copies of it.  A pass moves NT / kPieces rows (a multiple of 16, so a lane's
+// piece is the same in every pass).
+template <int D, int ROWS, int NT>
+struct Copier {
+  using TL = Tile<D>;
+  static constexpr int kPass = NT / TL::kPieces, kPasses = ROWS / kPass;
+  static_assert(kPass % 16 == 0 && ROWS % kPass == 0, "whole passes");
+  const uint16_t* src;
+  int64_t ld;
+  int rows;          // of the matrix
+  int row, piece;    // of this lane in the first pass
+  uint32_t ofs;      // its byte offset where that fits 31 bits
+  bool small;
+  __device__ __forceinline__ Copier(const uint16_t* s, int64_t ld_, int rows_) : src(s), ld(ld_), rows(rows_) {
+    const int tid = threadIdx.x;
+    row = tid / TL::kPieces;
+    piece = (tid % TL::kPieces) ^ TL::swz(row);
+    small = ld >= 0 && ld < (1 << 24);
+    ofs = (uint32_t)(row * (uint32_t)ld * 2u) + 16u * piece;
+  }
+  __device__ __forceinline__ void operator()(uint32_t tile, int row0) const {
+    const uint32_t at = tile + 16u * __builtin_amdgcn_readfirstlane(threadIdx.x & ~63);
+    if (small && row0 + ROWS <= rows) {
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i)
+        dma16(uniform_ptr(src + (int64_t)(row0 + i * kPass) * ld), ofs, at + i * NT * 16);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i)
+        dma16(src + (int64_t)min(row0 + i * kPass + row, rows - 1) * ld + 8 * piece, at + i * NT * 16);
+    }
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ typename Ops<T>::Vec as_vec(const uint4& u) {
+  return __builtin_bit_cast(typename Ops<T>::Vec, u);
+}
+
+// ---------------------------------------------------------------------------
+// sequences
+// ---------------------------------------------------------------------------
+
+struct Seq {
+  int b;             // batch index
+  int64_t q0, k0;    // first query and key row along t
+  int nq, nk;        // rows
+};
+
+struct SeqArgs {
+  const int64_t* cu;
+  int Tq, Tk, N;
+};
+
+__device__ __forceinline__ int64_t clamp_row(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : (v > hi ? hi : v); }
+
+__device__ __forceinline__ Seq get_seq(const SeqArgs& a, int i) {
+  Seq s;
+  if (a.cu == nullptr) {
+    s.b = i;
+    s.q0 = s.k0 = 0;
+    s.nq = a.Tq;
+    s.nk = a.Tk;
+  } else {
+    const int64_t b = clamp_row(a.cu[i], 0, a.Tq), e = clamp_row(a.cu[i + 1], b, a.Tq);
+    s.b = 0;
+    s.q0 = s.k0 = b;
+    s.nq = s.nk = (int)(e - b);
+  }
+  return s;
+}
+
+// Blocks of `rows` rows: a dense sequence has ceil(T / rows); packed sequence
+// i has its first at slot start / rows + i, which leaves each room for
+// ceil(len / rows) blocks.  Returns the sequence and the block in it (which
+// may lie past its end: nothing to do).
+__device__ __forceinline__ int find_block(const SeqArgs& a, int slot, int rows, int nblk, int& block) {
+  if (a.cu == nullptr) {
+    block = slot % nblk;
+    return slot / nblk;
+  }
+  auto first = [&](int i) { return (int)(clamp_row(a.cu[i], 0, a.Tq) / rows) + i; };
+  int lo = 0, hi = a.N;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (first(mid) <= slot) lo = mid; else hi = mid;
+  }
+  block = slot - first(lo);
+  return lo;
+}
+
+// Key tiles of TK keys that query positions [p0, p1] see: tiles [0, ns) of the
+// first keys, then [w0, w1).
+struct KeyRange {
+  int ns, w0, n;
+  __device__ __forceinline__ KeyRange(int p0, int p1, int nk, int window, int sinks, int tk) {
+    const int lo = (int)max((int64_t)p0 - window + 1, (int64_t)0);
+    const int hi = min(p1, nk - 1);
+    w0 = lo / tk;
+    const int w1 = hi < lo ? w0 : hi / tk + 1;
+    const int s = min(sinks, max(hi + 1, 0));
+    ns = min((s + tk - 1) / tk, w0);
+    n = ns + (w1 - w0);
+  }
+  __device__ __forceinline__ int tile(int i) const { return i < ns ? i : w0 + (i - ns); }
+};
+
+// Visibility of the accumulator rows of a lane whose column is query position
+// p: row c = 32 t + 8 (r / 4) + r % 4 of a key tile from j0 (the half's 4 rows
+// folded in) is seen where c <= hi and (c > lo or c < first).
+struct Mask {
+  int hi, lo, first;
+  __device__ __forceinline__ Mask(int p, int j0, int half, int nk, int window, int sinks) {
+    const int j = j0 + 4 * half;
+    hi = min(p, nk - 1) - j;
+    lo = (int)max((int64_t)p - window, (int64_t)-1) - j;
+    first = sinks - j;
+  }
+  __device__ __forceinline__ bool operator()(int t, int r) const {
+    const int c = 32 * t + 8 * (r >> 2) + (r & 3);
+    return (c <= hi) & ((c > lo) | (c < first));
+  }
+};
+
+// O^T += V^T P^T over one tile of which some keys are hidden from some rows,
+// where V holds infinities or NaN: those count only for the rows that see
+// them.  Their places are zero in the product; two products of 0/1 matrices
+// say which sums meet a +inf or NaN, and which a -inf or NaN.
+template <typename T, int D, int KS>
+__device__ __forceinline__ void pv_not_finite(f32x16 (&acc)[D / 32], const typename Ops<T>::Vec (&p)[2 * KS],
+                                           const Mask& seen, uint32_t v0, uint32_t v1) {
+  constexpr uint32_t E = Ops<T>::kExp, ONE = Ops<T>::kOne;
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt) {
+    f32x16 up = {}, dn = {};
+#pragma unroll
+    for (int s = 0; s < 2 * KS; ++s) {
+      const uint4 raw = Tile<D>::col8(v0, v1, dt, 16 * s * Tile<D>::kRowBytes);
+      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+      uint32_t f[4], u[4], d[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f[i] = u[i] = d[i] = 0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t x = (w[i] >> (16 * h)) & 0xffffu, mag = x & 0x7fffu;
+          if (mag < E) f[i] |= x << (16 * h);
+          if (mag > E || x == E) u[i] |= ONE << (16 * h);
+          if (mag > E || x == (E | 0x8000u)) d[i] |= ONE << (16 * h);
+        }
+      }
+      uint32_t one[4];    // the visible places of step s
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        one[i] = (seen(s >> 1, 8 * (s & 1) + 2 * i) ? ONE : 0u) | (seen(s >> 1, 8 * (s & 1) + 2 * i + 1) ? ONE << 16 : 0u);
+      const typename Ops<T>::Vec sv = as_vec<T>(make_uint4(one[0], one[1], one[2], one[3]));
+      acc[dt] = Ops<T>::mfma(as_vec<T>(make_uint4(f[0], f[1], f[2], f[3])), p[s], acc[dt]);
+      up = Ops<T>::mfma(as_vec<T>(make_uint4(u[0], u[1], u[2], u[3])), sv, up);
+      dn = Ops<T>::mfma(as_vec<T>(make_uint4(d[0], d[1], d[2], d[3])), sv, dn);
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      if (up[r] > 0.f) acc[dt][r] += __builtin_inff();
+      if (dn[r] > 0.f) acc[dt][r] -= __builtin_inff();
+    }
+  }
+}
+
+// Whether a tile of ROWS rows holds an infinity or NaN (a wave looks at all).
+template <typename T, int D, int ROWS>
+__device__ __forceinline__ bool tile_not_finite(uint32_t tile, int lane) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  u16x2 m = {0, 0};
+#pragma unroll
+  for (int i = 0; i < ROWS * D / 512; ++i) {
+    const u32x4 x = *(const lds_u32x4*)(tile + 16 * (i * 64 + lane));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t w = x[e] & 0x7fff7fffu;
+      m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w));
+    }
+  }
+  return __any(m[0] >= Ops<T>::kExp || m[1] >= Ops<T>::kExp);
+}
+
+// An operand with its sign turned where flip = 0x80008000 (else 0).
+template <typename T>
+__device__ __forceinline__ typename Ops<T>::Vec signed_vec(const uint4& x, uint32_t flip) {
+  return as_vec<T>(make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip));
+}
+
+// 32 query rows of a wave (lane l: row l % 32) against key tiles of 32 KS rows:
+// the running maximum m (in powers of 2, as the scores are), this lane's share
+// l of the sum, and O^T.
+template <typename T, int D, int KS>
+struct Rows {
+  using O = Ops<T>;
+  using Vec = typename O::Vec;
+  using TL = Tile<D>;
+  f32x16 acc[D / 32] = {};
+  float m = -__builtin_inff(), l = 0.f;
+
+  // kt: the lane's operand address in the key tile; vt: the value tile.
+  __device__ __forceinline__ void step(const Vec (&qf)[D / 16], uint32_t kt, uint32_t vt, uint32_t vofs0, uint32_t vofs1,
+                                       bool masked, const Mask& seen, float scale_log2, int lane) {
+    f32x16 s[KS] = {};
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+#pragma unroll
+      for (int t = 0; t < KS; ++t) s[t] = O::mfma(as_vec<T>(TL::row8(kt, i, 32 * t * TL::kRowBytes)), qf[i], s[t]);
+    }
+    if (masked) {
+#pragma unroll
+      for (int t = 0; t < KS; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[t][r] = seen(t, r) ? s[t][r] : -__builtin_inff();
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int t = 0; t < KS; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[t][r]);
+    mx = fmaxf(mx, swap_halves(mx)) * scale_log2;
+    if (__any(mx > m + kLazy)) {
+      // each row by its own scores, so that no row's bits depend on another's
+      const float mn = mx > m + kLazy ? mx : m;
+      const float f = mn == m ? 1.f : exp2_fast(m - mn);
+      m = mn;
+      l *= f;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][r] *= f;
+    }
+    const float mb = m == -__builtin_inff() ? 0.f : O::kShift - m;
+#pragma unroll
+    for (int t = 0; t < KS; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[t][r] = exp2_fast(__builtin_fmaf(s[t][r], scale_log2, mb));
+        l += s[t][r];
+      }
+    Vec pf[2 * KS];
+#pragma unroll
+    for (int t = 0; t < 2 * KS; ++t) pf[t] = acc_operand<T>(s[t >> 1], t & 1);
+    if (masked && tile_not_finite<T, D, 32 * KS>(vt, lane)) {
+      pv_not_finite<T, D, KS>(acc, pf, seen, vt + vofs0, vt + vofs1);
+    } else {
+#pragma unroll
+      for (int t = 0; t < 2 * KS; ++t)
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt)
+          acc[dt] = O::mfma(as_vec<T>(TL::col8(vt + vofs0, vt + vofs1, dt, 16 * t * TL::kRowBytes)), pf[t], acc[dt]);
+    }
+  }
+};
+
+// Whether every key of [j0, j1] is visible to every position of [p0, p1].
+__device__ __forceinline__ bool all_visible(int j0, int j1, int p0, int p1, int window, int sinks) {
+  return j1 <= p0 && (p1 - j0 < window || j1 < sinks);
+}
+// Whether none is.
+__device__ __forceinline__ bool none_visible(int j0, int j1, int p0, int p1, int window, int sinks) {
+  return j0 > p1 || (p0 - j1 >= window && j0 >= sinks);
+}
+
+// Rows of D 16-bit elements are read 16 bytes at a time; a stride that no
+// index uses may be anything.
+inline bool rows16(const void* p, const int64_t* s, int64_t b, int64_t t, int64_t h) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (b <= 1 || s[0] % 8 == 0) && (t <= 1 || s[1] % 8 == 0) &&
+         (h <= 1 || s[2] % 8 == 0);
+}
+
+// The scale in powers of 2 and the sign that goes into q: the running maximum
+// is taken of the products, so the factor after it is positive (of a scale of
+// zero, so small that every visible score is zero and hidden ones stay -inf).
+inline void split_scale(float scale, float& log2, uint32_t& flip) {
+  flip = scale < 0.f ? 0x80008000u : 0u;
+  log2 = scale == 0.f ? 1e-30f : (scale < 0.f ? -scale : scale) * kLog2e;
+}
+
+int check_attn(const GdnAttnParams& P);
+
+}  // namespace attn
+}  // namespace gdn

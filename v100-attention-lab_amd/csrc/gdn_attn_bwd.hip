@@ -1,0 +1,682 @@
+// Windowed attention, backward:
+//     P = e^{scale q k^T - lse},  dP = dO v^T,  dS = P (dP - D),  D = dO . o
+//     dv = P^T dO,  dk = scale dS^T q,  dq = scale dS k
+// in three steps, each sum in one workgroup and in a fixed order:
+//   prep  per query row lse in powers of 2, D, and (fp16) the largest |dO|;
+//   kv    128 key rows a workgroup, 32 a wave: query rows of all heads that
+//         share the key head pass in tiles of 32 (S and dP with a lane on one
+//         key; P and dS enter dV^T += dO^T P and dK^T += Q^T dS straight from
+//         their accumulators);
+//   q     128 query rows a workgroup, 32 a wave, key tiles of 64 as in the
+//         forward: S^T, dP^T, dQ^T += K^T dS^T.
+// Blocks of the first keys (the sinks) are seen by every later query row: the
+// rows beyond the block's window are cut into segments with workgroups of
+// their own, whose fp32 sums a last kernel adds in order.
+//
+// fp16 keeps P times 2^14 and dS in a unit of its own, 2^-7 of the product of
+// the largest |dO| (of the row, or of the tiles so far) and the largest |v| of
+// the head: |dS| <= 2 D of that product, so none overflows and small gradients
+// keep their precision.
+
+#include <algorithm>
+
+#include "gdn_attn.h"
+
+namespace gdn {
+namespace attn {
+
+constexpr int kKB = 128;       // key rows a workgroup (kv)
+constexpr int kQT = 32;        // query rows a tile (kv)
+constexpr int kQB = 128;       // query rows a workgroup (q)
+constexpr int kKT = 64;        // keys a tile (q)
+constexpr int kVParts = 64;    // partial maxima of |v| a head
+
+struct BArgs {
+  const uint16_t* q;
+  const uint16_t* k;
+  const uint16_t* v;
+  const uint16_t* o;
+  const uint16_t* dO;
+  const float* lse;
+  uint16_t* dq;
+  uint16_t* dk;
+  uint16_t* dv;
+  float* stat;      // [Hq][rows][2]: lse in powers of 2, D
+  float* rmax;      // [Hq][rows] largest |dO| (fp16)
+  float* vmax;      // [units_k][kVParts] (fp16)
+  float* part;      // [units_k][sink blocks][segments][2][kKB][D]
+  SeqArgs seq;
+  int64_t qs[3], ks[3], vs[3], os[3], dos[3], dqs[3], dks[3], dvs[3];
+  int64_t rows;     // B Tq
+  int Hq, Hk, G, B;
+  int units_q, units_k;         // (batch and) heads of the q and kv grids
+  int slots_q, slots_k;         // blocks of each
+  int sink_blocks, seg, slots_s;  // blocks of the first keys, rows a segment, segment slots
+  int window, sinks;
+  float scale, scale_log2;
+};
+
+template <typename T>
+constexpr bool kScaled = std::is_same<T, f16>::value;
+// P is kept times 2^kPUp in the products of the backward.
+template <typename T>
+constexpr float kPUp = kScaled<T> ? 14.f : 0.f;
+
+// The power of 2 at or above x (of fp16 values; 2^-24 for zero).
+__device__ __forceinline__ float pow2_above(float x) {
+  int e = 0;
+  (void)frexpf(fmaxf(x, 0x1p-24f), &e);
+  return ldexpf(1.f, e);
+}
+
+// ---------------------------------------------------------------------------
+// prep
+// ---------------------------------------------------------------------------
+
+__device__ __forceinline__ float finite_abs(float x) {
+  const float y = fabsf(x);
+  return y < __builtin_inff() ? y : 0.f;
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(256) void prep_kernel(const BArgs a, int row_blocks) {
+  constexpr int L = D / 8, RPB = 256 / L;      // lanes a row, rows a workgroup
+  if ((int)blockIdx.x < row_blocks) {
+    // heads of a row are neighbours: reads of o and dO are in order
+    const int64_t at = (int64_t)blockIdx.x * RPB + threadIdx.x / L;
+    const int c = threadIdx.x % L;
+    const bool ok = at < a.rows * a.Hq;
+    const int64_t row = ok ? at / a.Hq : 0;
+    const int h = ok ? (int)(at % a.Hq) : 0;
+    const int64_t b = row / a.seq.Tq, t = row % a.seq.Tq;
+    rowio::Pack<T, 8> po, pd;
+    po.load(reinterpret_cast<const T*>(a.o) + b * a.os[0] + t * a.os[1] + h * a.os[2] + 8 * c);
+    pd.load(reinterpret_cast<const T*>(a.dO) + b * a.dos[0] + t * a.dos[1] + h * a.dos[2] + 8 * c);
+    float d = 0.f, m = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = pd.get(e);
+      d = __builtin_fmaf(x, po.get(e), d);
+      if constexpr (kScaled<T>) m = fmaxf(m, finite_abs(x));
+    }
+#pragma unroll
+    for (int s = L / 2; s >= 1; s >>= 1) {
+      d += __shfl_xor(d, s, 64);
+      if constexpr (kScaled<T>) m = fmaxf(m, __shfl_xor(m, s, 64));
+    }
+    if (ok && c == 0) {
+      const float l = a.lse[at];
+      float* st = a.stat + ((int64_t)h * a.rows + row) * 2;
+      st[0] = l == -__builtin_inff() ? __builtin_inff() : l * kLog2e;
+      st[1] = d;
+      if constexpr (kScaled<T>) a.rmax[(int64_t)h * a.rows + row] = m;
+    }
+    return;
+  }
+  if constexpr (kScaled<T>) {
+    // one part of one head's keys
+    const int e = blockIdx.x - row_blocks, part = e % kVParts, unit = e / kVParts;
+    const int b = unit / a.Hk, hk = unit % a.Hk;
+    const int n = (a.seq.Tk + kVParts - 1) / kVParts, t0 = part * n, t1 = min(t0 + n, a.seq.Tk);
+    float m = 0.f;
+    for (int t = t0 + threadIdx.x / L; t < t1; t += RPB) {
+      rowio::Pack<T, 8> pv;
+      pv.load(reinterpret_cast<const T*>(a.v) + b * a.vs[0] + (int64_t)t * a.vs[1] + hk * a.vs[2] + 8 * (threadIdx.x % L));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m = fmaxf(m, finite_abs(pv.get(i)));
+    }
+#pragma unroll
+    for (int s = 32; s >= 1; s >>= 1) m = fmaxf(m, __shfl_xor(m, s, 64));
+    __shared__ float sm[4];
+    if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
+    __syncthreads();
+    if (threadIdx.x == 0) a.vmax[unit * kVParts + part] = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+  }
+}
+
+// The largest |v| of a head, as a power of 2.
+__device__ __forceinline__ float v_unit(const BArgs& a, int b, int hk, int lane) {
+  float m = a.vmax[(b * a.Hk + hk) * kVParts + lane];
+#pragma unroll
+  for (int s = 32; s >= 1; s >>= 1) m = fmaxf(m, __shfl_xor(m, s, 64));
+  return pow2_above(m);
+}
+
+// An operand with its infinities and NaN replaced by zero.
+template <typename T>
+__device__ __forceinline__ uint4 only_finite(const uint4& x) {
+  constexpr uint32_t E = Ops<T>::kExp;
+  uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if ((w[i] & E) == E) w[i] &= 0xffff0000u;
+    if ((w[i] & (E << 16)) == (E << 16)) w[i] &= 0x0000ffffu;
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Output rows from transposed accumulators: lane l holds row l % 32.
+template <typename T, int D>
+__device__ __forceinline__ void store_rows(uint16_t* row, const f32x16 (&acc)[D / 32], float f, int half) {
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      *reinterpret_cast<uint2*>(row + 32 * dt + 8 * c + 4 * half) =
+          make_uint2(Ops<T>::pack(acc[dt][4 * c] * f, acc[dt][4 * c + 1] * f),
+                     Ops<T>::pack(acc[dt][4 * c + 2] * f, acc[dt][4 * c + 3] * f));
+}
+
+// ---------------------------------------------------------------------------
+// kv
+// ---------------------------------------------------------------------------
+
+// Query rows that a key block takes itself: those in reach of its window; the
+// rest of a block of first keys goes to segments.  Rows of the sequence.
+struct QRange {
+  int r0, r1;        // [r0, r1)
+};
+__device__ __forceinline__ QRange own_rows(const BArgs& a, const Seq& s, int k0) {
+  const int shift = s.nk - s.nq;
+  QRange q;
+  q.r0 = max(k0 - shift, 0);
+  q.r1 = (int)min((int64_t)s.nq, max((int64_t)k0 + kKB - 1 + a.window - shift, (int64_t)0));
+  return q;
+}
+__device__ __forceinline__ QRange seg_rows(const BArgs& a, const Seq& s, int k0, int seg) {
+  const QRange own = own_rows(a, s, k0);
+  QRange q;
+  q.r0 = max(max(own.r0, own.r1), seg * a.seg);
+  q.r1 = (int)min((int64_t)s.nq, (int64_t)(seg + 1) * a.seg);
+  return q;
+}
+
+// 4 bytes per lane from global memory to LDS at `at` + 4 * lane.
+__device__ __forceinline__ void dma4(const void* src, uint32_t at) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(at) : "memory");
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(256, 1) void kv_kernel(const BArgs a) {
+  using O = Ops<T>;
+  using Vec = typename O::Vec;
+  using TL = Tile<D>;
+  constexpr uint32_t kTile = kQT * TL::kRowBytes, kBuf = 2 * kTile + 512;    // Q, dO, 32 x (lse, D), 32 x max
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kBuf];
+  const int unit_ix = blockIdx.x % a.units_k, item = blockIdx.x / a.units_k;
+  const int unit = a.units_k % 8 == 0 ? (unit_ix % 8) * (a.units_k / 8) + unit_ix / 8 : unit_ix;
+  const bool extra = item >= a.slots_k;
+  int si, hk, block, seg = 0;
+  if (!extra) {
+    if (a.seq.cu == nullptr) {
+      si = unit / a.Hk;
+      hk = unit % a.Hk;
+      block = item;
+    } else {
+      hk = unit;
+      si = find_block(a.seq, item, kKB, 0, block);
+    }
+  } else {
+    const int e = item - a.slots_k;
+    block = e % a.sink_blocks;
+    if (a.seq.cu == nullptr) {
+      si = unit / a.Hk;
+      hk = unit % a.Hk;
+      seg = e / a.sink_blocks;
+    } else {
+      hk = unit;
+      si = find_block(a.seq, e / a.sink_blocks, a.seg, 0, seg);
+    }
+  }
+  const Seq sq = get_seq(a.seq, si);
+  const int k0 = block * kKB;
+  if (block < 0 || k0 >= sq.nk || seg < 0 || (int64_t)seg * a.seg > sq.nq) return;
+  const int shift = sq.nk - sq.nq;
+  const QRange rg = extra ? seg_rows(a, sq, k0, seg) : own_rows(a, sq, k0);
+  if (extra && rg.r1 <= rg.r0) return;
+  const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int key = k0 + wv * 32 + l32;          // this lane's key row
+  const int j0 = k0 + wv * 32, j1 = min(j0 + 32, sq.nk) - 1;
+
+  Vec kf[D / 16], vf[D / 16];
+  {
+    const int64_t r = sq.k0 + min(key, sq.nk - 1);
+    const uint16_t* kr = a.k + sq.b * a.ks[0] + r * a.ks[1] + hk * a.ks[2];
+    const uint16_t* vr = a.v + sq.b * a.vs[0] + r * a.vs[1] + hk * a.vs[2];
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      kf[i] = as_vec<T>(*reinterpret_cast<const uint4*>(kr + 16 * i + 8 * half));
+      vf[i] = as_vec<T>(*reinterpret_cast<const uint4*>(vr + 16 * i + 8 * half));
+    }
+  }
+  const int nt = (max(rg.r1 - rg.r0, 0) + kQT - 1) / kQT, n = nt * a.G;
+  float vu = 1.f;
+  if constexpr (kScaled<T>)
+    if (n > 0) vu = v_unit(a, sq.b, hk, lane);
+  float unit_do = 0x1p-24f;                     // unit of dO so far (fp16)
+  f32x16 dk[D / 32] = {}, dv[D / 32] = {};
+
+  const uint32_t base = lds_addr(lds);
+  const uint32_t rofs = TL::row_ofs(lane), cofs0 = TL::col_ofs(lane, 0), cofs1 = TL::col_ofs(lane, 1);
+  auto fetch = [&](int it) {
+    const int g = it / nt, r0 = rg.r0 + (it % nt) * kQT, h = hk * a.G + g;
+    const uint32_t at = base + (it & 1) * kBuf;
+    const Copier<D, kQT, 256> cq(a.q + sq.b * a.qs[0] + sq.q0 * a.qs[1] + h * a.qs[2], a.qs[1], sq.nq);
+    const Copier<D, kQT, 256> cd(a.dO + sq.b * a.dos[0] + sq.q0 * a.dos[1] + h * a.dos[2], a.dos[1], sq.nq);
+    cq(at, r0);
+    cd(at + kTile, r0);
+    const int64_t row = (int64_t)h * a.rows + (int64_t)sq.b * a.seq.Tq + sq.q0 + min(r0 + (lane & 31), sq.nq - 1);
+    if (wv == 0) {
+      // lanes 0..31 bring lse, 32..63 D
+      dma4(a.stat + row * 2 + half, __builtin_amdgcn_readfirstlane(at + 2 * kTile));
+      if constexpr (kScaled<T>) dma4(a.rmax + row, __builtin_amdgcn_readfirstlane(at + 2 * kTile + 256));
+    }
+  };
+  dma_wait();
+  if (n > 0) fetch(0);
+  for (int it = 0; it < n; ++it) {
+    dma_wait();
+    __syncthreads();
+    if (it + 1 < n) fetch(it + 1);
+    const uint32_t qt = base + (it & 1) * kBuf, dt_ = qt + kTile, st = qt + 2 * kTile;
+    const int r0 = rg.r0 + (it % nt) * kQT, nr = min(kQT, rg.r1 - r0);
+    const int p0 = r0 + shift, p1 = p0 + nr - 1;
+    float sc = 1.f;
+    if constexpr (kScaled<T>) {
+      // the tile's unit, in every wave alike
+      typedef __attribute__((address_space(3))) const float lds_float;
+      float m = *(lds_float*)(st + 256 + 4 * l32);
+#pragma unroll
+      for (int s = 16; s >= 1; s >>= 1) m = fmaxf(m, __shfl_xor(m, s, 64));
+      const float u = pow2_above(m);
+      if (u > unit_do) {
+        const float f = unit_do / u;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) dk[i][r] *= f;
+        unit_do = u;
+      }
+      sc = 0x1p-7f / (unit_do * vu);            // 2^7 / unit, and P's 2^14 taken out
+    }
+    if (none_visible(j0, j1, p0, p1, a.window, a.sinks)) continue;
+    const bool masked = !(nr == kQT && j0 + 32 <= sq.nk && all_visible(j0, j1, p0, p1, a.window, a.sinks));
+
+    f32x16 s = {}, dp = {};
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) s = O::mfma(as_vec<T>(TL::row8(qt + rofs, i, 0)), kf[i], s);
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) dp = O::mfma(as_vec<T>(TL::row8(dt_ + rofs, i, 0)), vf[i], dp);
+    typedef float f32x4v __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) const f32x4v lds_f32x4;
+    bool bad = false;
+    if (masked) bad = tile_not_finite<T, D, kQT>(qt, lane) || tile_not_finite<T, D, kQT>(dt_, lane);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const f32x4v ls = *(lds_f32x4*)(st + 32 * c + 16 * half), de = *(lds_f32x4*)(st + 128 + 32 * c + 16 * half);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = 4 * c + e;
+        const float x = exp2_fast(__builtin_fmaf(s[r], a.scale_log2, kPUp<T> - ls[e]));
+        dp[r] = x * __builtin_fmaf(dp[r], sc, -de[e] * sc);
+        s[r] = x;
+      }
+      if (masked) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = 4 * c + e, row = acc_row(r, half), p = p0 + row;
+          const bool ok = (row < nr) & (key <= p) & ((p - key < a.window) | (key < a.sinks)) & (key < sq.nk);
+          // a row of dO that is not finite reaches the keys that see it
+          const float hit = fabsf(de[e]) < __builtin_inff() ? 0.f : __builtin_nanf("");
+          s[r] = ok ? (bad ? s[r] + hit : s[r]) : 0.f;
+          dp[r] = ok ? dp[r] : 0.f;
+        }
+      }
+    }
+    Vec pf[2], df[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      pf[t] = acc_operand<T>(s, t);
+      df[t] = acc_operand<T>(dp, t);
+    }
+    if (bad) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          dv[i] = O::mfma(as_vec<T>(only_finite<T>(TL::col8(dt_ + cofs0, dt_ + cofs1, i, 16 * t * TL::kRowBytes))), pf[t], dv[i]);
+          dk[i] = O::mfma(as_vec<T>(only_finite<T>(TL::col8(qt + cofs0, qt + cofs1, i, 16 * t * TL::kRowBytes))), df[t], dk[i]);
+        }
+    } else {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          dv[i] = O::mfma(as_vec<T>(TL::col8(dt_ + cofs0, dt_ + cofs1, i, 16 * t * TL::kRowBytes)), pf[t], dv[i]);
+          dk[i] = O::mfma(as_vec<T>(TL::col8(qt + cofs0, qt + cofs1, i, 16 * t * TL::kRowBytes)), df[t], dk[i]);
+        }
+    }
+  }
+  const float fv = exp2f(-kPUp<T>);
+  const float fk = kScaled<T> ? a.scale * unit_do * vu * 0x1p-7f : a.scale;
+  if (block < a.sink_blocks) {
+    // fp32 parts: slot 0 the block's own rows, then the segments
+    const int64_t slots = a.slots_s + 1;
+    const int64_t slot = a.seq.cu == nullptr ? (extra ? 1 + seg : 0)
+                                             : (extra ? (item - a.slots_k) / a.sink_blocks + 1 : 0);
+    // packed: a row of parts per sequence for the own rows
+    const int64_t u = a.seq.cu == nullptr ? unit : hk;
+    float* part = extra || a.seq.cu == nullptr
+                      ? a.part + ((u * a.sink_blocks + block) * slots + slot) * (2 * kKB * D)
+                      : a.part + ((int64_t)a.units_k * a.sink_blocks * slots + (u * a.sink_blocks + block) * a.seq.N + si) * (2 * kKB * D);
+    float* pk = part + (wv * 32 + l32) * D;
+    float* pv = pk + kKB * D;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int d = 32 * i + 8 * c + 4 * half;
+        *reinterpret_cast<float4*>(pk + d) = make_float4(dk[i][4 * c] * fk, dk[i][4 * c + 1] * fk, dk[i][4 * c + 2] * fk, dk[i][4 * c + 3] * fk);
+        *reinterpret_cast<float4*>(pv + d) = make_float4(dv[i][4 * c] * fv, dv[i][4 * c + 1] * fv, dv[i][4 * c + 2] * fv, dv[i][4 * c + 3] * fv);
+      }
+    return;
+  }
+  if (key >= sq.nk) return;
+  store_rows<T, D>(a.dk + sq.b * a.dks[0] + (sq.k0 + key) * a.dks[1] + hk * a.dks[2], dk, fk, half);
+  store_rows<T, D>(a.dv + sq.b * a.dvs[0] + (sq.k0 + key) * a.dvs[1] + hk * a.dvs[2], dv, fv, half);
+}
+
+// Sums of the parts of a block of first keys: a workgroup a block, sequence
+// and 8 key rows.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void sink_sum_kernel(const BArgs a) {
+  constexpr int kRowsWg = 8;
+  const int rg = blockIdx.x % (kKB / kRowsWg), rest = blockIdx.x / (kKB / kRowsWg);
+  const int block = rest % a.sink_blocks, us = rest / a.sink_blocks;   // us: unit (dense) or (head, sequence)
+  const int si = a.seq.cu == nullptr ? us / a.Hk : us % a.seq.N;
+  const int hk = a.seq.cu == nullptr ? us % a.Hk : us / a.seq.N;
+  const int64_t u = a.seq.cu == nullptr ? us : hk;
+  const Seq sq = get_seq(a.seq, si);
+  const int k0 = block * kKB;
+  if (k0 >= sq.nk) return;
+  const int64_t slots = a.slots_s + 1, one = 2 * kKB * D;
+  const float* parts = a.part + (u * a.sink_blocks + block) * slots * one;
+  const float* own = a.seq.cu == nullptr
+                         ? parts
+                         : a.part + ((int64_t)a.units_k * a.sink_blocks * slots + (u * a.sink_blocks + block) * a.seq.N + si) * one;
+  const int first = a.seq.cu == nullptr ? 0 : (int)(sq.q0 / a.seg) + si;
+  const int nseg = (sq.nq + a.seg - 1) / a.seg;
+  for (int e = threadIdx.x; e < kRowsWg * D / 4; e += 256) {
+    const int r = rg * kRowsWg + e / (D / 4), d = 4 * (e % (D / 4)), key = k0 + r;
+    if (key >= sq.nk) continue;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      float4 s = *reinterpret_cast<const float4*>(own + (w * kKB + r) * D + d);
+      for (int g = 0; g < nseg; ++g) {
+        const QRange q = seg_rows(a, sq, k0, g);
+        if (q.r1 <= q.r0) continue;
+        const float4 x = *reinterpret_cast<const float4*>(parts + (1 + first + g) * one + (w * kKB + r) * D + d);
+        s.x += x.x;
+        s.y += x.y;
+        s.z += x.z;
+        s.w += x.w;
+      }
+      uint16_t* out = w == 0 ? a.dk + sq.b * a.dks[0] + (sq.k0 + key) * a.dks[1] + hk * a.dks[2]
+                             : a.dv + sq.b * a.dvs[0] + (sq.k0 + key) * a.dvs[1] + hk * a.dvs[2];
+      *reinterpret_cast<uint2*>(out + d) = make_uint2(Ops<T>::pack(s.x, s.y), Ops<T>::pack(s.z, s.w));
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// q
+// ---------------------------------------------------------------------------
+
+template <typename T, int D>
+__global__ __launch_bounds__(256, 2) void q_kernel(const BArgs a) {
+  using O = Ops<T>;
+  using Vec = typename O::Vec;
+  using TL = Tile<D>;
+  constexpr uint32_t kTile = kKT * TL::kRowBytes;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * kTile];
+  const int unit_ix = blockIdx.x % a.units_q, slot = a.slots_q - 1 - blockIdx.x / a.units_q;
+  const int unit = a.units_q % 8 == 0 ? (unit_ix % 8) * (a.units_q / 8) + unit_ix / 8 : unit_ix;
+  int block, si, head;
+  if (a.seq.cu == nullptr) {
+    si = unit / a.Hq;
+    head = unit % a.Hq;
+    block = slot;
+  } else {
+    head = unit;
+    si = find_block(a.seq, slot, kQB, 0, block);
+  }
+  const Seq sq = get_seq(a.seq, si);
+  const int m0 = block * kQB;
+  if (block < 0 || m0 >= sq.nq) return;
+  const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int shift = sq.nk - sq.nq;
+  const int row = m0 + wv * 32 + l32, p = row + shift;
+  const int hk = head / a.G;
+  const int p0 = m0 + shift, p1 = min(m0 + kQB, sq.nq) - 1 + shift;
+  const KeyRange kr(p0, p1, sq.nk, a.window, a.sinks, kKT);
+  const int wp0 = m0 + wv * 32 + shift, wp1 = min(wp0 + 31, sq.nq - 1 + shift);
+
+  Vec qf[D / 16], df[D / 16];
+  const int64_t at = sq.q0 + min(row, sq.nq - 1);
+  {
+    const uint16_t* qr = a.q + sq.b * a.qs[0] + at * a.qs[1] + head * a.qs[2];
+    const uint16_t* dr = a.dO + sq.b * a.dos[0] + at * a.dos[1] + head * a.dos[2];
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      qf[i] = as_vec<T>(*reinterpret_cast<const uint4*>(qr + 16 * i + 8 * half));
+      df[i] = as_vec<T>(*reinterpret_cast<const uint4*>(dr + 16 * i + 8 * half));
+    }
+  }
+  const int64_t sat = (int64_t)head * a.rows + (int64_t)sq.b * a.seq.Tq + at;
+  const float2 st = *reinterpret_cast<const float2*>(a.stat + sat * 2);
+  float u = 1.f, sc = 1.f;
+  if constexpr (kScaled<T>) {
+    u = pow2_above(a.rmax[sat]) * v_unit(a, sq.b, hk, lane);
+    sc = 0x1p-7f / u;
+  }
+  const float lb = kPUp<T> - st.x, de = -st.y * sc;
+  f32x16 dq[D / 32] = {};
+
+  const Copier<D, kKT, 256> ck(a.k + sq.b * a.ks[0] + sq.k0 * a.ks[1] + hk * a.ks[2], a.ks[1], sq.nk);
+  const Copier<D, kKT, 256> cv(a.v + sq.b * a.vs[0] + sq.k0 * a.vs[1] + hk * a.vs[2], a.vs[1], sq.nk);
+  const uint32_t base = lds_addr(lds);
+  const uint32_t rofs = TL::row_ofs(lane), cofs0 = TL::col_ofs(lane, 0), cofs1 = TL::col_ofs(lane, 1);
+  dma_wait();
+  if (kr.n > 0) {
+    ck(base, kr.tile(0) * kKT);
+    cv(base + kTile, kr.tile(0) * kKT);
+  }
+  for (int it = 0; it < kr.n; ++it) {
+    const uint32_t kt = base + (it & 1) * 2 * kTile, vt = kt + kTile;
+    dma_wait();
+    __syncthreads();
+    if (it + 1 < kr.n) {
+      const uint32_t other = base + ((it + 1) & 1) * 2 * kTile;
+      ck(other, kr.tile(it + 1) * kKT);
+      cv(other + kTile, kr.tile(it + 1) * kKT);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int j0 = kr.tile(it) * kKT + 32 * h, j1 = min(j0 + 32, sq.nk) - 1;
+      if (j0 >= sq.nk || none_visible(j0, j1, wp0, wp1, a.window, a.sinks)) continue;
+      const bool masked = !(j0 + 32 <= sq.nk && all_visible(j0, j1, wp0, wp1, a.window, a.sinks));
+      const uint32_t kh = kt + 32 * h * TL::kRowBytes, vh = vt + 32 * h * TL::kRowBytes;
+      f32x16 s = {}, dp = {};
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) s = O::mfma(as_vec<T>(TL::row8(kh + rofs, i, 0)), qf[i], s);
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) dp = O::mfma(as_vec<T>(TL::row8(vh + rofs, i, 0)), df[i], dp);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float x = exp2_fast(__builtin_fmaf(s[r], a.scale_log2, lb));
+        dp[r] = x * __builtin_fmaf(dp[r], sc, de);
+      }
+      bool bad = false;
+      if (masked) {
+        const Mask seen(p, j0, half, sq.nk, a.window, a.sinks);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dp[r] = seen(0, r) ? dp[r] : 0.f;
+        bad = tile_not_finite<T, D, 32>(kh, lane);
+      }
+      Vec sf[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) sf[t] = acc_operand<T>(dp, t);
+      if (bad) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i)
+            dq[i] = O::mfma(as_vec<T>(only_finite<T>(TL::col8(kh + cofs0, kh + cofs1, i, 16 * t * TL::kRowBytes))), sf[t], dq[i]);
+      } else {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i)
+            dq[i] = O::mfma(as_vec<T>(TL::col8(kh + cofs0, kh + cofs1, i, 16 * t * TL::kRowBytes)), sf[t], dq[i]);
+      }
+    }
+  }
+  if (row >= sq.nq) return;
+  const float f = kScaled<T> ? a.scale * u * 0x1p-7f : a.scale;
+  store_rows<T, D>(a.dq + sq.b * a.dqs[0] + (sq.q0 + row) * a.dqs[1] + head * a.dqs[2], dq, f, half);
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+
+int64_t up256(int64_t n) { return (n + 255) & ~(int64_t)255; }
+
+// Blocks of first keys, rows a segment and segment slots of a call (none where
+// no row lies beyond the first block's window).
+void sink_plan(const GdnAttnParams& P, int& blocks, int& seg, int& slots) {
+  blocks = seg = slots = 0;
+  const int64_t sinks = std::min<int64_t>(P.sinks, P.Tk);
+  if (sinks == 0 || P.Tq == 0 || (int64_t)P.window + kKB >= P.Tk) return;
+  blocks = (int)((sinks + kKB - 1) / kKB);
+  // as much work as a block's own rows, and few enough parts: they take at
+  // most as many rows of D floats as there are query rows, twice
+  seg = (int)std::max<int64_t>({(int64_t)P.window + kKB, (int64_t)blocks * kKB, 512});
+  seg = (seg + kQT - 1) / kQT * kQT;
+  slots = P.cu_seqlens == nullptr ? (P.Tq + seg - 1) / seg : P.Tq / seg + P.N;
+}
+
+struct Space {
+  int64_t stat, rmax, vmax, part, total;
+};
+Space space(const GdnAttnParams& P) {
+  Space s;
+  const int64_t rows = (int64_t)P.B * P.Tq;
+  int blocks, seg, slots;
+  sink_plan(P, blocks, seg, slots);
+  s.stat = 0;
+  s.rmax = s.stat + up256(rows * P.Hq * 8);
+  s.vmax = s.rmax + (P.dtype == GDN_DTYPE_F16 ? up256(rows * P.Hq * 4) : 0);
+  s.part = s.vmax + (P.dtype == GDN_DTYPE_F16 ? up256((int64_t)P.B * P.Hk * kVParts * 4) : 0);
+  const int64_t units = P.cu_seqlens == nullptr ? (int64_t)P.B * P.Hk : P.Hk;
+  const int64_t n = units * blocks * (slots + 1 + (P.cu_seqlens == nullptr ? 0 : P.N));
+  s.total = s.part + up256(n * 2 * kKB * P.D * 4);
+  return s;
+}
+
+template <typename T, int D>
+int launch(const BArgs& a, hipStream_t s) {
+  const int64_t rb = (a.rows * a.Hq + 256 / (D / 8) - 1) / (256 / (D / 8));
+  const int64_t vb = kScaled<T> ? (int64_t)a.B * a.Hk * kVParts : 0;
+  const int64_t kvb = (int64_t)a.units_k * (a.slots_k + (int64_t)a.sink_blocks * a.slots_s);
+  const int64_t qb = (int64_t)a.units_q * a.slots_q;
+  if (rb + vb > 0x7fffffffLL || kvb > 0x7fffffffLL || qb > 0x7fffffffLL) return GDN_ERR_BAD_SHAPE;
+  if (rb > 0) hipLaunchKernelGGL((prep_kernel<T, D>), dim3((uint32_t)(rb + vb)), dim3(256), 0, s, a, (int)rb);
+  if (kvb > 0) hipLaunchKernelGGL((kv_kernel<T, D>), dim3((uint32_t)kvb), dim3(256), 0, s, a);
+  if (a.sink_blocks > 0) {
+    const int64_t us = a.seq.cu == nullptr ? a.units_k : (int64_t)a.Hk * a.seq.N;
+    hipLaunchKernelGGL((sink_sum_kernel<T, D>), dim3((uint32_t)(us * a.sink_blocks * (kKB / 8))), dim3(256), 0, s, a);
+  }
+  if (qb > 0) hipLaunchKernelGGL((q_kernel<T, D>), dim3((uint32_t)qb), dim3(256), 0, s, a);
+  return (int)hipGetLastError();
+}
+
+}  // namespace attn
+}  // namespace gdn
+
+using namespace gdn;
+using namespace gdn::attn;
+
+extern "C" {
+
+int64_t gdn_attn_bwd_workspace_size(const GdnAttnParams* prm) {
+  if (prm == nullptr || check_attn(*prm) != GDN_OK) return -1;
+  return space(*prm).total;
+}
+
+int gdn_attn_bwd_launch(const GdnAttnParams* prm, void* stream) {
+  if (prm == nullptr) return GDN_ERR_NULL_POINTER;
+  const GdnAttnParams& P = *prm;
+  const int st = check_attn(P);
+  if (st != GDN_OK) return st;
+  if (P.Tq > 0 && (P.q == nullptr || P.o == nullptr || P.lse == nullptr || P.d_o == nullptr || P.dq == nullptr))
+    return GDN_ERR_NULL_POINTER;
+  if (P.Tk > 0 && (P.k == nullptr || P.v == nullptr || P.dk == nullptr || P.dv == nullptr)) return GDN_ERR_NULL_POINTER;
+  if (!rows16(P.q, P.q_stride, P.B, P.Tq, P.Hq) || !rows16(P.o, P.o_stride, P.B, P.Tq, P.Hq) ||
+      !rows16(P.d_o, P.do_stride, P.B, P.Tq, P.Hq) || !rows16(P.dq, P.dq_stride, P.B, P.Tq, P.Hq) ||
+      !rows16(P.k, P.k_stride, P.B, P.Tk, P.Hk) || !rows16(P.v, P.v_stride, P.B, P.Tk, P.Hk) ||
+      !rows16(P.dk, P.dk_stride, P.B, P.Tk, P.Hk) || !rows16(P.dv, P.dv_stride, P.B, P.Tk, P.Hk))
+    return GDN_ERR_MISALIGNED;
+  const Space sp = space(P);
+  if (sp.total > 0 && (P.workspace == nullptr || P.workspace_bytes < sp.total ||
+                       reinterpret_cast<uintptr_t>(P.workspace) % 256 != 0))
+    return GDN_ERR_WORKSPACE;
+  BArgs a = {};
+  a.q = static_cast<const uint16_t*>(P.q);
+  a.k = static_cast<const uint16_t*>(P.k);
+  a.v = static_cast<const uint16_t*>(P.v);
+  a.o = static_cast<const uint16_t*>(P.o);
+  a.dO = static_cast<const uint16_t*>(P.d_o);
+  a.lse = P.lse;
+  a.dq = static_cast<uint16_t*>(P.dq);
+  a.dk = static_cast<uint16_t*>(P.dk);
+  a.dv = static_cast<uint16_t*>(P.dv);
+  char* ws = static_cast<char*>(P.workspace);
+  a.stat = reinterpret_cast<float*>(ws + sp.stat);
+  a.rmax = reinterpret_cast<float*>(ws + sp.rmax);
+  a.vmax = reinterpret_cast<float*>(ws + sp.vmax);
+  a.part = reinterpret_cast<float*>(ws + sp.part);
+  a.seq = SeqArgs{P.cu_seqlens, P.Tq, P.Tk, P.N};
+  for (int d = 0; d < 3; ++d) {
+    a.qs[d] = P.q_stride[d];
+    a.ks[d] = P.k_stride[d];
+    a.vs[d] = P.v_stride[d];
+    a.os[d] = P.o_stride[d];
+    a.dos[d] = P.do_stride[d];
+    a.dqs[d] = P.dq_stride[d];
+    a.dks[d] = P.dk_stride[d];
+    a.dvs[d] = P.dv_stride[d];
+  }
+  a.rows = (int64_t)P.B * P.Tq;
+  a.B = P.B;
+  a.Hq = P.Hq;
+  a.Hk = P.Hk;
+  a.G = P.Hq / P.Hk;
+  const bool packed = P.cu_seqlens != nullptr;
+  a.units_q = packed ? P.Hq : P.B * P.Hq;
+  a.units_k = packed ? P.Hk : P.B * P.Hk;
+  a.slots_q = packed ? P.Tq / kQB + P.N : (P.Tq + kQB - 1) / kQB;
+  a.slots_k = packed ? P.Tk / kKB + P.N : (P.Tk + kKB - 1) / kKB;
+  sink_plan(P, a.sink_blocks, a.seg, a.slots_s);
+  a.window = P.window;
+  a.sinks = P.sinks;
+  a.scale = P.scale;
+  a.scale_log2 = P.scale * kLog2e;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (P.dtype == GDN_DTYPE_F16) return P.D == 128 ? launch<f16, 128>(a, s) : launch<f16, 64>(a, s);
+  return P.D == 128 ? launch<bf16_t, 128>(a, s) : launch<bf16_t, 64>(a, s);
+}
+
+}  // extern "C"

@@ -1,0 +1,188 @@
+// Windowed attention, forward: o = softmax(scale q k^T) v over the keys that
+// each query row sees, one pass over the keys with the running maximum and sum.
+//
+// A workgroup is 4 waves on 128 query rows of one head, 32 rows a wave.  Key
+// and value tiles of 64 rows come by LDS-DMA into two buffers, one ahead of
+// the products.  A wave forms S^T = K Q^T (a lane then holds one query row's
+// scores, so the softmax needs one exchange, between the lane's two halves)
+// and O^T += V^T P^T with P^T straight from the accumulators.  Only tiles on
+// the edges of the visible range are masked.
+
+#include <algorithm>
+
+#include "gdn_attn.h"
+
+namespace gdn {
+namespace attn {
+
+constexpr int kBM = 128;       // query rows a workgroup
+constexpr int kBN = 64;        // keys a tile
+constexpr int kNT = 256;
+
+struct FArgs {
+  const uint16_t* q;
+  const uint16_t* k;
+  const uint16_t* v;
+  uint16_t* o;
+  float* lse;
+  SeqArgs seq;
+  int64_t qs[3], ks[3], vs[3], os[3];
+  int Hq, G, units, nblk, slots, window, sinks;
+  float scale_log2;
+  uint32_t flip;
+};
+
+template <typename T, int D>
+__global__ __launch_bounds__(kNT, 2) void fwd_kernel(const FArgs a) {
+  using O = Ops<T>;
+  using Vec = typename O::Vec;
+  using TL = Tile<D>;
+  constexpr uint32_t kTile = kBN * TL::kRowBytes;     // K0 V0 K1 V1
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * kTile];
+  // unit = (batch, head); neighbouring units share key heads, and workgroups
+  // blockIdx.x % 8 run on one XCD: give each XCD a run of units.  Later blocks
+  // see more keys and start first.
+  const int unit_ix = blockIdx.x % a.units, slot = a.slots - 1 - blockIdx.x / a.units;
+  const int unit = a.units % 8 == 0 ? (unit_ix % 8) * (a.units / 8) + unit_ix / 8 : unit_ix;
+  int block, si, head;
+  if (a.seq.cu == nullptr) {
+    si = unit / a.Hq;
+    head = unit % a.Hq;
+    block = slot;
+  } else {
+    head = unit;
+    si = find_block(a.seq, slot, kBM, 0, block);
+  }
+  const Seq sq = get_seq(a.seq, si);
+  const int m0 = block * kBM;
+  if (block < 0 || m0 >= sq.nq) return;
+  const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int shift = sq.nk - sq.nq;            // position of query row 0
+  const int row = m0 + wv * 32 + l32;         // this lane's query row
+  const int p = row + shift;
+  const int hk = head / a.G;
+  const uint16_t* kb = a.k + sq.b * a.ks[0] + sq.k0 * a.ks[1] + hk * a.ks[2];
+  const uint16_t* vb = a.v + sq.b * a.vs[0] + sq.k0 * a.vs[1] + hk * a.vs[2];
+
+  const int p0 = m0 + shift, p1 = min(m0 + kBM, sq.nq) - 1 + shift;
+  const KeyRange kr(p0, p1, sq.nk, a.window, a.sinks, kBN);
+  const int wp0 = m0 + wv * 32 + shift, wp1 = min(wp0 + 31, sq.nq - 1 + shift);
+
+  Vec qf[D / 16];
+  {
+    const uint16_t* qr = a.q + sq.b * a.qs[0] + (sq.q0 + min(row, sq.nq - 1)) * a.qs[1] + head * a.qs[2];
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) qf[i] = signed_vec<T>(*reinterpret_cast<const uint4*>(qr + 16 * i + 8 * half), a.flip);
+  }
+  Rows<T, D, kBN / 32> rows;
+  const Copier<D, kBN, kNT> ck(kb, a.ks[1], sq.nk), cv(vb, a.vs[1], sq.nk);
+  const uint32_t base = lds_addr(lds);
+  const uint32_t kofs = TL::row_ofs(lane), vofs0 = TL::col_ofs(lane, 0), vofs1 = TL::col_ofs(lane, 1);
+  dma_wait();     // q is here: no load but the tiles' is waited for in the loop
+  if (kr.n > 0) {
+    ck(base, kr.tile(0) * kBN);
+    cv(base + kTile, kr.tile(0) * kBN);
+  }
+  for (int it = 0; it < kr.n; ++it) {
+    const int j0 = kr.tile(it) * kBN;
+    const uint32_t kt = base + (it & 1) * 2 * kTile, vt = kt + kTile;
+    dma_wait();
+    __syncthreads();                          // tile `it` is here; every wave is done with the other buffer
+    if (it + 1 < kr.n) {
+      const int jn = kr.tile(it + 1) * kBN;
+      const uint32_t other = base + ((it + 1) & 1) * 2 * kTile;
+      ck(other, jn);
+      cv(other + kTile, jn);
+    }
+    const int j1 = min(j0 + kBN, sq.nk) - 1;
+    if (!none_visible(j0, j1, wp0, wp1, a.window, a.sinks)) {
+      const bool masked = !(j0 + kBN <= sq.nk && all_visible(j0, j1, wp0, wp1, a.window, a.sinks));
+      rows.step(qf, kt + kofs, vt, vofs0, vofs1, masked, Mask(p, j0, half, sq.nk, a.window, a.sinks), a.scale_log2, lane);
+    }
+  }
+
+  const float l = rows.l + swap_halves(rows.l);
+  if (row >= sq.nq) return;
+  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+  uint16_t* orow = a.o + sq.b * a.os[0] + (sq.q0 + row) * a.os[1] + head * a.os[2];
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const uint2 w = make_uint2(O::pack(rows.acc[dt][4 * c] * inv, rows.acc[dt][4 * c + 1] * inv),
+                                 O::pack(rows.acc[dt][4 * c + 2] * inv, rows.acc[dt][4 * c + 3] * inv));
+      *reinterpret_cast<uint2*>(orow + 32 * dt + 8 * c + 4 * half) = w;
+    }
+  if (a.lse != nullptr && half == 0) {
+    const int64_t at = ((int64_t)sq.b * a.seq.Tq + sq.q0 + row) * a.Hq + head;
+    a.lse[at] = l > 0.f || l != l ? (rows.m - O::kShift) * kLn2 + logf(l) : -__builtin_inff();
+  }
+}
+
+int check_attn(const GdnAttnParams& P) {
+  if (P.B <= 0 || P.Tq < 0 || P.Tk < 0 || P.N <= 0 || P.N > (1 << 22) || P.Hq <= 0 || P.Hk <= 0 || P.Hq % P.Hk != 0) return GDN_ERR_BAD_SHAPE;
+  if (P.cu_seqlens == nullptr ? P.N != P.B : (P.B != 1 || P.Tq != P.Tk)) return GDN_ERR_BAD_SHAPE;
+  if (P.window < 1 || P.sinks < 0) return GDN_ERR_BAD_SHAPE;
+  if (P.D != 64 && P.D != 128) return GDN_ERR_UNSUPPORTED;
+  if (P.dtype != GDN_DTYPE_F16 && P.dtype != GDN_DTYPE_BF16) return GDN_ERR_BAD_DTYPE;
+  // positions are 32-bit
+  if ((int64_t)P.Tq + P.Tk > 0x3fffffffLL) return GDN_ERR_BAD_SHAPE;
+  return GDN_OK;
+}
+
+template <typename T>
+int launch_t(const FArgs& a, int D, hipStream_t s) {
+  const dim3 grid((uint32_t)a.units * a.slots);
+  if (D == 128) hipLaunchKernelGGL((fwd_kernel<T, 128>), grid, dim3(kNT), 0, s, a);
+  else hipLaunchKernelGGL((fwd_kernel<T, 64>), grid, dim3(kNT), 0, s, a);
+  return (int)hipGetLastError();
+}
+
+}  // namespace attn
+}  // namespace gdn
+
+using namespace gdn;
+using namespace gdn::attn;
+
+extern "C" int gdn_attn_launch(const GdnAttnParams* prm, void* stream) {
+  if (prm == nullptr) return GDN_ERR_NULL_POINTER;
+  const GdnAttnParams& P = *prm;
+  const int st = check_attn(P);
+  if (st != GDN_OK) return st;
+  if (P.Tq == 0) return GDN_OK;
+  if (P.q == nullptr || P.o == nullptr || (P.Tk > 0 && (P.k == nullptr || P.v == nullptr))) return GDN_ERR_NULL_POINTER;
+  if (!rows16(P.q, P.q_stride, P.B, P.Tq, P.Hq) || !rows16(P.o, P.o_stride, P.B, P.Tq, P.Hq) ||
+      !rows16(P.k, P.k_stride, P.B, P.Tk, P.Hk) || !rows16(P.v, P.v_stride, P.B, P.Tk, P.Hk))
+    return GDN_ERR_MISALIGNED;
+  FArgs a = {};
+  a.q = static_cast<const uint16_t*>(P.q);
+  a.k = static_cast<const uint16_t*>(P.k);
+  a.v = static_cast<const uint16_t*>(P.v);
+  a.o = static_cast<uint16_t*>(P.o);
+  a.lse = P.lse;
+  a.seq = SeqArgs{P.cu_seqlens, P.Tq, P.Tk, P.N};
+  for (int d = 0; d < 3; ++d) {
+    a.qs[d] = P.q_stride[d];
+    a.ks[d] = P.k_stride[d];
+    a.vs[d] = P.v_stride[d];
+    a.os[d] = P.o_stride[d];
+  }
+  a.Hq = P.Hq;
+  a.G = P.Hq / P.Hk;
+  a.window = P.window;
+  a.sinks = P.sinks;
+  split_scale(P.scale, a.scale_log2, a.flip);
+  int64_t units = P.Hq, slots = 0;
+  if (P.cu_seqlens == nullptr) {
+    units *= P.B;
+    slots = (P.Tq + kBM - 1) / kBM;
+  } else {
+    slots = P.Tq / kBM + P.N;
+  }
+  if (units * slots > 0x7fffffffLL) return GDN_ERR_BAD_SHAPE;
+  a.units = (int)units;
+  a.slots = (int)slots;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  return P.dtype == GDN_DTYPE_F16 ? launch_t<f16>(a, P.D, s) : launch_t<bf16_t>(a, P.D, s);
+}

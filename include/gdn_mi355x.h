@@ -405,7 +405,7 @@ int gdn_scan_bwd_launch(const GdnScanParams* params, void* stream);
  *   - y: x_dtype, or e4m3 bytes when `scale` is set: y / scale rounded to the
  *     nearest, scale = max|y| / 448 over the row (group 0) or over each 128
  *     columns (group 128, D a multiple of it); scale is dense
- *     [rows, D / group] (or [rows]); a group of zeros has scale 0.
+ *     [rows, D / group] (or [rows, 1]); a group of zeros has scale 0.
  *   - backward: r, dy (x_dtype), dr_in (nullable, r_dtype); dr (r_dtype), dx
  *     (nullable: the same in x_dtype), dw (w_dtype).
  *   - w and dw: w_dtype (x_dtype or fp32), dense. */

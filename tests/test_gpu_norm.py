@@ -90,7 +90,7 @@ def _fp8_check(pkg, x, w, res, group):
     want, _ = _norm(x.double() + (res.double() if res is not None else 0.0), w.double(), 1e-6)
     D = x.shape[-1]
     assert y.dtype == torch.float8_e4m3fn and y.shape == x.shape
-    assert scale.shape == ((*x.shape[:-1], D // group) if group else x.shape[:-1])
+    assert scale.shape == (*x.shape[:-1], D // (group or D))
     top = want.unflatten(-1, (-1, group or D)).abs().amax(-1)
     s = scale.double().view(top.shape)
     assert ((s - top / 448).abs() <= 2.0 ** -18 * top / 448).all()
@@ -180,7 +180,7 @@ def test_shapes_and_strides(pkg, cuda):
     d0, dw = pkg.add_rms_norm_bwd(res[:0], w, dy[:0], dr[:0])
     assert d0.shape == (0, 6, 136) and (dw == 0).all()
     q, s, _ = pkg.add_rms_norm_fp8(x[:0], w, res[:0])
-    assert q.shape == (0, 6, 136) and s.shape == (0, 6)
+    assert q.shape == (0, 6, 136) and s.shape == (0, 6, 1)
 
 
 @pytest.mark.parametrize("xd,rd", TYPES)

@@ -279,58 +279,30 @@ struct Mask {
   }
 };
 
-// O^T += V^T P^T over one tile of which some keys are hidden from some rows,
-// where V holds infinities or NaN: those count only for the rows that see
-// them.  Their places are zero in the product; two products of 0/1 matrices
-// say which sums meet a +inf or NaN, and which a -inf or NaN.
-template <typename T, int D, int KS>
-__device__ __forceinline__ void pv_not_finite(f32x16 (&acc)[D / 32], const typename Ops<T>::Vec (&p)[2 * KS],
-                                           const Mask& seen, uint32_t v0, uint32_t v1) {
-  constexpr uint32_t E = Ops<T>::kExp, ONE = Ops<T>::kOne;
+// An operand with its infinities and NaN replaced by zero.
+template <typename T>
+__device__ __forceinline__ uint4 only_finite(const uint4& x) {
+  constexpr uint32_t E = Ops<T>::kExp;
+  uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-  for (int dt = 0; dt < D / 32; ++dt) {
-    f32x16 up = {}, dn = {};
-#pragma unroll
-    for (int s = 0; s < 2 * KS; ++s) {
-      const uint4 raw = Tile<D>::col8(v0, v1, dt, 16 * s * Tile<D>::kRowBytes);
-      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-      uint32_t f[4], u[4], d[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        f[i] = u[i] = d[i] = 0;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t x = (w[i] >> (16 * h)) & 0xffffu, mag = x & 0x7fffu;
-          if (mag < E) f[i] |= x << (16 * h);
-          if (mag > E || x == E) u[i] |= ONE << (16 * h);
-          if (mag > E || x == (E | 0x8000u)) d[i] |= ONE << (16 * h);
-        }
-      }
-      uint32_t one[4];    // the visible places of step s
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        one[i] = (seen(s >> 1, 8 * (s & 1) + 2 * i) ? ONE : 0u) | (seen(s >> 1, 8 * (s & 1) + 2 * i + 1) ? ONE << 16 : 0u);
-      const typename Ops<T>::Vec sv = as_vec<T>(make_uint4(one[0], one[1], one[2], one[3]));
-      acc[dt] = Ops<T>::mfma(as_vec<T>(make_uint4(f[0], f[1], f[2], f[3])), p[s], acc[dt]);
-      up = Ops<T>::mfma(as_vec<T>(make_uint4(u[0], u[1], u[2], u[3])), sv, up);
-      dn = Ops<T>::mfma(as_vec<T>(make_uint4(d[0], d[1], d[2], d[3])), sv, dn);
-    }
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      if (up[r] > 0.f) acc[dt][r] += __builtin_inff();
-      if (dn[r] > 0.f) acc[dt][r] -= __builtin_inff();
-    }
+  for (int i = 0; i < 4; ++i) {
+    if ((w[i] & E) == E) w[i] &= 0xffff0000u;
+    if ((w[i] & (E << 16)) == (E << 16)) w[i] &= 0x0000ffffu;
   }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Whether a tile of ROWS rows holds an infinity or NaN (a wave looks at all).
-template <typename T, int D, int ROWS>
-__device__ __forceinline__ bool tile_not_finite(uint32_t tile, int lane) {
+// A product over rows of which some are hidden from some columns adds 0 times
+// what the hidden places hold.  Where that is an infinity or NaN, the tile is
+// made finite before the product: these look at and change N KB of LDS, one
+// wave, 16 bytes a lane and step.
+template <typename T, int N>
+__device__ __forceinline__ bool not_finite(uint32_t at, int lane) {
   typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
   u16x2 m = {0, 0};
 #pragma unroll
-  for (int i = 0; i < ROWS * D / 512; ++i) {
-    const u32x4 x = *(const lds_u32x4*)(tile + 16 * (i * 64 + lane));
+  for (int i = 0; i < N; ++i) {
+    const u32x4 x = *(const lds_u32x4*)(at + 16 * (i * 64 + lane));
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const uint32_t w = x[e] & 0x7fff7fffu;
@@ -338,6 +310,16 @@ __device__ __forceinline__ bool tile_not_finite(uint32_t tile, int lane) {
     }
   }
   return __any(m[0] >= Ops<T>::kExp || m[1] >= Ops<T>::kExp);
+}
+template <typename T, int N>
+__device__ __forceinline__ void make_finite(uint32_t at, int lane) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    lds_u32x4* p = (lds_u32x4*)(at + 16 * (i * 64 + lane));
+    const u32x4 x = *p;
+    const uint4 y = only_finite<T>(make_uint4(x[0], x[1], x[2], x[3]));
+    *p = u32x4{y.x, y.y, y.z, y.w};
+  }
 }
 
 // An operand with its sign turned where flip = 0x80008000 (else 0).
@@ -357,9 +339,11 @@ struct Rows {
   f32x16 acc[D / 32] = {};
   float m = -__builtin_inff(), l = 0.f;
 
-  // kt: the lane's operand address in the key tile; vt: the value tile.
-  __device__ __forceinline__ void step(const Vec (&qf)[D / 16], uint32_t kt, uint32_t vt, uint32_t vofs0, uint32_t vofs1,
-                                       bool masked, const Mask& seen, float scale_log2, int lane) {
+  Vec pf[2 * KS];
+
+  // Scores and probabilities of one tile; kt: the lane's operand address.
+  __device__ __forceinline__ void scores(const Vec (&qf)[D / 16], uint32_t kt, bool masked, const Mask& seen,
+                                         float scale_log2) {
     f32x16 s[KS] = {};
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) {
@@ -397,18 +381,53 @@ struct Rows {
         s[t][r] = exp2_fast(__builtin_fmaf(s[t][r], scale_log2, mb));
         l += s[t][r];
       }
-    Vec pf[2 * KS];
 #pragma unroll
     for (int t = 0; t < 2 * KS; ++t) pf[t] = acc_operand<T>(s[t >> 1], t & 1);
-    if (masked && tile_not_finite<T, D, 32 * KS>(vt, lane)) {
-      pv_not_finite<T, D, KS>(acc, pf, seen, vt + vofs0, vt + vofs1);
-    } else {
+  }
+
+  // What the infinities and NaN of a value tile add to the rows that see them
+  // (v0, v1: the lane's transposed addresses): two products of 0/1 matrices
+  // say which sums meet a +inf or NaN, and which a -inf or NaN.
+  __device__ __forceinline__ void add_not_finite(const Mask& seen, uint32_t v0, uint32_t v1) {
+    constexpr uint32_t E = O::kExp, ONE = O::kOne;
 #pragma unroll
-      for (int t = 0; t < 2 * KS; ++t)
+    for (int dt = 0; dt < D / 32; ++dt) {
+      f32x16 up = {}, dn = {};
 #pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt)
-          acc[dt] = O::mfma(as_vec<T>(TL::col8(vt + vofs0, vt + vofs1, dt, 16 * t * TL::kRowBytes)), pf[t], acc[dt]);
+      for (int s = 0; s < 2 * KS; ++s) {
+        const uint4 raw = TL::col8(v0, v1, dt, 16 * s * TL::kRowBytes);
+        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+        uint32_t u[4], d[4], one[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          u[i] = d[i] = one[i] = 0;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t x = (w[i] >> (16 * h)) & 0xffffu, mag = x & 0x7fffu;
+            if (mag > E || x == E) u[i] |= ONE << (16 * h);
+            if (mag > E || x == (E | 0x8000u)) d[i] |= ONE << (16 * h);
+            if (seen(s >> 1, 8 * (s & 1) + 2 * i + h)) one[i] |= ONE << (16 * h);
+          }
+        }
+        const Vec sv = as_vec<T>(make_uint4(one[0], one[1], one[2], one[3]));
+        up = O::mfma(as_vec<T>(make_uint4(u[0], u[1], u[2], u[3])), sv, up);
+        dn = O::mfma(as_vec<T>(make_uint4(d[0], d[1], d[2], d[3])), sv, dn);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        acc[dt][r] += up[r] > 0.f ? __builtin_inff() : 0.f;
+        acc[dt][r] -= dn[r] > 0.f ? __builtin_inff() : 0.f;
+      }
     }
+  }
+
+  // O^T += V^T P^T
+  __device__ __forceinline__ void values(uint32_t v0, uint32_t v1) {
+#pragma unroll
+    for (int t = 0; t < 2 * KS; ++t)
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt)
+        acc[dt] = O::mfma(as_vec<T>(TL::col8(v0, v1, dt, 16 * t * TL::kRowBytes)), pf[t], acc[dt]);
   }
 };
 

@@ -3,10 +3,10 @@
 //     dv = P^T dO,  dk = scale dS^T q,  dq = scale dS k
 // in three steps, each sum in one workgroup and in a fixed order:
 //   prep  per query row lse in powers of 2, D, and (fp16) the largest |dO|;
-//   kv    128 key rows a workgroup, 32 a wave: query rows of all heads that
-//         share the key head pass in tiles of 32 (S and dP with a lane on one
-//         key; P and dS enter dV^T += dO^T P and dK^T += Q^T dS straight from
-//         their accumulators);
+//   kv    128 key rows a workgroup of 8 waves: query rows of all heads that
+//         share the key head pass in tiles of 64, a wave taking 32 keys and 32
+//         of the rows (S and dP with a lane on one key; P and dS enter dV^T +=
+//         dO^T P and dK^T += Q^T dS straight from their accumulators);
 //   q     128 query rows a workgroup, 32 a wave, key tiles of 64 as in the
 //         forward: S^T, dP^T, dQ^T += K^T dS^T.
 // Blocks of the first keys (the sinks) are seen by every later query row: the
@@ -26,7 +26,8 @@ namespace gdn {
 namespace attn {
 
 constexpr int kKB = 128;       // key rows a workgroup (kv)
-constexpr int kQT = 32;        // query rows a tile (kv)
+constexpr int kQT = 64;        // query rows a tile (kv)
+constexpr int kKVT = 512;      // threads (kv)
 constexpr int kQB = 128;       // query rows a workgroup (q)
 constexpr int kKT = 64;        // keys a tile (q)
 constexpr int kVParts = 64;    // partial maxima of |v| a head
@@ -142,19 +143,6 @@ __device__ __forceinline__ float v_unit(const BArgs& a, int b, int hk, int lane)
   return pow2_above(m);
 }
 
-// An operand with its infinities and NaN replaced by zero.
-template <typename T>
-__device__ __forceinline__ uint4 only_finite(const uint4& x) {
-  constexpr uint32_t E = Ops<T>::kExp;
-  uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if ((w[i] & E) == E) w[i] &= 0xffff0000u;
-    if ((w[i] & (E << 16)) == (E << 16)) w[i] &= 0x0000ffffu;
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
 // Output rows from transposed accumulators: lane l holds row l % 32.
 template <typename T, int D>
 __device__ __forceinline__ void store_rows(uint16_t* row, const f32x16 (&acc)[D / 32], float f, int half) {
@@ -197,35 +185,32 @@ __device__ __forceinline__ void dma4(const void* src, uint32_t at) {
 }
 
 template <typename T, int D>
-__global__ __launch_bounds__(256, 1) void kv_kernel(const BArgs a) {
+__global__ __launch_bounds__(kKVT, 2) void kv_kernel(const BArgs a) {
   using O = Ops<T>;
   using Vec = typename O::Vec;
   using TL = Tile<D>;
-  constexpr uint32_t kTile = kQT * TL::kRowBytes, kBuf = 2 * kTile + 512;    // Q, dO, 32 x (lse, D), 32 x max
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kBuf];
-  const int unit_ix = blockIdx.x % a.units_k, item = blockIdx.x / a.units_k;
+  constexpr uint32_t kTile = kQT * TL::kRowBytes, kBuf = 2 * kTile + 1024;    // Q, dO, 64 x lse, D, max
+  constexpr uint32_t kK = 2 * kBuf, kV = kK + kKB * TL::kRowBytes;            // the block's k and v rows
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kV + kKB * TL::kRowBytes];
+  const int unit_ix = blockIdx.x % a.units_k;
   const int unit = a.units_k % 8 == 0 ? (unit_ix % 8) * (a.units_k / 8) + unit_ix / 8 : unit_ix;
-  const bool extra = item >= a.slots_k;
+  // the segments first: they are short, and the blocks fill up behind them
+  const int extras = a.sink_blocks * a.slots_s, at_item = blockIdx.x / a.units_k;
+  const bool extra = at_item < extras;
+  const int item = extra ? at_item : at_item - extras;
   int si, hk, block, seg = 0;
-  if (!extra) {
-    if (a.seq.cu == nullptr) {
-      si = unit / a.Hk;
-      hk = unit % a.Hk;
-      block = item;
-    } else {
-      hk = unit;
-      si = find_block(a.seq, item, kKB, 0, block);
-    }
+  if (a.seq.cu == nullptr) {
+    si = unit / a.Hk;
+    hk = unit % a.Hk;
+    block = extra ? item % a.sink_blocks : item;
+    seg = extra ? item / a.sink_blocks : 0;
   } else {
-    const int e = item - a.slots_k;
-    block = e % a.sink_blocks;
-    if (a.seq.cu == nullptr) {
-      si = unit / a.Hk;
-      hk = unit % a.Hk;
-      seg = e / a.sink_blocks;
+    hk = unit;
+    if (extra) {
+      block = item % a.sink_blocks;
+      si = find_block(a.seq, item / a.sink_blocks, a.seg, 0, seg);
     } else {
-      hk = unit;
-      si = find_block(a.seq, e / a.sink_blocks, a.seg, 0, seg);
+      si = find_block(a.seq, item, kKB, 0, block);
     }
   }
   const Seq sq = get_seq(a.seq, si);
@@ -235,43 +220,37 @@ __global__ __launch_bounds__(256, 1) void kv_kernel(const BArgs a) {
   const QRange rg = extra ? seg_rows(a, sq, k0, seg) : own_rows(a, sq, k0);
   if (extra && rg.r1 <= rg.r0) return;
   const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
-  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int key = k0 + wv * 32 + l32;          // this lane's key row
-  const int j0 = k0 + wv * 32, j1 = min(j0 + 32, sq.nk) - 1;
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kg = wv & 3, qh = wv >> 2;
+  const int key = k0 + kg * 32 + l32;          // this lane's key row
+  const int j0 = k0 + kg * 32, j1 = min(j0 + 32, sq.nk) - 1;
+  const uint32_t base = lds_addr(lds);
 
-  Vec kf[D / 16], vf[D / 16];
-  {
-    const int64_t r = sq.k0 + min(key, sq.nk - 1);
-    const uint16_t* kr = a.k + sq.b * a.ks[0] + r * a.ks[1] + hk * a.ks[2];
-    const uint16_t* vr = a.v + sq.b * a.vs[0] + r * a.vs[1] + hk * a.vs[2];
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-      kf[i] = as_vec<T>(*reinterpret_cast<const uint4*>(kr + 16 * i + 8 * half));
-      vf[i] = as_vec<T>(*reinterpret_cast<const uint4*>(vr + 16 * i + 8 * half));
-    }
-  }
   const int nt = (max(rg.r1 - rg.r0, 0) + kQT - 1) / kQT, n = nt * a.G;
+  {
+    const Copier<D, kKB, kKVT> ck(a.k + sq.b * a.ks[0] + sq.k0 * a.ks[1] + hk * a.ks[2], a.ks[1], sq.nk);
+    const Copier<D, kKB, kKVT> cv(a.v + sq.b * a.vs[0] + sq.k0 * a.vs[1] + hk * a.vs[2], a.vs[1], sq.nk);
+    ck(base + kK, k0);
+    cv(base + kV, k0);
+  }
   float vu = 1.f;
   if constexpr (kScaled<T>)
     if (n > 0) vu = v_unit(a, sq.b, hk, lane);
   float unit_do = 0x1p-24f;                     // unit of dO so far (fp16)
   f32x16 dk[D / 32] = {}, dv[D / 32] = {};
 
-  const uint32_t base = lds_addr(lds);
   const uint32_t rofs = TL::row_ofs(lane), cofs0 = TL::col_ofs(lane, 0), cofs1 = TL::col_ofs(lane, 1);
+  const uint32_t kt = base + kK + 32 * kg * TL::kRowBytes + rofs, vt = base + kV + 32 * kg * TL::kRowBytes + rofs;
   auto fetch = [&](int it) {
     const int g = it / nt, r0 = rg.r0 + (it % nt) * kQT, h = hk * a.G + g;
     const uint32_t at = base + (it & 1) * kBuf;
-    const Copier<D, kQT, 256> cq(a.q + sq.b * a.qs[0] + sq.q0 * a.qs[1] + h * a.qs[2], a.qs[1], sq.nq);
-    const Copier<D, kQT, 256> cd(a.dO + sq.b * a.dos[0] + sq.q0 * a.dos[1] + h * a.dos[2], a.dos[1], sq.nq);
+    const Copier<D, kQT, kKVT> cq(a.q + sq.b * a.qs[0] + sq.q0 * a.qs[1] + h * a.qs[2], a.qs[1], sq.nq);
+    const Copier<D, kQT, kKVT> cd(a.dO + sq.b * a.dos[0] + sq.q0 * a.dos[1] + h * a.dos[2], a.dos[1], sq.nq);
     cq(at, r0);
     cd(at + kTile, r0);
-    const int64_t row = (int64_t)h * a.rows + (int64_t)sq.b * a.seq.Tq + sq.q0 + min(r0 + (lane & 31), sq.nq - 1);
-    if (wv == 0) {
-      // lanes 0..31 bring lse, 32..63 D
-      dma4(a.stat + row * 2 + half, __builtin_amdgcn_readfirstlane(at + 2 * kTile));
-      if constexpr (kScaled<T>) dma4(a.rmax + row, __builtin_amdgcn_readfirstlane(at + 2 * kTile + 256));
-    }
+    const int64_t row = (int64_t)h * a.rows + (int64_t)sq.b * a.seq.Tq + sq.q0 + min(r0 + lane, sq.nq - 1);
+    if (wv < 2) dma4(a.stat + row * 2 + wv, __builtin_amdgcn_readfirstlane(at + 2 * kTile + 256 * wv));
+    if constexpr (kScaled<T>)
+      if (wv == 2) dma4(a.rmax + row, __builtin_amdgcn_readfirstlane(at + 2 * kTile + 512));
   };
   dma_wait();
   if (n > 0) fetch(0);
@@ -279,76 +258,86 @@ __global__ __launch_bounds__(256, 1) void kv_kernel(const BArgs a) {
     dma_wait();
     __syncthreads();
     if (it + 1 < n) fetch(it + 1);
-    const uint32_t qt = base + (it & 1) * kBuf, dt_ = qt + kTile, st = qt + 2 * kTile;
-    const int r0 = rg.r0 + (it % nt) * kQT, nr = min(kQT, rg.r1 - r0);
-    const int p0 = r0 + shift, p1 = p0 + nr - 1;
-    float sc = 1.f;
-    if constexpr (kScaled<T>) {
-      // the tile's unit, in every wave alike
-      typedef __attribute__((address_space(3))) const float lds_float;
-      float m = *(lds_float*)(st + 256 + 4 * l32);
-#pragma unroll
-      for (int s = 16; s >= 1; s >>= 1) m = fmaxf(m, __shfl_xor(m, s, 64));
-      const float u = pow2_above(m);
-      if (u > unit_do) {
-        const float f = unit_do / u;
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) dk[i][r] *= f;
-        unit_do = u;
-      }
-      sc = 0x1p-7f / (unit_do * vu);            // 2^7 / unit, and P's 2^14 taken out
-    }
-    if (none_visible(j0, j1, p0, p1, a.window, a.sinks)) continue;
-    const bool masked = !(nr == kQT && j0 + 32 <= sq.nk && all_visible(j0, j1, p0, p1, a.window, a.sinks));
-
-    f32x16 s = {}, dp = {};
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i) s = O::mfma(as_vec<T>(TL::row8(qt + rofs, i, 0)), kf[i], s);
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i) dp = O::mfma(as_vec<T>(TL::row8(dt_ + rofs, i, 0)), vf[i], dp);
-    typedef float f32x4v __attribute__((ext_vector_type(4)));
-    typedef __attribute__((address_space(3))) const f32x4v lds_f32x4;
+    const uint32_t buf = base + (it & 1) * kBuf;
+    const uint32_t qt = buf + 32 * qh * TL::kRowBytes, dt_ = qt + kTile, st = buf + 2 * kTile + 128 * qh;
+    const int t0 = rg.r0 + (it % nt) * kQT;                        // the tile's rows, and the wave's
+    const int r0 = t0 + 32 * qh, nr = min(32, rg.r1 - r0), p0 = r0 + shift, p1 = p0 + nr - 1;
+    const bool active = nr > 0 && !none_visible(j0, j1, p0, p1, a.window, a.sinks);
+    const bool masked = !(nr == 32 && j0 + 32 <= sq.nk && all_visible(j0, j1, p0, p1, a.window, a.sinks));
+    // a tile on an edge of any wave's range: are all its rows finite?
+    constexpr int kShare = 2 * kTile / 8192;
     bool bad = false;
-    if (masked) bad = tile_not_finite<T, D, kQT>(qt, lane) || tile_not_finite<T, D, kQT>(dt_, lane);
+    if (!(t0 + kQT <= rg.r1 && k0 + kKB <= sq.nk &&
+          all_visible(k0, k0 + kKB - 1, t0 + shift, t0 + kQT - 1 + shift, a.window, a.sinks)))
+      bad = __syncthreads_or(not_finite<T, kShare>(buf + wv * kShare * 1024, lane));
+    Vec pf[2], df[2];
+    if (active) {
+      float sc = 1.f;
+      if constexpr (kScaled<T>) {
+        // the unit of the wave's rows
+        typedef __attribute__((address_space(3))) const float lds_float;
+        float m = *(lds_float*)(st + 512 + 4 * l32);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const f32x4v ls = *(lds_f32x4*)(st + 32 * c + 16 * half), de = *(lds_f32x4*)(st + 128 + 32 * c + 16 * half);
+        for (int s = 16; s >= 1; s >>= 1) m = fmaxf(m, __shfl_xor(m, s, 64));
+        const float u = pow2_above(m);
+        if (u > unit_do) {
+          const float f = unit_do / u;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = 4 * c + e;
-        const float x = exp2_fast(__builtin_fmaf(s[r], a.scale_log2, kPUp<T> - ls[e]));
-        dp[r] = x * __builtin_fmaf(dp[r], sc, -de[e] * sc);
-        s[r] = x;
+          for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) dk[i][r] *= f;
+          unit_do = u;
+        }
+        sc = 0x1p-7f / (unit_do * vu);            // 2^7 / unit, and P's 2^14 taken out
       }
-      if (masked) {
+      // not kept across iterations: the addresses of 2 D / 16 steps
+      uint32_t ka = kt, va = vt;
+      asm volatile("" : "+v"(ka), "+v"(va));
+      f32x16 s = {}, dp = {};
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) s = O::mfma(as_vec<T>(TL::row8(qt + rofs, i, 0)), as_vec<T>(TL::row8(ka, i, 0)), s);
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) dp = O::mfma(as_vec<T>(TL::row8(dt_ + rofs, i, 0)), as_vec<T>(TL::row8(va, i, 0)), dp);
+      typedef float f32x4v __attribute__((ext_vector_type(4)));
+      typedef __attribute__((address_space(3))) const f32x4v lds_f32x4;
+      // row c + 4 half of the tile sees the lane's key where lo <= c < top
+      const int rel = p0 + 4 * half - key;
+      const int64_t reach = key < a.sinks ? (int64_t)1 << 32 : (int64_t)a.window - rel;
+      const int lo = -rel, top = key < sq.nk ? (int)min((int64_t)(nr - 4 * half), reach) : -1;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const f32x4v ls = *(lds_f32x4*)(st + 32 * c + 16 * half), de = *(lds_f32x4*)(st + 256 + 32 * c + 16 * half);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int r = 4 * c + e, row = acc_row(r, half), p = p0 + row;
-          const bool ok = (row < nr) & (key <= p) & ((p - key < a.window) | (key < a.sinks)) & (key < sq.nk);
+          const int r = 4 * c + e;
+          const float x = exp2_fast(__builtin_fmaf(s[r], a.scale_log2, kPUp<T> - ls[e]));
+          dp[r] = x * __builtin_fmaf(dp[r], sc, -de[e] * sc);
+          s[r] = x;
           // a row of dO that is not finite reaches the keys that see it
-          const float hit = fabsf(de[e]) < __builtin_inff() ? 0.f : __builtin_nanf("");
-          s[r] = ok ? (bad ? s[r] + hit : s[r]) : 0.f;
-          dp[r] = ok ? dp[r] : 0.f;
+          if (bad) s[r] += fabsf(de[e]) < __builtin_inff() ? 0.f : __builtin_nanf("");
+        }
+        if (masked) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = 4 * c + e, at = 8 * c + e;
+            const bool ok = (at >= lo) & (at < top);
+            s[r] = ok ? s[r] : 0.f;
+            dp[r] = ok ? dp[r] : 0.f;
+          }
         }
       }
-    }
-    Vec pf[2], df[2];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      pf[t] = acc_operand<T>(s, t);
-      df[t] = acc_operand<T>(dp, t);
+      for (int t = 0; t < 2; ++t) {
+        pf[t] = acc_operand<T>(s, t);
+        df[t] = acc_operand<T>(dp, t);
+      }
     }
     if (bad) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-          dv[i] = O::mfma(as_vec<T>(only_finite<T>(TL::col8(dt_ + cofs0, dt_ + cofs1, i, 16 * t * TL::kRowBytes))), pf[t], dv[i]);
-          dk[i] = O::mfma(as_vec<T>(only_finite<T>(TL::col8(qt + cofs0, qt + cofs1, i, 16 * t * TL::kRowBytes))), df[t], dk[i]);
-        }
-    } else {
+      __syncthreads();
+      make_finite<T, kShare>(buf + wv * kShare * 1024, lane);
+      __syncthreads();
+    }
+    if (active) {
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -360,31 +349,62 @@ __global__ __launch_bounds__(256, 1) void kv_kernel(const BArgs a) {
   }
   const float fv = exp2f(-kPUp<T>);
   const float fk = kScaled<T> ? a.scale * unit_do * vu * 0x1p-7f : a.scale;
+  // the two halves of the query rows: the second's sums pass through LDS
+  typedef float f32x4v __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) f32x4v lds_f32x4;
+  static_assert(4 * 32 * D * 4 <= sizeof(lds), "a half's sums fit");
+  const uint32_t mine = base + (kg * 64 + lane) * 16;
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    f32x16(&x)[D / 32] = w == 0 ? dk : dv;
+    const float f = w == 0 ? fk : fv;
+    dma_wait();
+    __syncthreads();
+    if (qh == 1) {
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          *(lds_f32x4*)(mine + (4 * i + c) * 4096) =
+              f32x4v{x[i][4 * c] * f, x[i][4 * c + 1] * f, x[i][4 * c + 2] * f, x[i][4 * c + 3] * f};
+    }
+    __syncthreads();
+    if (qh == 0) {
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const f32x4v y = *(lds_f32x4*)(mine + (4 * i + c) * 4096);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[i][4 * c + e] = __builtin_fmaf(x[i][4 * c + e], f, y[e]);
+        }
+    }
+  }
+  if (qh == 1) return;
   if (block < a.sink_blocks) {
-    // fp32 parts: slot 0 the block's own rows, then the segments
-    const int64_t slots = a.slots_s + 1;
-    const int64_t slot = a.seq.cu == nullptr ? (extra ? 1 + seg : 0)
-                                             : (extra ? (item - a.slots_k) / a.sink_blocks + 1 : 0);
-    // packed: a row of parts per sequence for the own rows
+    // fp32 parts: the block's own rows (dense: before the segments' parts;
+    // packed: one for each sequence, behind all of those), then the segments
+    if (extra && j0 >= a.sinks) return;
+    const int64_t slots = a.slots_s + (a.seq.cu == nullptr ? 1 : 0);
     const int64_t u = a.seq.cu == nullptr ? unit : hk;
-    float* part = extra || a.seq.cu == nullptr
-                      ? a.part + ((u * a.sink_blocks + block) * slots + slot) * (2 * kKB * D)
-                      : a.part + ((int64_t)a.units_k * a.sink_blocks * slots + (u * a.sink_blocks + block) * a.seq.N + si) * (2 * kKB * D);
-    float* pk = part + (wv * 32 + l32) * D;
+    const int64_t ub = u * a.sink_blocks + block;
+    const int64_t at = extra ? ub * slots + item / a.sink_blocks + (a.seq.cu == nullptr ? 1 : 0)
+                             : (a.seq.cu == nullptr ? ub * slots : (int64_t)a.units_k * a.sink_blocks * slots + ub * a.seq.N + si);
+    float* pk = a.part + at * (2 * kKB * D) + (kg * 32 + l32) * D;
     float* pv = pk + kKB * D;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const int d = 32 * i + 8 * c + 4 * half;
-        *reinterpret_cast<float4*>(pk + d) = make_float4(dk[i][4 * c] * fk, dk[i][4 * c + 1] * fk, dk[i][4 * c + 2] * fk, dk[i][4 * c + 3] * fk);
-        *reinterpret_cast<float4*>(pv + d) = make_float4(dv[i][4 * c] * fv, dv[i][4 * c + 1] * fv, dv[i][4 * c + 2] * fv, dv[i][4 * c + 3] * fv);
+        *reinterpret_cast<float4*>(pk + d) = make_float4(dk[i][4 * c], dk[i][4 * c + 1], dk[i][4 * c + 2], dk[i][4 * c + 3]);
+        *reinterpret_cast<float4*>(pv + d) = make_float4(dv[i][4 * c], dv[i][4 * c + 1], dv[i][4 * c + 2], dv[i][4 * c + 3]);
       }
     return;
   }
   if (key >= sq.nk) return;
-  store_rows<T, D>(a.dk + sq.b * a.dks[0] + (sq.k0 + key) * a.dks[1] + hk * a.dks[2], dk, fk, half);
-  store_rows<T, D>(a.dv + sq.b * a.dvs[0] + (sq.k0 + key) * a.dvs[1] + hk * a.dvs[2], dv, fv, half);
+  store_rows<T, D>(a.dk + sq.b * a.dks[0] + (sq.k0 + key) * a.dks[1] + hk * a.dks[2], dk, 1.f, half);
+  store_rows<T, D>(a.dv + sq.b * a.dvs[0] + (sq.k0 + key) * a.dvs[1] + hk * a.dvs[2], dv, 1.f, half);
 }
 
 // Sums of the parts of a block of first keys: a workgroup a block, sequence
@@ -400,12 +420,10 @@ __global__ __launch_bounds__(256) void sink_sum_kernel(const BArgs a) {
   const Seq sq = get_seq(a.seq, si);
   const int k0 = block * kKB;
   if (k0 >= sq.nk) return;
-  const int64_t slots = a.slots_s + 1, one = 2 * kKB * D;
-  const float* parts = a.part + (u * a.sink_blocks + block) * slots * one;
-  const float* own = a.seq.cu == nullptr
-                         ? parts
-                         : a.part + ((int64_t)a.units_k * a.sink_blocks * slots + (u * a.sink_blocks + block) * a.seq.N + si) * one;
-  const int first = a.seq.cu == nullptr ? 0 : (int)(sq.q0 / a.seg) + si;
+  const int64_t slots = a.slots_s + (a.seq.cu == nullptr ? 1 : 0), one = 2 * kKB * D, ub = u * a.sink_blocks + block;
+  const float* parts = a.part + ub * slots * one;
+  const float* own = a.seq.cu == nullptr ? parts : a.part + ((int64_t)a.units_k * a.sink_blocks * slots + ub * a.seq.N + si) * one;
+  const int first = a.seq.cu == nullptr ? 1 : (int)(sq.q0 / a.seg) + si;
   const int nseg = (sq.nq + a.seg - 1) / a.seg;
   for (int e = threadIdx.x; e < kRowsWg * D / 4; e += 256) {
     const int r = rg * kRowsWg + e / (D / 4), d = 4 * (e % (D / 4)), key = k0 + r;
@@ -413,10 +431,10 @@ __global__ __launch_bounds__(256) void sink_sum_kernel(const BArgs a) {
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
       float4 s = *reinterpret_cast<const float4*>(own + (w * kKB + r) * D + d);
-      for (int g = 0; g < nseg; ++g) {
+      for (int g = 0; g < nseg && key < a.sinks; ++g) {
         const QRange q = seg_rows(a, sq, k0, g);
         if (q.r1 <= q.r0) continue;
-        const float4 x = *reinterpret_cast<const float4*>(parts + (1 + first + g) * one + (w * kKB + r) * D + d);
+        const float4 x = *reinterpret_cast<const float4*>(parts + (first + g) * one + (w * kKB + r) * D + d);
         s.x += x.x;
         s.y += x.y;
         s.z += x.z;
@@ -523,7 +541,7 @@ __global__ __launch_bounds__(256, 2) void q_kernel(const BArgs a) {
         const Mask seen(p, j0, half, sq.nk, a.window, a.sinks);
 #pragma unroll
         for (int r = 0; r < 16; ++r) dp[r] = seen(0, r) ? dp[r] : 0.f;
-        bad = tile_not_finite<T, D, 32>(kh, lane);
+        bad = not_finite<T, 32 * TL::kRowBytes / 1024>(kh, lane);
       }
       Vec sf[2];
 #pragma unroll
@@ -561,10 +579,10 @@ void sink_plan(const GdnAttnParams& P, int& blocks, int& seg, int& slots) {
   const int64_t sinks = std::min<int64_t>(P.sinks, P.Tk);
   if (sinks == 0 || P.Tq == 0 || (int64_t)P.window + kKB >= P.Tk) return;
   blocks = (int)((sinks + kKB - 1) / kKB);
-  // as much work as a block's own rows, and few enough parts: they take at
-  // most as many rows of D floats as there are query rows, twice
-  seg = (int)std::max<int64_t>({(int64_t)P.window + kKB, (int64_t)blocks * kKB, 512});
-  seg = (seg + kQT - 1) / kQT * kQT;
+  // about 16 tiles of all heads a segment, short beside a block's own rows, and
+  // no more parts than rows of D floats for every query row, twice
+  const int64_t group = P.Hq / P.Hk;
+  seg = (int)std::max<int64_t>((16 + group - 1) / group * kQT, (int64_t)blocks * kKB);
   slots = P.cu_seqlens == nullptr ? (P.Tq + seg - 1) / seg : P.Tq / seg + P.N;
 }
 
@@ -581,7 +599,7 @@ Space space(const GdnAttnParams& P) {
   s.vmax = s.rmax + (P.dtype == GDN_DTYPE_F16 ? up256(rows * P.Hq * 4) : 0);
   s.part = s.vmax + (P.dtype == GDN_DTYPE_F16 ? up256((int64_t)P.B * P.Hk * kVParts * 4) : 0);
   const int64_t units = P.cu_seqlens == nullptr ? (int64_t)P.B * P.Hk : P.Hk;
-  const int64_t n = units * blocks * (slots + 1 + (P.cu_seqlens == nullptr ? 0 : P.N));
+  const int64_t n = units * blocks * (slots + (P.cu_seqlens == nullptr ? 1 : P.N));
   s.total = s.part + up256(n * 2 * kKB * P.D * 4);
   return s;
 }
@@ -594,7 +612,7 @@ int launch(const BArgs& a, hipStream_t s) {
   const int64_t qb = (int64_t)a.units_q * a.slots_q;
   if (rb + vb > 0x7fffffffLL || kvb > 0x7fffffffLL || qb > 0x7fffffffLL) return GDN_ERR_BAD_SHAPE;
   if (rb > 0) hipLaunchKernelGGL((prep_kernel<T, D>), dim3((uint32_t)(rb + vb)), dim3(256), 0, s, a, (int)rb);
-  if (kvb > 0) hipLaunchKernelGGL((kv_kernel<T, D>), dim3((uint32_t)kvb), dim3(256), 0, s, a);
+  if (kvb > 0) hipLaunchKernelGGL((kv_kernel<T, D>), dim3((uint32_t)kvb), dim3(kKVT), 0, s, a);
   if (a.sink_blocks > 0) {
     const int64_t us = a.seq.cu == nullptr ? a.units_k : (int64_t)a.Hk * a.seq.N;
     hipLaunchKernelGGL((sink_sum_kernel<T, D>), dim3((uint32_t)(us * a.sink_blocks * (kKB / 8))), dim3(256), 0, s, a);

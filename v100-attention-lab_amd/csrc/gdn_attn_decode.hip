@@ -110,8 +110,14 @@ __global__ __launch_bounds__(64 * kDWaves) void decode_kernel(const DArgs a) {
     const uint32_t kt = base + (k & 1) * 2 * kTile;
     const int j0 = kr.tile(t) * kDN, j1 = min(j0 + kDN, n) - 1;
     const bool masked = !(j0 + kDN <= n && all_visible(j0, j1, p0, p1, a.window, a.sinks));
-    rows.step(qf, kt + kofs, kt + kTile, vofs0, vofs1, masked, Mask(p, j0, half, n, a.window, a.sinks), a.scale_log2,
-              lane);
+    const Mask seen(p, j0, half, n, a.window, a.sinks);
+    rows.scores(qf, kt + kofs, masked, seen, a.scale_log2);
+    const uint32_t vt = kt + kTile;
+    if (masked && not_finite<T, kTile / 1024>(vt, lane)) {
+      rows.add_not_finite(seen, vt + vofs0, vt + vofs1);
+      make_finite<T, kTile / 1024>(vt, lane);
+    }
+    rows.values(vt + vofs0, vt + vofs1);
   }
   rows.l += swap_halves(rows.l);
 

@@ -96,10 +96,22 @@ __global__ __launch_bounds__(kNT, 2) void fwd_kernel(const FArgs a) {
       cv(other + kTile, jn);
     }
     const int j1 = min(j0 + kBN, sq.nk) - 1;
-    if (!none_visible(j0, j1, wp0, wp1, a.window, a.sinks)) {
-      const bool masked = !(j0 + kBN <= sq.nk && all_visible(j0, j1, wp0, wp1, a.window, a.sinks));
-      rows.step(qf, kt + kofs, vt, vofs0, vofs1, masked, Mask(p, j0, half, sq.nk, a.window, a.sinks), a.scale_log2, lane);
+    const bool whole = j0 + kBN <= sq.nk, active = !none_visible(j0, j1, wp0, wp1, a.window, a.sinks);
+    const bool masked = !(whole && all_visible(j0, j1, wp0, wp1, a.window, a.sinks));
+    const Mask seen(p, j0, half, sq.nk, a.window, a.sinks);
+    // a tile on an edge of any wave's range: are all its values finite?
+    constexpr int kShare = kTile / 4096;
+    bool bad = false;
+    if (!(whole && all_visible(j0, j1, p0, p1, a.window, a.sinks)))
+      bad = __syncthreads_or(not_finite<T, kShare>(vt + wv * kShare * 1024, lane));
+    if (active) rows.scores(qf, kt + kofs, masked, seen, a.scale_log2);
+    if (bad) {
+      if (active) rows.add_not_finite(seen, vt + vofs0, vt + vofs1);
+      __syncthreads();
+      make_finite<T, kShare>(vt + wv * kShare * 1024, lane);
+      __syncthreads();
     }
+    if (active) rows.values(vt + vofs0, vt + vofs1);
   }
 
   const float l = rows.l + swap_halves(rows.l);

@@ -74,7 +74,7 @@ def _fwd_plan(x, weight, residual, eps, fp8, group):
     P.D, P.eps, P.group = D, float(eps), group or 0
     P.x_dtype, P.w_dtype = _DTYPE_CODE[x.dtype], _DTYPE_CODE[weight.dtype]
     P.r_dtype = _DTYPE_CODE[x.dtype if residual is None else residual.dtype]
-    return bytes(P), (*x.shape[:-1], D // group) if group else x.shape[:-1]
+    return bytes(P), (*x.shape[:-1], D // (group or D))
 
 
 def _run(x, weight, residual, eps, fp8, group):
@@ -90,7 +90,7 @@ def _run(x, weight, residual, eps, fp8, group):
             raise ValueError(f"residual must have shape {shape and tuple(shape)}")
         plan = _fwd_plan(x3, weight, residual3, eps, fp8, group)
         if x3 is not x:
-            plan = plan[0], (*shape[:-1], shape[-1] // group) if group else shape[:-1]
+            plan = plan[0], (*shape[:-1], shape[-1] // (group or shape[-1]))
         if key is not None:
             if len(_FWD_PLANS) >= _PLANS_MAX:
                 _FWD_PLANS.clear()
@@ -144,7 +144,7 @@ def add_rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[t
 
     Returns ``(y, scale, r)``: ``y`` float8_e4m3fn, ``scale`` float32 with
     ``y * scale`` the norm's output; scale is ``max|.| / 448`` over each row
-    (``[...]``) or, with ``group=128``, over each 128 columns
+    (``[..., 1]``) or, with ``group=128``, over each 128 columns
     (``[..., D / 128]``).  A group of zeros has scale 0.  Not differentiable.
     """
     if _needs_grad(x, weight, residual):

@@ -75,6 +75,26 @@ __device__ __forceinline__ typename Ops<T>::Vec acc_operand(const f32x16& p, int
   return v;
 }
 
+// N products, each with its LDS operand read AHEAD products before it: left
+// alone the compiler puts each read right before its product, and the wave
+// waits for it there.
+template <int N, int AHEAD, typename Load, typename Use>
+__device__ __forceinline__ void fed_products(Load load, Use use) {
+  decltype(load(0)) f[AHEAD];
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) f[i] = load(i);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    use(i, f[i % AHEAD]);
+    if (i + AHEAD < N) f[i % AHEAD] = load(i + AHEAD);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+struct Pair {
+  uint4 a, b;
+};
+
 // Accumulator row of register r.
 __device__ __forceinline__ int acc_row(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
 
@@ -345,11 +365,8 @@ struct Rows {
   __device__ __forceinline__ void scores(const Vec (&qf)[D / 16], uint32_t kt, bool masked, const Mask& seen,
                                          float scale_log2) {
     f32x16 s[KS] = {};
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-#pragma unroll
-      for (int t = 0; t < KS; ++t) s[t] = O::mfma(as_vec<T>(TL::row8(kt, i, 32 * t * TL::kRowBytes)), qf[i], s[t]);
-    }
+    fed_products<KS * D / 16, 4>([&](int i) { return TL::row8(kt, i / KS, 32 * (i % KS) * TL::kRowBytes); },
+                                 [&](int i, const uint4& x) { s[i % KS] = O::mfma(as_vec<T>(x), qf[i / KS], s[i % KS]); });
     if (masked) {
 #pragma unroll
       for (int t = 0; t < KS; ++t)
@@ -423,11 +440,9 @@ struct Rows {
 
   // O^T += V^T P^T
   __device__ __forceinline__ void values(uint32_t v0, uint32_t v1) {
-#pragma unroll
-    for (int t = 0; t < 2 * KS; ++t)
-#pragma unroll
-      for (int dt = 0; dt < D / 32; ++dt)
-        acc[dt] = O::mfma(as_vec<T>(TL::col8(v0, v1, dt, 16 * t * TL::kRowBytes)), pf[t], acc[dt]);
+    constexpr int N = D / 32;
+    fed_products<2 * KS * N, 4>([&](int i) { return TL::col8(v0, v1, i % N, 16 * (i / N) * TL::kRowBytes); },
+                                [&](int i, const uint4& x) { acc[i % N] = O::mfma(as_vec<T>(x), pf[i / N], acc[i % N]); });
   }
 };
 

@@ -294,10 +294,16 @@ __global__ __launch_bounds__(kKVT, 2) void kv_kernel(const BArgs a) {
       uint32_t ka = kt, va = vt;
       asm volatile("" : "+v"(ka), "+v"(va));
       f32x16 s = {}, dp = {};
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) s = O::mfma(as_vec<T>(TL::row8(qt + rofs, i, 0)), as_vec<T>(TL::row8(ka, i, 0)), s);
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) dp = O::mfma(as_vec<T>(TL::row8(dt_ + rofs, i, 0)), as_vec<T>(TL::row8(va, i, 0)), dp);
+      // steps of S and dP in turn
+      fed_products<D / 8, 4>(
+          [&](int i) {
+            return (i & 1) ? Pair{TL::row8(dt_ + rofs, i / 2, 0), TL::row8(va, i / 2, 0)}
+                           : Pair{TL::row8(qt + rofs, i / 2, 0), TL::row8(ka, i / 2, 0)};
+          },
+          [&](int i, const Pair& x) {
+            f32x16& c = (i & 1) ? dp : s;
+            c = O::mfma(as_vec<T>(x.a), as_vec<T>(x.b), c);
+          });
       typedef float f32x4v __attribute__((ext_vector_type(4)));
       typedef __attribute__((address_space(3))) const f32x4v lds_f32x4;
       // row c + 4 half of the tile sees the lane's key where lo <= c < top
@@ -338,13 +344,14 @@ __global__ __launch_bounds__(kKVT, 2) void kv_kernel(const BArgs a) {
       __syncthreads();
     }
     if (active) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-          dv[i] = O::mfma(as_vec<T>(TL::col8(dt_ + cofs0, dt_ + cofs1, i, 16 * t * TL::kRowBytes)), pf[t], dv[i]);
-          dk[i] = O::mfma(as_vec<T>(TL::col8(qt + cofs0, qt + cofs1, i, 16 * t * TL::kRowBytes)), df[t], dk[i]);
-        }
+      constexpr int N = D / 32;
+      fed_products<4 * N, 4>(
+          [&](int i) { return TL::col8((i & 1 ? qt : dt_) + cofs0, (i & 1 ? qt : dt_) + cofs1, i / 2 % N, 16 * (i / (2 * N)) * TL::kRowBytes); },
+          [&](int i, const uint4& x) {
+            const int t = i / (2 * N), d = i / 2 % N;
+            if (i & 1) dk[d] = O::mfma(as_vec<T>(x), df[t], dk[d]);
+            else dv[d] = O::mfma(as_vec<T>(x), pf[t], dv[d]);
+          });
     }
   }
   const float fv = exp2f(-kPUp<T>);
@@ -527,10 +534,11 @@ __global__ __launch_bounds__(256, 2) void q_kernel(const BArgs a) {
       const bool masked = !(j0 + 32 <= sq.nk && all_visible(j0, j1, wp0, wp1, a.window, a.sinks));
       const uint32_t kh = kt + 32 * h * TL::kRowBytes, vh = vt + 32 * h * TL::kRowBytes;
       f32x16 s = {}, dp = {};
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) s = O::mfma(as_vec<T>(TL::row8(kh + rofs, i, 0)), qf[i], s);
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) dp = O::mfma(as_vec<T>(TL::row8(vh + rofs, i, 0)), df[i], dp);
+      fed_products<D / 8, 4>([&](int i) { return TL::row8((i & 1 ? vh : kh) + rofs, i / 2, 0); },
+                             [&](int i, const uint4& x) {
+                               if (i & 1) dp = O::mfma(as_vec<T>(x), df[i / 2], dp);
+                               else s = O::mfma(as_vec<T>(x), qf[i / 2], s);
+                             });
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const float x = exp2_fast(__builtin_fmaf(s[r], a.scale_log2, lb));
@@ -553,11 +561,9 @@ __global__ __launch_bounds__(256, 2) void q_kernel(const BArgs a) {
           for (int i = 0; i < D / 32; ++i)
             dq[i] = O::mfma(as_vec<T>(only_finite<T>(TL::col8(kh + cofs0, kh + cofs1, i, 16 * t * TL::kRowBytes))), sf[t], dq[i]);
       } else {
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int i = 0; i < D / 32; ++i)
-            dq[i] = O::mfma(as_vec<T>(TL::col8(kh + cofs0, kh + cofs1, i, 16 * t * TL::kRowBytes)), sf[t], dq[i]);
+        constexpr int N = D / 32;
+        fed_products<2 * N, 4>([&](int i) { return TL::col8(kh + cofs0, kh + cofs1, i % N, 16 * (i / N) * TL::kRowBytes); },
+                               [&](int i, const uint4& x) { dq[i % N] = O::mfma(as_vec<T>(x), sf[i / N], dq[i % N]); });
       }
     }
   }

@@ -181,6 +181,7 @@ __device__ __forceinline__ QRange seg_rows(const BArgs& a, const Seq& s, int k0,
 
 // 4 bytes per lane from global memory to LDS at `at` + 4 * lane.
 __device__ __forceinline__ void dma4(const void* src, uint32_t at) {
+  at = __builtin_amdgcn_readfirstlane(at);
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(at) : "memory");
 }
 
@@ -240,27 +241,38 @@ __global__ __launch_bounds__(kKVT, 2) void kv_kernel(const BArgs a) {
 
   const uint32_t rofs = TL::row_ofs(lane), cofs0 = TL::col_ofs(lane, 0), cofs1 = TL::col_ofs(lane, 1);
   const uint32_t kt = base + kK + 32 * kg * TL::kRowBytes + rofs, vt = base + kV + 32 * kg * TL::kRowBytes + rofs;
-  auto fetch = [&](int it) {
-    const int g = it / nt, r0 = rg.r0 + (it % nt) * kQT, h = hk * a.G + g;
-    const uint32_t at = base + (it & 1) * kBuf;
-    const Copier<D, kQT, kKVT> cq(a.q + sq.b * a.qs[0] + sq.q0 * a.qs[1] + h * a.qs[2], a.qs[1], sq.nq);
-    const Copier<D, kQT, kKVT> cd(a.dO + sq.b * a.dos[0] + sq.q0 * a.dos[1] + h * a.dos[2], a.dos[1], sq.nq);
-    cq(at, r0);
-    cd(at + kTile, r0);
-    const int64_t row = (int64_t)h * a.rows + (int64_t)sq.b * a.seq.Tq + sq.q0 + min(r0 + lane, sq.nq - 1);
-    if (wv < 2) dma4(a.stat + row * 2 + wv, __builtin_amdgcn_readfirstlane(at + 2 * kTile + 256 * wv));
+  // the tile that is brought next: its rows and head
+  int fr0 = rg.r0, fh = hk * a.G;
+  Copier<D, kQT, kKVT> cq(a.q + sq.b * a.qs[0] + sq.q0 * a.qs[1] + fh * a.qs[2], a.qs[1], sq.nq);
+  Copier<D, kQT, kKVT> cd(a.dO + sq.b * a.dos[0] + sq.q0 * a.dos[1] + fh * a.dos[2], a.dos[1], sq.nq);
+  int64_t frow = (int64_t)fh * a.rows + (int64_t)sq.b * a.seq.Tq + sq.q0;
+  auto fetch = [&](uint32_t at) {
+    cq(at, fr0);
+    cd(at + kTile, fr0);
+    const int64_t row = frow + min(fr0 + lane, sq.nq - 1);
+    if (wv < 2) dma4(a.stat + row * 2 + wv, at + 2 * kTile + 256 * wv);
     if constexpr (kScaled<T>)
-      if (wv == 2) dma4(a.rmax + row, __builtin_amdgcn_readfirstlane(at + 2 * kTile + 512));
+      if (wv == 2) dma4(a.rmax + row, at + 2 * kTile + 512);
+    fr0 += kQT;
+    if (fr0 >= rg.r1) {
+      fr0 = rg.r0;
+      cq.src += a.qs[2];
+      cd.src += a.dos[2];
+      frow += a.rows;
+    }
   };
   dma_wait();
-  if (n > 0) fetch(0);
+  // two waves share a SIMD: with one of them ahead, its exponentials run beside
+  // the other's products
+  if (qh == 1) __builtin_amdgcn_s_setprio(1);
+  if (n > 0) fetch(base);
+  int t0 = rg.r0;                                 // the tile's first row
   for (int it = 0; it < n; ++it) {
     dma_wait();
     __syncthreads();
-    if (it + 1 < n) fetch(it + 1);
+    if (it + 1 < n) fetch(base + ((it + 1) & 1) * kBuf);
     const uint32_t buf = base + (it & 1) * kBuf;
     const uint32_t qt = buf + 32 * qh * TL::kRowBytes, dt_ = qt + kTile, st = buf + 2 * kTile + 128 * qh;
-    const int t0 = rg.r0 + (it % nt) * kQT;                        // the tile's rows, and the wave's
     const int r0 = t0 + 32 * qh, nr = min(32, rg.r1 - r0), p0 = r0 + shift, p1 = p0 + nr - 1;
     const bool active = nr > 0 && !none_visible(j0, j1, p0, p1, a.window, a.sinks);
     const bool masked = !(nr == 32 && j0 + 32 <= sq.nk && all_visible(j0, j1, p0, p1, a.window, a.sinks));
@@ -306,6 +318,15 @@ __global__ __launch_bounds__(kKVT, 2) void kv_kernel(const BArgs a) {
           });
       typedef float f32x4v __attribute__((ext_vector_type(4)));
       typedef __attribute__((address_space(3))) const f32x4v lds_f32x4;
+      if (bad) {
+        // a row of dO that is not finite reaches the keys that see it: its S is NaN
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const f32x4v de = *(lds_f32x4*)(st + 256 + 32 * c + 16 * half);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[4 * c + e] += fabsf(de[e]) < __builtin_inff() ? 0.f : __builtin_nanf("");
+        }
+      }
       // row c + 4 half of the tile sees the lane's key where lo <= c < top
       const int rel = p0 + 4 * half - key;
       const int64_t reach = key < a.sinks ? (int64_t)1 << 32 : (int64_t)a.window - rel;
@@ -319,8 +340,6 @@ __global__ __launch_bounds__(kKVT, 2) void kv_kernel(const BArgs a) {
           const float x = exp2_fast(__builtin_fmaf(s[r], a.scale_log2, kPUp<T> - ls[e]));
           dp[r] = x * __builtin_fmaf(dp[r], sc, -de[e] * sc);
           s[r] = x;
-          // a row of dO that is not finite reaches the keys that see it
-          if (bad) s[r] += fabsf(de[e]) < __builtin_inff() ? 0.f : __builtin_nanf("");
         }
         if (masked) {
 #pragma unroll
@@ -353,6 +372,7 @@ __global__ __launch_bounds__(kKVT, 2) void kv_kernel(const BArgs a) {
             else dv[d] = O::mfma(as_vec<T>(x), pf[t], dv[d]);
           });
     }
+    t0 = t0 + kQT < rg.r1 ? t0 + kQT : rg.r0;
   }
   const float fv = exp2f(-kPUp<T>);
   const float fk = kScaled<T> ? a.scale * unit_do * vu * 0x1p-7f : a.scale;

@@ -91,8 +91,8 @@ __device__ __forceinline__ void fed_products(Load load, Use use) {
     __builtin_amdgcn_sched_barrier(0);
   }
 }
-struct Pair {
-  uint4 a, b;
+struct Triple {
+  uint4 a, b, c;
 };
 
 // Accumulator row of register r.
@@ -131,57 +131,62 @@ __device__ __forceinline__ const void* uniform_ptr(const void* p) {
   return (const void*)(uintptr_t)(((uint64_t)hi << 32) | lo);
 }
 
-// ROWS rows of D 16-bit elements in LDS, in 16-byte pieces; piece c of row r
-// lies at piece c ^ swz(r) of the row.  16 rows at one piece (a product's
-// operand) and 4 rows at 64 neighbouring bytes (a transposing read) then each
-// cover all banks once.  swz depends on r % 16 only.
+// Rows of D 16-bit elements in LDS: groups of 1 KB (kGroup rows, one LDS-DMA of
+// a wave) 1040 bytes apart, in 16-byte pieces; piece c of row r lies at place
+// c ^ swz(r) of the row.  16 rows at one piece (a product's operand) and 4 rows
+// at 64 neighbouring bytes (a transposing read) then each cover all banks once,
+// and a lane's addresses differ by constants but for four of them.
 template <int D>
 struct Tile {
-  static constexpr int kPieces = D / 8;
-  static constexpr int kRowBytes = 2 * D;
+  static constexpr int kPieces = D / 8, kRowBytes = 2 * D, kGroup = 1024 / kRowBytes;
+  static constexpr uint32_t kGroupBytes = 1040;
+  static constexpr uint32_t bytes(int rows) { return rows / kGroup * kGroupBytes; }   // rows: a multiple of kGroup
   __device__ static __forceinline__ int swz(int row) {
-    return D == 128 ? ((row & 3) << 2) | ((row >> 2) & 3) : (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+    return D == 128 ? (row & 3) << 2 : (((row >> 1) & 1) << 2) | (((row >> 2) & 1) << 1);
   }
-  // Byte offset in a tile of this lane's operand rows: row l % 32, elements
-  // 8 (l / 32) ...  Step i is at offset ^ (32 i), 32 rows on at + 32 rows.
-  __device__ static __forceinline__ uint32_t row_ofs(int lane) {
-    const int r = lane & 31, h = lane >> 5;
-    return r * kRowBytes + ((h ^ swz(r)) << 4);
+  __device__ static __forceinline__ uint32_t place(int row, int piece) {
+    return row / kGroup * kGroupBytes + row % kGroup * kRowBytes + 16 * (piece ^ swz(row));
   }
-  __device__ static __forceinline__ uint4 row8(uint32_t addr, int i, int imm) {
-    const u32x4 v = *(const lds_u32x4*)((addr ^ (uint32_t)(32 * i)) + imm);
+  // A lane's byte offsets in a tile.
+  uint32_t row[4], col[D / 32];
+  __device__ __forceinline__ explicit Tile(int lane) {
+    const int h = lane >> 5, a = lane & 15;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) row[j] = place(lane & 31, h + (D == 128 ? 4 : 2) * j);
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+      col[dt] = place(4 * h + (a >> 2), 4 * dt + 2 * ((lane >> 4) & 1) + ((a & 3) >> 1)) + 8 * (a & 1);
+  }
+  // Operand of step i: row r0 + l % 32, elements 16 i + 8 (l / 32) .. (r0 a
+  // multiple of kGroup).
+  __device__ __forceinline__ uint4 row8(uint32_t tile, int i, int r0 = 0) const {
+    const u32x4 v = *(const lds_u32x4*)(tile + row[D == 128 ? i >> 1 : i] + (D == 128 ? 32 * (i & 1) : 0) + bytes(r0));
     return make_uint4(v[0], v[1], v[2], v[3]);
   }
-  // Transposed operand: lane l receives element d0 + l % 32 of rows k0 + 4 h +
-  // {0..3} and k0 + 8 + 4 h + {0..3}, h = l / 32 (k0 a multiple of 16, d0 =
-  // 32 dt).  ds_read_b64_tr_b16: lane i of 16 receives halfword i % 4 of the 8
-  // bytes addressed by lanes 4 j + i / 4, j = 0..3.  The offsets of the two
-  // reads at k0 = 0, dt = 0; dt is at offset ^ (64 dt), k0 at + k0 rows.
-  __device__ static __forceinline__ uint32_t col_ofs(int lane, int which) {
-    const int a = lane & 15, h = lane >> 5, d = 16 * ((lane >> 4) & 1) + 4 * (a & 3);
-    const int r = 8 * which + 4 * h + (a >> 2);
-    return r * kRowBytes + (((d >> 3) ^ swz(r)) << 4) + 2 * (d & 7);
-  }
-  __device__ static __forceinline__ uint4 col8(uint32_t addr0, uint32_t addr1, int dt, int imm) {
+  // Transposed operand: lane l receives element 32 dt + l % 32 of rows k0 + 4 h
+  // + {0..3} and k0 + 8 + 4 h + {0..3}, h = l / 32 (k0 a multiple of 16).
+  // ds_read_b64_tr_b16: lane i of 16 receives halfword i % 4 of the 8 bytes
+  // addressed by lanes 4 j + i / 4, j = 0..3.
+  __device__ __forceinline__ uint4 col8(uint32_t tile, int dt, int k0) const {
     union {
       s16x4 h[2];
       uint4 v;
     } u;
-    u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)((addr0 ^ (uint32_t)(64 * dt)) + imm));
-    u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)((addr1 ^ (uint32_t)(64 * dt)) + imm));
+    u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + col[dt] + bytes(k0)));
+    u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + col[dt] + bytes(k0 + 8)));
     return u.v;
   }
 };
 
 // Copies rows row0 .. row0 + ROWS - 1 of a [rows, D] matrix (row stride ld
 // elements) into a tile by LDS-DMA, NT threads; rows past the last one are
-// copies of it.  A pass moves NT / kPieces rows (a multiple of 16, so a lane's
-// piece is the same in every pass).
+// copies of it.  A pass moves NT / kPieces rows (a multiple of kGroup, so a
+// lane's piece is the same in every pass).
 template <int D, int ROWS, int NT>
 struct Copier {
   using TL = Tile<D>;
   static constexpr int kPass = NT / TL::kPieces, kPasses = ROWS / kPass;
-  static_assert(kPass % 16 == 0 && ROWS % kPass == 0, "whole passes");
+  static_assert(kPass % TL::kGroup == 0 && ROWS % kPass == 0, "whole passes");
   const uint16_t* src;
   int64_t ld;
   int rows;          // of the matrix
@@ -189,22 +194,23 @@ struct Copier {
   uint32_t ofs;      // its byte offset where that fits 31 bits
   bool small;
   __device__ __forceinline__ Copier(const uint16_t* s, int64_t ld_, int rows_) : src(s), ld(ld_), rows(rows_) {
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x % NT;
     row = tid / TL::kPieces;
     piece = (tid % TL::kPieces) ^ TL::swz(row);
     small = ld >= 0 && ld < (1 << 24);
     ofs = (uint32_t)(row * (uint32_t)ld * 2u) + 16u * piece;
   }
   __device__ __forceinline__ void operator()(uint32_t tile, int row0) const {
-    const uint32_t at = tile + 16u * __builtin_amdgcn_readfirstlane(threadIdx.x & ~63);
+    constexpr uint32_t kStep = NT / 64 * TL::kGroupBytes;
+    const uint32_t at = tile + TL::kGroupBytes * __builtin_amdgcn_readfirstlane(threadIdx.x % NT / 64);
     if (small && row0 + ROWS <= rows) {
 #pragma unroll
       for (int i = 0; i < kPasses; ++i)
-        dma16(uniform_ptr(src + (int64_t)(row0 + i * kPass) * ld), ofs, at + i * NT * 16);
+        dma16(uniform_ptr(src + (int64_t)(row0 + i * kPass) * ld), ofs, at + i * kStep);
     } else {
 #pragma unroll
       for (int i = 0; i < kPasses; ++i)
-        dma16(src + (int64_t)min(row0 + i * kPass + row, rows - 1) * ld + 8 * piece, at + i * NT * 16);
+        dma16(src + (int64_t)min(row0 + i * kPass + row, rows - 1) * ld + 8 * piece, at + i * kStep);
     }
   }
 };
@@ -314,15 +320,15 @@ __device__ __forceinline__ uint4 only_finite(const uint4& x) {
 
 // A product over rows of which some are hidden from some columns adds 0 times
 // what the hidden places hold.  Where that is an infinity or NaN, the tile is
-// made finite before the product: these look at and change N KB of LDS, one
-// wave, 16 bytes a lane and step.
+// made finite before the product: these look at and change N groups of a tile,
+// one wave, a group a step.
 template <typename T, int N>
 __device__ __forceinline__ bool not_finite(uint32_t at, int lane) {
   typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
   u16x2 m = {0, 0};
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const u32x4 x = *(const lds_u32x4*)(at + 16 * (i * 64 + lane));
+    const u32x4 x = *(const lds_u32x4*)(at + i * 1040 + 16 * lane);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const uint32_t w = x[e] & 0x7fff7fffu;
@@ -335,7 +341,7 @@ template <typename T, int N>
 __device__ __forceinline__ void make_finite(uint32_t at, int lane) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    lds_u32x4* p = (lds_u32x4*)(at + 16 * (i * 64 + lane));
+    lds_u32x4* p = (lds_u32x4*)(at + i * 1040 + 16 * lane);
     const u32x4 x = *p;
     const uint4 y = only_finite<T>(make_uint4(x[0], x[1], x[2], x[3]));
     *p = u32x4{y.x, y.y, y.z, y.w};
@@ -361,11 +367,11 @@ struct Rows {
 
   Vec pf[2 * KS];
 
-  // Scores and probabilities of one tile; kt: the lane's operand address.
-  __device__ __forceinline__ void scores(const Vec (&qf)[D / 16], uint32_t kt, bool masked, const Mask& seen,
+  // Scores and probabilities of one tile.
+  __device__ __forceinline__ void scores(const Vec (&qf)[D / 16], const TL& tl, uint32_t kt, bool masked, const Mask& seen,
                                          float scale_log2) {
     f32x16 s[KS] = {};
-    fed_products<KS * D / 16, 4>([&](int i) { return TL::row8(kt, i / KS, 32 * (i % KS) * TL::kRowBytes); },
+    fed_products<KS * D / 16, 4>([&](int i) { return tl.row8(kt, i / KS, 32 * (i % KS)); },
                                  [&](int i, const uint4& x) { s[i % KS] = O::mfma(as_vec<T>(x), qf[i / KS], s[i % KS]); });
     if (masked) {
 #pragma unroll
@@ -402,17 +408,17 @@ struct Rows {
     for (int t = 0; t < 2 * KS; ++t) pf[t] = acc_operand<T>(s[t >> 1], t & 1);
   }
 
-  // What the infinities and NaN of a value tile add to the rows that see them
-  // (v0, v1: the lane's transposed addresses): two products of 0/1 matrices
-  // say which sums meet a +inf or NaN, and which a -inf or NaN.
-  __device__ __forceinline__ void add_not_finite(const Mask& seen, uint32_t v0, uint32_t v1) {
+  // What the infinities and NaN of a value tile add to the rows that see them:
+  // two products of 0/1 matrices say which sums meet a +inf or NaN, and which a
+  // -inf or NaN.
+  __device__ __forceinline__ void add_not_finite(const Mask& seen, const TL& tl, uint32_t vt) {
     constexpr uint32_t E = O::kExp, ONE = O::kOne;
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt) {
       f32x16 up = {}, dn = {};
 #pragma unroll
       for (int s = 0; s < 2 * KS; ++s) {
-        const uint4 raw = TL::col8(v0, v1, dt, 16 * s * TL::kRowBytes);
+        const uint4 raw = tl.col8(vt, dt, 16 * s);
         const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
         uint32_t u[4], d[4], one[4];
 #pragma unroll
@@ -439,9 +445,9 @@ struct Rows {
   }
 
   // O^T += V^T P^T
-  __device__ __forceinline__ void values(uint32_t v0, uint32_t v1) {
+  __device__ __forceinline__ void values(const TL& tl, uint32_t vt) {
     constexpr int N = D / 32;
-    fed_products<2 * KS * N, 4>([&](int i) { return TL::col8(v0, v1, i % N, 16 * (i / N) * TL::kRowBytes); },
+    fed_products<2 * KS * N, 4>([&](int i) { return tl.col8(vt, i % N, 16 * (i / N)); },
                                 [&](int i, const uint4& x) { acc[i % N] = O::mfma(as_vec<T>(x), pf[i / N], acc[i % N]); });
   }
 };

@@ -190,15 +190,16 @@ __global__ __launch_bounds__(kKVT, 2) void kv_kernel(const BArgs a) {
   using O = Ops<T>;
   using Vec = typename O::Vec;
   using TL = Tile<D>;
-  constexpr uint32_t kTile = kQT * TL::kRowBytes, kBuf = 2 * kTile + 1024;    // Q, dO, 64 x lse, D, max
-  constexpr uint32_t kK = 2 * kBuf, kV = kK + kKB * TL::kRowBytes;            // the block's k and v rows
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[kV + kKB * TL::kRowBytes];
+  constexpr uint32_t kTile = TL::bytes(kQT), kBuf = 2 * kTile + 1024;    // Q, dO, 64 x lse, D, max
+  constexpr uint32_t kV = 2 * kBuf;                                           // the block's v rows
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kV + TL::bytes(kKB)];
   const int unit_ix = blockIdx.x % a.units_k;
   const int unit = a.units_k % 8 == 0 ? (unit_ix % 8) * (a.units_k / 8) + unit_ix / 8 : unit_ix;
-  // the segments first: they are short, and the blocks fill up behind them
-  const int extras = a.sink_blocks * a.slots_s, at_item = blockIdx.x / a.units_k;
-  const bool extra = at_item < extras;
-  const int item = extra ? at_item : at_item - extras;
+  // the segments last: they are short and fill the places of the blocks at the
+  // sequences' ends
+  const int at_item = blockIdx.x / a.units_k;
+  const bool extra = at_item >= a.slots_k;
+  const int item = extra ? at_item - a.slots_k : at_item;
   int si, hk, block, seg = 0;
   if (a.seq.cu == nullptr) {
     si = unit / a.Hk;
@@ -227,10 +228,12 @@ __global__ __launch_bounds__(kKVT, 2) void kv_kernel(const BArgs a) {
   const uint32_t base = lds_addr(lds);
 
   const int nt = (max(rg.r1 - rg.r0, 0) + kQT - 1) / kQT, n = nt * a.G;
+  Vec kf[D / 16];
   {
-    const Copier<D, kKB, kKVT> ck(a.k + sq.b * a.ks[0] + sq.k0 * a.ks[1] + hk * a.ks[2], a.ks[1], sq.nk);
+    const uint16_t* kr = a.k + sq.b * a.ks[0] + (sq.k0 + min(key, sq.nk - 1)) * a.ks[1] + hk * a.ks[2];
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) kf[i] = as_vec<T>(*reinterpret_cast<const uint4*>(kr + 16 * i + 8 * half));
     const Copier<D, kKB, kKVT> cv(a.v + sq.b * a.vs[0] + sq.k0 * a.vs[1] + hk * a.vs[2], a.vs[1], sq.nk);
-    ck(base + kK, k0);
     cv(base + kV, k0);
   }
   float vu = 1.f;
@@ -239,8 +242,8 @@ __global__ __launch_bounds__(kKVT, 2) void kv_kernel(const BArgs a) {
   float unit_do = 0x1p-24f;                     // unit of dO so far (fp16)
   f32x16 dk[D / 32] = {}, dv[D / 32] = {};
 
-  const uint32_t rofs = TL::row_ofs(lane), cofs0 = TL::col_ofs(lane, 0), cofs1 = TL::col_ofs(lane, 1);
-  const uint32_t kt = base + kK + 32 * kg * TL::kRowBytes + rofs, vt = base + kV + 32 * kg * TL::kRowBytes + rofs;
+  const TL tl(lane);
+  const uint32_t vt = base + kV + TL::bytes(32) * kg;
   // the tile that is brought next: its rows and head
   int fr0 = rg.r0, fh = hk * a.G;
   Copier<D, kQT, kKVT> cq(a.q + sq.b * a.qs[0] + sq.q0 * a.qs[1] + fh * a.qs[2], a.qs[1], sq.nq);
@@ -272,16 +275,16 @@ __global__ __launch_bounds__(kKVT, 2) void kv_kernel(const BArgs a) {
     __syncthreads();
     if (it + 1 < n) fetch(base + ((it + 1) & 1) * kBuf);
     const uint32_t buf = base + (it & 1) * kBuf;
-    const uint32_t qt = buf + 32 * qh * TL::kRowBytes, dt_ = qt + kTile, st = buf + 2 * kTile + 128 * qh;
+    const uint32_t qt = buf + TL::bytes(32) * qh, dt_ = qt + kTile, st = buf + 2 * kTile + 128 * qh;
     const int r0 = t0 + 32 * qh, nr = min(32, rg.r1 - r0), p0 = r0 + shift, p1 = p0 + nr - 1;
     const bool active = nr > 0 && !none_visible(j0, j1, p0, p1, a.window, a.sinks);
     const bool masked = !(nr == 32 && j0 + 32 <= sq.nk && all_visible(j0, j1, p0, p1, a.window, a.sinks));
     // a tile on an edge of any wave's range: are all its rows finite?
-    constexpr int kShare = 2 * kTile / 8192;
+    constexpr int kShare = 2 * kQT / TL::kGroup / 8;
     bool bad = false;
     if (!(t0 + kQT <= rg.r1 && k0 + kKB <= sq.nk &&
           all_visible(k0, k0 + kKB - 1, t0 + shift, t0 + kQT - 1 + shift, a.window, a.sinks)))
-      bad = __syncthreads_or(not_finite<T, kShare>(buf + wv * kShare * 1024, lane));
+      bad = __syncthreads_or(not_finite<T, kShare>(buf + wv * kShare * TL::kGroupBytes, lane));
     Vec pf[2], df[2];
     if (active) {
       float sc = 1.f;
@@ -302,20 +305,12 @@ __global__ __launch_bounds__(kKVT, 2) void kv_kernel(const BArgs a) {
         }
         sc = 0x1p-7f / (unit_do * vu);            // 2^7 / unit, and P's 2^14 taken out
       }
-      // not kept across iterations: the addresses of 2 D / 16 steps
-      uint32_t ka = kt, va = vt;
-      asm volatile("" : "+v"(ka), "+v"(va));
       f32x16 s = {}, dp = {};
-      // steps of S and dP in turn
-      fed_products<D / 8, 4>(
-          [&](int i) {
-            return (i & 1) ? Pair{TL::row8(dt_ + rofs, i / 2, 0), TL::row8(va, i / 2, 0)}
-                           : Pair{TL::row8(qt + rofs, i / 2, 0), TL::row8(ka, i / 2, 0)};
-          },
-          [&](int i, const Pair& x) {
-            f32x16& c = (i & 1) ? dp : s;
-            c = O::mfma(as_vec<T>(x.a), as_vec<T>(x.b), c);
-          });
+      fed_products<D / 16, 2>([&](int i) { return Triple{tl.row8(qt, i), tl.row8(dt_, i), tl.row8(vt, i)}; },
+                              [&](int i, const Triple& x) {
+                                s = O::mfma(as_vec<T>(x.a), kf[i], s);
+                                dp = O::mfma(as_vec<T>(x.b), as_vec<T>(x.c), dp);
+                              });
       typedef float f32x4v __attribute__((ext_vector_type(4)));
       typedef __attribute__((address_space(3))) const f32x4v lds_f32x4;
       if (bad) {
@@ -359,13 +354,13 @@ __global__ __launch_bounds__(kKVT, 2) void kv_kernel(const BArgs a) {
     }
     if (bad) {
       __syncthreads();
-      make_finite<T, kShare>(buf + wv * kShare * 1024, lane);
+      make_finite<T, kShare>(buf + wv * kShare * TL::kGroupBytes, lane);
       __syncthreads();
     }
     if (active) {
       constexpr int N = D / 32;
       fed_products<4 * N, 4>(
-          [&](int i) { return TL::col8((i & 1 ? qt : dt_) + cofs0, (i & 1 ? qt : dt_) + cofs1, i / 2 % N, 16 * (i / (2 * N)) * TL::kRowBytes); },
+          [&](int i) { return tl.col8(i & 1 ? qt : dt_, i / 2 % N, 16 * (i / (2 * N))); },
           [&](int i, const uint4& x) {
             const int t = i / (2 * N), d = i / 2 % N;
             if (i & 1) dk[d] = O::mfma(as_vec<T>(x), df[t], dk[d]);
@@ -483,7 +478,7 @@ __global__ __launch_bounds__(256, 2) void q_kernel(const BArgs a) {
   using O = Ops<T>;
   using Vec = typename O::Vec;
   using TL = Tile<D>;
-  constexpr uint32_t kTile = kKT * TL::kRowBytes;
+  constexpr uint32_t kTile = TL::bytes(kKT);
   __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * kTile];
   const int unit_ix = blockIdx.x % a.units_q, slot = a.slots_q - 1 - blockIdx.x / a.units_q;
   const int unit = a.units_q % 8 == 0 ? (unit_ix % 8) * (a.units_q / 8) + unit_ix / 8 : unit_ix;
@@ -532,7 +527,7 @@ __global__ __launch_bounds__(256, 2) void q_kernel(const BArgs a) {
   const Copier<D, kKT, 256> ck(a.k + sq.b * a.ks[0] + sq.k0 * a.ks[1] + hk * a.ks[2], a.ks[1], sq.nk);
   const Copier<D, kKT, 256> cv(a.v + sq.b * a.vs[0] + sq.k0 * a.vs[1] + hk * a.vs[2], a.vs[1], sq.nk);
   const uint32_t base = lds_addr(lds);
-  const uint32_t rofs = TL::row_ofs(lane), cofs0 = TL::col_ofs(lane, 0), cofs1 = TL::col_ofs(lane, 1);
+  const TL tl(lane);
   dma_wait();
   if (kr.n > 0) {
     ck(base, kr.tile(0) * kKT);
@@ -552,9 +547,9 @@ __global__ __launch_bounds__(256, 2) void q_kernel(const BArgs a) {
       const int j0 = kr.tile(it) * kKT + 32 * h, j1 = min(j0 + 32, sq.nk) - 1;
       if (j0 >= sq.nk || none_visible(j0, j1, wp0, wp1, a.window, a.sinks)) continue;
       const bool masked = !(j0 + 32 <= sq.nk && all_visible(j0, j1, wp0, wp1, a.window, a.sinks));
-      const uint32_t kh = kt + 32 * h * TL::kRowBytes, vh = vt + 32 * h * TL::kRowBytes;
+      const uint32_t kh = kt + TL::bytes(32) * h, vh = vt + TL::bytes(32) * h;
       f32x16 s = {}, dp = {};
-      fed_products<D / 8, 4>([&](int i) { return TL::row8((i & 1 ? vh : kh) + rofs, i / 2, 0); },
+      fed_products<D / 8, 4>([&](int i) { return tl.row8(i & 1 ? vh : kh, i / 2); },
                              [&](int i, const uint4& x) {
                                if (i & 1) dp = O::mfma(as_vec<T>(x), df[i / 2], dp);
                                else s = O::mfma(as_vec<T>(x), qf[i / 2], s);
@@ -569,7 +564,7 @@ __global__ __launch_bounds__(256, 2) void q_kernel(const BArgs a) {
         const Mask seen(p, j0, half, sq.nk, a.window, a.sinks);
 #pragma unroll
         for (int r = 0; r < 16; ++r) dp[r] = seen(0, r) ? dp[r] : 0.f;
-        bad = not_finite<T, 32 * TL::kRowBytes / 1024>(kh, lane);
+        bad = not_finite<T, 32 / TL::kGroup>(kh, lane);
       }
       Vec sf[2];
 #pragma unroll
@@ -579,10 +574,10 @@ __global__ __launch_bounds__(256, 2) void q_kernel(const BArgs a) {
         for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int i = 0; i < D / 32; ++i)
-            dq[i] = O::mfma(as_vec<T>(only_finite<T>(TL::col8(kh + cofs0, kh + cofs1, i, 16 * t * TL::kRowBytes))), sf[t], dq[i]);
+            dq[i] = O::mfma(as_vec<T>(only_finite<T>(tl.col8(kh, i, 16 * t))), sf[t], dq[i]);
       } else {
         constexpr int N = D / 32;
-        fed_products<2 * N, 4>([&](int i) { return TL::col8(kh + cofs0, kh + cofs1, i % N, 16 * (i / N) * TL::kRowBytes); },
+        fed_products<2 * N, 4>([&](int i) { return tl.col8(kh, i % N, 16 * (i / N)); },
                                [&](int i, const uint4& x) { dq[i % N] = O::mfma(as_vec<T>(x), sf[i / N], dq[i % N]); });
       }
     }

@@ -56,7 +56,7 @@ __global__ __launch_bounds__(64 * kDWaves) void decode_kernel(const DArgs a) {
   using O = Ops<T>;
   using Vec = typename O::Vec;
   using TL = Tile<D>;
-  constexpr uint32_t kTile = kDN * TL::kRowBytes, kWave = 4 * kTile;
+  constexpr uint32_t kTile = TL::bytes(kDN), kWave = 4 * kTile;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[kDWaves * kWave];
   const int split = blockIdx.x % a.splits, unit = blockIdx.x / a.splits;
   const int rt = unit % a.tiles_r, bh = unit / a.tiles_r, hk = bh % a.Hk, b = bh / a.Hk;
@@ -88,10 +88,10 @@ __global__ __launch_bounds__(64 * kDWaves) void decode_kernel(const DArgs a) {
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
       const int e = i * 64 + lane, row = e / TL::kPieces, c = (e % TL::kPieces) ^ TL::swz(row);
-      dma16(src + (int64_t)min(row0 + row, n - 1) * ld + 8 * c, at + i * 1024);
+      dma16(src + (int64_t)min(row0 + row, n - 1) * ld + 8 * c, at + i * TL::kGroupBytes);
     }
   };
-  const uint32_t kofs = TL::row_ofs(lane), vofs0 = TL::col_ofs(lane, 0), vofs1 = TL::col_ofs(lane, 1);
+  const TL tl(lane);
   Rows<T, D, 1> rows;
   dma_wait();
   if (t0 + wv < t1) {
@@ -111,13 +111,13 @@ __global__ __launch_bounds__(64 * kDWaves) void decode_kernel(const DArgs a) {
     const int j0 = kr.tile(t) * kDN, j1 = min(j0 + kDN, n) - 1;
     const bool masked = !(j0 + kDN <= n && all_visible(j0, j1, p0, p1, a.window, a.sinks));
     const Mask seen(p, j0, half, n, a.window, a.sinks);
-    rows.scores(qf, kt + kofs, masked, seen, a.scale_log2);
+    rows.scores(qf, tl, kt, masked, seen, a.scale_log2);
     const uint32_t vt = kt + kTile;
-    if (masked && not_finite<T, kTile / 1024>(vt, lane)) {
-      rows.add_not_finite(seen, vt + vofs0, vt + vofs1);
-      make_finite<T, kTile / 1024>(vt, lane);
+    if (masked && not_finite<T, kDN / TL::kGroup>(vt, lane)) {
+      rows.add_not_finite(seen, tl, vt);
+      make_finite<T, kDN / TL::kGroup>(vt, lane);
     }
-    rows.values(vt + vofs0, vt + vofs1);
+    rows.values(tl, vt);
   }
   rows.l += swap_halves(rows.l);
 

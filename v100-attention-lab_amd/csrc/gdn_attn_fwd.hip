@@ -37,7 +37,7 @@ __global__ __launch_bounds__(kNT, 2) void fwd_kernel(const FArgs a) {
   using O = Ops<T>;
   using Vec = typename O::Vec;
   using TL = Tile<D>;
-  constexpr uint32_t kTile = kBN * TL::kRowBytes;     // K0 V0 K1 V1
+  constexpr uint32_t kTile = TL::bytes(kBN);     // K0 V0 K1 V1
   __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * kTile];
   // unit = (batch, head); neighbouring units share key heads, and workgroups
   // blockIdx.x % 8 run on one XCD: give each XCD a run of units.  Later blocks
@@ -78,7 +78,7 @@ __global__ __launch_bounds__(kNT, 2) void fwd_kernel(const FArgs a) {
   Rows<T, D, kBN / 32> rows;
   const Copier<D, kBN, kNT> ck(kb, a.ks[1], sq.nk), cv(vb, a.vs[1], sq.nk);
   const uint32_t base = lds_addr(lds);
-  const uint32_t kofs = TL::row_ofs(lane), vofs0 = TL::col_ofs(lane, 0), vofs1 = TL::col_ofs(lane, 1);
+  const TL tl(lane);
   dma_wait();     // q is here: no load but the tiles' is waited for in the loop
   if (kr.n > 0) {
     ck(base, kr.tile(0) * kBN);
@@ -100,18 +100,18 @@ __global__ __launch_bounds__(kNT, 2) void fwd_kernel(const FArgs a) {
     const bool masked = !(whole && all_visible(j0, j1, wp0, wp1, a.window, a.sinks));
     const Mask seen(p, j0, half, sq.nk, a.window, a.sinks);
     // a tile on an edge of any wave's range: are all its values finite?
-    constexpr int kShare = kTile / 4096;
+    constexpr int kShare = kBN / TL::kGroup / 4;
     bool bad = false;
     if (!(whole && all_visible(j0, j1, p0, p1, a.window, a.sinks)))
-      bad = __syncthreads_or(not_finite<T, kShare>(vt + wv * kShare * 1024, lane));
-    if (active) rows.scores(qf, kt + kofs, masked, seen, a.scale_log2);
+      bad = __syncthreads_or(not_finite<T, kShare>(vt + wv * kShare * TL::kGroupBytes, lane));
+    if (active) rows.scores(qf, tl, kt, masked, seen, a.scale_log2);
     if (bad) {
-      if (active) rows.add_not_finite(seen, vt + vofs0, vt + vofs1);
+      if (active) rows.add_not_finite(seen, tl, vt);
       __syncthreads();
-      make_finite<T, kShare>(vt + wv * kShare * 1024, lane);
+      make_finite<T, kShare>(vt + wv * kShare * TL::kGroupBytes, lane);
       __syncthreads();
     }
-    if (active) rows.values(vt + vofs0, vt + vofs1);
+    if (active) rows.values(tl, vt);
   }
 
   const float l = rows.l + swap_halves(rows.l);

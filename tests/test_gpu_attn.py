@@ -408,3 +408,13 @@ def test_stream_graph_and_repeat(pkg, cuda):
         torch.cuda.synchronize()
         assert torch.equal(og, pkg.window_attn_decode(q[:, :1], k, v, lens, 200, 4))
         assert torch.equal(ag, pkg.window_attn(q, k, v, 100, 4))
+
+
+@pytest.mark.parametrize("D,dtype", [(64, torch.float16), (128, torch.bfloat16)])
+def test_many_key_blocks(pkg, cuda, D, dtype):
+    """Enough key blocks for workgroups of 4 waves (the smaller tests have the
+    blocks shared by several)."""
+    q, k, v, do = _inputs(cuda, 8, 700, 700, 12, 12, D, dtype, seed=21)
+    _check(pkg, q, k, v, do, 130, 3)
+    q, k, v, do = _inputs(cuda, 1, 5000, 5000, 16, 16, D, dtype, seed=22)
+    _check(pkg, q, k, v, do, 200, 20, lens=[1999, 0, 1, 3000])

@@ -26,8 +26,7 @@ namespace gdn {
 namespace attn {
 
 constexpr int kKB = 128;       // key rows a workgroup (kv)
-constexpr int kQT = 64;        // query rows a tile (kv)
-constexpr int kKVT = 512;      // threads (kv)
+constexpr int kSegRows = 64;   // rows of segments come in multiples of it
 constexpr int kQB = 128;       // query rows a workgroup (q)
 constexpr int kKT = 64;        // keys a tile (q)
 constexpr int kVParts = 64;    // partial maxima of |v| a head
@@ -52,6 +51,8 @@ struct BArgs {
   int Hq, Hk, G, B;
   int units_q, units_k;         // (batch and) heads of the q and kv grids
   int slots_q, slots_k;         // blocks of each
+  int kv_halves;                // waves of a workgroup / 4 (kv)
+  int splits;                   // workgroups a key block
   int sink_blocks, seg, slots_s;  // blocks of the first keys, rows a segment, segment slots
   int window, sinks;
   float scale, scale_log2;
@@ -179,27 +180,36 @@ __device__ __forceinline__ QRange seg_rows(const BArgs& a, const Seq& s, int k0,
   return q;
 }
 
+// Place of the part of a key block's own rows: with splits one for each slot
+// and split, else one for each block of first keys of each sequence.
+__device__ __forceinline__ int64_t own_part(const BArgs& a, int unit, int si, int block, int slot, int split) {
+  const int64_t first = (int64_t)a.units_k * a.sink_blocks * a.slots_s;
+  if (a.splits > 1) return first + ((int64_t)unit * a.slots_k + slot) * a.splits + split;
+  return first + ((int64_t)unit * (a.seq.cu == nullptr ? 1 : a.seq.N) + (a.seq.cu == nullptr ? 0 : si)) * a.sink_blocks + block;
+}
+
 // 4 bytes per lane from global memory to LDS at `at` + 4 * lane.
 __device__ __forceinline__ void dma4(const void* src, uint32_t at) {
   at = __builtin_amdgcn_readfirstlane(at);
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(at) : "memory");
 }
 
-template <typename T, int D>
-__global__ __launch_bounds__(kKVT, 2) void kv_kernel(const BArgs a) {
+template <typename T, int D, int QH>
+__global__ __launch_bounds__(256 * QH, D == 64 && QH == 1 ? 3 : 2) void kv_kernel(const BArgs a) {
+  constexpr int kQT = 32 * QH, kKVT = 256 * QH;     // query rows a tile, threads
   using O = Ops<T>;
   using Vec = typename O::Vec;
   using TL = Tile<D>;
-  constexpr uint32_t kTile = TL::bytes(kQT), kBuf = 2 * kTile + 1024;    // Q, dO, 64 x lse, D, max
+  constexpr uint32_t kTile = TL::bytes(kQT), kBuf = 2 * kTile + 1024;    // Q, dO, lse, D, max
   constexpr uint32_t kV = 2 * kBuf;                                           // the block's v rows
   __shared__ __attribute__((aligned(1024))) uint8_t lds[kV + TL::bytes(kKB)];
   const int unit_ix = blockIdx.x % a.units_k;
   const int unit = a.units_k % 8 == 0 ? (unit_ix % 8) * (a.units_k / 8) + unit_ix / 8 : unit_ix;
   // the segments last: they are short and fill the places of the blocks at the
   // sequences' ends
-  const int at_item = blockIdx.x / a.units_k;
-  const bool extra = at_item >= a.slots_k;
-  const int item = extra ? at_item - a.slots_k : at_item;
+  const int at_item = blockIdx.x / a.units_k, own_items = a.slots_k * a.splits;
+  const bool extra = at_item >= own_items;
+  const int item = extra ? at_item - own_items : at_item / a.splits, split = extra ? 0 : at_item % a.splits;
   int si, hk, block, seg = 0;
   if (a.seq.cu == nullptr) {
     si = unit / a.Hk;
@@ -227,7 +237,10 @@ __global__ __launch_bounds__(kKVT, 2) void kv_kernel(const BArgs a) {
   const int j0 = k0 + kg * 32, j1 = min(j0 + 32, sq.nk) - 1;
   const uint32_t base = lds_addr(lds);
 
-  const int nt = (max(rg.r1 - rg.r0, 0) + kQT - 1) / kQT, n = nt * a.G;
+  // the tiles of all heads in a row, of which this workgroup takes its share
+  const int nt = (max(rg.r1 - rg.r0, 0) + kQT - 1) / kQT, all = nt * a.G;
+  const int n0 = extra ? 0 : (int)((int64_t)all * split / a.splits);
+  const int n = extra ? all : (int)((int64_t)all * (split + 1) / a.splits) - n0;
   Vec kf[D / 16];
   {
     const uint16_t* kr = a.k + sq.b * a.ks[0] + (sq.k0 + min(key, sq.nk - 1)) * a.ks[1] + hk * a.ks[2];
@@ -245,7 +258,8 @@ __global__ __launch_bounds__(kKVT, 2) void kv_kernel(const BArgs a) {
   const TL tl(lane);
   const uint32_t vt = base + kV + TL::bytes(32) * kg;
   // the tile that is brought next: its rows and head
-  int fr0 = rg.r0, fh = hk * a.G;
+  int fr0 = rg.r0 + (n > 0 ? n0 % nt : 0) * kQT;
+  const int fh = hk * a.G + (n > 0 ? n0 / nt : 0);
   Copier<D, kQT, kKVT> cq(a.q + sq.b * a.qs[0] + sq.q0 * a.qs[1] + fh * a.qs[2], a.qs[1], sq.nq);
   Copier<D, kQT, kKVT> cd(a.dO + sq.b * a.dos[0] + sq.q0 * a.dos[1] + fh * a.dos[2], a.dos[1], sq.nq);
   int64_t frow = (int64_t)fh * a.rows + (int64_t)sq.b * a.seq.Tq + sq.q0;
@@ -253,6 +267,7 @@ __global__ __launch_bounds__(kKVT, 2) void kv_kernel(const BArgs a) {
     cq(at, fr0);
     cd(at + kTile, fr0);
     const int64_t row = frow + min(fr0 + lane, sq.nq - 1);
+    // (rows past the tile's are not read)
     if (wv < 2) dma4(a.stat + row * 2 + wv, at + 2 * kTile + 256 * wv);
     if constexpr (kScaled<T>)
       if (wv == 2) dma4(a.rmax + row, at + 2 * kTile + 512);
@@ -268,8 +283,8 @@ __global__ __launch_bounds__(kKVT, 2) void kv_kernel(const BArgs a) {
   // two waves share a SIMD: with one of them ahead, its exponentials run beside
   // the other's products
   if (qh == 1) __builtin_amdgcn_s_setprio(1);
+  int t0 = fr0;                                   // the tile's first row
   if (n > 0) fetch(base);
-  int t0 = rg.r0;                                 // the tile's first row
   for (int it = 0; it < n; ++it) {
     dma_wait();
     __syncthreads();
@@ -280,7 +295,7 @@ __global__ __launch_bounds__(kKVT, 2) void kv_kernel(const BArgs a) {
     const bool active = nr > 0 && !none_visible(j0, j1, p0, p1, a.window, a.sinks);
     const bool masked = !(nr == 32 && j0 + 32 <= sq.nk && all_visible(j0, j1, p0, p1, a.window, a.sinks));
     // a tile on an edge of any wave's range: are all its rows finite?
-    constexpr int kShare = 2 * kQT / TL::kGroup / 8;
+    constexpr int kShare = 2 * kQT / TL::kGroup / (4 * QH);
     bool bad = false;
     if (!(t0 + kQT <= rg.r1 && k0 + kKB <= sq.nk &&
           all_visible(k0, k0 + kKB - 1, t0 + shift, t0 + kQT - 1 + shift, a.window, a.sinks)))
@@ -374,12 +389,18 @@ __global__ __launch_bounds__(kKVT, 2) void kv_kernel(const BArgs a) {
   // the two halves of the query rows: the second's sums pass through LDS
   typedef float f32x4v __attribute__((ext_vector_type(4)));
   typedef __attribute__((address_space(3))) f32x4v lds_f32x4;
-  static_assert(4 * 32 * D * 4 <= sizeof(lds), "a half's sums fit");
+  static_assert(QH == 1 || 4 * 32 * D * 4 <= sizeof(lds), "a half's sums fit");
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      dk[i][r] *= fk;
+      dv[i][r] *= fv;
+    }
   const uint32_t mine = base + (kg * 64 + lane) * 16;
 #pragma unroll
-  for (int w = 0; w < 2; ++w) {
+  for (int w = 0; w < 2 * (QH - 1); ++w) {
     f32x16(&x)[D / 32] = w == 0 ? dk : dv;
-    const float f = w == 0 ? fk : fv;
     dma_wait();
     __syncthreads();
     if (qh == 1) {
@@ -388,7 +409,7 @@ __global__ __launch_bounds__(kKVT, 2) void kv_kernel(const BArgs a) {
 #pragma unroll
         for (int c = 0; c < 4; ++c)
           *(lds_f32x4*)(mine + (4 * i + c) * 4096) =
-              f32x4v{x[i][4 * c] * f, x[i][4 * c + 1] * f, x[i][4 * c + 2] * f, x[i][4 * c + 3] * f};
+              f32x4v{x[i][4 * c], x[i][4 * c + 1], x[i][4 * c + 2], x[i][4 * c + 3]};
     }
     __syncthreads();
     if (qh == 0) {
@@ -398,20 +419,16 @@ __global__ __launch_bounds__(kKVT, 2) void kv_kernel(const BArgs a) {
         for (int c = 0; c < 4; ++c) {
           const f32x4v y = *(lds_f32x4*)(mine + (4 * i + c) * 4096);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[i][4 * c + e] = __builtin_fmaf(x[i][4 * c + e], f, y[e]);
+          for (int e = 0; e < 4; ++e) x[i][4 * c + e] += y[e];
         }
     }
   }
   if (qh == 1) return;
-  if (block < a.sink_blocks) {
-    // fp32 parts: the block's own rows (dense: before the segments' parts;
-    // packed: one for each sequence, behind all of those), then the segments
+  if (block < a.sink_blocks || a.splits > 1) {
+    // fp32 parts: of segments and, behind them, of the blocks' own rows
     if (extra && j0 >= a.sinks) return;
-    const int64_t slots = a.slots_s + (a.seq.cu == nullptr ? 1 : 0);
-    const int64_t u = a.seq.cu == nullptr ? unit : hk;
-    const int64_t ub = u * a.sink_blocks + block;
-    const int64_t at = extra ? ub * slots + item / a.sink_blocks + (a.seq.cu == nullptr ? 1 : 0)
-                             : (a.seq.cu == nullptr ? ub * slots : (int64_t)a.units_k * a.sink_blocks * slots + ub * a.seq.N + si);
+    const int64_t at = extra ? ((int64_t)unit * a.sink_blocks + block) * a.slots_s + item / a.sink_blocks
+                             : own_part(a, unit, si, block, item, split);
     float* pk = a.part + at * (2 * kKB * D) + (kg * 32 + l32) * D;
     float* pv = pk + kKB * D;
 #pragma unroll
@@ -429,38 +446,54 @@ __global__ __launch_bounds__(kKVT, 2) void kv_kernel(const BArgs a) {
   store_rows<T, D>(a.dv + sq.b * a.dvs[0] + (sq.k0 + key) * a.dvs[1] + hk * a.dvs[2], dv, 1.f, half);
 }
 
-// Sums of the parts of a block of first keys: a workgroup a block, sequence
-// and 8 key rows.
+// Sums of the parts of a key block, in order: a workgroup a block and 8 rows.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void sink_sum_kernel(const BArgs a) {
+__global__ __launch_bounds__(256) void part_sum_kernel(const BArgs a, int blocks) {
   constexpr int kRowsWg = 8;
   const int rg = blockIdx.x % (kKB / kRowsWg), rest = blockIdx.x / (kKB / kRowsWg);
-  const int block = rest % a.sink_blocks, us = rest / a.sink_blocks;   // us: unit (dense) or (head, sequence)
-  const int si = a.seq.cu == nullptr ? us / a.Hk : us % a.seq.N;
-  const int hk = a.seq.cu == nullptr ? us % a.Hk : us / a.seq.N;
-  const int64_t u = a.seq.cu == nullptr ? us : hk;
+  const int e = rest % blocks, unit = rest / blocks;
+  int si, hk, block, slot = 0;
+  if (a.seq.cu == nullptr) {
+    si = unit / a.Hk;
+    hk = unit % a.Hk;
+    block = slot = e;
+  } else {
+    hk = unit;
+    if (a.splits > 1) {
+      slot = e;
+      si = find_block(a.seq, slot, kKB, 0, block);
+    } else {
+      si = e / a.sink_blocks;
+      block = e % a.sink_blocks;
+    }
+  }
   const Seq sq = get_seq(a.seq, si);
   const int k0 = block * kKB;
-  if (k0 >= sq.nk) return;
-  const int64_t slots = a.slots_s + (a.seq.cu == nullptr ? 1 : 0), one = 2 * kKB * D, ub = u * a.sink_blocks + block;
-  const float* parts = a.part + ub * slots * one;
-  const float* own = a.seq.cu == nullptr ? parts : a.part + ((int64_t)a.units_k * a.sink_blocks * slots + ub * a.seq.N + si) * one;
-  const int first = a.seq.cu == nullptr ? 1 : (int)(sq.q0 / a.seg) + si;
-  const int nseg = (sq.nq + a.seg - 1) / a.seg;
+  if (block < 0 || k0 >= sq.nk) return;
+  const int64_t one = 2 * kKB * D;
+  const float* own = a.part + own_part(a, unit, si, block, slot, 0) * one;
+  const int first = a.seq.cu == nullptr || a.seg == 0 ? 0 : (int)(sq.q0 / a.seg) + si;
+  const int nseg = block < a.sink_blocks ? (sq.nq + a.seg - 1) / a.seg : 0;
+  const float* segs = a.part + (((int64_t)unit * a.sink_blocks + block) * a.slots_s + first) * one;
   for (int e = threadIdx.x; e < kRowsWg * D / 4; e += 256) {
     const int r = rg * kRowsWg + e / (D / 4), d = 4 * (e % (D / 4)), key = k0 + r;
     if (key >= sq.nk) continue;
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
-      float4 s = *reinterpret_cast<const float4*>(own + (w * kKB + r) * D + d);
-      for (int g = 0; g < nseg && key < a.sinks; ++g) {
-        const QRange q = seg_rows(a, sq, k0, g);
-        if (q.r1 <= q.r0) continue;
-        const float4 x = *reinterpret_cast<const float4*>(parts + (first + g) * one + (w * kKB + r) * D + d);
+      const int64_t at = (w * kKB + r) * D + d;
+      float4 s = *reinterpret_cast<const float4*>(own + at);
+      auto add = [&](const float* p) {
+        const float4 x = *reinterpret_cast<const float4*>(p + at);
         s.x += x.x;
         s.y += x.y;
         s.z += x.z;
         s.w += x.w;
+      };
+#pragma unroll 4
+      for (int g = 1; g < a.splits; ++g) add(own + g * one);
+      for (int g = 0; g < nseg && key < a.sinks; ++g) {
+        const QRange q = seg_rows(a, sq, k0, g);
+        if (q.r1 > q.r0) add(segs + g * one);
       }
       uint16_t* out = w == 0 ? a.dk + sq.b * a.dks[0] + (sq.k0 + key) * a.dks[1] + hk * a.dks[2]
                              : a.dv + sq.b * a.dvs[0] + (sq.k0 + key) * a.dvs[1] + hk * a.dvs[2];
@@ -600,11 +633,24 @@ void sink_plan(const GdnAttnParams& P, int& blocks, int& seg, int& slots) {
   const int64_t sinks = std::min<int64_t>(P.sinks, P.Tk);
   if (sinks == 0 || P.Tq == 0 || (int64_t)P.window + kKB >= P.Tk) return;
   blocks = (int)((sinks + kKB - 1) / kKB);
-  // about 16 tiles of all heads a segment, short beside a block's own rows, and
-  // no more parts than rows of D floats for every query row, twice
-  const int64_t group = P.Hq / P.Hk;
-  seg = (int)std::max<int64_t>((16 + group - 1) / group * kQT, (int64_t)blocks * kKB);
+  // half of a block's own tiles a segment, 16 at most (of all heads together),
+  // and no more parts than rows of D floats for every query row, twice
+  const int64_t group = P.Hq / P.Hk, own = ((int64_t)P.window + kKB) / kSegRows;
+  const int64_t tiles = std::max<int64_t>(1, std::min<int64_t>(16 / group, own / 2));
+  seg = (int)std::max<int64_t>(tiles * kSegRows, (int64_t)blocks * kKB);
   slots = P.cu_seqlens == nullptr ? (P.Tq + seg - 1) / seg : P.Tq / seg + P.N;
+}
+
+// Key blocks (slots) of a call, and the workgroups that share one: where the
+// blocks leave CUs empty, each is cut into as many as fill them, of at least 4
+// tiles of 64 rows.
+int64_t key_slots(const GdnAttnParams& P) { return P.cu_seqlens == nullptr ? (P.Tk + kKB - 1) / kKB : P.Tk / kKB + P.N; }
+int64_t key_units(const GdnAttnParams& P) { return P.cu_seqlens == nullptr ? (int64_t)P.B * P.Hk : P.Hk; }
+int key_splits(const GdnAttnParams& P) {
+  const int64_t blocks = std::max<int64_t>(1, key_units(P) * key_slots(P));
+  const int64_t rows = std::min<int64_t>((int64_t)P.window + kKB, P.Tq);
+  const int64_t tiles = (rows + 63) / 64 * (P.Hq / P.Hk);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(256 / blocks, tiles / 4));
 }
 
 struct Space {
@@ -619,9 +665,9 @@ Space space(const GdnAttnParams& P) {
   s.rmax = s.stat + up256(rows * P.Hq * 8);
   s.vmax = s.rmax + (P.dtype == GDN_DTYPE_F16 ? up256(rows * P.Hq * 4) : 0);
   s.part = s.vmax + (P.dtype == GDN_DTYPE_F16 ? up256((int64_t)P.B * P.Hk * kVParts * 4) : 0);
-  const int64_t units = P.cu_seqlens == nullptr ? (int64_t)P.B * P.Hk : P.Hk;
-  const int64_t n = units * blocks * (slots + (P.cu_seqlens == nullptr ? 1 : P.N));
-  s.total = s.part + up256(n * 2 * kKB * P.D * 4);
+  const int64_t units = key_units(P), splits = key_splits(P);
+  const int64_t own = splits > 1 ? key_slots(P) * splits : (int64_t)blocks * (P.cu_seqlens == nullptr ? 1 : P.N);
+  s.total = s.part + up256(units * ((int64_t)blocks * slots + own) * 2 * kKB * P.D * 4);
   return s;
 }
 
@@ -629,14 +675,19 @@ template <typename T, int D>
 int launch(const BArgs& a, hipStream_t s) {
   const int64_t rb = (a.rows * a.Hq + 256 / (D / 8) - 1) / (256 / (D / 8));
   const int64_t vb = kScaled<T> ? (int64_t)a.B * a.Hk * kVParts : 0;
-  const int64_t kvb = (int64_t)a.units_k * (a.slots_k + (int64_t)a.sink_blocks * a.slots_s);
+  const int64_t kvb = (int64_t)a.units_k * ((int64_t)a.slots_k * a.splits + (int64_t)a.sink_blocks * a.slots_s);
   const int64_t qb = (int64_t)a.units_q * a.slots_q;
   if (rb + vb > 0x7fffffffLL || kvb > 0x7fffffffLL || qb > 0x7fffffffLL) return GDN_ERR_BAD_SHAPE;
   if (rb > 0) hipLaunchKernelGGL((prep_kernel<T, D>), dim3((uint32_t)(rb + vb)), dim3(256), 0, s, a, (int)rb);
-  if (kvb > 0) hipLaunchKernelGGL((kv_kernel<T, D>), dim3((uint32_t)kvb), dim3(kKVT), 0, s, a);
-  if (a.sink_blocks > 0) {
-    const int64_t us = a.seq.cu == nullptr ? a.units_k : (int64_t)a.Hk * a.seq.N;
-    hipLaunchKernelGGL((sink_sum_kernel<T, D>), dim3((uint32_t)(us * a.sink_blocks * (kKB / 8))), dim3(256), 0, s, a);
+  if (kvb > 0) {
+    if (a.kv_halves == 1) hipLaunchKernelGGL((kv_kernel<T, D, 1>), dim3((uint32_t)kvb), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((kv_kernel<T, D, 2>), dim3((uint32_t)kvb), dim3(512), 0, s, a);
+  }
+  if (a.sink_blocks > 0 || a.splits > 1) {
+    const int64_t blocks = a.splits > 1 ? a.slots_k : (int64_t)a.sink_blocks * (a.seq.cu == nullptr ? 1 : a.seq.N);
+    const int64_t pb = a.units_k * blocks * (kKB / 8);
+    if (pb > 0x7fffffffLL) return GDN_ERR_BAD_SHAPE;
+    if (pb > 0) hipLaunchKernelGGL((part_sum_kernel<T, D>), dim3((uint32_t)pb), dim3(256), 0, s, a, (int)blocks);
   }
   if (qb > 0) hipLaunchKernelGGL((q_kernel<T, D>), dim3((uint32_t)qb), dim3(256), 0, s, a);
   return (int)hipGetLastError();
@@ -705,9 +756,15 @@ int gdn_attn_bwd_launch(const GdnAttnParams* prm, void* stream) {
   a.G = P.Hq / P.Hk;
   const bool packed = P.cu_seqlens != nullptr;
   a.units_q = packed ? P.Hq : P.B * P.Hq;
-  a.units_k = packed ? P.Hk : P.B * P.Hk;
+  a.units_k = (int)key_units(P);
   a.slots_q = packed ? P.Tq / kQB + P.N : (P.Tq + kQB - 1) / kQB;
-  a.slots_k = packed ? P.Tk / kKB + P.N : (P.Tk + kKB - 1) / kKB;
+  a.slots_k = (int)key_slots(P);
+  a.splits = key_splits(P);
+  // 4 waves a workgroup, several workgroups a CU, where there are that many;
+  // else 8 waves, so that a SIMD still has two (B2 Hk4 T4096 window 1024 bf16,
+  // 256 blocks: 348 us of backward with 8 waves, 390 with 4; B4, 512 blocks:
+  // 602 and 581; 1040 blocks of D 64: 219 and 170)
+  a.kv_halves = (int64_t)a.units_k * a.slots_k >= 512 ? 1 : 2;
   sink_plan(P, a.sink_blocks, a.seg, a.slots_s);
   a.window = P.window;
   a.sinks = P.sinks;

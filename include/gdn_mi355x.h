@@ -354,7 +354,7 @@ int gdn_bwd_launch(const GdnBwdParams* params, void* stream);
  *     outputs dense.
  *   - states: fp32 [slots, D], the state at the start of every chunk of
  *     gdn_scan_chunk() rows; slots = gdn_scan_slots().  The forward writes
- *     it (nullable there: then it lies in the workspace); the backward reads
+ *     it (nullable there); the backward reads
  *     it (nullable: recomputed from x, g and h0).
  *   - workspace: gdn_scan_workspace_size() / gdn_scan_bwd_workspace_size()
  *     bytes, 256-byte aligned. */

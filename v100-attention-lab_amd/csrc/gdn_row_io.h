@@ -71,6 +71,15 @@ struct Pack {
   __device__ __forceinline__ void load(const E* p) { raw = *reinterpret_cast<const Raw*>(p); }
   __device__ __forceinline__ void store(E* p) const { *reinterpret_cast<Raw*>(p) = raw; }
   __device__ __forceinline__ void zero() { raw = Raw{}; }
+  // From here on the elements are unpacked again where they are used (the
+  // compiler would keep them unpacked, in twice the registers).
+  __device__ __forceinline__ void repack() {
+    uint32_t w[(sizeof(Raw) + 3) / 4] = {};
+    __builtin_memcpy(w, &raw, sizeof(Raw));
+#pragma unroll
+    for (auto& x : w) asm volatile("" : "+v"(x));
+    __builtin_memcpy(&raw, w, sizeof(Raw));
+  }
   __device__ __forceinline__ float get(int i) const {
     E e[V];
     __builtin_memcpy(e, &raw, sizeof(raw));

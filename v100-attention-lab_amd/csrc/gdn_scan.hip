@@ -5,18 +5,27 @@
 //
 // Rows s..t together are h_t = e^G h_{s-1} + H with G the sum of their g, so a
 // chunk of rows is one pair (G, H) per channel.  A gate near 1 enters as
-// e^g - 1 (Decay below): its rounding does not add up over the rows that a
-// state lives through.  A call of more than one chunk runs
-//   agg    the pair of every chunk (forward from x, backward from dy),
-//   carry  the state before every chunk, from the pairs of those before it,
-//   main   every chunk from its state: rows in order, so that a row's value
-//          comes from its own sequence of products and sums.
-// A workgroup is kWaves waves on one chunk and 64 V channels; wave w holds R
-// consecutive rows in registers and the waves exchange their pairs in LDS.
-// Every sum has a fixed order.
+// e^g - 1 (decay() below): its rounding does not add up over the rows that a
+// state lives through.
 //
-// Bound by memory: x, g read and y written once, and the pairs' pass reads x
-// and g once more, from the 256 MB cache where they fit.
+// A workgroup is kWaves waves on one chunk and 64 V channels; wave w holds
+// kRows consecutive rows in registers and the waves exchange their pairs in
+// LDS.  Sequences of one chunk need no more.  Else every workgroup leaves its
+// chunk's pair in the workspace, takes the pairs of the chunks before it (in
+// the backward, after it) and walks its rows from the state that they give: x,
+// g and y pass through memory once.  Every 16th workgroup also leaves the pair
+// of its 16 chunks, so that a chunk reads at most 30 pairs and one for each 16
+// chunks between.  All sums have a fixed order.
+//
+// Waiting: chunks are dealt by a counter in the order of the walk, so whatever
+// a workgroup waits for is left by workgroups that already run; each leaves its
+// own pair before it waits for any, and what it leaves later depends on earlier
+// ones alone.  A place in the workspace holds ~0 until its pair is there (one
+// 8-byte store, seen by 8-byte loads past the caches), so no other order of
+// memory is needed.  Chunk places that no sequence uses get a pair as well:
+// offsets that make no sense give no meaningful rows, but every wait ends.
+//
+// Bound by memory.
 
 #include <algorithm>
 
@@ -27,8 +36,8 @@ namespace scan {
 
 using namespace rowio;
 
-constexpr int kWaves = 16;
-constexpr int kRows = 8;                   // rows a wave
+constexpr int kWaves = 8;
+constexpr int kRows = 16;                  // rows a wave
 constexpr int kChunk = kWaves * kRows;     // rows a workgroup
 constexpr int kThreads = 64 * kWaves;
 
@@ -44,8 +53,9 @@ struct Args {
   float* fs;
   float* dh0;
   float* states;    // state before each chunk
-  float* rstates;   // backward: D after each chunk
-  float2* agg;      // pairs of the chunks
+  uint64_t* agg;    // pairs of the chunks in the order of the walk
+  uint64_t* agg16;  // pairs of 16 chunks
+  uint32_t* ticket;
   const int64_t* cu;
   int64_t xs[2], gs[2], ys[2], dys[2], dxs[2], dgs[2];
   int64_t h0s, dfs;
@@ -103,7 +113,7 @@ __device__ __forceinline__ Job slot_job(const Args& p, int slot) {
   }
   Job j = seq_job(p, seq);
   j.chunk = slot - j.first;
-  if (j.chunk * kChunk >= j.len && !(j.chunk == 0 && j.len == 0)) j.chunk = -1;
+  if (j.chunk < 0 || (j.chunk * kChunk >= j.len && !(j.chunk == 0 && j.len == 0))) j.chunk = -1;
   return j;
 }
 
@@ -130,12 +140,6 @@ __device__ __forceinline__ float step(float t, float h, float x) {
   return near1 && fabsf(base) == __builtin_inff() ? base : r;
 }
 
-// Exchange of the waves' pairs: decay(G) and H.
-template <int V>
-struct Exchange {
-  float t[kWaves][64 * V], h[kWaves][64 * V];
-};
-
 template <typename TX, typename TG, int V>
 __device__ __forceinline__ void load_rows(const TX* x, const TG* g, int64_t xs, int64_t gs, int n, bool ok,
                                           Pack<TX, V> (&xr)[kRows], Pack<TG, V> (&gr)[kRows]) {
@@ -150,135 +154,180 @@ __device__ __forceinline__ void load_rows(const TX* x, const TG* g, int64_t xs, 
   }
 }
 
-// The pair of every chunk.  REV: rows from the last to the first, D <- e^g (v + D).
-template <typename TX, typename TG, int V, bool REV>
-__global__ __launch_bounds__(kThreads) void agg_kernel(const Args p) {
-  const uint32_t slot = blockIdx.x / p.nblk, blk = blockIdx.x % p.nblk;
-  const Job j = slot_job(p, (int)slot);
-  if (j.chunk < 0 || j.len == 0) return;
+// ---------------------------------------------------------------------------
+// pairs in the workspace
+// ---------------------------------------------------------------------------
+
+constexpr uint64_t kAbsent = ~(uint64_t)0;
+constexpr int kSet = 16;                   // chunks whose pairs are joined to one
+
+__device__ __forceinline__ void leave_pair(uint64_t* at, float g, float h) {
+  uint64_t v = ((uint64_t)__float_as_uint(h) << 32) | __float_as_uint(g);
+  if (v == kAbsent) v = 0x7fc000007fc00000ull;   // a NaN of other bits
+  __hip_atomic_store(at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ uint64_t look(const uint64_t* at) {
+  return __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float pair_g(uint64_t v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float pair_h(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
+
+// Every place of n pairs absent, and the counter at zero.
+__global__ __launch_bounds__(256) void clear_kernel(uint64_t* agg, int64_t n, uint32_t* ticket) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i == 0) *ticket = 0;
+  for (int64_t k = i; k < n / 2; k += (int64_t)gridDim.x * 256)
+    reinterpret_cast<ulonglong2*>(agg)[k] = make_ulonglong2(kAbsent, kAbsent);
+}
+
+// Chunk of a workgroup and its place u in the order of the walk (REV: from the
+// last chunk to the first).
+template <bool REV>
+__device__ __forceinline__ uint32_t next_place(const Args& p, bool single, uint32_t& blk) {
+  uint32_t at = blockIdx.x;
+  if (!single) {
+    __shared__ uint32_t sh;
+    if (threadIdx.x == 0) sh = atomicAdd(p.ticket, 1u);
+    __syncthreads();
+    at = sh;
+  }
+  blk = at % p.nblk;
+  return at / p.nblk;
+}
+
+// Scratch of the joins below.
+template <int V>
+struct Join {
+  float g[kWaves][64 * V], h[kWaves][64 * V];
+};
+
+// Leaves the chunk's pair (from the waves' pairs in sh, in the order of the
+// walk) and, at the end of a set, the set's.  u: the chunk's place.
+template <int V, bool REV>
+__device__ __forceinline__ void leave(const Args& p, const Join<V>& sh, uint32_t u, int c0) {
+  const int ch = threadIdx.x, c = c0 + ch;
+  if (ch >= 64 * V || c >= p.D) return;
+  float g = 0.f, h = 0.f;
+#pragma unroll
+  for (int s = 0; s < kWaves; ++s) {
+    const int i = REV ? kWaves - 1 - s : s;
+    h = step(decay(sh.g[i][ch]), h, sh.h[i][ch]);
+    g += sh.g[i][ch];
+  }
+  leave_pair(p.agg + (int64_t)u * p.D + c, g, h);
+  if (u % kSet != kSet - 1) return;
+  const uint64_t* first = p.agg + (int64_t)(u - (kSet - 1)) * p.D + c;
+  constexpr int kBatch = 5;
+  static_assert((kSet - 1) % kBatch == 0, "whole batches");
+  float gs = 0.f, hs = 0.f;
+#pragma unroll 1
+  for (int k = 0; k < kSet - 1; k += kBatch) {
+    uint64_t v[kBatch];
+    bool all;
+    do {
+      all = true;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) v[i] = look(first + (int64_t)(k + i) * p.D);
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) all &= v[i] != kAbsent;
+    } while (!all);
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      hs = step(decay(pair_g(v[i])), hs, pair_h(v[i]));
+      gs += pair_g(v[i]);
+    }
+  }
+  leave_pair(p.agg16 + (int64_t)(u / kSet) * p.D + c, gs + g, step(decay(g), hs, h));
+}
+
+// The state h (of this lane's V channels) behind the places first .. u - 1, in
+// order: single places up to a set's start, whole sets, single places again.
+// Each wave takes a share of these pairs; the shares are joined in LDS.
+template <int V>
+__device__ __forceinline__ void carry(const Args& p, Join<V>& sh, uint32_t first, uint32_t u, int c, bool ok,
+                                      float (&h)[V]) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int c = (int)blk * 64 * V + lane * V;
-  const bool ok = c < p.D;
-  const int r0 = j.chunk * kChunk + w * kRows;
-  const int n = min(max(j.len - r0, 0), kRows);
-  const int64_t* vs = REV ? p.dys : p.xs;
-  const TX* v = static_cast<const TX*>(REV ? p.dy : p.x) + j.b * vs[0] + (j.row + r0) * vs[1] + c;
-  const TG* g = static_cast<const TG*>(p.g) + j.b * p.gs[0] + (j.row + r0) * p.gs[1] + c;
-  Pack<TX, V> vr[kRows];
-  Pack<TG, V> gr[kRows];
-  load_rows<TX, TG, V>(v, g, vs[1], p.gs[1], n, ok, vr, gr);
+  const int up = (int)(first + kSet - 1) / kSet * kSet;       // the first whole set's start
+  const int head = min((int)u, up) - (int)first;
+  const int sets = max((int)u / kSet - up / kSet, 0);
+  const int tail = max((int)u - max((int)u / kSet * kSet, up), 0);
+  const int n = max(head, 0) + sets + tail;
+  const int share = (n + kWaves - 1) / kWaves, k0 = min(w * share, n), k1 = min(k0 + share, n);
+  auto at = [&](int k) -> const uint64_t* {
+    if (k < head) return p.agg + ((int64_t)first + k) * p.D + c;
+    if (k < head + sets) return p.agg16 + ((int64_t)(up / kSet) + (k - head)) * p.D + c;
+    return p.agg + ((int64_t)(u - tail) + (k - head - sets)) * p.D + c;
+  };
   float G[V], H[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) G[e] = H[e] = 0.f;
+  if (ok) {
+    constexpr int kBatch = 4;
+#pragma unroll 1
+    for (int k = k0; k < k1; k += kBatch) {
+      uint64_t v[kBatch][V];
+      bool all;
+      do {
+        all = true;
 #pragma unroll
-  for (int s = 0; s < kRows; ++s) {
-    const int i = REV ? kRows - 1 - s : s;
-    if (i < n) {
+        for (int i = 0; i < kBatch; ++i) {
+          const uint64_t* a = at(min(k + i, k1 - 1));
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float gv = gr[i].get(e), t = decay(gv);
-        H[e] = REV ? step(t, vr[i].get(e) + H[e], 0.f) : step(t, H[e], vr[i].get(e));
-        G[e] += gv;
+          for (int e = 0; e < V; ++e) v[i][e] = look(a + e);
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+#pragma unroll
+          for (int e = 0; e < V; ++e) all &= v[i][e] != kAbsent;
+      } while (!all);
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        if (k + i < k1) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            H[e] = step(decay(pair_g(v[i][e])), H[e], pair_h(v[i][e]));
+            G[e] += pair_g(v[i][e]);
+          }
+        }
       }
     }
   }
-  __shared__ float sh_g[kWaves][64 * V], sh_h[kWaves][64 * V];
 #pragma unroll
   for (int e = 0; e < V; ++e) {
-    sh_g[w][lane * V + e] = G[e];
-    sh_h[w][lane * V + e] = H[e];
+    sh.g[w][lane * V + e] = G[e];
+    sh.h[w][lane * V + e] = H[e];
   }
   __syncthreads();
-  const int ch = threadIdx.x;
-  if (ch < 64 * V && (int)blk * 64 * V + ch < p.D) {
-    float gs = 0.f, h = 0.f;
+  for (int i = 0; i < kWaves && i * share < n; ++i) {
 #pragma unroll
-    for (int s = 0; s < kWaves; ++s) {
-      const int i = REV ? kWaves - 1 - s : s;
-      h = step(decay(sh_g[i][ch]), h, sh_h[i][ch]);
-      gs += sh_g[i][ch];
-    }
-    p.agg[(int64_t)slot * p.D + (int)blk * 64 * V + ch] = make_float2(gs, h);
+    for (int e = 0; e < V; ++e) h[e] = step(decay(sh.g[i][lane * V + e]), h[e], sh.h[i][lane * V + e]);
   }
 }
 
-// The state before every chunk of a sequence (REV: D after every chunk): wave
-// w folds the pairs of its share of the chunks, the shares are joined in LDS,
-// then every wave walks its share again.
-template <bool REV>
-__global__ __launch_bounds__(kThreads) void carry_kernel(const Args p) {
-  const int nb = (p.D + 63) / 64;
-  const int seq = blockIdx.x / nb, blk = blockIdx.x % nb;
-  const Job j = seq_job(p, seq);
-  const int n = (j.len + kChunk - 1) / kChunk;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int c = blk * 64 + lane;
-  const bool ok = c < p.D;
-  const int share = (n + kWaves - 1) / kWaves;
-  const int k0 = min(w * share, n), k1 = min(k0 + share, n);
-  // chunk of step k, in the order of the walk
-  auto at = [&](int k) -> int64_t { return (int64_t)(j.first + (REV ? n - 1 - k : k)) * p.D + c; };
-  float G = 0.f, H = 0.f;
-  if (ok) {
-#pragma unroll 8
-    for (int k = k0; k < k1; ++k) {
-      const float2 t = p.agg[at(k)];
-      H = step(decay(t.x), H, t.y);
-      G += t.x;
-    }
-  }
-  __shared__ Exchange<1> sh;
-  sh.t[w][lane] = decay(G);
-  sh.h[w][lane] = H;
-  __syncthreads();
-  if (!ok) return;
-  const float* init = REV ? p.dfinal : p.h0;
-  const int64_t is = REV ? p.dfs : p.h0s;
-  float h = init != nullptr ? init[seq * is + c] : 0.f;
-  for (int i = 0; i < w; ++i) h = step(sh.t[i][lane], h, sh.h[i][lane]);
-  float* out = REV ? p.rstates : p.states;
-#pragma unroll 8
-  for (int k = k0; k < k1; ++k) {
-    const float2 t = p.agg[at(k)];
-    out[at(k)] = h;
-    h = step(decay(t.x), h, t.y);
-  }
-}
+// ---------------------------------------------------------------------------
+// forward
+// ---------------------------------------------------------------------------
 
-// y and the final state of every chunk; the state before it from `states`,
-// or h0 where every sequence is one chunk (single).
-template <typename TX, typename TG, int V>
-__global__ __launch_bounds__(kThreads) void main_kernel(const Args p, bool single) {
-  const uint32_t slot = blockIdx.x / p.nblk, blk = blockIdx.x % p.nblk;
+// y, the final states and (not nullptr) the states at the chunks' starts.
+// ONLY_STATES: those alone.  single: every sequence is one chunk.
+template <typename TX, typename TG, int V, bool ONLY_STATES>
+__global__ __launch_bounds__(kThreads, 4) void fwd_kernel(const Args p, bool single) {
+  uint32_t blk;
+  const uint32_t slot = next_place<false>(p, single, blk);
   const Job j = slot_job(p, (int)slot);
-  if (j.chunk < 0) return;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int c = (int)blk * 64 * V + lane * V;
   const bool ok = c < p.D;
-  const int r0 = j.chunk * kChunk + w * kRows;
-  const int n = min(max(j.len - r0, 0), kRows);
+  const int r0 = max(j.chunk, 0) * kChunk + w * kRows;
+  const int n = j.chunk < 0 ? 0 : min(max(j.len - r0, 0), kRows);
   const TX* x = static_cast<const TX*>(p.x) + j.b * p.xs[0] + (j.row + r0) * p.xs[1] + c;
   const TG* g = static_cast<const TG*>(p.g) + j.b * p.gs[0] + (j.row + r0) * p.gs[1] + c;
-  TX* y = static_cast<TX*>(p.y) + j.b * p.ys[0] + (j.row + r0) * p.ys[1] + c;
   Pack<TX, V> xr[kRows];
   Pack<TG, V> gr[kRows];
   load_rows<TX, TG, V>(x, g, p.xs[1], p.gs[1], n, ok, xr, gr);
   float h[V];
 #pragma unroll
-  for (int e = 0; e < V; ++e) h[e] = 0.f;
-  if (ok) {
-    if (!single && j.len > 0) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) h[e] = p.states[(int64_t)slot * p.D + c + e];
-    } else if (p.h0 != nullptr) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) h[e] = p.h0[j.seq * p.h0s + c + e];
-    }
-    if (single && p.states != nullptr && w == 0) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) p.states[(int64_t)slot * p.D + c + e] = h[e];
-    }
-  }
+  for (int e = 0; e < V; ++e) h[e] = ok && p.h0 != nullptr ? p.h0[j.seq * p.h0s + c + e] : 0.f;
   float a[kRows][V], G[V], H[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) G[e] = H[e] = 0.f;
@@ -292,17 +341,30 @@ __global__ __launch_bounds__(kThreads) void main_kernel(const Args p, bool singl
       G[e] += gr[i].get(e);
     }
   }
-  __shared__ Exchange<V> sh;
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) xr[i].repack();
+  __shared__ Join<V> waves, shares;
 #pragma unroll
   for (int e = 0; e < V; ++e) {
-    sh.t[w][lane * V + e] = decay(G[e]);
-    sh.h[w][lane * V + e] = H[e];
+    waves.g[w][lane * V + e] = G[e];
+    waves.h[w][lane * V + e] = H[e];
   }
   __syncthreads();
-  if (!ok) return;
+  if (!single) {
+    leave<V, false>(p, waves, slot, (int)blk * 64 * V);
+    if (j.chunk < 0) return;
+    carry<V>(p, shares, (uint32_t)j.first, slot, c, ok, h);
+  }
+  if (j.chunk < 0 || !ok) return;
+  if (p.states != nullptr && w == 0) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) p.states[(int64_t)slot * p.D + c + e] = h[e];
+  }
+  if constexpr (ONLY_STATES) return;
+  TX* y = static_cast<TX*>(p.y) + j.b * p.ys[0] + (j.row + r0) * p.ys[1] + c;
   for (int i = 0; i < w; ++i) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) h[e] = step(sh.t[i][lane * V + e], h[e], sh.h[i][lane * V + e]);
+    for (int e = 0; e < V; ++e) h[e] = step(decay(waves.g[i][lane * V + e]), h[e], waves.h[i][lane * V + e]);
   }
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
@@ -321,24 +383,25 @@ __global__ __launch_bounds__(kThreads) void main_kernel(const Args p, bool singl
   }
 }
 
-// dx, dg of every chunk and dh0; the state before it from `states`, D after
-// it from `rstates`, or h0 and dfinal where every sequence is one chunk.
+// ---------------------------------------------------------------------------
+// backward
+// ---------------------------------------------------------------------------
+
+// dx, dg and dh0, the states at the chunks' starts from `states` (single: h0).
 template <typename TX, typename TG, int V>
-__global__ __launch_bounds__(kThreads) void bwd_kernel(const Args p, bool single) {
-  const uint32_t slot = blockIdx.x / p.nblk, blk = blockIdx.x % p.nblk;
+__global__ __launch_bounds__(kThreads, 4) void bwd_kernel(const Args p, bool single) {
+  uint32_t blk;
+  const uint32_t u = next_place<true>(p, single, blk), slot = p.slots - 1 - u;
   const Job j = slot_job(p, (int)slot);
-  if (j.chunk < 0) return;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int c = (int)blk * 64 * V + lane * V;
   const bool ok = c < p.D;
-  const int r0 = j.chunk * kChunk + w * kRows;
-  const int n = min(max(j.len - r0, 0), kRows);
+  const int r0 = max(j.chunk, 0) * kChunk + w * kRows;
+  const int n = j.chunk < 0 ? 0 : min(max(j.len - r0, 0), kRows);
   const int64_t row = j.row + r0;
   const TX* x = static_cast<const TX*>(p.x) + j.b * p.xs[0] + row * p.xs[1] + c;
   const TG* g = static_cast<const TG*>(p.g) + j.b * p.gs[0] + row * p.gs[1] + c;
   const TX* dy = static_cast<const TX*>(p.dy) + j.b * p.dys[0] + row * p.dys[1] + c;
-  TX* dx = static_cast<TX*>(p.dx) + j.b * p.dxs[0] + row * p.dxs[1] + c;
-  TG* dg = static_cast<TG*>(p.dg) + j.b * p.dgs[0] + row * p.dgs[1] + c;
   Pack<TX, V> xr[kRows], dr[kRows];
   Pack<TG, V> gr[kRows];
   load_rows<TX, TG, V>(x, g, p.xs[1], p.gs[1], n, ok, xr, gr);
@@ -349,22 +412,13 @@ __global__ __launch_bounds__(kThreads) void bwd_kernel(const Args p, bool single
   }
   float h[V], d[V];
 #pragma unroll
-  for (int e = 0; e < V; ++e) h[e] = d[e] = 0.f;
-  if (ok) {
-    const bool many = !single && j.len > 0;
-    if (many) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        h[e] = p.states[(int64_t)slot * p.D + c + e];
-        d[e] = p.rstates[(int64_t)slot * p.D + c + e];
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        if (p.h0 != nullptr) h[e] = p.h0[j.seq * p.h0s + c + e];
-        if (p.dfinal != nullptr) d[e] = p.dfinal[j.seq * p.dfs + c + e];
-      }
+  for (int e = 0; e < V; ++e) {
+    h[e] = 0.f;
+    if (ok && j.chunk >= 0) {
+      if (!single && j.len > 0) h[e] = p.states[(int64_t)slot * p.D + c + e];
+      else if (p.h0 != nullptr) h[e] = p.h0[j.seq * p.h0s + c + e];
     }
+    d[e] = ok && p.dfinal != nullptr ? p.dfinal[j.seq * p.dfs + c + e] : 0.f;
   }
   float a[kRows][V], G[V], H[V], R[V];
 #pragma unroll
@@ -373,7 +427,6 @@ __global__ __launch_bounds__(kThreads) void bwd_kernel(const Args p, bool single
   for (int i = 0; i < kRows; ++i) {
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      // rows past the end: g = 0 and x = 0 keep the state
       a[i][e] = decay(gr[i].get(e));
       H[e] = step(a[i][e], H[e], xr[i].get(e));
       G[e] += gr[i].get(e);
@@ -384,23 +437,36 @@ __global__ __launch_bounds__(kThreads) void bwd_kernel(const Args p, bool single
 #pragma unroll
     for (int e = 0; e < V; ++e) R[e] = step(a[i][e], dr[i].get(e) + R[e], 0.f);
   }
-  __shared__ Exchange<V> sh;
-  __shared__ float sh_r[kWaves][64 * V];
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    xr[i].repack();
+    dr[i].repack();
+  }
+  __shared__ Join<V> waves, shares;          // waves: G and the pairs of the backward walk
+  __shared__ float sh_h[kWaves][64 * V];     // H of the forward walk
 #pragma unroll
   for (int e = 0; e < V; ++e) {
-    sh.t[w][lane * V + e] = decay(G[e]);
-    sh.h[w][lane * V + e] = H[e];
-    sh_r[w][lane * V + e] = R[e];
+    waves.g[w][lane * V + e] = G[e];
+    waves.h[w][lane * V + e] = R[e];
+    sh_h[w][lane * V + e] = H[e];
   }
   __syncthreads();
-  if (!ok) return;
+  if (!single) {
+    leave<V, true>(p, waves, u, (int)blk * 64 * V);
+    if (j.chunk < 0) return;
+    const uint32_t last = j.first + (uint32_t)max((j.len + kChunk - 1) / kChunk, 1) - 1;
+    carry<V>(p, shares, p.slots - 1 - last, u, c, ok, d);
+  }
+  if (j.chunk < 0 || !ok) return;
+  TX* dx = static_cast<TX*>(p.dx) + j.b * p.dxs[0] + row * p.dxs[1] + c;
+  TG* dg = static_cast<TG*>(p.dg) + j.b * p.dgs[0] + row * p.dgs[1] + c;
   for (int i = 0; i < w; ++i) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) h[e] = step(sh.t[i][lane * V + e], h[e], sh.h[i][lane * V + e]);
+    for (int e = 0; e < V; ++e) h[e] = step(decay(waves.g[i][lane * V + e]), h[e], sh_h[i][lane * V + e]);
   }
   for (int i = kWaves - 1; i > w; --i) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) d[e] = step(sh.t[i][lane * V + e], d[e], sh_r[i][lane * V + e]);
+    for (int e = 0; e < V; ++e) d[e] = step(decay(waves.g[i][lane * V + e]), d[e], waves.h[i][lane * V + e]);
   }
   float ah[kRows][V];   // e^{g_t} h_{t-1}
 #pragma unroll
@@ -486,6 +552,14 @@ bool pairs_ok(const void* p, const int64_t* s, int eb) {
   return reinterpret_cast<uintptr_t>(p) % (2 * eb) == 0 && s[0] % 2 == 0 && s[1] % 2 == 0;
 }
 
+// The pairs' places before a walk.
+void clear(const Args& a, hipStream_t s) {
+  // agg, then agg16 (an even number of pairs in all, see pair_bytes)
+  const int64_t n = ((int64_t)a.slots * a.D + 1) / 2 * 2 + (((int64_t)a.slots / kSet) * a.D + 1) / 2 * 2;
+  const uint32_t grid = (uint32_t)std::min<int64_t>((n / 2 + 255) / 256, 2048);
+  hipLaunchKernelGGL(clear_kernel, dim3(grid), dim3(256), 0, s, a.agg, n, a.ticket);
+}
+
 template <typename TX, typename TG, int V>
 int run_fwd(Args& a, bool single, hipStream_t s) {
   a.nblk = (a.D + 64 * V - 1) / (64 * V);
@@ -493,29 +567,23 @@ int run_fwd(Args& a, bool single, hipStream_t s) {
     hipLaunchKernelGGL((short_kernel<TX, TG, V>), dim3((uint32_t)a.N * a.nblk), dim3(64), 0, s, a);
     return (int)hipGetLastError();
   }
-  const uint32_t grid = a.slots * a.nblk;
-  if (!single) {
-    hipLaunchKernelGGL((agg_kernel<TX, TG, V, false>), dim3(grid), dim3(kThreads), 0, s, a);
-    hipLaunchKernelGGL((carry_kernel<false>), dim3((uint32_t)a.N * ((a.D + 63) / 64)), dim3(kThreads), 0, s, a);
-  }
-  hipLaunchKernelGGL((main_kernel<TX, TG, V>), dim3(grid), dim3(kThreads), 0, s, a, single);
+  if (!single) clear(a, s);
+  hipLaunchKernelGGL((fwd_kernel<TX, TG, V, false>), dim3(a.slots * a.nblk), dim3(kThreads), 0, s, a, single);
   return (int)hipGetLastError();
 }
 
 template <typename TX, typename TG, int V>
 int run_bwd(Args& a, bool single, bool have_states, hipStream_t s) {
   a.nblk = (a.D + 64 * V - 1) / (64 * V);
-  const uint32_t grid = a.slots * a.nblk;
+  const dim3 grid(a.slots * a.nblk);
   if (!single) {
-    const dim3 cg((uint32_t)a.N * ((a.D + 63) / 64));
+    clear(a, s);
     if (!have_states) {
-      hipLaunchKernelGGL((agg_kernel<TX, TG, V, false>), dim3(grid), dim3(kThreads), 0, s, a);
-      hipLaunchKernelGGL((carry_kernel<false>), cg, dim3(kThreads), 0, s, a);
+      hipLaunchKernelGGL((fwd_kernel<TX, TG, V, true>), grid, dim3(kThreads), 0, s, a, single);
+      clear(a, s);
     }
-    hipLaunchKernelGGL((agg_kernel<TX, TG, V, true>), dim3(grid), dim3(kThreads), 0, s, a);
-    hipLaunchKernelGGL((carry_kernel<true>), cg, dim3(kThreads), 0, s, a);
   }
-  hipLaunchKernelGGL((bwd_kernel<TX, TG, V>), dim3(grid), dim3(kThreads), 0, s, a, single);
+  hipLaunchKernelGGL((bwd_kernel<TX, TG, V>), grid, dim3(kThreads), 0, s, a, single);
   return (int)hipGetLastError();
 }
 
@@ -573,11 +641,23 @@ struct Bwd {
   hipStream_t s;
   template <typename TX, typename TG, int V>
   int operator()() {
-    return run_bwd<TX, TG, V>(a, single, have, s);
+    return run_bwd<TX, TG, std::is_same<TX, float>::value ? 1 : V>(a, single, have, s);
   }
 };
 
 int64_t up256(int64_t n) { return (n + 255) & ~(int64_t)255; }
+
+// Workspace of a walk: the pairs (of chunks, then of sets, each an even number
+// of places), the counter.
+int64_t pair_bytes(int64_t slots, int64_t D) {
+  return ((slots * D + 1) / 2 * 2 + (slots / kSet * D + 1) / 2 * 2) * 8;
+}
+int64_t walk_bytes(int64_t slots, int64_t D) { return up256(pair_bytes(slots, D) + 4); }
+void walk_space(Args& a, void* ws) {
+  a.agg = static_cast<uint64_t*>(ws);
+  a.agg16 = a.agg + ((int64_t)a.slots * a.D + 1) / 2 * 2;
+  a.ticket = reinterpret_cast<uint32_t*>(static_cast<char*>(ws) + pair_bytes(a.slots, a.D));
+}
 
 }  // namespace scan
 }  // namespace gdn
@@ -597,15 +677,14 @@ int64_t gdn_scan_slots(int B, int T, int N, int packed) {
 int64_t gdn_scan_workspace_size(const GdnScanParams* prm) {
   if (prm == nullptr || check(*prm) != GDN_OK) return -1;
   if (is_single(*prm)) return 0;
-  const int64_t n = slots_of(prm->B, prm->T, prm->N, prm->cu_seqlens != nullptr) * prm->D;
-  return up256(8 * n) + (prm->states == nullptr ? up256(4 * n) : 0);
+  return walk_bytes(slots_of(prm->B, prm->T, prm->N, prm->cu_seqlens != nullptr), prm->D);
 }
 
 int64_t gdn_scan_bwd_workspace_size(const GdnScanParams* prm) {
   if (prm == nullptr || check(*prm) != GDN_OK) return -1;
   if (is_single(*prm)) return 0;
-  const int64_t n = slots_of(prm->B, prm->T, prm->N, prm->cu_seqlens != nullptr) * prm->D;
-  return up256(8 * n) + up256(4 * n) + (prm->states == nullptr ? up256(4 * n) : 0);
+  const int64_t slots = slots_of(prm->B, prm->T, prm->N, prm->cu_seqlens != nullptr);
+  return walk_bytes(slots, prm->D) + (prm->states == nullptr ? up256(4 * slots * prm->D) : 0);
 }
 
 int gdn_scan_launch(const GdnScanParams* prm, void* stream) {
@@ -625,11 +704,7 @@ int gdn_scan_launch(const GdnScanParams* prm, void* stream) {
   a.fs = P.final_state;
   a.states = P.states;
   for (int d = 0; d < 2; ++d) a.ys[d] = P.y_stride[d];
-  if (need > 0) {
-    a.agg = static_cast<float2*>(P.workspace);
-    if (P.states == nullptr)
-      a.states = reinterpret_cast<float*>(static_cast<char*>(P.workspace) + up256(8 * (int64_t)a.slots * a.D));
-  }
+  if (need > 0) walk_space(a, P.workspace);
   const int eb = dtype_bytes(P.x_dtype), gb = dtype_bytes(P.g_dtype);
   const bool two = P.D % 2 == 0 && pairs_ok(P.x, P.x_stride, eb) && pairs_ok(P.g, P.g_stride, gb) &&
                    pairs_ok(P.y, P.y_stride, eb);
@@ -663,18 +738,17 @@ int gdn_scan_bwd_launch(const GdnScanParams* prm, void* stream) {
     a.dgs[d] = P.dg_stride[d];
   }
   if (need > 0) {
-    char* ws = static_cast<char*>(P.workspace);
-    const int64_t n = (int64_t)a.slots * a.D;
-    a.agg = reinterpret_cast<float2*>(ws);
-    a.rstates = reinterpret_cast<float*>(ws + up256(8 * n));
-    if (P.states == nullptr) a.states = reinterpret_cast<float*>(ws + up256(8 * n) + up256(4 * n));
+    walk_space(a, P.workspace);
+    if (P.states == nullptr)
+      a.states = reinterpret_cast<float*>(static_cast<char*>(P.workspace) + walk_bytes(a.slots, a.D));
   }
   const int eb = dtype_bytes(P.x_dtype), gb = dtype_bytes(P.g_dtype);
   const bool two = P.D % 2 == 0 && pairs_ok(P.x, P.x_stride, eb) && pairs_ok(P.g, P.g_stride, gb) &&
                    pairs_ok(P.dy, P.dy_stride, eb) && pairs_ok(P.dx, P.dx_stride, eb) &&
                    pairs_ok(P.dg, P.dg_stride, gb);
   Bwd f{a, is_single(P), P.states != nullptr, static_cast<hipStream_t>(stream)};
-  return two ? by_type<2>(P.x_dtype, P.g_dtype, f) : by_type<1>(P.x_dtype, P.g_dtype, f);
+  // fp32 rows of x, g and dy two channels wide do not fit the registers
+  return two && P.x_dtype != GDN_DTYPE_F32 ? by_type<2>(P.x_dtype, P.g_dtype, f) : by_type<1>(P.x_dtype, P.g_dtype, f);
 }
 
 }  // extern "C"

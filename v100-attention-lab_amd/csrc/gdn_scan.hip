@@ -17,7 +17,8 @@
 // of its 16 chunks, so that a chunk reads at most 30 pairs and one for each 16
 // chunks between.  All sums have a fixed order.
 //
-// Waiting: chunks are dealt by a counter in the order of the walk, so whatever
+// Waiting: a channel block's chunks are dealt by its counter in the order of
+// the walk, so whatever
 // a workgroup waits for is left by workgroups that already run; each leaves its
 // own pair before it waits for any, and what it leaves later depends on earlier
 // ones alone.  A place in the workspace holds ~0 until its pair is there (one
@@ -160,6 +161,7 @@ __device__ __forceinline__ void load_rows(const TX* x, const TG* g, int64_t xs, 
 
 constexpr uint64_t kAbsent = ~(uint64_t)0;
 constexpr int kSet = 16;                   // chunks whose pairs are joined to one
+constexpr int kLine = 32;                  // floats between two counters
 
 __device__ __forceinline__ void leave_pair(uint64_t* at, float g, float h) {
   uint64_t v = ((uint64_t)__float_as_uint(h) << 32) | __float_as_uint(g);
@@ -172,27 +174,22 @@ __device__ __forceinline__ uint64_t look(const uint64_t* at) {
 __device__ __forceinline__ float pair_g(uint64_t v) { return __uint_as_float((uint32_t)v); }
 __device__ __forceinline__ float pair_h(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
 
-// Every place of n pairs absent, and the counter at zero.
-__global__ __launch_bounds__(256) void clear_kernel(uint64_t* agg, int64_t n, uint32_t* ticket) {
+// Every place of n pairs absent, and the counters at zero.
+__global__ __launch_bounds__(256) void clear_kernel(uint64_t* agg, int64_t n, uint32_t* ticket, int nblk) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i == 0) *ticket = 0;
+  for (int64_t k = i; k < nblk; k += (int64_t)gridDim.x * 256) ticket[k * kLine] = 0;
   for (int64_t k = i; k < n / 2; k += (int64_t)gridDim.x * 256)
     reinterpret_cast<ulonglong2*>(agg)[k] = make_ulonglong2(kAbsent, kAbsent);
 }
 
-// Chunk of a workgroup and its place u in the order of the walk (REV: from the
-// last chunk to the first).
-template <bool REV>
+// Channel block of a workgroup and its chunk's place in the order of the walk.
 __device__ __forceinline__ uint32_t next_place(const Args& p, bool single, uint32_t& blk) {
-  uint32_t at = blockIdx.x;
-  if (!single) {
-    __shared__ uint32_t sh;
-    if (threadIdx.x == 0) sh = atomicAdd(p.ticket, 1u);
-    __syncthreads();
-    at = sh;
-  }
-  blk = at % p.nblk;
-  return at / p.nblk;
+  blk = blockIdx.x % p.nblk;
+  if (single) return blockIdx.x / p.nblk;
+  __shared__ uint32_t sh;
+  if (threadIdx.x == 0) sh = atomicAdd(p.ticket + (int64_t)blk * kLine, 1u);
+  __syncthreads();
+  return sh;
 }
 
 // Scratch of the joins below.
@@ -249,8 +246,10 @@ __device__ __forceinline__ void carry(const Args& p, Join<V>& sh, uint32_t first
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int up = (int)(first + kSet - 1) / kSet * kSet;       // the first whole set's start
   const int head = min((int)u, up) - (int)first;
-  const int sets = max((int)u / kSet - up / kSet, 0);
-  const int tail = max((int)u - max((int)u / kSet * kSet, up), 0);
+  // (the last 16 to 31 singly: by then a set before them has had its time)
+  const int end = max(((int)u / kSet - 1) * kSet, up);
+  const int sets = max((end - up) / kSet, 0);
+  const int tail = max((int)u - end, 0);
   const int n = max(head, 0) + sets + tail;
   const int share = (n + kWaves - 1) / kWaves, k0 = min(w * share, n), k1 = min(k0 + share, n);
   auto at = [&](int k) -> const uint64_t* {
@@ -313,7 +312,7 @@ __device__ __forceinline__ void carry(const Args& p, Join<V>& sh, uint32_t first
 template <typename TX, typename TG, int V, bool ONLY_STATES>
 __global__ __launch_bounds__(kThreads, 4) void fwd_kernel(const Args p, bool single) {
   uint32_t blk;
-  const uint32_t slot = next_place<false>(p, single, blk);
+  const uint32_t slot = next_place(p, single, blk);
   const Job j = slot_job(p, (int)slot);
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int c = (int)blk * 64 * V + lane * V;
@@ -391,7 +390,7 @@ __global__ __launch_bounds__(kThreads, 4) void fwd_kernel(const Args p, bool sin
 template <typename TX, typename TG, int V>
 __global__ __launch_bounds__(kThreads, 4) void bwd_kernel(const Args p, bool single) {
   uint32_t blk;
-  const uint32_t u = next_place<true>(p, single, blk), slot = p.slots - 1 - u;
+  const uint32_t u = next_place(p, single, blk), slot = p.slots - 1 - u;
   const Job j = slot_job(p, (int)slot);
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int c = (int)blk * 64 * V + lane * V;
@@ -557,7 +556,7 @@ void clear(const Args& a, hipStream_t s) {
   // agg, then agg16 (an even number of pairs in all, see pair_bytes)
   const int64_t n = ((int64_t)a.slots * a.D + 1) / 2 * 2 + (((int64_t)a.slots / kSet) * a.D + 1) / 2 * 2;
   const uint32_t grid = (uint32_t)std::min<int64_t>((n / 2 + 255) / 256, 2048);
-  hipLaunchKernelGGL(clear_kernel, dim3(grid), dim3(256), 0, s, a.agg, n, a.ticket);
+  hipLaunchKernelGGL(clear_kernel, dim3(grid), dim3(256), 0, s, a.agg, n, a.ticket, a.nblk);
 }
 
 template <typename TX, typename TG, int V>
@@ -648,11 +647,11 @@ struct Bwd {
 int64_t up256(int64_t n) { return (n + 255) & ~(int64_t)255; }
 
 // Workspace of a walk: the pairs (of chunks, then of sets, each an even number
-// of places), the counter.
+// of places), the counters (of channel blocks of 64 or 128).
 int64_t pair_bytes(int64_t slots, int64_t D) {
   return ((slots * D + 1) / 2 * 2 + (slots / kSet * D + 1) / 2 * 2) * 8;
 }
-int64_t walk_bytes(int64_t slots, int64_t D) { return up256(pair_bytes(slots, D) + 4); }
+int64_t walk_bytes(int64_t slots, int64_t D) { return up256(pair_bytes(slots, D) + (D + 63) / 64 * kLine * 4); }
 void walk_space(Args& a, void* ws) {
   a.agg = static_cast<uint64_t*>(ws);
   a.agg16 = a.agg + ((int64_t)a.slots * a.D + 1) / 2 * 2;

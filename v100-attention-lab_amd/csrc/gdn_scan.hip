@@ -118,27 +118,27 @@ __device__ __forceinline__ Job slot_job(const Args& p, int slot) {
   return j;
 }
 
-// e^g in one float: for -1/8 < g <= 0 it is e^g - 1 (sign bit set, by its
-// series, truncated below 2^-30), else e^g (sign bit clear).  e^g h is then
-// h + (e^g - 1) h, exact to the rounding of the sum, where e^g itself would
-// carry an error of 2^-25 a row.
+// e^g in one float: for -1/16 < g <= -0 it is e^g - 1 (sign bit set; four terms
+// of its series, the next below 2^-26 of 1), else e^g (sign bit clear).  e^g h is
+// then h + (e^g - 1) h, exact to the rounding of the sum, where e^g itself would
+// carry an error of 2^-25 a row.  Below -1/16 a state lives for a few rows, and
+// the hardware's 2^x of the rounded exponent is enough (2^-24 |g| beside the
+// result's own unit).
 __device__ __forceinline__ float decay(float g) {
   const float n = -g;
-  float s = -1.f / 720.f;
-  s = __builtin_fmaf(s, n, 1.f / 120.f);
-  s = __builtin_fmaf(s, n, -1.f / 24.f);
-  s = __builtin_fmaf(s, n, 1.f / 6.f);
+  float s = __builtin_fmaf(n, -1.f / 24.f, 1.f / 6.f);
   s = __builtin_fmaf(s, n, -0.5f);
   s = __builtin_fmaf(s, n, 1.f);
-  return n >= 0.f && n < 0.125f ? -fabsf(n * s) : expf(g);
+  const float e = __builtin_amdgcn_exp2f(g * 1.4426950408889634f);
+  return __float_as_uint(n) < __float_as_uint(0.0625f) ? g * s : e;
 }
 
-// e^g h + x from t = decay(g); an infinite sum stays what it is.
+// e^g h + x from t = decay(g).  Near 1 an infinite state stays what it is:
+// (e^g - 1) times the largest finite number does not reach it.
 __device__ __forceinline__ float step(float t, float h, float x) {
   const bool near1 = __float_as_int(t) < 0;
-  const float base = near1 ? h + x : x;
-  const float r = __builtin_fmaf(t, h, base);
-  return near1 && fabsf(base) == __builtin_inff() ? base : r;
+  const float top = 3.402823466e38f;
+  return __builtin_fmaf(t, near1 ? __builtin_amdgcn_fmed3f(h, -top, top) : h, near1 ? h + x : x);
 }
 
 template <typename TX, typename TG, int V>

@@ -11,7 +11,7 @@ import torch
 
 from . import _lib
 from .ops import _DTYPE_CODE, _PLANS_MAX, _check_devices, _launch, _needs_grad, _offsets
-from .scan import _failed, _sig
+from .scan import _failed, _like, _sig
 
 SUPPORTED_D = (64, 128)
 MAX_DECODE_T = 16
@@ -115,7 +115,7 @@ def _run(q, k, v, window, sinks, scale, cu, n_seq, need_lse):
             _FWD_PLANS[key] = plan
     elif not _aligned(q, k, v):
         _validate(q, k, v)
-    o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    o = _like(q)
     lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if need_lse else None
     P = _lib.GdnAttnParams.from_buffer_copy(plan)
     P.q, P.k, P.v, P.o = q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr()
@@ -205,7 +205,7 @@ def _run_bwd(q, k, v, o, lse, do, window, sinks, scale, cu, n_seq):
         _bwd_plan(q, k, v, o, lse, do, window, sinks, scale, n_seq)
     params, ws_bytes = plan
     dev = q.device
-    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
+    dq, dk, dv = _like(q), _like(k), _like(v)
     ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=dev)
     P = _lib.GdnAttnParams.from_buffer_copy(params)
     P.q, P.k, P.v, P.o, P.lse, P.d_o = (t.data_ptr() for t in (q, k, v, o, lse, do))
@@ -306,7 +306,7 @@ def window_attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
     lens = cache_seqlens
     if lens.dtype != torch.int32 or not lens.is_contiguous():
         lens = lens.clamp(0, k_cache.shape[1]).to(torch.int32).contiguous()
-    o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    o = _like(q)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes > 0 else None
     P = _lib.GdnAttnDecodeParams.from_buffer_copy(params)
     P.q, P.k, P.v, P.o = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr()

@@ -279,7 +279,6 @@ __global__ __launch_bounds__(256 * QH, D == 64 && QH == 1 ? 3 : 2) void kv_kerne
       frow += a.rows;
     }
   };
-  dma_wait();
   // two waves share a SIMD: with one of them ahead, its exponentials run beside
   // the other's products
   if (qh == 1) __builtin_amdgcn_s_setprio(1);
@@ -561,7 +560,6 @@ __global__ __launch_bounds__(256, 2) void q_kernel(const BArgs a) {
   const Copier<D, kKT, 256> cv(a.v + sq.b * a.vs[0] + sq.k0 * a.vs[1] + hk * a.vs[2], a.vs[1], sq.nk);
   const uint32_t base = lds_addr(lds);
   const TL tl(lane);
-  dma_wait();
   if (kr.n > 0) {
     ck(base, kr.tile(0) * kKT);
     cv(base + kTile, kr.tile(0) * kKT);

@@ -19,6 +19,7 @@ namespace attn {
 constexpr int kDN = 32;          // keys a tile
 constexpr int kDWaves = 4;
 constexpr int kMaxT = 16;
+constexpr int kMaxSplits = 64;
 
 struct DArgs {
   const uint16_t* q;
@@ -93,7 +94,6 @@ __global__ __launch_bounds__(64 * kDWaves) void decode_kernel(const DArgs a) {
   };
   const TL tl(lane);
   Rows<T, D, 1> rows;
-  dma_wait();
   if (t0 + wv < t1) {
     const int j = kr.tile(t0 + wv) * kDN;
     fetch(base, kb, a.ks[1], j);
@@ -174,29 +174,57 @@ __global__ __launch_bounds__(64 * kDWaves) void decode_kernel(const DArgs a) {
   for (int e = 0; e < D / 8; e += 2) *reinterpret_cast<uint32_t*>(o + e) = O::pack(out[e] * inv, out[e + 1] * inv);
 }
 
-// One workgroup a query row: D threads, the splits in order.
+// One workgroup a query row: every wave weighs the splits (one a lane), then
+// groups of D / 4 threads add the splits g, g + groups, .. and the groups' sums
+// are added in order.
+constexpr int kJT = 256;
 template <typename T, int D>
-__global__ __launch_bounds__(D) void join_kernel(const DArgs a) {
-  const int c = blockIdx.x % 32, unit = blockIdx.x / 32;
-  const int rt = unit % a.tiles_r, bh = unit / a.tiles_r, hk = bh % a.Hk, b = bh / a.Hk;
-  const QRow w(a, hk, rt, c);
-  if (!w.ok) return;
+__global__ __launch_bounds__(kJT) void join_kernel(const DArgs a) {
+  constexpr int L = D / 4, kGroups = kJT / L;
+  const int rows = a.G * a.T, r = blockIdx.x % rows, bh = blockIdx.x / rows, hk = bh % a.Hk, b = bh / a.Hk;
+  const int c = r % 32, unit = bh * a.tiles_r + r / 32;
   const float* part = a.part + (int64_t)unit * a.splits * 32 * (D + 2);
   const int64_t step = 32 * (D + 2);
-  float top = -__builtin_inff();
-  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, part[s * step + c]);
-  float l = 0.f, out = 0.f;
-#pragma unroll 4
-  for (int s = 0; s < a.splits; ++s) {
-    const float f = weight(part[s * step + c], top);
-    if (f != 0.f) {
-      l += f * part[s * step + 32 + c];
-      out += f * part[s * step + 64 + c * D + threadIdx.x];
+  const int lane = threadIdx.x & 63, g = threadIdx.x / L, d = threadIdx.x % L;
+  static_assert(kMaxSplits <= 64, "a split a lane");
+  const float m = lane < a.splits ? part[lane * step + c] : -__builtin_inff();
+  const float ls = lane < a.splits ? part[lane * step + 32 + c] : 0.f;
+  float top = m;
+#pragma unroll
+  for (int s = 32; s >= 1; s >>= 1) top = fmaxf(top, __shfl_xor(top, s, 64));
+  const float f = weight(m, top);
+  float l = f != 0.f ? f * ls : 0.f;
+#pragma unroll
+  for (int s = 32; s >= 1; s >>= 1) l += __shfl_xor(l, s, 64);
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int k = 0; k < kMaxSplits / kGroups; ++k) {
+    const int s = k * kGroups + g;
+    const float fs = __shfl(f, s < a.splits ? s : 0, 64);
+    if (s < a.splits && fs != 0.f) {
+      const float4 x = *reinterpret_cast<const float4*>(part + s * step + 64 + c * D + 4 * d);
+      o.x += fs * x.x;
+      o.y += fs * x.y;
+      o.z += fs * x.z;
+      o.w += fs * x.w;
     }
   }
+  __shared__ float4 sums[kGroups][L];
+  sums[g][d] = o;
+  __syncthreads();
+  if (g != 0) return;
+#pragma unroll
+  for (int k = 1; k < kGroups; ++k) {
+    const float4 x = sums[k][d];
+    o.x += x.x;
+    o.y += x.y;
+    o.z += x.z;
+    o.w += x.w;
+  }
   const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-  const uint32_t bits = Ops<T>::pack(out * inv, 0.f);
-  a.o[b * a.os[0] + w.t * a.os[1] + w.h * a.os[2] + threadIdx.x] = (uint16_t)(bits & 0xffffu);
+  const QRow w(a, hk, r / 32, c);
+  *reinterpret_cast<uint2*>(a.o + b * a.os[0] + w.t * a.os[1] + w.h * a.os[2] + 4 * d) =
+      make_uint2(Ops<T>::pack(o.x * inv, o.y * inv), Ops<T>::pack(o.z * inv, o.w * inv));
 }
 
 int check(const GdnAttnDecodeParams& P) {
@@ -209,21 +237,23 @@ int check(const GdnAttnDecodeParams& P) {
 
 int row_tiles(const GdnAttnDecodeParams& P) { return (P.Hq / P.Hk * P.T + 31) / 32; }
 
-// Workgroups a sequence and key head: enough for two a CU, of at least one
-// tile a wave, over the tiles that the longest sequence can have.
+// Workgroups a sequence and key head: one a CU (their tiles fill its LDS; 32
+// sequences of 4 key heads with 4100 keys: 55 us with 256 workgroups, 60 with
+// 512, 66 with 1024), of at least one tile a wave, over the tiles that the
+// longest sequence can have.
 int splits_of(const GdnAttnDecodeParams& P) {
   const int64_t keys = std::min<int64_t>(P.S, (int64_t)P.window + P.T - 1 + P.sinks);
   const int64_t tiles = keys / kDN + 2;
   const int64_t units = (int64_t)P.B * P.Hk * row_tiles(P);
-  const int64_t want = (512 + units - 1) / units;
-  return (int)std::max<int64_t>(1, std::min({want, (tiles + kDWaves - 1) / kDWaves, (int64_t)64}));
+  const int64_t want = (256 + units - 1) / units;
+  return (int)std::max<int64_t>(1, std::min({want, (tiles + kDWaves - 1) / kDWaves, (int64_t)kMaxSplits}));
 }
 
 template <typename T, int D>
 int launch(const DArgs& a, hipStream_t s) {
   const uint32_t units = (uint32_t)a.B * a.Hk * a.tiles_r;
   hipLaunchKernelGGL((decode_kernel<T, D>), dim3(units * a.splits), dim3(64 * kDWaves), 0, s, a);
-  if (a.splits > 1) hipLaunchKernelGGL((join_kernel<T, D>), dim3(units * 32), dim3(D), 0, s, a);
+  if (a.splits > 1) hipLaunchKernelGGL((join_kernel<T, D>), dim3((uint32_t)(a.B * a.Hk * a.G * a.T)), dim3(kJT), 0, s, a);
   return (int)hipGetLastError();
 }
 
@@ -251,7 +281,7 @@ int gdn_attn_decode_launch(const GdnAttnDecodeParams* prm, void* stream) {
   if (!rows16(P.q, P.q_stride, P.B, P.T, P.Hq) || !rows16(P.o, P.o_stride, P.B, P.T, P.Hq) ||
       !rows16(P.k, P.k_stride, P.B, P.S, P.Hk) || !rows16(P.v, P.v_stride, P.B, P.S, P.Hk))
     return GDN_ERR_MISALIGNED;
-  if ((int64_t)P.B * P.Hk * row_tiles(P) * 64 > 0x7fffffffLL) return GDN_ERR_BAD_SHAPE;
+  if ((int64_t)P.B * P.Hk * row_tiles(P) * kMaxSplits > 0x7fffffffLL) return GDN_ERR_BAD_SHAPE;
   const int64_t need = gdn_attn_decode_workspace_size(prm);
   if (need > 0 && (P.workspace == nullptr || P.workspace_bytes < need ||
                    reinterpret_cast<uintptr_t>(P.workspace) % 256 != 0))

@@ -79,7 +79,6 @@ __global__ __launch_bounds__(kNT, 2) void fwd_kernel(const FArgs a) {
   const Copier<D, kBN, kNT> ck(kb, a.ks[1], sq.nk), cv(vb, a.vs[1], sq.nk);
   const uint32_t base = lds_addr(lds);
   const TL tl(lane);
-  dma_wait();     // q is here: no load but the tiles' is waited for in the loop
   if (kr.n > 0) {
     ck(base, kr.tile(0) * kBN);
     cv(base + kTile, kr.tile(0) * kBN);

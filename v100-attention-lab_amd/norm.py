@@ -10,7 +10,7 @@ import torch
 
 from . import _lib
 from .ops import _DTYPE_CODE, _PLANS_MAX, _check_devices, _code, _launch, _needs_grad
-from .scan import _check_columns, _failed, _sig
+from .scan import _check_columns, _failed, _like, _sig
 
 _FWD_PLANS = {}
 _BWD_PLANS = {}
@@ -97,13 +97,13 @@ def _run(x, weight, residual, eps, fp8, group):
             _FWD_PLANS[key] = plan
     params, shape_scale = plan
     dev = x.device
-    y = torch.empty(shape, dtype=torch.float8_e4m3fn if fp8 else x.dtype, device=dev)
+    y = _like(x, torch.float8_e4m3fn if fp8 else None)
     scale = torch.empty(shape_scale, dtype=torch.float32, device=dev) if fp8 else None
     P = _lib.GdnNormParams.from_buffer_copy(params)
     P.x, P.w, P.y = x3.data_ptr(), weight.data_ptr(), y.data_ptr()
     r = x
     if residual is not None:
-        r = torch.empty(shape, dtype=residual.dtype, device=dev)
+        r = _like(residual)
         P.res, P.r_out = residual3.data_ptr(), r.data_ptr()
     if fp8:
         P.scale = scale.data_ptr()
@@ -178,7 +178,6 @@ def _bwd_plan(r, weight, dy, dr, eps, x_dtype):
 
 
 def _run_bwd(r, weight, dy, dr, eps, need_dx):
-    shape = r.shape if isinstance(r, torch.Tensor) else None
     # autograd may hand over any layout, e.g. the expansion of a scalar
     dy, dr = (t.contiguous() if isinstance(t, torch.Tensor) and t.dim() > 0 and t.stride(-1) != 1 else t
               for t in (dy, dr))
@@ -199,9 +198,9 @@ def _run_bwd(r, weight, dy, dr, eps, need_dx):
             _BWD_PLANS[key] = plan
     params, ws_bytes = plan
     dev = r.device
-    out = torch.empty(shape, dtype=r.dtype, device=dev)
-    dx = torch.empty(shape, dtype=dy.dtype, device=dev) if need_dx else None
-    dw = torch.empty(weight.shape, dtype=weight.dtype, device=dev)
+    out = _like(r)
+    dx = _like(dy) if need_dx else None
+    dw = _like(weight)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
     P = _lib.GdnNormParams.from_buffer_copy(params)
     P.r, P.w, P.dy = r3.data_ptr(), weight.data_ptr(), dy3.data_ptr()

@@ -20,6 +20,14 @@ def _sig(t):
     return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
 
 
+def _like(t, dtype=None):
+    """A new dense tensor of t's shape (empty_like, the cheaper call, keeps the
+    order of dense strides)."""
+    if t.is_contiguous():
+        return torch.empty_like(t, dtype=dtype)
+    return torch.empty(t.shape, dtype=dtype or t.dtype, device=t.device)
+
+
 def _failed(name, status):
     return RuntimeError(f"{name} failed ({status}): {_lib.op_status_string(status)}")
 
@@ -102,8 +110,8 @@ def _run(x, g, h0, cu, n_seq, return_states):
             _FWD_PLANS[key] = plan
     params, ws_bytes, shape_fs, shape_st = plan
     dev = x.device
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    fs = torch.empty(shape_fs, dtype=torch.float32, device=dev)
+    y = _like(x)
+    fs = _like(h0) if h0 is not None else torch.empty(shape_fs, dtype=torch.float32, device=dev)
     states = torch.empty(shape_st, dtype=torch.float32, device=dev) if return_states else None
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes > 0 else None
     P = _lib.GdnScanParams.from_buffer_copy(params)
@@ -204,8 +212,7 @@ def _run_bwd(x, g, h0, dy, dfinal, states, cu, n_seq, need_dh0):
             _BWD_PLANS[key] = plan
     params, ws_bytes, shape_dh0 = plan
     dev = x.device
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    dg = torch.empty(g.shape, dtype=g.dtype, device=dev)
+    dx, dg = _like(x), _like(g)
     dh0 = torch.empty(shape_dh0, dtype=torch.float32, device=dev) if shape_dh0 is not None else None
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes > 0 else None
     P = _lib.GdnScanParams.from_buffer_copy(params)

@@ -208,9 +208,11 @@ struct Copier {
       for (int i = 0; i < kPasses; ++i)
         dma16(uniform_ptr(src + (int64_t)(row0 + i * kPass) * ld), ofs, at + i * kStep);
     } else {
+      int r = row0 + row;
+      asm volatile("" : "+v"(r));     // (not kept in registers from tile to tile)
 #pragma unroll
       for (int i = 0; i < kPasses; ++i)
-        dma16(src + (int64_t)min(row0 + i * kPass + row, rows - 1) * ld + 8 * piece, at + i * kStep);
+        dma16(src + (int64_t)min(r + i * kPass, rows - 1) * ld + 8 * piece, at + i * kStep);
     }
   }
 };
@@ -366,6 +368,13 @@ struct Rows {
   float m = -__builtin_inff(), l = 0.f;
 
   Vec pf[2 * KS];
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) acc[i] = f32x16{};
+    m = -__builtin_inff();
+    l = 0.f;
+  }
 
   // Scores and probabilities of one tile.
   __device__ __forceinline__ void scores(const Vec (&qf)[D / 16], const TL& tl, uint32_t kt, bool masked, const Mask& seen,

@@ -257,12 +257,15 @@ __global__ __launch_bounds__(256 * QH, D == 64 && QH == 1 ? 3 : 2) void kv_kerne
 
   const TL tl(lane);
   const uint32_t vt = base + kV + TL::bytes(32) * kg;
-  // the tile that is brought next: its rows and head
-  int fr0 = rg.r0 + (n > 0 ? n0 % nt : 0) * kQT;
+  const int fr_first = rg.r0 + (n > 0 ? n0 % nt : 0) * kQT;
   const int fh = hk * a.G + (n > 0 ? n0 / nt : 0);
-  Copier<D, kQT, kKVT> cq(a.q + sq.b * a.qs[0] + sq.q0 * a.qs[1] + fh * a.qs[2], a.qs[1], sq.nq);
-  Copier<D, kQT, kKVT> cd(a.dO + sq.b * a.dos[0] + sq.q0 * a.dos[1] + fh * a.dos[2], a.dos[1], sq.nq);
-  int64_t frow = (int64_t)fh * a.rows + (int64_t)sq.b * a.seq.Tq + sq.q0;
+  const uint16_t* const q_first = a.q + sq.b * a.qs[0] + sq.q0 * a.qs[1] + fh * a.qs[2];
+  const uint16_t* const d_first = a.dO + sq.b * a.dos[0] + sq.q0 * a.dos[1] + fh * a.dos[2];
+  const int64_t row_first = (int64_t)fh * a.rows + (int64_t)sq.b * a.seq.Tq + sq.q0;
+  // the tile that is brought next: its rows and head
+  int fr0;
+  int64_t frow;
+  Copier<D, kQT, kKVT> cq(q_first, a.qs[1], sq.nq), cd(d_first, a.dos[1], sq.nq);
   auto fetch = [&](uint32_t at) {
     cq(at, fr0);
     cd(at + kTile, fr0);
@@ -282,6 +285,15 @@ __global__ __launch_bounds__(256 * QH, D == 64 && QH == 1 ? 3 : 2) void kv_kerne
   // two waves share a SIMD: with one of them ahead, its exponentials run beside
   // the other's products
   if (qh == 1) __builtin_amdgcn_s_setprio(1);
+  // One pass over the tiles.  careful: tiles on an edge of any wave's range are
+  // made finite where they are not, after S and dP.
+  // An infinity or NaN in a hidden place shows in the sums (0 times it is NaN):
+  // only then the careful pass is taken.
+  for (bool careful = false;; careful = true) {
+  fr0 = fr_first;
+  cq.src = q_first;
+  cd.src = d_first;
+  frow = row_first;
   int t0 = fr0;                                   // the tile's first row
   if (n > 0) fetch(base);
   for (int it = 0; it < n; ++it) {
@@ -296,7 +308,7 @@ __global__ __launch_bounds__(256 * QH, D == 64 && QH == 1 ? 3 : 2) void kv_kerne
     // a tile on an edge of any wave's range: are all its rows finite?
     constexpr int kShare = 2 * kQT / TL::kGroup / (4 * QH);
     bool bad = false;
-    if (!(t0 + kQT <= rg.r1 && k0 + kKB <= sq.nk &&
+    if (careful && !(t0 + kQT <= rg.r1 && k0 + kKB <= sq.nk &&
           all_visible(k0, k0 + kKB - 1, t0 + shift, t0 + kQT - 1 + shift, a.window, a.sinks)))
       bad = __syncthreads_or(not_finite<T, kShare>(buf + wv * kShare * TL::kGroupBytes, lane));
     Vec pf[2], df[2];
@@ -382,6 +394,16 @@ __global__ __launch_bounds__(256 * QH, D == 64 && QH == 1 ? 3 : 2) void kv_kerne
           });
     }
     t0 = t0 + kQT < rg.r1 ? t0 + kQT : rg.r0;
+  }
+  bool odd = false;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) odd |= !(fabsf(dk[i][r]) < __builtin_inff()) | !(fabsf(dv[i][r]) < __builtin_inff());
+  if (careful || !__syncthreads_or(odd)) break;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) dk[i] = dv[i] = f32x16{};
+  unit_do = 0x1p-24f;
   }
   const float fv = exp2f(-kPUp<T>);
   const float fk = kScaled<T> ? a.scale * unit_do * vu * 0x1p-7f : a.scale;
@@ -560,6 +582,7 @@ __global__ __launch_bounds__(256, 2) void q_kernel(const BArgs a) {
   const Copier<D, kKT, 256> cv(a.v + sq.b * a.vs[0] + sq.k0 * a.vs[1] + hk * a.vs[2], a.vs[1], sq.nk);
   const uint32_t base = lds_addr(lds);
   const TL tl(lane);
+  auto pass = [&](bool careful) {
   if (kr.n > 0) {
     ck(base, kr.tile(0) * kKT);
     cv(base + kTile, kr.tile(0) * kKT);
@@ -595,7 +618,7 @@ __global__ __launch_bounds__(256, 2) void q_kernel(const BArgs a) {
         const Mask seen(p, j0, half, sq.nk, a.window, a.sinks);
 #pragma unroll
         for (int r = 0; r < 16; ++r) dp[r] = seen(0, r) ? dp[r] : 0.f;
-        bad = not_finite<T, 32 / TL::kGroup>(kh, lane);
+        bad = careful && not_finite<T, 32 / TL::kGroup>(kh, lane);
       }
       Vec sf[2];
 #pragma unroll
@@ -612,6 +635,19 @@ __global__ __launch_bounds__(256, 2) void q_kernel(const BArgs a) {
                                [&](int i, const uint4& x) { dq[i % N] = O::mfma(as_vec<T>(x), sf[i / N], dq[i % N]); });
       }
     }
+  }
+  };
+  // (see kv_kernel)
+  pass(false);
+  bool odd = false;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) odd |= !(fabsf(dq[i][r]) < __builtin_inff());
+  if (__syncthreads_or(odd)) {
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) dq[i] = f32x16{};
+    pass(true);
   }
   if (row >= sq.nq) return;
   const float f = kScaled<T> ? a.scale * u * 0x1p-7f : a.scale;

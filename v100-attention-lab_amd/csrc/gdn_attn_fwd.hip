@@ -79,38 +79,53 @@ __global__ __launch_bounds__(kNT, 2) void fwd_kernel(const FArgs a) {
   const Copier<D, kBN, kNT> ck(kb, a.ks[1], sq.nk), cv(vb, a.vs[1], sq.nk);
   const uint32_t base = lds_addr(lds);
   const TL tl(lane);
-  if (kr.n > 0) {
-    ck(base, kr.tile(0) * kBN);
-    cv(base + kTile, kr.tile(0) * kBN);
-  }
-  for (int it = 0; it < kr.n; ++it) {
-    const int j0 = kr.tile(it) * kBN;
-    const uint32_t kt = base + (it & 1) * 2 * kTile, vt = kt + kTile;
-    dma_wait();
-    __syncthreads();                          // tile `it` is here; every wave is done with the other buffer
-    if (it + 1 < kr.n) {
-      const int jn = kr.tile(it + 1) * kBN;
-      const uint32_t other = base + ((it + 1) & 1) * 2 * kTile;
-      ck(other, jn);
-      cv(other + kTile, jn);
+  // One pass over the tiles.  careful: tiles on an edge of any wave's range are
+  // made finite where they are not, after what they hold has reached the rows
+  // that see it.
+  auto pass = [&](bool careful) {
+    if (kr.n > 0) {
+      ck(base, kr.tile(0) * kBN);
+      cv(base + kTile, kr.tile(0) * kBN);
     }
-    const int j1 = min(j0 + kBN, sq.nk) - 1;
-    const bool whole = j0 + kBN <= sq.nk, active = !none_visible(j0, j1, wp0, wp1, a.window, a.sinks);
-    const bool masked = !(whole && all_visible(j0, j1, wp0, wp1, a.window, a.sinks));
-    const Mask seen(p, j0, half, sq.nk, a.window, a.sinks);
-    // a tile on an edge of any wave's range: are all its values finite?
-    constexpr int kShare = kBN / TL::kGroup / 4;
-    bool bad = false;
-    if (!(whole && all_visible(j0, j1, p0, p1, a.window, a.sinks)))
-      bad = __syncthreads_or(not_finite<T, kShare>(vt + wv * kShare * TL::kGroupBytes, lane));
-    if (active) rows.scores(qf, tl, kt, masked, seen, a.scale_log2);
-    if (bad) {
-      if (active) rows.add_not_finite(seen, tl, vt);
-      __syncthreads();
-      make_finite<T, kShare>(vt + wv * kShare * TL::kGroupBytes, lane);
-      __syncthreads();
+    for (int it = 0; it < kr.n; ++it) {
+      const int j0 = kr.tile(it) * kBN;
+      const uint32_t kt = base + (it & 1) * 2 * kTile, vt = kt + kTile;
+      dma_wait();
+      __syncthreads();                        // tile `it` is here; every wave is done with the other buffer
+      if (it + 1 < kr.n) {
+        const int jn = kr.tile(it + 1) * kBN;
+        const uint32_t other = base + ((it + 1) & 1) * 2 * kTile;
+        ck(other, jn);
+        cv(other + kTile, jn);
+      }
+      const int j1 = min(j0 + kBN, sq.nk) - 1;
+      const bool whole = j0 + kBN <= sq.nk, active = !none_visible(j0, j1, wp0, wp1, a.window, a.sinks);
+      const bool masked = !(whole && all_visible(j0, j1, wp0, wp1, a.window, a.sinks));
+      const Mask seen(p, j0, half, sq.nk, a.window, a.sinks);
+      constexpr int kShare = kBN / TL::kGroup / 4;
+      const uint32_t share = vt + wv * kShare * TL::kGroupBytes;
+      if (active) rows.scores(qf, tl, kt, masked, seen, a.scale_log2);
+      if (careful && !(whole && all_visible(j0, j1, p0, p1, a.window, a.sinks)) &&
+          __syncthreads_or(not_finite<T, kShare>(share, lane))) {
+        if (active) rows.add_not_finite(seen, tl, vt);
+        __syncthreads();
+        make_finite<T, kShare>(share, lane);
+        __syncthreads();
+      }
+      if (active) rows.values(tl, vt);
     }
-    if (active) rows.values(tl, vt);
+  };
+  // An infinity or NaN in a hidden place would show in the sums (0 times it is
+  // NaN): only then the careful pass is taken.
+  pass(false);
+  bool odd = !(fabsf(rows.l) < __builtin_inff());
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) odd |= !(fabsf(rows.acc[dt][r]) < __builtin_inff());
+  if (__syncthreads_or(odd)) {
+    rows.clear();
+    pass(true);
   }
 
   const float l = rows.l + swap_halves(rows.l);

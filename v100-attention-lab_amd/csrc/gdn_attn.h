@@ -62,7 +62,18 @@ struct Ops<bf16_t> {
 constexpr float kLazy = 8.f;
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
-__device__ __forceinline__ float swap_halves(float x) { return __shfl_xor(x, 32, 64); }
+// The value of the lane in the other half (l ^ 32), without a way through LDS.
+__device__ __forceinline__ float swap_halves(float x) {
+  const uint32_t u = __float_as_uint(x);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+}
+// The larger of the two halves' values, in both.
+__device__ __forceinline__ float max_halves(float x) {
+  const uint32_t u = __float_as_uint(x);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
 
 // Registers 8 s .. 8 s + 7 of a product as the operand of the next one.
 template <typename T>
@@ -91,8 +102,8 @@ __device__ __forceinline__ void fed_products(Load load, Use use) {
     __builtin_amdgcn_sched_barrier(0);
   }
 }
-struct Triple {
-  uint4 a, b, c;
+struct Quad {
+  uint4 a, b, c, d;
 };
 
 // Accumulator row of register r.
@@ -124,11 +135,13 @@ __device__ __forceinline__ void dma_wait() {
   __builtin_amdgcn_s_waitcnt(7 << 4);   // vmcnt(0) lgkmcnt(0)
   asm volatile("" ::: "memory");
 }
-// A pointer that is the same in every lane, in scalar registers.
-__device__ __forceinline__ const void* uniform_ptr(const void* p) {
-  const uint64_t u = (uint64_t)(uintptr_t)p;
-  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)u), hi = __builtin_amdgcn_readfirstlane((uint32_t)(u >> 32));
-  return (const void*)(uintptr_t)(((uint64_t)hi << 32) | lo);
+// A value that is the same in every lane, in scalar registers.
+__device__ __forceinline__ int64_t uniform64(int64_t v) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+  return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ const uint16_t* uniform_ptr(const uint16_t* p) {
+  return (const uint16_t*)(uintptr_t)uniform64((int64_t)(uintptr_t)p);
 }
 
 // Rows of D 16-bit elements in LDS: groups of 1 KB (kGroup rows, one LDS-DMA of
@@ -193,7 +206,8 @@ struct Copier {
   int row, piece;    // of this lane in the first pass
   uint32_t ofs;      // its byte offset where that fits 31 bits
   bool small;
-  __device__ __forceinline__ Copier(const uint16_t* s, int64_t ld_, int rows_) : src(s), ld(ld_), rows(rows_) {
+  __device__ __forceinline__ Copier(const uint16_t* s, int64_t ld_, int rows_)
+      : src(uniform_ptr(s)), ld(ld_), rows(__builtin_amdgcn_readfirstlane(rows_)) {
     const int tid = threadIdx.x % NT;
     row = tid / TL::kPieces;
     piece = (tid % TL::kPieces) ^ TL::swz(row);
@@ -206,7 +220,7 @@ struct Copier {
     if (small && row0 + ROWS <= rows) {
 #pragma unroll
       for (int i = 0; i < kPasses; ++i)
-        dma16(uniform_ptr(src + (int64_t)(row0 + i * kPass) * ld), ofs, at + i * kStep);
+        dma16(src + (int64_t)(row0 + i * kPass) * ld, ofs, at + i * kStep);
     } else {
       int r = row0 + row;
       asm volatile("" : "+v"(r));     // (not kept in registers from tile to tile)
@@ -249,8 +263,8 @@ __device__ __forceinline__ Seq get_seq(const SeqArgs& a, int i) {
   } else {
     const int64_t b = clamp_row(a.cu[i], 0, a.Tq), e = clamp_row(a.cu[i + 1], b, a.Tq);
     s.b = 0;
-    s.q0 = s.k0 = b;
-    s.nq = s.nk = (int)(e - b);
+    s.q0 = s.k0 = uniform64(b);
+    s.nq = s.nk = __builtin_amdgcn_readfirstlane((int)(e - b));
   }
   return s;
 }
@@ -393,7 +407,7 @@ struct Rows {
     for (int t = 0; t < KS; ++t)
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[t][r]);
-    mx = fmaxf(mx, swap_halves(mx)) * scale_log2;
+    mx = max_halves(mx) * scale_log2;
     if (__any(mx > m + kLazy)) {
       // each row by its own scores, so that no row's bits depend on another's
       const float mn = mx > m + kLazy ? mx : m;

@@ -64,11 +64,23 @@ constexpr bool kScaled = std::is_same<T, f16>::value;
 template <typename T>
 constexpr float kPUp = kScaled<T> ? 14.f : 0.f;
 
-// The power of 2 at or above x (of fp16 values; 2^-24 for zero).
+// The power of 2 above x (of fp16 magnitudes; above 2^-24 for zero), and the
+// inverse of a power of 2: from the exponent's bits.
 __device__ __forceinline__ float pow2_above(float x) {
-  int e = 0;
-  (void)frexpf(fmaxf(x, 0x1p-24f), &e);
-  return ldexpf(1.f, e);
+  return __uint_as_float((__float_as_uint(fmaxf(x, 0x1p-24f)) & 0x7f800000u) + 0x00800000u);
+}
+__device__ __forceinline__ float pow2_inverse(float u) { return __uint_as_float(0x7f000000u - __float_as_uint(u)); }
+
+// The largest x of each 32 lanes, in all of them (16 by rotations of a row).
+__device__ __forceinline__ float max32(float x) {
+#define ROTATED(c) __uint_as_float(__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), c, 0xf, 0xf, false))
+  x = fmaxf(x, ROTATED(0x128));
+  x = fmaxf(x, ROTATED(0x124));
+  x = fmaxf(x, ROTATED(0x122));
+  x = fmaxf(x, ROTATED(0x121));
+#undef ROTATED
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
 // ---------------------------------------------------------------------------
@@ -202,7 +214,10 @@ __global__ __launch_bounds__(256 * QH, D == 64 && QH == 1 ? 3 : 2) void kv_kerne
   using TL = Tile<D>;
   constexpr uint32_t kTile = TL::bytes(kQT), kBuf = 2 * kTile + 1024;    // Q, dO, lse, D, max
   constexpr uint32_t kV = 2 * kBuf;                                           // the block's v rows
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[kV + TL::bytes(kKB)];
+  // the keys in registers, or (3 waves a SIMD) in LDS as well
+  constexpr bool kKeysInLds = D == 64 && QH == 1;
+  constexpr uint32_t kK = kV + TL::bytes(kKB);
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kK + (kKeysInLds ? TL::bytes(kKB) : 0)];
   const int unit_ix = blockIdx.x % a.units_k;
   const int unit = a.units_k % 8 == 0 ? (unit_ix % 8) * (a.units_k / 8) + unit_ix / 8 : unit_ix;
   // the segments last: they are short and fill the places of the blocks at the
@@ -243,9 +258,14 @@ __global__ __launch_bounds__(256 * QH, D == 64 && QH == 1 ? 3 : 2) void kv_kerne
   const int n = extra ? all : (int)((int64_t)all * (split + 1) / a.splits) - n0;
   Vec kf[D / 16];
   {
-    const uint16_t* kr = a.k + sq.b * a.ks[0] + (sq.k0 + min(key, sq.nk - 1)) * a.ks[1] + hk * a.ks[2];
+    if constexpr (kKeysInLds) {
+      const Copier<D, kKB, kKVT> ck(a.k + sq.b * a.ks[0] + sq.k0 * a.ks[1] + hk * a.ks[2], a.ks[1], sq.nk);
+      ck(base + kK, k0);
+    } else {
+      const uint16_t* kr = a.k + sq.b * a.ks[0] + (sq.k0 + min(key, sq.nk - 1)) * a.ks[1] + hk * a.ks[2];
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) kf[i] = as_vec<T>(*reinterpret_cast<const uint4*>(kr + 16 * i + 8 * half));
+      for (int i = 0; i < D / 16; ++i) kf[i] = as_vec<T>(*reinterpret_cast<const uint4*>(kr + 16 * i + 8 * half));
+    }
     const Copier<D, kKB, kKVT> cv(a.v + sq.b * a.vs[0] + sq.k0 * a.vs[1] + hk * a.vs[2], a.vs[1], sq.nk);
     cv(base + kV, k0);
   }
@@ -259,8 +279,8 @@ __global__ __launch_bounds__(256 * QH, D == 64 && QH == 1 ? 3 : 2) void kv_kerne
   const uint32_t vt = base + kV + TL::bytes(32) * kg;
   const int fr_first = rg.r0 + (n > 0 ? n0 % nt : 0) * kQT;
   const int fh = hk * a.G + (n > 0 ? n0 / nt : 0);
-  const uint16_t* const q_first = a.q + sq.b * a.qs[0] + sq.q0 * a.qs[1] + fh * a.qs[2];
-  const uint16_t* const d_first = a.dO + sq.b * a.dos[0] + sq.q0 * a.dos[1] + fh * a.dos[2];
+  const uint16_t* const q_first = uniform_ptr(a.q + sq.b * a.qs[0] + sq.q0 * a.qs[1] + fh * a.qs[2]);
+  const uint16_t* const d_first = uniform_ptr(a.dO + sq.b * a.dos[0] + sq.q0 * a.dos[1] + fh * a.dos[2]);
   const int64_t row_first = (int64_t)fh * a.rows + (int64_t)sq.b * a.seq.Tq + sq.q0;
   // the tile that is brought next: its rows and head
   int fr0;
@@ -317,26 +337,29 @@ __global__ __launch_bounds__(256 * QH, D == 64 && QH == 1 ? 3 : 2) void kv_kerne
       if constexpr (kScaled<T>) {
         // the unit of the wave's rows
         typedef __attribute__((address_space(3))) const float lds_float;
-        float m = *(lds_float*)(st + 512 + 4 * l32);
-#pragma unroll
-        for (int s = 16; s >= 1; s >>= 1) m = fmaxf(m, __shfl_xor(m, s, 64));
-        const float u = pow2_above(m);
-        if (u > unit_do) {
-          const float f = unit_do / u;
+        const float u = pow2_above(max32(*(lds_float*)(st + 512 + 4 * l32)));
+        if (__any(u > unit_do)) {
+          const float f = unit_do * pow2_inverse(u);
 #pragma unroll
           for (int i = 0; i < D / 32; ++i)
 #pragma unroll
             for (int r = 0; r < 16; ++r) dk[i][r] *= f;
           unit_do = u;
         }
-        sc = 0x1p-7f / (unit_do * vu);            // 2^7 / unit, and P's 2^14 taken out
+        sc = 0x1p-7f * pow2_inverse(unit_do * vu);   // 2^7 / unit, and P's 2^14 taken out
       }
       f32x16 s = {}, dp = {};
-      fed_products<D / 16, 2>([&](int i) { return Triple{tl.row8(qt, i), tl.row8(dt_, i), tl.row8(vt, i)}; },
-                              [&](int i, const Triple& x) {
-                                s = O::mfma(as_vec<T>(x.a), kf[i], s);
-                                dp = O::mfma(as_vec<T>(x.b), as_vec<T>(x.c), dp);
-                              });
+      fed_products<D / 16, 2>(
+          [&](int i) {
+            Quad x{tl.row8(qt, i), tl.row8(dt_, i), tl.row8(vt, i), {}};
+            if constexpr (kKeysInLds) x.d = tl.row8(vt + (kK - kV), i);
+            return x;
+          },
+          [&](int i, const Quad& x) {
+            if constexpr (kKeysInLds) s = O::mfma(as_vec<T>(x.a), as_vec<T>(x.d), s);
+            else s = O::mfma(as_vec<T>(x.a), kf[i], s);
+            dp = O::mfma(as_vec<T>(x.b), as_vec<T>(x.c), dp);
+          });
       typedef float f32x4v __attribute__((ext_vector_type(4)));
       typedef __attribute__((address_space(3))) const f32x4v lds_f32x4;
       if (bad) {
@@ -385,7 +408,7 @@ __global__ __launch_bounds__(256 * QH, D == 64 && QH == 1 ? 3 : 2) void kv_kerne
     }
     if (active) {
       constexpr int N = D / 32;
-      fed_products<4 * N, 4>(
+      fed_products<4 * N, D == 128 ? 4 : 2>(
           [&](int i) { return tl.col8(i & 1 ? qt : dt_, i / 2 % N, 16 * (i / (2 * N))); },
           [&](int i, const uint4& x) {
             const int t = i / (2 * N), d = i / 2 % N;
@@ -573,7 +596,7 @@ __global__ __launch_bounds__(256, 2) void q_kernel(const BArgs a) {
   float u = 1.f, sc = 1.f;
   if constexpr (kScaled<T>) {
     u = pow2_above(a.rmax[sat]) * v_unit(a, sq.b, hk, lane);
-    sc = 0x1p-7f / u;
+    sc = 0x1p-7f * pow2_inverse(u);
   }
   const float lb = kPUp<T> - st.x, de = -st.y * sc;
   f32x16 dq[D / 32] = {};

@@ -1,14 +1,14 @@
 // Windowed attention, backward:
 //     P = e^{scale q k^T - lse},  dP = dO v^T,  dS = P (dP - D),  D = dO . o
 //     dv = P^T dO,  dk = scale dS^T q,  dq = scale dS k
-// in three steps, each sum in one workgroup and in a fixed order:
-//   prep  per query row lse in powers of 2, D, and (fp16) the largest |dO|;
-//   kv    128 key rows a workgroup of 8 waves: query rows of all heads that
-//         share the key head pass in tiles of 64, a wave taking 32 keys and 32
-//         of the rows (S and dP with a lane on one key; P and dS enter dV^T +=
-//         dO^T P and dK^T += Q^T dS straight from their accumulators);
+// in two steps, each sum in one workgroup and in a fixed order:
 //   q     128 query rows a workgroup, 32 a wave, key tiles of 64 as in the
-//         forward: S^T, dP^T, dQ^T += K^T dS^T.
+//         forward: S^T, dP^T, dQ^T += K^T dS^T; it also leaves, per query row,
+//         lse in powers of 2, D and (fp16) the largest |dO|;
+//   kv    128 key rows a workgroup of 4 or 8 waves: query rows of all heads that
+//         share the key head pass in tiles of 32 or 64, a wave taking 32 keys
+//         and 32 of the rows (S and dP with a lane on one key; P and dS enter dV^T +=
+//         dO^T P and dK^T += Q^T dS straight from their accumulators);
 // Blocks of the first keys (the sinks) are seen by every later query row: the
 // rows beyond the block's window are cut into segments with workgroups of
 // their own, whose fp32 sums a last kernel adds in order.
@@ -84,7 +84,7 @@ __device__ __forceinline__ float max32(float x) {
 }
 
 // ---------------------------------------------------------------------------
-// prep
+// v
 // ---------------------------------------------------------------------------
 
 __device__ __forceinline__ float finite_abs(float x) {
@@ -92,60 +92,26 @@ __device__ __forceinline__ float finite_abs(float x) {
   return y < __builtin_inff() ? y : 0.f;
 }
 
-template <typename T, int D>
-__global__ __launch_bounds__(256) void prep_kernel(const BArgs a, int row_blocks) {
+// One part of the keys of one head: the largest |v|.
+template <int D>
+__global__ __launch_bounds__(256) void v_max_kernel(const BArgs a) {
   constexpr int L = D / 8, RPB = 256 / L;      // lanes a row, rows a workgroup
-  if ((int)blockIdx.x < row_blocks) {
-    // heads of a row are neighbours: reads of o and dO are in order
-    const int64_t at = (int64_t)blockIdx.x * RPB + threadIdx.x / L;
-    const int c = threadIdx.x % L;
-    const bool ok = at < a.rows * a.Hq;
-    const int64_t row = ok ? at / a.Hq : 0;
-    const int h = ok ? (int)(at % a.Hq) : 0;
-    const int64_t b = row / a.seq.Tq, t = row % a.seq.Tq;
-    rowio::Pack<T, 8> po, pd;
-    po.load(reinterpret_cast<const T*>(a.o) + b * a.os[0] + t * a.os[1] + h * a.os[2] + 8 * c);
-    pd.load(reinterpret_cast<const T*>(a.dO) + b * a.dos[0] + t * a.dos[1] + h * a.dos[2] + 8 * c);
-    float d = 0.f, m = 0.f;
+  const int part = blockIdx.x % kVParts, unit = blockIdx.x / kVParts;
+  const int b = unit / a.Hk, hk = unit % a.Hk;
+  const int n = (a.seq.Tk + kVParts - 1) / kVParts, t0 = part * n, t1 = min(t0 + n, a.seq.Tk);
+  float m = 0.f;
+  for (int t = t0 + threadIdx.x / L; t < t1; t += RPB) {
+    rowio::Pack<f16, 8> pv;
+    pv.load(reinterpret_cast<const f16*>(a.v) + b * a.vs[0] + (int64_t)t * a.vs[1] + hk * a.vs[2] + 8 * (threadIdx.x % L));
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float x = pd.get(e);
-      d = __builtin_fmaf(x, po.get(e), d);
-      if constexpr (kScaled<T>) m = fmaxf(m, finite_abs(x));
-    }
-#pragma unroll
-    for (int s = L / 2; s >= 1; s >>= 1) {
-      d += __shfl_xor(d, s, 64);
-      if constexpr (kScaled<T>) m = fmaxf(m, __shfl_xor(m, s, 64));
-    }
-    if (ok && c == 0) {
-      const float l = a.lse[at];
-      float* st = a.stat + ((int64_t)h * a.rows + row) * 2;
-      st[0] = l == -__builtin_inff() ? __builtin_inff() : l * kLog2e;
-      st[1] = d;
-      if constexpr (kScaled<T>) a.rmax[(int64_t)h * a.rows + row] = m;
-    }
-    return;
+    for (int i = 0; i < 8; ++i) m = fmaxf(m, finite_abs(pv.get(i)));
   }
-  if constexpr (kScaled<T>) {
-    // one part of one head's keys
-    const int e = blockIdx.x - row_blocks, part = e % kVParts, unit = e / kVParts;
-    const int b = unit / a.Hk, hk = unit % a.Hk;
-    const int n = (a.seq.Tk + kVParts - 1) / kVParts, t0 = part * n, t1 = min(t0 + n, a.seq.Tk);
-    float m = 0.f;
-    for (int t = t0 + threadIdx.x / L; t < t1; t += RPB) {
-      rowio::Pack<T, 8> pv;
-      pv.load(reinterpret_cast<const T*>(a.v) + b * a.vs[0] + (int64_t)t * a.vs[1] + hk * a.vs[2] + 8 * (threadIdx.x % L));
 #pragma unroll
-      for (int i = 0; i < 8; ++i) m = fmaxf(m, finite_abs(pv.get(i)));
-    }
-#pragma unroll
-    for (int s = 32; s >= 1; s >>= 1) m = fmaxf(m, __shfl_xor(m, s, 64));
-    __shared__ float sm[4];
-    if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
-    __syncthreads();
-    if (threadIdx.x == 0) a.vmax[unit * kVParts + part] = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-  }
+  for (int s = 32; s >= 1; s >>= 1) m = fmaxf(m, __shfl_xor(m, s, 64));
+  __shared__ float sm[4];
+  if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) a.vmax[unit * kVParts + part] = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
 }
 
 // The largest |v| of a head, as a power of 2.
@@ -518,6 +484,9 @@ __global__ __launch_bounds__(256) void part_sum_kernel(const BArgs a, int blocks
   const float* own = a.part + own_part(a, unit, si, block, slot, 0) * one;
   const int first = a.seq.cu == nullptr || a.seg == 0 ? 0 : (int)(sq.q0 / a.seg) + si;
   const int nseg = block < a.sink_blocks ? (sq.nq + a.seg - 1) / a.seg : 0;
+  // segments that end before the rows beyond the block's own have no part
+  const QRange mine = own_rows(a, sq, k0);
+  const int end = max(mine.r0, mine.r1), seg0 = nseg == 0 ? 0 : (end < sq.nq ? end / a.seg : nseg);
   const float* segs = a.part + (((int64_t)unit * a.sink_blocks + block) * a.slots_s + first) * one;
   for (int e = threadIdx.x; e < kRowsWg * D / 4; e += 256) {
     const int r = rg * kRowsWg + e / (D / 4), d = 4 * (e % (D / 4)), key = k0 + r;
@@ -535,9 +504,9 @@ __global__ __launch_bounds__(256) void part_sum_kernel(const BArgs a, int blocks
       };
 #pragma unroll 4
       for (int g = 1; g < a.splits; ++g) add(own + g * one);
-      for (int g = 0; g < nseg && key < a.sinks; ++g) {
-        const QRange q = seg_rows(a, sq, k0, g);
-        if (q.r1 > q.r0) add(segs + g * one);
+      if (key < a.sinks) {
+#pragma unroll 8
+        for (int g = seg0; g < nseg; ++g) add(segs + g * one);
       }
       uint16_t* out = w == 0 ? a.dk + sq.b * a.dks[0] + (sq.k0 + key) * a.dks[1] + hk * a.dks[2]
                              : a.dv + sq.b * a.dvs[0] + (sq.k0 + key) * a.dvs[1] + hk * a.dvs[2];
@@ -591,14 +560,38 @@ __global__ __launch_bounds__(256, 2) void q_kernel(const BArgs a) {
       df[i] = as_vec<T>(*reinterpret_cast<const uint4*>(dr + 16 * i + 8 * half));
     }
   }
-  const int64_t sat = (int64_t)head * a.rows + (int64_t)sq.b * a.seq.Tq + at;
-  const float2 st = *reinterpret_cast<const float2*>(a.stat + sat * 2);
+  // D = dO . o and the largest |dO| of the row, left for the kv step
+  float dsum = 0.f, dmax = 0.f;
+  {
+    const uint16_t* orow = a.o + sq.b * a.os[0] + at * a.os[1] + head * a.os[2];
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      rowio::Pack<T, 8> po, pd;
+      po.load(reinterpret_cast<const T*>(orow + 16 * i + 8 * half));
+      pd.raw = __builtin_bit_cast(uint4, df[i]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x = pd.get(e);
+        dsum = __builtin_fmaf(x, po.get(e), dsum);
+        if constexpr (kScaled<T>) dmax = fmaxf(dmax, finite_abs(x));
+      }
+    }
+  }
+  dsum += swap_halves(dsum);
+  const float l = a.lse[((int64_t)sq.b * a.seq.Tq + at) * a.Hq + head];
+  const float lse2 = l == -__builtin_inff() ? __builtin_inff() : l * kLog2e;
+  if constexpr (kScaled<T>) dmax = max_halves(dmax);
+  if (half == 0 && row < sq.nq) {
+    const int64_t sat = (int64_t)head * a.rows + (int64_t)sq.b * a.seq.Tq + at;
+    *reinterpret_cast<float2*>(a.stat + sat * 2) = make_float2(lse2, dsum);
+    if constexpr (kScaled<T>) a.rmax[sat] = dmax;
+  }
   float u = 1.f, sc = 1.f;
   if constexpr (kScaled<T>) {
-    u = pow2_above(a.rmax[sat]) * v_unit(a, sq.b, hk, lane);
+    u = pow2_above(dmax) * v_unit(a, sq.b, hk, lane);
     sc = 0x1p-7f * pow2_inverse(u);
   }
-  const float lb = kPUp<T> - st.x, de = -st.y * sc;
+  const float lb = kPUp<T> - lse2, de = -dsum * sc;
   f32x16 dq[D / 32] = {};
 
   const Copier<D, kKT, 256> ck(a.k + sq.b * a.ks[0] + sq.k0 * a.ks[1] + hk * a.ks[2], a.ks[1], sq.nk);
@@ -730,12 +723,12 @@ Space space(const GdnAttnParams& P) {
 
 template <typename T, int D>
 int launch(const BArgs& a, hipStream_t s) {
-  const int64_t rb = (a.rows * a.Hq + 256 / (D / 8) - 1) / (256 / (D / 8));
-  const int64_t vb = kScaled<T> ? (int64_t)a.B * a.Hk * kVParts : 0;
+  const int64_t vb = kScaled<T> && a.rows > 0 ? (int64_t)a.B * a.Hk * kVParts : 0;
   const int64_t kvb = (int64_t)a.units_k * ((int64_t)a.slots_k * a.splits + (int64_t)a.sink_blocks * a.slots_s);
   const int64_t qb = (int64_t)a.units_q * a.slots_q;
-  if (rb + vb > 0x7fffffffLL || kvb > 0x7fffffffLL || qb > 0x7fffffffLL) return GDN_ERR_BAD_SHAPE;
-  if (rb > 0) hipLaunchKernelGGL((prep_kernel<T, D>), dim3((uint32_t)(rb + vb)), dim3(256), 0, s, a, (int)rb);
+  if (vb > 0x7fffffffLL || kvb > 0x7fffffffLL || qb > 0x7fffffffLL) return GDN_ERR_BAD_SHAPE;
+  if (vb > 0) hipLaunchKernelGGL((v_max_kernel<D>), dim3((uint32_t)vb), dim3(256), 0, s, a);
+  if (qb > 0) hipLaunchKernelGGL((q_kernel<T, D>), dim3((uint32_t)qb), dim3(256), 0, s, a);
   if (kvb > 0) {
     if (a.kv_halves == 1) hipLaunchKernelGGL((kv_kernel<T, D, 1>), dim3((uint32_t)kvb), dim3(256), 0, s, a);
     else hipLaunchKernelGGL((kv_kernel<T, D, 2>), dim3((uint32_t)kvb), dim3(512), 0, s, a);
@@ -746,7 +739,6 @@ int launch(const BArgs& a, hipStream_t s) {
     if (pb > 0x7fffffffLL) return GDN_ERR_BAD_SHAPE;
     if (pb > 0) hipLaunchKernelGGL((part_sum_kernel<T, D>), dim3((uint32_t)pb), dim3(256), 0, s, a, (int)blocks);
   }
-  if (qb > 0) hipLaunchKernelGGL((q_kernel<T, D>), dim3((uint32_t)qb), dim3(256), 0, s, a);
   return (int)hipGetLastError();
 }
 

@@ -306,18 +306,50 @@ struct KeyRange {
 
 // Visibility of the accumulator rows of a lane whose column is query position
 // p: row c = 32 t + 8 (r / 4) + r % 4 of a key tile from j0 (the half's 4 rows
-// folded in) is seen where c <= hi and (c > lo or c < first).
+// folded in) is seen where c <= hi and (c > lo or c < first).  `ends` and
+// `starts` say (for the wave) whether any row's visible keys end, or start,
+// inside the tile, `firsts` whether the first keys reach into it.
 struct Mask {
   int hi, lo, first;
-  __device__ __forceinline__ Mask(int p, int j0, int half, int nk, int window, int sinks) {
+  bool ends, starts, firsts;
+  // The tile's keys [j0, j0 + n), the wave's positions [p0, p1].
+  __device__ __forceinline__ Mask(int p, int j0, int n, int half, int nk, int p0, int p1, int window, int sinks) {
     const int j = j0 + 4 * half;
     hi = min(p, nk - 1) - j;
     lo = (int)max((int64_t)p - window, (int64_t)-1) - j;
     first = sinks - j;
+    ends = j0 + n - 1 > p0 || j0 + n > nk;
+    starts = p1 - j0 >= window && j0 + n > sinks;
+    firsts = j0 < sinks;
   }
+  __device__ __forceinline__ bool any() const { return ends || starts; }
+  __device__ __forceinline__ static int at(int t, int r) { return 32 * t + 8 * (r >> 2) + (r & 3); }
   __device__ __forceinline__ bool operator()(int t, int r) const {
-    const int c = 32 * t + 8 * (r >> 2) + (r & 3);
+    const int c = at(t, r);
     return (c <= hi) & ((c > lo) | (c < first));
+  }
+  // x where it is seen, else `hidden`
+  template <int KS>
+  __device__ __forceinline__ void apply(f32x16 (&x)[KS], float hidden) const {
+    if (ends) {
+#pragma unroll
+      for (int t = 0; t < KS; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[t][r] = at(t, r) <= hi ? x[t][r] : hidden;
+    }
+    if (starts) {
+      if (firsts) {
+#pragma unroll
+        for (int t = 0; t < KS; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) x[t][r] = (at(t, r) > lo) | (at(t, r) < first) ? x[t][r] : hidden;
+      } else {
+#pragma unroll
+        for (int t = 0; t < KS; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) x[t][r] = at(t, r) > lo ? x[t][r] : hidden;
+      }
+    }
   }
 };
 
@@ -370,10 +402,10 @@ __device__ __forceinline__ typename Ops<T>::Vec signed_vec(const uint4& x, uint3
   return as_vec<T>(make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip));
 }
 
-// 32 query rows of a wave (lane l: row l % 32) against key tiles of 32 KS rows:
-// the running maximum m (in powers of 2, as the scores are), this lane's share
-// l of the sum, and O^T.
-template <typename T, int D, int KS>
+// 32 query rows of a wave (lane l: row l % 32) against key tiles of 32 KS rows
+// (KS up to MAX): the running maximum m (in powers of 2, as the scores are),
+// this lane's share l of the sum, and O^T.
+template <typename T, int D, int MAX>
 struct Rows {
   using O = Ops<T>;
   using Vec = typename O::Vec;
@@ -381,7 +413,7 @@ struct Rows {
   f32x16 acc[D / 32] = {};
   float m = -__builtin_inff(), l = 0.f;
 
-  Vec pf[2 * KS];
+  Vec pf[2 * MAX];
 
   __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -391,17 +423,13 @@ struct Rows {
   }
 
   // Scores and probabilities of one tile.
-  __device__ __forceinline__ void scores(const Vec (&qf)[D / 16], const TL& tl, uint32_t kt, bool masked, const Mask& seen,
+  template <int KS>
+  __device__ __forceinline__ void scores(const Vec (&qf)[D / 16], const TL& tl, uint32_t kt, const Mask& seen,
                                          float scale_log2) {
     f32x16 s[KS] = {};
     fed_products<KS * D / 16, 4>([&](int i) { return tl.row8(kt, i / KS, 32 * (i % KS)); },
                                  [&](int i, const uint4& x) { s[i % KS] = O::mfma(as_vec<T>(x), qf[i / KS], s[i % KS]); });
-    if (masked) {
-#pragma unroll
-      for (int t = 0; t < KS; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[t][r] = seen(t, r) ? s[t][r] : -__builtin_inff();
-    }
+    seen.apply<KS>(s, -__builtin_inff());
     float mx = s[0][0];
 #pragma unroll
     for (int t = 0; t < KS; ++t)
@@ -434,6 +462,7 @@ struct Rows {
   // What the infinities and NaN of a value tile add to the rows that see them:
   // two products of 0/1 matrices say which sums meet a +inf or NaN, and which a
   // -inf or NaN.
+  template <int KS>
   __device__ __forceinline__ void add_not_finite(const Mask& seen, const TL& tl, uint32_t vt) {
     constexpr uint32_t E = O::kExp, ONE = O::kOne;
 #pragma unroll
@@ -468,6 +497,7 @@ struct Rows {
   }
 
   // O^T += V^T P^T
+  template <int KS>
   __device__ __forceinline__ void values(const TL& tl, uint32_t vt) {
     constexpr int N = D / 32;
     fed_products<2 * KS * N, 4>([&](int i) { return tl.col8(vt, i % N, 16 * (i / N)); },

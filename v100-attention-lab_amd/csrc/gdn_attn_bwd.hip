@@ -616,9 +616,10 @@ __global__ __launch_bounds__(256, 2) void q_kernel(const BArgs a) {
     for (int h = 0; h < 2; ++h) {
       const int j0 = kr.tile(it) * kKT + 32 * h, j1 = min(j0 + 32, sq.nk) - 1;
       if (j0 >= sq.nk || none_visible(j0, j1, wp0, wp1, a.window, a.sinks)) continue;
-      const bool masked = !(j0 + 32 <= sq.nk && all_visible(j0, j1, wp0, wp1, a.window, a.sinks));
+      const Mask seen(p, j0, 32, half, sq.nk, wp0, wp1, a.window, a.sinks);
       const uint32_t kh = kt + TL::bytes(32) * h, vh = vt + TL::bytes(32) * h;
-      f32x16 s = {}, dp = {};
+      f32x16 s = {}, dps[1] = {};
+      f32x16& dp = dps[0];
       fed_products<D / 8, 4>([&](int i) { return tl.row8(i & 1 ? vh : kh, i / 2); },
                              [&](int i, const uint4& x) {
                                if (i & 1) dp = O::mfma(as_vec<T>(x), df[i / 2], dp);
@@ -629,13 +630,8 @@ __global__ __launch_bounds__(256, 2) void q_kernel(const BArgs a) {
         const float x = exp2_fast(__builtin_fmaf(s[r], a.scale_log2, lb));
         dp[r] = x * __builtin_fmaf(dp[r], sc, de);
       }
-      bool bad = false;
-      if (masked) {
-        const Mask seen(p, j0, half, sq.nk, a.window, a.sinks);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) dp[r] = seen(0, r) ? dp[r] : 0.f;
-        bad = careful && not_finite<T, 32 / TL::kGroup>(kh, lane);
-      }
+      seen.apply<1>(dps, 0.f);
+      const bool bad = careful && seen.any() && not_finite<T, 32 / TL::kGroup>(kh, lane);
       Vec sf[2];
 #pragma unroll
       for (int t = 0; t < 2; ++t) sf[t] = acc_operand<T>(dp, t);

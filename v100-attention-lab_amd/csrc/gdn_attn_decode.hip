@@ -108,16 +108,14 @@ __global__ __launch_bounds__(64 * kDWaves) void decode_kernel(const DArgs a) {
       fetch(other + kTile, vb, a.vs[1], j);
     }
     const uint32_t kt = base + (k & 1) * 2 * kTile;
-    const int j0 = kr.tile(t) * kDN, j1 = min(j0 + kDN, n) - 1;
-    const bool masked = !(j0 + kDN <= n && all_visible(j0, j1, p0, p1, a.window, a.sinks));
-    const Mask seen(p, j0, half, n, a.window, a.sinks);
-    rows.scores(qf, tl, kt, masked, seen, a.scale_log2);
+    const Mask seen(p, kr.tile(t) * kDN, kDN, half, n, p0, p1, a.window, a.sinks);
+    rows.template scores<1>(qf, tl, kt, seen, a.scale_log2);
     const uint32_t vt = kt + kTile;
-    if (masked && not_finite<T, kDN / TL::kGroup>(vt, lane)) {
-      rows.add_not_finite(seen, tl, vt);
+    if (seen.any() && not_finite<T, kDN / TL::kGroup>(vt, lane)) {
+      rows.template add_not_finite<1>(seen, tl, vt);
       make_finite<T, kDN / TL::kGroup>(vt, lane);
     }
-    rows.values(tl, vt);
+    rows.template values<1>(tl, vt);
   }
   rows.l += swap_halves(rows.l);
 

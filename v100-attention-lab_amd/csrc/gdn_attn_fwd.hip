@@ -79,10 +79,11 @@ __global__ __launch_bounds__(kNT, 2) void fwd_kernel(const FArgs a) {
   const Copier<D, kBN, kNT> ck(kb, a.ks[1], sq.nk), cv(vb, a.vs[1], sq.nk);
   const uint32_t base = lds_addr(lds);
   const TL tl(lane);
-  // One pass over the tiles.  careful: tiles on an edge of any wave's range are
-  // made finite where they are not, after what they hold has reached the rows
-  // that see it.
-  auto pass = [&](bool careful) {
+  // An infinity or NaN in a hidden place shows in the sums (0 times it is NaN):
+  // only then the pass over the tiles is taken again, carefully.  Tiles on an
+  // edge of any wave's range are then made finite where they are not, after
+  // what they hold has reached the rows that see it.
+  for (bool careful = false;; careful = true) {
     if (kr.n > 0) {
       ck(base, kr.tile(0) * kBN);
       cv(base + kTile, kr.tile(0) * kBN);
@@ -99,33 +100,27 @@ __global__ __launch_bounds__(kNT, 2) void fwd_kernel(const FArgs a) {
         cv(other + kTile, jn);
       }
       const int j1 = min(j0 + kBN, sq.nk) - 1;
-      const bool whole = j0 + kBN <= sq.nk, active = !none_visible(j0, j1, wp0, wp1, a.window, a.sinks);
-      const bool masked = !(whole && all_visible(j0, j1, wp0, wp1, a.window, a.sinks));
-      const Mask seen(p, j0, half, sq.nk, a.window, a.sinks);
+      const bool active = !none_visible(j0, j1, wp0, wp1, a.window, a.sinks);
+      const Mask seen(p, j0, kBN, half, sq.nk, wp0, wp1, a.window, a.sinks);
       constexpr int kShare = kBN / TL::kGroup / 4;
       const uint32_t share = vt + wv * kShare * TL::kGroupBytes;
-      if (active) rows.scores(qf, tl, kt, masked, seen, a.scale_log2);
-      if (careful && !(whole && all_visible(j0, j1, p0, p1, a.window, a.sinks)) &&
+      if (active) rows.template scores<2>(qf, tl, kt, seen, a.scale_log2);
+      if (careful && !(j0 + kBN <= sq.nk && all_visible(j0, j1, p0, p1, a.window, a.sinks)) &&
           __syncthreads_or(not_finite<T, kShare>(share, lane))) {
-        if (active) rows.add_not_finite(seen, tl, vt);
+        if (active) rows.template add_not_finite<2>(seen, tl, vt);
         __syncthreads();
         make_finite<T, kShare>(share, lane);
         __syncthreads();
       }
-      if (active) rows.values(tl, vt);
+      if (active) rows.template values<2>(tl, vt);
     }
-  };
-  // An infinity or NaN in a hidden place would show in the sums (0 times it is
-  // NaN): only then the careful pass is taken.
-  pass(false);
-  bool odd = !(fabsf(rows.l) < __builtin_inff());
+    bool odd = !(fabsf(rows.l) < __builtin_inff());
 #pragma unroll
-  for (int dt = 0; dt < D / 32; ++dt)
+    for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) odd |= !(fabsf(rows.acc[dt][r]) < __builtin_inff());
-  if (__syncthreads_or(odd)) {
+      for (int r = 0; r < 16; ++r) odd |= !(fabsf(rows.acc[dt][r]) < __builtin_inff());
+    if (careful || !__syncthreads_or(odd)) break;
     rows.clear();
-    pass(true);
   }
 
   const float l = rows.l + swap_halves(rows.l);

@@ -418,3 +418,38 @@ def test_many_key_blocks(pkg, cuda, D, dtype):
     _check(pkg, q, k, v, do, 130, 3)
     q, k, v, do = _inputs(cuda, 1, 5000, 5000, 16, 16, D, dtype, seed=22)
     _check(pkg, q, k, v, do, 200, 20, lens=[1999, 0, 1, 3000])
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_gradient_over_few_keys(pkg, cuda, D):
+    """Rows of few keys: D = sum P dP beside dP, where the rounding of o would
+    show.  In packed sequences of 1 to 40 rows what is left is the rounding of dS
+    and of the result, each uniform up to 2^-8: 3^-0.5 2^-8 each, (2 / 3)^0.5
+    2^-8 of the norm together.  A row with one key has dq = 0 but for the sums'
+    own rounding, 2^-20 of |dO| |v| |k|."""
+    lens = [1, 3, 40, 1, 17, 8, 25, 2, 9]
+    T, Hq, Hk = sum(lens), 4, 2
+    gen = torch.Generator().manual_seed(3)
+    q, k, v, do = (torch.randn(1, T, h, D, generator=gen).to(torch.bfloat16) for h in (Hq, Hk, Hk, Hq))
+    cu = torch.tensor([0] + lens).cumsum(0)
+    qc, kc, vc, dc = (t.to(cuda) for t in (q, k, v, do))
+    o, lse = pkg.window_attn(qc, kc, vc, 16, 1, cu_seqlens=cu.to(cuda), return_lse=True)
+    got = pkg.window_attn_bwd(qc, kc, vc, o, lse, dc, 16, 1, cu_seqlens=cu.to(cuda))
+    want = [torch.zeros_like(t, dtype=torch.float64) for t in (q, k, v)]
+    for s, e in zip(cu[:-1].tolist(), cu[1:].tolist()):
+        x, kk, vv, dd = (t[0, s:e].double() for t in (q, k, v, do))
+        kr, vr = kk.repeat_interleave(Hq // Hk, 1), vv.repeat_interleave(Hq // Hk, 1)
+        sc = torch.einsum("thd,shd->hts", x, kr) * D ** -0.5
+        i, j = torch.arange(e - s)[:, None], torch.arange(e - s)[None]
+        P = sc.masked_fill(~((j <= i) & ((j > i - 16) | (j < 1))), -torch.inf).softmax(-1)
+        dP = torch.einsum("thd,shd->hts", dd, vr)
+        dS = P * (dP - (P * dP).sum(-1, keepdim=True)) * D ** -0.5
+        want[0][0, s:e] = torch.einsum("hts,shd->thd", dS, kr)
+        want[1][0, s:e] = torch.einsum("hts,thd->shd", dS, x).view(e - s, Hk, -1, D).sum(2)
+        want[2][0, s:e] = torch.einsum("hts,thd->shd", P, dd).view(e - s, Hk, -1, D).sum(2)
+    for g, w in zip(got, want):
+        assert (g.cpu().double() - w).norm() <= (2 / 3) ** 0.5 * 2.0 ** -8 * w.norm()
+    first = [s for s in cu[:-1].tolist()]
+    size = (do[0, first].double().norm(dim=-1) * v[0, first].double().norm(dim=-1).repeat_interleave(2, -1)
+            * k[0, first].double().norm(dim=-1).repeat_interleave(2, -1))
+    assert (got[0][0, first].cpu().double().norm(dim=-1) <= 2.0 ** -20 * size).all()

@@ -29,6 +29,7 @@ constexpr int kKB = 128;       // key rows a workgroup (kv)
 constexpr int kSegRows = 64;   // rows of segments come in multiples of it
 constexpr int kQB = 128;       // query rows a workgroup (q)
 constexpr int kKT = 64;        // keys a tile (q)
+constexpr int kFewTiles = 4;   // up to so many key tiles a block of rows sums D itself (q)
 constexpr int kVParts = 64;    // partial maxima of |v| a head
 
 struct BArgs {
@@ -560,9 +561,68 @@ __global__ __launch_bounds__(256, 2) void q_kernel(const BArgs a) {
       df[i] = as_vec<T>(*reinterpret_cast<const uint4*>(dr + 16 * i + 8 * half));
     }
   }
-  // D = dO . o and the largest |dO| of the row, left for the kv step
-  float dsum = 0.f, dmax = 0.f;
-  {
+  // the largest |dO| of the row, left for the kv step
+  float dmax = 0.f;
+  if constexpr (kScaled<T>) {
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) dmax = fmaxf(dmax, finite_abs((float)df[i][e]));
+    dmax = max_halves(dmax);
+  }
+  const float l = a.lse[((int64_t)sq.b * a.seq.Tq + at) * a.Hq + head];
+  const float lse2 = l == -__builtin_inff() ? __builtin_inff() : l * kLog2e;
+  const Copier<D, kKT, 256> ck(a.k + sq.b * a.ks[0] + sq.k0 * a.ks[1] + hk * a.ks[2], a.ks[1], sq.nk);
+  const Copier<D, kKT, 256> cv(a.v + sq.b * a.vs[0] + sq.k0 * a.vs[1] + hk * a.vs[2], a.vs[1], sq.nk);
+  const uint32_t base = lds_addr(lds);
+  const TL tl(lane);
+  // One walk over the key tiles: f(tile's K and V, its first key) for each half
+  // of a tile that any of the wave's rows sees.
+  auto walk = [&](auto f) {
+    if (kr.n > 0) {
+      ck(base, kr.tile(0) * kKT);
+      cv(base + kTile, kr.tile(0) * kKT);
+    }
+    for (int it = 0; it < kr.n; ++it) {
+      const uint32_t kt = base + (it & 1) * 2 * kTile, vt = kt + kTile;
+      dma_wait();
+      __syncthreads();
+      if (it + 1 < kr.n) {
+        const uint32_t other = base + ((it + 1) & 1) * 2 * kTile;
+        ck(other, kr.tile(it + 1) * kKT);
+        cv(other + kTile, kr.tile(it + 1) * kKT);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int j0 = kr.tile(it) * kKT + 32 * h, j1 = min(j0 + 32, sq.nk) - 1;
+        if (j0 >= sq.nk || none_visible(j0, j1, wp0, wp1, a.window, a.sinks)) continue;
+        f(kt + TL::bytes(32) * h, vt + TL::bytes(32) * h, j0);
+      }
+    }
+  };
+  auto products = [&](uint32_t kh, uint32_t vh, f32x16& s, f32x16& dp) {
+    fed_products<D / 8, 4>([&](int i) { return tl.row8(i & 1 ? vh : kh, i / 2); },
+                           [&](int i, const uint4& x) {
+                             if (i & 1) dp = O::mfma(as_vec<T>(x), df[i / 2], dp);
+                             else s = O::mfma(as_vec<T>(x), qf[i / 2], s);
+                           });
+  };
+  // D = dO . o.  Over few keys the rounding of o shows in dP - D (a row with one
+  // key has dP = D): there D is the sum of P dP instead, from a walk of its own.
+  float dsum = 0.f;
+  if (kr.n <= kFewTiles) {
+    walk([&](uint32_t kh, uint32_t vh, int j0) {
+      const Mask seen(p, j0, 32, half, sq.nk, wp0, wp1, a.window, a.sinks);
+      f32x16 s = {}, x[1] = {};
+      products(kh, vh, s, x[0]);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[0][r] *= exp2_fast(__builtin_fmaf(s[r], a.scale_log2, -lse2));
+      seen.apply<1>(x, 0.f);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dsum += x[0][r];
+    });
+    __syncthreads();      // the next walk begins with the first buffer
+  } else {
     const uint16_t* orow = a.o + sq.b * a.os[0] + at * a.os[1] + head * a.os[2];
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) {
@@ -570,17 +630,10 @@ __global__ __launch_bounds__(256, 2) void q_kernel(const BArgs a) {
       po.load(reinterpret_cast<const T*>(orow + 16 * i + 8 * half));
       pd.raw = __builtin_bit_cast(uint4, df[i]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float x = pd.get(e);
-        dsum = __builtin_fmaf(x, po.get(e), dsum);
-        if constexpr (kScaled<T>) dmax = fmaxf(dmax, finite_abs(x));
-      }
+      for (int e = 0; e < 8; ++e) dsum = __builtin_fmaf(pd.get(e), po.get(e), dsum);
     }
   }
   dsum += swap_halves(dsum);
-  const float l = a.lse[((int64_t)sq.b * a.seq.Tq + at) * a.Hq + head];
-  const float lse2 = l == -__builtin_inff() ? __builtin_inff() : l * kLog2e;
-  if constexpr (kScaled<T>) dmax = max_halves(dmax);
   if (half == 0 && row < sq.nq) {
     const int64_t sat = (int64_t)head * a.rows + (int64_t)sq.b * a.seq.Tq + at;
     *reinterpret_cast<float2*>(a.stat + sat * 2) = make_float2(lse2, dsum);
@@ -594,37 +647,12 @@ __global__ __launch_bounds__(256, 2) void q_kernel(const BArgs a) {
   const float lb = kPUp<T> - lse2, de = -dsum * sc;
   f32x16 dq[D / 32] = {};
 
-  const Copier<D, kKT, 256> ck(a.k + sq.b * a.ks[0] + sq.k0 * a.ks[1] + hk * a.ks[2], a.ks[1], sq.nk);
-  const Copier<D, kKT, 256> cv(a.v + sq.b * a.vs[0] + sq.k0 * a.vs[1] + hk * a.vs[2], a.vs[1], sq.nk);
-  const uint32_t base = lds_addr(lds);
-  const TL tl(lane);
   auto pass = [&](bool careful) {
-  if (kr.n > 0) {
-    ck(base, kr.tile(0) * kKT);
-    cv(base + kTile, kr.tile(0) * kKT);
-  }
-  for (int it = 0; it < kr.n; ++it) {
-    const uint32_t kt = base + (it & 1) * 2 * kTile, vt = kt + kTile;
-    dma_wait();
-    __syncthreads();
-    if (it + 1 < kr.n) {
-      const uint32_t other = base + ((it + 1) & 1) * 2 * kTile;
-      ck(other, kr.tile(it + 1) * kKT);
-      cv(other + kTile, kr.tile(it + 1) * kKT);
-    }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int j0 = kr.tile(it) * kKT + 32 * h, j1 = min(j0 + 32, sq.nk) - 1;
-      if (j0 >= sq.nk || none_visible(j0, j1, wp0, wp1, a.window, a.sinks)) continue;
+    walk([&](uint32_t kh, uint32_t vh, int j0) {
       const Mask seen(p, j0, 32, half, sq.nk, wp0, wp1, a.window, a.sinks);
-      const uint32_t kh = kt + TL::bytes(32) * h, vh = vt + TL::bytes(32) * h;
       f32x16 s = {}, dps[1] = {};
       f32x16& dp = dps[0];
-      fed_products<D / 8, 4>([&](int i) { return tl.row8(i & 1 ? vh : kh, i / 2); },
-                             [&](int i, const uint4& x) {
-                               if (i & 1) dp = O::mfma(as_vec<T>(x), df[i / 2], dp);
-                               else s = O::mfma(as_vec<T>(x), qf[i / 2], s);
-                             });
+      products(kh, vh, s, dp);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const float x = exp2_fast(__builtin_fmaf(s[r], a.scale_log2, lb));
@@ -646,8 +674,7 @@ __global__ __launch_bounds__(256, 2) void q_kernel(const BArgs a) {
         fed_products<2 * N, 4>([&](int i) { return tl.col8(kh, i % N, 16 * (i / N)); },
                                [&](int i, const uint4& x) { dq[i % N] = O::mfma(as_vec<T>(x), sf[i / N], dq[i % N]); });
       }
-    }
-  }
+    });
   };
   // (see kv_kernel)
   pass(false);

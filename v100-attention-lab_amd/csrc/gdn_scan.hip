@@ -240,7 +240,7 @@ __device__ __forceinline__ void leave(const Args& p, const Join<V>& sh, uint32_t
 // The state h (of this lane's V channels) behind the places first .. u - 1, in
 // order: single places up to a set's start, whole sets, single places again.
 // Each wave takes a share of these pairs; the shares are joined in LDS.
-template <int V>
+template <int V, int BATCH>
 __device__ __forceinline__ void carry(const Args& p, Join<V>& sh, uint32_t first, uint32_t u, int c, bool ok,
                                       float (&h)[V]) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
@@ -261,26 +261,25 @@ __device__ __forceinline__ void carry(const Args& p, Join<V>& sh, uint32_t first
 #pragma unroll
   for (int e = 0; e < V; ++e) G[e] = H[e] = 0.f;
   if (ok) {
-    constexpr int kBatch = 4;
 #pragma unroll 1
-    for (int k = k0; k < k1; k += kBatch) {
-      uint64_t v[kBatch][V];
+    for (int k = k0; k < k1; k += BATCH) {
+      uint64_t v[BATCH][V];
       bool all;
       do {
         all = true;
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
+        for (int i = 0; i < BATCH; ++i) {
           const uint64_t* a = at(min(k + i, k1 - 1));
 #pragma unroll
           for (int e = 0; e < V; ++e) v[i][e] = look(a + e);
         }
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i)
+        for (int i = 0; i < BATCH; ++i)
 #pragma unroll
           for (int e = 0; e < V; ++e) all &= v[i][e] != kAbsent;
       } while (!all);
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
+      for (int i = 0; i < BATCH; ++i) {
         if (k + i < k1) {
 #pragma unroll
           for (int e = 0; e < V; ++e) {
@@ -307,10 +306,16 @@ __device__ __forceinline__ void carry(const Args& p, Join<V>& sh, uint32_t first
 // forward
 // ---------------------------------------------------------------------------
 
+// 16-bit gates: e^g is formed again in the second walk instead of held, which
+// leaves room for 6 waves a SIMD (B4 T4096 D2048 bf16: 67.3 us; held, 4 waves,
+// 73.5).  32-bit gates hold it: 6 waves would spill (90 us; 4 waves 75.5).
+template <typename TX, typename TG>
+constexpr bool kMore = sizeof(TX) == 2 && sizeof(TG) == 2;
+
 // y, the final states and (not nullptr) the states at the chunks' starts.
 // ONLY_STATES: those alone.  single: every sequence is one chunk.
 template <typename TX, typename TG, int V, bool ONLY_STATES>
-__global__ __launch_bounds__(kThreads, 4) void fwd_kernel(const Args p, bool single) {
+__global__ __launch_bounds__(kThreads, (kMore<TX, TG> ? 6 : 4)) void fwd_kernel(const Args p, bool single) {
   uint32_t blk;
   const uint32_t slot = next_place(p, single, blk);
   const Job j = slot_job(p, (int)slot);
@@ -327,7 +332,8 @@ __global__ __launch_bounds__(kThreads, 4) void fwd_kernel(const Args p, bool sin
   float h[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) h[e] = ok && p.h0 != nullptr ? p.h0[j.seq * p.h0s + c + e] : 0.f;
-  float a[kRows][V], G[V], H[V];
+  constexpr bool kHold = sizeof(TG) == 4;
+  float a[kHold ? kRows : 1][V], G[V], H[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) G[e] = H[e] = 0.f;
 #pragma unroll
@@ -335,13 +341,17 @@ __global__ __launch_bounds__(kThreads, 4) void fwd_kernel(const Args p, bool sin
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       // rows past the end: g = 0 and x = 0 keep the state
-      a[i][e] = decay(gr[i].get(e));
-      H[e] = step(a[i][e], H[e], xr[i].get(e));
+      const float t = decay(gr[i].get(e));
+      if constexpr (kHold) a[i][e] = t;
+      H[e] = step(t, H[e], xr[i].get(e));
       G[e] += gr[i].get(e);
     }
   }
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) xr[i].repack();
+  for (int i = 0; i < kRows; ++i) {
+    xr[i].repack();
+    if constexpr (!kHold) gr[i].repack();
+  }
   __shared__ Join<V> waves, shares;
 #pragma unroll
   for (int e = 0; e < V; ++e) {
@@ -352,7 +362,7 @@ __global__ __launch_bounds__(kThreads, 4) void fwd_kernel(const Args p, bool sin
   if (!single) {
     leave<V, false>(p, waves, slot, (int)blk * 64 * V);
     if (j.chunk < 0) return;
-    carry<V>(p, shares, (uint32_t)j.first, slot, c, ok, h);
+    carry<V, kMore<TX, TG> ? 2 : 4>(p, shares, (uint32_t)j.first, slot, c, ok, h);
   }
   if (j.chunk < 0 || !ok) return;
   if (p.states != nullptr && w == 0) {
@@ -369,7 +379,12 @@ __global__ __launch_bounds__(kThreads, 4) void fwd_kernel(const Args p, bool sin
   for (int i = 0; i < kRows; ++i) {
     if (i < n) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) h[e] = step(a[i][e], h[e], xr[i].get(e));
+      for (int e = 0; e < V; ++e) {
+        float t;
+        if constexpr (kHold) t = a[i][e];
+        else t = decay(gr[i].get(e));
+        h[e] = step(t, h[e], xr[i].get(e));
+      }
       Pack<TX, V> o;
       o.set(h);
       o.store(y + i * p.ys[1]);
@@ -454,7 +469,7 @@ __global__ __launch_bounds__(kThreads, 4) void bwd_kernel(const Args p, bool sin
     leave<V, true>(p, waves, u, (int)blk * 64 * V);
     if (j.chunk < 0) return;
     const uint32_t last = j.first + (uint32_t)max((j.len + kChunk - 1) / kChunk, 1) - 1;
-    carry<V>(p, shares, p.slots - 1 - last, u, c, ok, d);
+    carry<V, 4>(p, shares, p.slots - 1 - last, u, c, ok, d);
   }
   if (j.chunk < 0 || !ok) return;
   TX* dx = static_cast<TX*>(p.dx) + j.b * p.dxs[0] + row * p.dxs[1] + c;

@@ -136,6 +136,8 @@ __global__ __launch_bounds__(64 * kDWaves) void decode_kernel(const DArgs a) {
   __syncthreads();
   // thread: row c = tid / 8, D / 8 columns from 8 neighbouring threads
   const int c = threadIdx.x >> 3, d0 = (threadIdx.x & 7) * (D / 8);
+  const QRow row(a, hk, rt, c);
+  if (!row.ok) return;
   float top = sm[c];
 #pragma unroll
   for (int w = 1; w < kDWaves; ++w) top = fmaxf(top, sm[w * 32 + c]);
@@ -164,10 +166,8 @@ __global__ __launch_bounds__(64 * kDWaves) void decode_kernel(const DArgs a) {
       *reinterpret_cast<float4*>(part + 64 + c * D + d0 + e) = make_float4(out[e], out[e + 1], out[e + 2], out[e + 3]);
     return;
   }
-  const QRow w(a, hk, rt, c);
-  if (!w.ok) return;
   const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-  uint16_t* o = a.o + b * a.os[0] + w.t * a.os[1] + w.h * a.os[2] + d0;
+  uint16_t* o = a.o + b * a.os[0] + row.t * a.os[1] + row.h * a.os[2] + d0;
 #pragma unroll
   for (int e = 0; e < D / 8; e += 2) *reinterpret_cast<uint32_t*>(o + e) = O::pack(out[e] * inv, out[e + 1] * inv);
 }
@@ -237,11 +237,14 @@ int row_tiles(const GdnAttnDecodeParams& P) { return (P.Hq / P.Hk * P.T + 31) / 
 
 // Workgroups a sequence and key head: one a CU (their tiles fill its LDS; 32
 // sequences of 4 key heads with 4100 keys: 55 us with 256 workgroups, 60 with
-// 512, 66 with 1024), of at least one tile a wave, over the tiles that the
-// longest sequence can have.
+// 512, 66 with 1024), over the tiles that the longest sequence can have.  Up to
+// 4 tiles a wave stay in one workgroup: the join costs as much (a sequence of 4
+// key heads, head size 128, one workgroup / joined: 128 keys 7.5 / 10.0 us, 512
+// keys 10.6 / 10.8, 1024 keys 15.0 / 11.0, 4096 keys 40.0 / 11.9).
 int splits_of(const GdnAttnDecodeParams& P) {
   const int64_t keys = std::min<int64_t>(P.S, (int64_t)P.window + P.T - 1 + P.sinks);
   const int64_t tiles = keys / kDN + 2;
+  if (tiles <= 4 * kDWaves + 2) return 1;
   const int64_t units = (int64_t)P.B * P.Hk * row_tiles(P);
   const int64_t want = (256 + units - 1) / units;
   return (int)std::max<int64_t>(1, std::min({want, (tiles + kDWaves - 1) / kDWaves, (int64_t)kMaxSplits}));

@@ -116,7 +116,7 @@ def _run(q, k, v, window, sinks, scale, cu, n_seq, need_lse):
     elif not _aligned(q, k, v):
         _validate(q, k, v)
     o = _like(q)
-    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if need_lse else None
+    lse = q.new_empty(q.shape[:3], dtype=torch.float32) if need_lse else None
     P = _lib.GdnAttnParams.from_buffer_copy(plan)
     P.q, P.k, P.v, P.o = q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr()
     P.lse = lse.data_ptr() if lse is not None else None
@@ -307,7 +307,7 @@ def window_attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
     if lens.dtype != torch.int32 or not lens.is_contiguous():
         lens = lens.clamp(0, k_cache.shape[1]).to(torch.int32).contiguous()
     o = _like(q)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes > 0 else None
+    ws = q.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes > 0 else None
     P = _lib.GdnAttnDecodeParams.from_buffer_copy(params)
     P.q, P.k, P.v, P.o = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr()
     P.cache_seqlens = lens.data_ptr()

@@ -98,7 +98,7 @@ def _run(x, weight, residual, eps, fp8, group):
     params, shape_scale = plan
     dev = x.device
     y = _like(x, torch.float8_e4m3fn if fp8 else None)
-    scale = torch.empty(shape_scale, dtype=torch.float32, device=dev) if fp8 else None
+    scale = x.new_empty(shape_scale, dtype=torch.float32) if fp8 else None
     P = _lib.GdnNormParams.from_buffer_copy(params)
     P.x, P.w, P.y = x3.data_ptr(), weight.data_ptr(), y.data_ptr()
     r = x
@@ -201,7 +201,7 @@ def _run_bwd(r, weight, dy, dr, eps, need_dx):
     out = _like(r)
     dx = _like(dy) if need_dx else None
     dw = _like(weight)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    ws = r.new_empty(ws_bytes, dtype=torch.uint8)
     P = _lib.GdnNormParams.from_buffer_copy(params)
     P.r, P.w, P.dy = r3.data_ptr(), weight.data_ptr(), dy3.data_ptr()
     P.dr_in = dr3.data_ptr() if dr is not None else None

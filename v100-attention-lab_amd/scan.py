@@ -111,9 +111,9 @@ def _run(x, g, h0, cu, n_seq, return_states):
     params, ws_bytes, shape_fs, shape_st = plan
     dev = x.device
     y = _like(x)
-    fs = _like(h0) if h0 is not None else torch.empty(shape_fs, dtype=torch.float32, device=dev)
-    states = torch.empty(shape_st, dtype=torch.float32, device=dev) if return_states else None
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes > 0 else None
+    fs = _like(h0) if h0 is not None else x.new_empty(shape_fs, dtype=torch.float32)
+    states = x.new_empty(shape_st, dtype=torch.float32) if return_states else None
+    ws = x.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes > 0 else None
     P = _lib.GdnScanParams.from_buffer_copy(params)
     P.x, P.g = x.data_ptr(), g.data_ptr()
     P.h0 = h0.data_ptr() if h0 is not None else None
@@ -213,8 +213,8 @@ def _run_bwd(x, g, h0, dy, dfinal, states, cu, n_seq, need_dh0):
     params, ws_bytes, shape_dh0 = plan
     dev = x.device
     dx, dg = _like(x), _like(g)
-    dh0 = torch.empty(shape_dh0, dtype=torch.float32, device=dev) if shape_dh0 is not None else None
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes > 0 else None
+    dh0 = x.new_empty(shape_dh0, dtype=torch.float32) if shape_dh0 is not None else None
+    ws = x.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes > 0 else None
     P = _lib.GdnScanParams.from_buffer_copy(params)
     P.x, P.g, P.dy = x.data_ptr(), g.data_ptr(), dy.data_ptr()
     P.h0 = h0.data_ptr() if h0 is not None else None

@@ -111,6 +111,19 @@ def test_fp8(pkg, cuda, xd, rd, rows, D, group):
     _fp8_check(pkg, x, w, None, group)
 
 
+@pytest.mark.parametrize("rows,D", [(33, 64), (17, 72), (19, 128), (9, 136), (2100, 256), (5, 264), (13, 512), (6, 1016),
+                                    (37, 63), (40, 65), (9, 101), (21, 133), (3, 255), (7, 257), (9000, 101), (5, 513)])
+def test_rows_of_part_of_a_wave(pkg, cuda, rows, D):
+    """Rows held by 8, 16 or 32 lanes, 8 columns and one column at a time."""
+    for xd, rd in TYPES:
+        x, res, w, dy, dr = _inputs(cuda, (rows, D), xd, rd, torch.float32, seed=rows + D)
+        r = _fwd_check(pkg, x, w, res)
+        _bwd_check(pkg, r, w, dy, dr)
+        _fp8_check(pkg, x, w, res, None)
+        if D % 128 == 0:
+            _fp8_check(pkg, x, w, res, 128)
+
+
 @pytest.mark.parametrize("group", [None, 128])
 def test_fp8_misaligned(pkg, cuda, group):
     x, res, w, _, _ = _inputs(cuda, (6, 258), torch.bfloat16, torch.bfloat16, torch.float32, seed=2)

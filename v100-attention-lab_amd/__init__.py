@@ -2,7 +2,10 @@
 
 The hot path of ``v100-attention-lab`` (``gdn_chunk_fwd``,
 gdn_triton.py:113-140) as a hand-written gfx950 HIP kernel behind a C ABI
-(``include/gdn_mi355x.h``), called from PyTorch-ROCm through ctypes.
+(``include/gdn_mi355x.h``), called from PyTorch-ROCm through ctypes, and the
+operators that a hybrid model runs beside it: ``gated_scan`` (an elementwise
+gated recurrence), ``window_attn`` (softmax attention with a sliding window and
+sinks) and ``add_rms_norm``, with their backward and single-token forms.
 
 The directory name is not a Python identifier; import it with
 ``importlib.import_module("v100-attention-lab_amd")`` -- it also registers

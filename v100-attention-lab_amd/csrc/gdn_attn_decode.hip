@@ -7,7 +7,10 @@
 // The waves are joined in LDS; with more than one split the workgroups leave
 // (m, l, O) in the workspace and a second kernel joins them, in order.
 //
-// Bound by reading the cache rows once.
+// Bound by reading the cache rows once (32 sequences, 4 key heads of 128, 4100
+// visible keys, bf16: 51 us with the call, 5.3 TB/s), and for few sequences by the
+// chain of one workgroup and the join (one sequence of the same: 8 us and 4 us
+// for 8.4 MB).
 
 #include <algorithm>
 

@@ -4,13 +4,16 @@
 //     dr = dr_in + rstd (w dy - n mean(w dy n)),  dw = sum_rows dy n
 //
 // A row is read once, held in registers in fp32 and written once: a team of
-// 64 or 256 threads takes a row, each thread P pieces of V columns.  Rows
+// 8 to 256 threads takes a row, each thread P pieces of V columns.  Rows
 // that do not fit the registers, and 128-column scales of rows without
 // 16-byte alignment, are read a second time (long kernels).
 // dw: every workgroup sums its rows' dy n in registers, in row order, and
 // writes one partial row; a second kernel adds the partial rows in order.
 //
-// Bound by memory.
+// Bound by memory.  16384 rows of 2048, bf16 with an fp32 residual stream:
+// forward 71 us (403 MB, 5.7 TB/s), backward 98 us (470 MB, 4.8 TB/s) and 5 us
+// for dw's partial rows; 8192 rows of 4096 to 8 bits with 128-column scales 47 us
+// with the call (235 MB, 5.0 TB/s).  A large copy: 4.9 TB/s.
 
 #include <algorithm>
 
@@ -52,9 +55,10 @@ __device__ __forceinline__ int64_t row_at(const Args& p, uint32_t row, const int
   return (int64_t)o * s[0] + (int64_t)i * s[1];
 }
 
-__device__ __forceinline__ float wave_sum(float v) {
+template <int W>
+__device__ __forceinline__ float lanes_sum(float v) {
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+  for (int o = W / 2; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
   return v;
 }
 // The larger of two; NaN where either is.
@@ -66,11 +70,12 @@ __device__ __forceinline__ float lanes_max(float v) {
   return v;
 }
 
-// Sum over a team of TEAM threads (a wave, or the block's waves through LDS;
+// Sum over a team of TEAM threads (a wave or less, or the block's waves through LDS;
 // each use has a slot of its own, so no wait is needed after the read).
 template <int TEAM, bool MAX>
 __device__ __forceinline__ float team_reduce(float v, float* slot) {
-  v = MAX ? lanes_max<64>(v) : wave_sum(v);
+  constexpr int W = TEAM < 64 ? TEAM : 64;
+  v = MAX ? lanes_max<W>(v) : lanes_sum<W>(v);
   if constexpr (TEAM > 64) {
     constexpr int NW = TEAM / 64;
     if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = v;
@@ -136,7 +141,7 @@ __global__ __launch_bounds__(kBlock) void fwd_kernel(const Args p) {
   constexpr int ROWS = kBlock / TEAM;
   const int t = threadIdx.x % TEAM;
   const uint32_t row = blockIdx.x * ROWS + threadIdx.x / TEAM;
-  if (TEAM == 64 && row >= p.rows) return;   // no barrier below for these
+  if (TEAM <= 64 && row >= p.rows) return;   // no barrier below for these
   const TX* x = static_cast<const TX*>(p.x) + row_at(p, row, p.xs);
   Pack<TX, V> xr[P];
   Pack<TR, V> rr[P];
@@ -340,13 +345,11 @@ __global__ __launch_bounds__(kBlock) void bwd_kernel(const Args p) {
         sd = __builtin_fmaf(w[i][e] * yr[i].get(e), v, sd);
       }
     }
-    if constexpr (TEAM == 64) {
-      ss = wave_sum(ss);
-      sd = wave_sum(sd);
-    } else {
+    constexpr int W = TEAM < 64 ? TEAM : 64;
+    ss = lanes_sum<W>(ss);
+    sd = lanes_sum<W>(sd);
+    if constexpr (TEAM > 64) {
       // two sums behind one barrier; the slots alternate between rows
-      ss = wave_sum(ss);
-      sd = wave_sum(sd);
       if ((threadIdx.x & 63) == 0) {
         slots[turn][0][threadIdx.x >> 6] = ss;
         slots[turn][1][threadIdx.x >> 6] = sd;
@@ -488,21 +491,39 @@ __global__ __launch_bounds__(1024) void dw_sum_kernel(const Args p) {
   }
 }
 
-// The team and pieces that hold a row, or 0 pieces: it does not fit.
+// The team and pieces that hold a row, or 0 pieces: it does not fit.  The
+// smallest team whose threads hold the row in 4 pieces of 8 columns (1 or 2 of
+// the shortest rows) or 16 of one: fewer steps between lanes, no barrier up to a
+// wave, and enough bytes in flight for the backward's 512 workgroups.  bf16, 2^25
+// columns in all, forward / backward in us:
+//   8 columns: D 64 8 lanes 41 / 47, 64 lanes 157 / 301; D 256 16 lanes 41 / 41,
+//     64 lanes 46 / 82; D 1024 32 lanes 42 / 39, 64 lanes 41 / 41, 256 lanes
+//     52 / 102; D 2048 64 lanes 43 / 38, 256 lanes 41 / 58; D 4096 256 lanes
+//     41 / 41, 64 lanes of 8 pieces 46 / 53; no registers (long) 76 / 114;
+//   one column: D 63 16 lanes 58 / 129, 256 lanes 506 / 1275; D 255 16 lanes
+//     58 / 103, 256 lanes 138 / 349; D 1001 64 lanes 53 / 118, 256 lanes 66 / 153;
+//     D 2047 256 lanes 59 / 137, 64 lanes 72 / 117.
 struct Shape {
   int v, p, team;
 };
 Shape shape_of(int D, bool wide) {
   if (wide) {
-    if (D <= 512) return {8, 1, 64};
-    if (D <= 1024) return {8, 2, 64};
+    if (D <= 64) return {8, 1, 8};
+    if (D <= 128) return {8, 1, 16};
+    if (D <= 256) return {8, 2, 16};
+    if (D <= 512) return {8, 4, 16};
+    if (D <= 1024) return {8, 4, 32};
     if (D <= 2048) return {8, 4, 64};
     if (D <= 4096) return {8, 2, 256};
     if (D <= 8192) return {8, 4, 256};
     if (D <= 16384) return {8, 8, 256};
     return {0, 0, 0};
   }
-  if (D <= 1024) return {1, 4, 256};
+  if (D <= 64) return {1, 4, 16};
+  if (D <= 128) return {1, 8, 16};
+  if (D <= 256) return {1, 16, 16};
+  if (D <= 512) return {1, 16, 32};
+  if (D <= 1024) return {1, 16, 64};
   if (D <= 4096) return {1, 16, 256};
   if (D <= 8192) return {1, 32, 256};
   return {0, 0, 0};
@@ -513,7 +534,7 @@ int fwd_shape(const Args& a, hipStream_t s) {
   const dim3 grid((a.rows + kBlock / TEAM - 1) / (kBlock / TEAM));
   if (a.scale == nullptr) hipLaunchKernelGGL((fwd_kernel<TX, TR, V, P, TEAM, 0>), grid, dim3(kBlock), 0, s, a);
   else if (a.group == 0) hipLaunchKernelGGL((fwd_kernel<TX, TR, V, P, TEAM, 1>), grid, dim3(kBlock), 0, s, a);
-  else if constexpr (V == 8) hipLaunchKernelGGL((fwd_kernel<TX, TR, V, P, TEAM, 2>), grid, dim3(kBlock), 0, s, a);
+  else if constexpr (V == 8 && TEAM >= 16) hipLaunchKernelGGL((fwd_kernel<TX, TR, V, P, TEAM, 2>), grid, dim3(kBlock), 0, s, a);
   return (int)hipGetLastError();
 }
 
@@ -522,11 +543,18 @@ int fwd_typed(const Args& a, bool wide, hipStream_t s) {
   Shape sh = shape_of(a.D, wide);
   if (!wide && a.scale != nullptr && a.group != 0) sh.p = 0;   // 128 columns are not a lane group there
   switch (sh.p * 1000 + sh.team) {
-    case 1064: return fwd_shape<TX, TR, 8, 1, 64>(a, s);
-    case 2064: return fwd_shape<TX, TR, 8, 2, 64>(a, s);
+    case 1008: return fwd_shape<TX, TR, 8, 1, 8>(a, s);
+    case 1016: return fwd_shape<TX, TR, 8, 1, 16>(a, s);
+    case 2016: return fwd_shape<TX, TR, 8, 2, 16>(a, s);
+    case 4016: return sh.v == 8 ? fwd_shape<TX, TR, 8, 4, 16>(a, s) : fwd_shape<TX, TR, 1, 4, 16>(a, s);
+    case 4032: return fwd_shape<TX, TR, 8, 4, 32>(a, s);
     case 4064: return fwd_shape<TX, TR, 8, 4, 64>(a, s);
+    case 8016: return fwd_shape<TX, TR, 1, 8, 16>(a, s);
+    case 16016: return fwd_shape<TX, TR, 1, 16, 16>(a, s);
+    case 16032: return fwd_shape<TX, TR, 1, 16, 32>(a, s);
+    case 16064: return fwd_shape<TX, TR, 1, 16, 64>(a, s);
     case 2256: return fwd_shape<TX, TR, 8, 2, 256>(a, s);
-    case 4256: return sh.v == 8 ? fwd_shape<TX, TR, 8, 4, 256>(a, s) : fwd_shape<TX, TR, 1, 4, 256>(a, s);
+    case 4256: return fwd_shape<TX, TR, 8, 4, 256>(a, s);
     case 8256: return fwd_shape<TX, TR, 8, 8, 256>(a, s);
     case 16256: return fwd_shape<TX, TR, 1, 16, 256>(a, s);
     case 32256: return fwd_shape<TX, TR, 1, 32, 256>(a, s);
@@ -548,11 +576,18 @@ template <typename TX, typename TR>
 int bwd_typed(const Args& a, bool wide, hipStream_t s) {
   const Shape sh = shape_of(a.D, wide);
   switch (sh.p * 1000 + sh.team) {
-    case 1064: bwd_shape<TX, TR, 8, 1, 64>(a, s); break;
-    case 2064: bwd_shape<TX, TR, 8, 2, 64>(a, s); break;
+    case 1008: bwd_shape<TX, TR, 8, 1, 8>(a, s); break;
+    case 1016: bwd_shape<TX, TR, 8, 1, 16>(a, s); break;
+    case 2016: bwd_shape<TX, TR, 8, 2, 16>(a, s); break;
+    case 4016: sh.v == 8 ? bwd_shape<TX, TR, 8, 4, 16>(a, s) : bwd_shape<TX, TR, 1, 4, 16>(a, s); break;
+    case 4032: bwd_shape<TX, TR, 8, 4, 32>(a, s); break;
     case 4064: bwd_shape<TX, TR, 8, 4, 64>(a, s); break;
+    case 8016: bwd_shape<TX, TR, 1, 8, 16>(a, s); break;
+    case 16016: bwd_shape<TX, TR, 1, 16, 16>(a, s); break;
+    case 16032: bwd_shape<TX, TR, 1, 16, 32>(a, s); break;
+    case 16064: bwd_shape<TX, TR, 1, 16, 64>(a, s); break;
     case 2256: bwd_shape<TX, TR, 8, 2, 256>(a, s); break;
-    case 4256: sh.v == 8 ? bwd_shape<TX, TR, 8, 4, 256>(a, s) : bwd_shape<TX, TR, 1, 4, 256>(a, s); break;
+    case 4256: bwd_shape<TX, TR, 8, 4, 256>(a, s); break;
     case 8256: bwd_shape<TX, TR, 8, 8, 256>(a, s); break;
     case 16256: bwd_shape<TX, TR, 1, 16, 256>(a, s); break;
     case 32256: bwd_shape<TX, TR, 1, 32, 256>(a, s); break;

@@ -18,15 +18,19 @@
 // chunks between.  All sums have a fixed order.
 //
 // Waiting: a channel block's chunks are dealt by its counter in the order of
-// the walk, so whatever
-// a workgroup waits for is left by workgroups that already run; each leaves its
-// own pair before it waits for any, and what it leaves later depends on earlier
-// ones alone.  A place in the workspace holds ~0 until its pair is there (one
+// the walk, so whatever a workgroup waits for is left by workgroups that already
+// run; each leaves its own pair before it waits for any, and what it leaves
+// later depends on earlier ones alone.  A place in the workspace holds ~0 until its pair is there (one
 // 8-byte store, seen by 8-byte loads past the caches), so no other order of
 // memory is needed.  Chunk places that no sequence uses get a pair as well:
 // offsets that make no sense give no meaningful rows, but every wait ends.
 //
-// Bound by memory.
+// Bound by memory, and by the walk's phases (rows in, pairs out and back, rows
+// out), which the workgroups of a CU pass through side by side.  B4 T4096 D2048,
+// bf16 with fp32 gates: forward 84 us (268 MB, 3.2 TB/s), backward from the
+// forward's states 104 us (470 MB, 4.5 TB/s), a large copy 4.9 TB/s.  Chunks of
+// 128 rows by 8 waves: forward and backward 188 us; by 4 waves 224 (more pairs),
+// 256 rows by 16 waves 215 (one workgroup a CU).
 
 #include <algorithm>
 
@@ -516,7 +520,8 @@ __global__ __launch_bounds__(kThreads, 4) void bwd_kernel(const Args p, bool sin
 }
 
 // Sequences of at most kShort rows, dense: a thread walks its channels' rows
-// in order, no exchange.
+// in order, no exchange.  16 single rows of 2048 channels: 2.8 us, of which most
+// is the launch.
 constexpr int kShort = 8;
 template <typename TX, typename TG, int V>
 __global__ __launch_bounds__(64) void short_kernel(const Args p) {

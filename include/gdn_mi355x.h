@@ -471,7 +471,7 @@ typedef struct GdnAttnParams {
   void* dk;
   void* dv;
   const int64_t* cu_seqlens;
-  void* workspace;          /* gdn_attn_bwd_workspace_size() bytes */
+  void* workspace;          /* gdn_attn[_bwd]_workspace_size() bytes, 256-byte aligned */
   int64_t workspace_bytes;
   int64_t q_stride[3];      /* (b, t, h), in elements */
   int64_t k_stride[3];
@@ -488,6 +488,7 @@ typedef struct GdnAttnParams {
   int32_t dtype;
 } GdnAttnParams;
 
+int64_t gdn_attn_workspace_size(const GdnAttnParams* params);
 int gdn_attn_launch(const GdnAttnParams* params, void* stream);
 int64_t gdn_attn_bwd_workspace_size(const GdnAttnParams* params);
 int gdn_attn_bwd_launch(const GdnAttnParams* params, void* stream);

@@ -453,3 +453,35 @@ def test_gradient_over_few_keys(pkg, cuda, D):
     size = (do[0, first].double().norm(dim=-1) * v[0, first].double().norm(dim=-1).repeat_interleave(2, -1)
             * k[0, first].double().norm(dim=-1).repeat_interleave(2, -1))
     assert (got[0][0, first].cpu().double().norm(dim=-1) <= 2.0 ** -20 * size).all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,T,S,Hq,Hk,window,sinks", [(1, 20, 4001, 4, 2, None, 0), (2, 1, 3000, 2, 1, 1500, 3),
+                                                      (1, 700, 1500, 2, 2, 400, 130), (1, 1100, 1100, 3, 1, None, 5),
+                                                      (1, 900, 640, 2, 1, None, 0)])
+def test_few_rows_over_long_keys(pkg, cuda, dtype, D, B, T, S, Hq, Hk, window, sinks):
+    """Blocks whose keys are shared by several workgroups: splits that see no
+    key, rows that see none at all, and infinities in hidden places of one split."""
+    gen = torch.Generator().manual_seed(T + S)
+    q, k, v = (torch.randn(B, n, h, D, generator=gen).to(dtype).to(cuda) for n, h in ((T, Hq), (S, Hk), (S, Hk)))
+    seen = visible(T, S, window, sinks, cuda)
+    hidden = ~seen.any(0)
+    kk, vv = (t.repeat_interleave(Hq // Hk, 2).transpose(1, 2).double() for t in (k, v))
+    s = torch.matmul(q.transpose(1, 2).double(), kk.transpose(2, 3).contiguous()) * D ** -0.5
+    s = s.masked_fill(~seen, -math.inf)
+    lse = torch.logsumexp(s, -1).transpose(1, 2)
+    P = torch.where(seen, torch.exp(s - torch.where(lse > -math.inf, lse, 0.0).transpose(1, 2)[..., None]), 0.0)
+    want = torch.matmul(P, vv.contiguous()).transpose(1, 2)
+    for value in (None, math.inf):
+        if value is not None:
+            if not hidden.any():
+                continue
+            v = v.clone()
+            v[:, hidden] = value
+        o, l = pkg.window_attn(q, k, v, window, sinks, return_lse=True)
+        torch.cuda.synchronize()
+        assert (o.double() - want).norm() <= 1.5 * UNIT[dtype] * want.norm()
+        none = ~seen.any(1)
+        assert (o[:, none] == 0).all() and (l[:, none] == -math.inf).all()
+        assert (l[:, ~none].double() - lse[:, ~none]).abs().max() <= 2.0 ** -18 * max(1.0, lse[:, ~none].abs().max().item())

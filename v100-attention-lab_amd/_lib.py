@@ -53,6 +53,7 @@ EXPORTED_SYMBOLS = (
     "gdn_norm_launch",
     "gdn_norm_bwd_workspace_size",
     "gdn_norm_bwd_launch",
+    "gdn_attn_workspace_size",
     "gdn_attn_launch",
     "gdn_attn_bwd_workspace_size",
     "gdn_attn_bwd_launch",

@@ -108,7 +108,13 @@ def _run(q, k, v, window, sinks, scale, cu, n_seq, need_lse):
     if plan is None:
         w, s = _check_window(window, sinks)
         dims = _validate(q, k, v)
-        plan = bytes(_params(q, k, v, *dims, n_seq, w, s, scale))
+        P = _params(q, k, v, *dims, n_seq, w, s, scale)
+        P.cu_seqlens = 1 if n_seq is not None else None     # only whether it is set counts here
+        ws_bytes = _lib.load_library().gdn_attn_workspace_size(ctypes.byref(P))
+        if ws_bytes < 0:
+            raise ValueError(f"window_attn does not support q {tuple(q.shape)}, k {tuple(k.shape)}")
+        P.cu_seqlens = None
+        plan = bytes(P), int(ws_bytes)
         if key is not None:
             if len(_FWD_PLANS) >= _PLANS_MAX:
                 _FWD_PLANS.clear()
@@ -117,7 +123,11 @@ def _run(q, k, v, window, sinks, scale, cu, n_seq, need_lse):
         _validate(q, k, v)
     o = _like(q)
     lse = q.new_empty(q.shape[:3], dtype=torch.float32) if need_lse else None
-    P = _lib.GdnAttnParams.from_buffer_copy(plan)
+    params, ws_bytes = plan
+    ws = q.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes > 0 else None
+    P = _lib.GdnAttnParams.from_buffer_copy(params)
+    if ws is not None:
+        P.workspace, P.workspace_bytes = ws.data_ptr(), ws_bytes
     P.q, P.k, P.v, P.o = q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr()
     P.lse = lse.data_ptr() if lse is not None else None
     P.cu_seqlens = cu.data_ptr() if cu is not None else None

@@ -6,7 +6,8 @@
 // the products.  A wave forms S^T = K Q^T (a lane then holds one query row's
 // scores, so the softmax needs one exchange, between the lane's two halves)
 // and O^T += V^T P^T with P^T straight from the accumulators.  Only tiles on
-// the edges of the visible range are masked.
+// the edges of the visible range are masked.  Few blocks of rows over many keys
+// are cut along the keys, and a second kernel joins the parts.
 //
 // Bound by the matrix cores and, beside them, the exponentials: of 64 keys a
 // wave's products take 1024 cycles of a SIMD at head size 128 and its softmax
@@ -30,6 +31,7 @@ namespace attn {
 constexpr int kBM = 128;       // query rows a workgroup
 constexpr int kBN = 64;        // keys a tile
 constexpr int kNT = 256;
+constexpr int kPlaces = 512;   // workgroups that the card holds at once
 
 struct FArgs {
   const uint16_t* q;
@@ -39,7 +41,9 @@ struct FArgs {
   float* lse;
   SeqArgs seq;
   int64_t qs[3], ks[3], vs[3], os[3];
-  int Hq, G, units, nblk, slots, window, sinks;
+  int Hq, G, units, slots, splits, window, sinks;
+  float* stat;      // [splits][B Tq Hq][2]: maximum (in powers of 2) and sum of a split
+  float* part;      // [splits][B Tq Hq][D]: its O
   float scale_log2;
   uint32_t flip;
 };
@@ -54,7 +58,8 @@ __global__ __launch_bounds__(kNT, 2) void fwd_kernel(const FArgs a) {
   // unit = (batch, head); neighbouring units share key heads, and workgroups
   // blockIdx.x % 8 run on one XCD: give each XCD a run of units.  Later blocks
   // see more keys and start first.
-  const int unit_ix = blockIdx.x % a.units, slot = a.slots - 1 - blockIdx.x / a.units;
+  const int unit_ix = blockIdx.x % a.units, rest = blockIdx.x / a.units;
+  const int slot = a.slots - 1 - rest % a.slots, split = rest / a.slots;
   const int unit = a.units % 8 == 0 ? (unit_ix % 8) * (a.units / 8) + unit_ix / 8 : unit_ix;
   int block, si, head;
   if (a.seq.cu == nullptr) {
@@ -79,6 +84,8 @@ __global__ __launch_bounds__(kNT, 2) void fwd_kernel(const FArgs a) {
 
   const int p0 = m0 + shift, p1 = min(m0 + kBM, sq.nq) - 1 + shift;
   const KeyRange kr(p0, p1, sq.nk, a.window, a.sinks, kBN);
+  const int per = (kr.n + a.splits - 1) / a.splits;
+  const int it0 = min(split * per, kr.n), n = min(per, kr.n - it0);
   const int wp0 = m0 + wv * 32 + shift, wp1 = min(wp0 + 31, sq.nq - 1 + shift);
 
   Vec qf[D / 16];
@@ -96,17 +103,17 @@ __global__ __launch_bounds__(kNT, 2) void fwd_kernel(const FArgs a) {
   // edge of any wave's range are then made finite where they are not, after
   // what they hold has reached the rows that see it.
   for (bool careful = false;; careful = true) {
-    if (kr.n > 0) {
-      ck(base, kr.tile(0) * kBN);
-      cv(base + kTile, kr.tile(0) * kBN);
+    if (n > 0) {
+      ck(base, kr.tile(it0) * kBN);
+      cv(base + kTile, kr.tile(it0) * kBN);
     }
-    for (int it = 0; it < kr.n; ++it) {
-      const int j0 = kr.tile(it) * kBN;
+    for (int it = 0; it < n; ++it) {
+      const int j0 = kr.tile(it0 + it) * kBN;
       const uint32_t kt = base + (it & 1) * 2 * kTile, vt = kt + kTile;
       dma_wait();
       __syncthreads();                        // tile `it` is here; every wave is done with the other buffer
-      if (it + 1 < kr.n) {
-        const int jn = kr.tile(it + 1) * kBN;
+      if (it + 1 < n) {
+        const int jn = kr.tile(it0 + it + 1) * kBN;
         const uint32_t other = base + ((it + 1) & 1) * 2 * kTile;
         ck(other, jn);
         cv(other + kTile, jn);
@@ -137,6 +144,19 @@ __global__ __launch_bounds__(kNT, 2) void fwd_kernel(const FArgs a) {
 
   const float l = rows.l + swap_halves(rows.l);
   if (row >= sq.nq) return;
+  const int64_t at = ((int64_t)sq.b * a.seq.Tq + sq.q0 + row) * a.Hq + head;
+  if (a.splits > 1) {
+    const int64_t to = (int64_t)split * a.units * a.seq.Tq + at;
+    if (half == 0) *reinterpret_cast<float2*>(a.stat + 2 * to) = make_float2(rows.m, l);
+    float* pr = a.part + to * D + 4 * half;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        *reinterpret_cast<float4*>(pr + 32 * dt + 8 * c) =
+            make_float4(rows.acc[dt][4 * c], rows.acc[dt][4 * c + 1], rows.acc[dt][4 * c + 2], rows.acc[dt][4 * c + 3]);
+    return;
+  }
   const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
   uint16_t* orow = a.o + sq.b * a.os[0] + (sq.q0 + row) * a.os[1] + head * a.os[2];
 #pragma unroll
@@ -147,10 +167,40 @@ __global__ __launch_bounds__(kNT, 2) void fwd_kernel(const FArgs a) {
                                  O::pack(rows.acc[dt][4 * c + 2] * inv, rows.acc[dt][4 * c + 3] * inv));
       *reinterpret_cast<uint2*>(orow + 32 * dt + 8 * c + 4 * half) = w;
     }
-  if (a.lse != nullptr && half == 0) {
-    const int64_t at = ((int64_t)sq.b * a.seq.Tq + sq.q0 + row) * a.Hq + head;
+  if (a.lse != nullptr && half == 0)
     a.lse[at] = l > 0.f || l != l ? (rows.m - O::kShift) * kLn2 + logf(l) : -__builtin_inff();
+}
+
+// The splits of a row joined, in order: D / 4 threads a row (of a dense batch).
+template <typename T, int D>
+__global__ __launch_bounds__(kNT) void join_rows_kernel(const FArgs a) {
+  constexpr int L = D / 4;
+  const int64_t rows = (int64_t)a.units * a.seq.Tq, at = (int64_t)blockIdx.x * (kNT / L) + threadIdx.x / L;
+  if (at >= rows) return;
+  const int d = 4 * (threadIdx.x % L);
+  float top = -__builtin_inff();
+  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.stat[2 * (s * rows + at)]);
+  float l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int s = 0; s < a.splits; ++s) {
+    const float2 ml = *reinterpret_cast<const float2*>(a.stat + 2 * (s * rows + at));
+    const float4 x = *reinterpret_cast<const float4*>(a.part + (s * rows + at) * D + d);
+    if (ml.x == -__builtin_inff()) continue;      // this split saw no key
+    const float f = exp2_fast(ml.x - top);
+    l += f * ml.y;
+    o.x += f * x.x;
+    o.y += f * x.y;
+    o.z += f * x.z;
+    o.w += f * x.w;
   }
+  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+  const int head = (int)(at % a.Hq);
+  const int64_t bt = at / a.Hq, b = bt / a.seq.Tq, t = bt % a.seq.Tq;
+  *reinterpret_cast<uint2*>(a.o + b * a.os[0] + t * a.os[1] + head * a.os[2] + d) =
+      make_uint2(Ops<T>::pack(o.x * inv, o.y * inv), Ops<T>::pack(o.z * inv, o.w * inv));
+  if (a.lse != nullptr && d == 0)
+    a.lse[at] = l > 0.f || l != l ? (top - Ops<T>::kShift) * kLn2 + logf(l) : -__builtin_inff();
 }
 
 int check_attn(const GdnAttnParams& P) {
@@ -164,12 +214,36 @@ int check_attn(const GdnAttnParams& P) {
   return GDN_OK;
 }
 
+// Workgroups that share a block's keys: where a dense batch leaves most places
+// on the card (two a CU) empty and has 1024 keys or more, as many as fill them,
+// of at least 4 tiles each.  (Packed lengths are not known on the host.)  One
+// workgroup a block / shared, bf16: 32 rows on 32768 keys, 16 heads of 128,
+// 639 / 65 us; 512 on 4096 88 / 45; 1024 causal rows, 8 heads, 28 / 25; 2048 causal
+// rows of 12 heads (192 blocks) 49 / 44, of 16 (256 blocks) 51 / 57; 512 causal
+// rows of 16 heads 18 / 20.
+int splits_of(const GdnAttnParams& P) {
+  const int64_t blocks = (int64_t)P.B * P.Hq * ((P.Tq + kBM - 1) / kBM);
+  const int64_t keys = std::min<int64_t>(P.Tk, (int64_t)P.window + kBM + P.sinks);
+  if (P.cu_seqlens != nullptr || blocks == 0 || blocks >= kPlaces / 2 || keys < 1024) return 1;
+  return (int)std::min<int64_t>(kPlaces / blocks, keys / kBN / 4);
+}
+int64_t stat_bytes(const GdnAttnParams& P, int splits) {
+  return ((int64_t)splits * P.B * P.Tq * P.Hq * 8 + 255) & ~(int64_t)255;
+}
+
+template <typename T, int D>
+int launch_td(const FArgs& a, hipStream_t s) {
+  hipLaunchKernelGGL((fwd_kernel<T, D>), dim3((uint32_t)a.units * a.slots * a.splits), dim3(kNT), 0, s, a);
+  if (a.splits > 1) {
+    constexpr int kRowsWg = kNT / (D / 4);
+    const int64_t rows = (int64_t)a.units * a.seq.Tq;
+    hipLaunchKernelGGL((join_rows_kernel<T, D>), dim3((uint32_t)((rows + kRowsWg - 1) / kRowsWg)), dim3(kNT), 0, s, a);
+  }
+  return (int)hipGetLastError();
+}
 template <typename T>
 int launch_t(const FArgs& a, int D, hipStream_t s) {
-  const dim3 grid((uint32_t)a.units * a.slots);
-  if (D == 128) hipLaunchKernelGGL((fwd_kernel<T, 128>), grid, dim3(kNT), 0, s, a);
-  else hipLaunchKernelGGL((fwd_kernel<T, 64>), grid, dim3(kNT), 0, s, a);
-  return (int)hipGetLastError();
+  return D == 128 ? launch_td<T, 128>(a, s) : launch_td<T, 64>(a, s);
 }
 
 }  // namespace attn
@@ -178,7 +252,15 @@ int launch_t(const FArgs& a, int D, hipStream_t s) {
 using namespace gdn;
 using namespace gdn::attn;
 
-extern "C" int gdn_attn_launch(const GdnAttnParams* prm, void* stream) {
+extern "C" {
+
+int64_t gdn_attn_workspace_size(const GdnAttnParams* prm) {
+  if (prm == nullptr || check_attn(*prm) != GDN_OK) return -1;
+  const int splits = splits_of(*prm);
+  return splits == 1 ? 0 : stat_bytes(*prm, splits) + (int64_t)splits * prm->B * prm->Tq * prm->Hq * prm->D * 4;
+}
+
+int gdn_attn_launch(const GdnAttnParams* prm, void* stream) {
   if (prm == nullptr) return GDN_ERR_NULL_POINTER;
   const GdnAttnParams& P = *prm;
   const int st = check_attn(P);
@@ -216,6 +298,16 @@ extern "C" int gdn_attn_launch(const GdnAttnParams* prm, void* stream) {
   if (units * slots > 0x7fffffffLL) return GDN_ERR_BAD_SHAPE;
   a.units = (int)units;
   a.slots = (int)slots;
+  a.splits = splits_of(P);
+  if (a.splits > 1) {
+    if (P.workspace == nullptr || P.workspace_bytes < gdn_attn_workspace_size(prm) ||
+        reinterpret_cast<uintptr_t>(P.workspace) % 256 != 0)
+      return GDN_ERR_WORKSPACE;
+    a.stat = static_cast<float*>(P.workspace);
+    a.part = reinterpret_cast<float*>(static_cast<char*>(P.workspace) + stat_bytes(P, a.splits));
+  }
   hipStream_t s = static_cast<hipStream_t>(stream);
   return P.dtype == GDN_DTYPE_F16 ? launch_t<f16>(a, P.D, s) : launch_t<bf16_t>(a, P.D, s);
 }
+
+}  // extern "C"

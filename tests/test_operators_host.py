@@ -195,6 +195,20 @@ def test_decode_refusals(lib, pkg, kw, code):
     assert lib.gdn_attn_decode_launch(ctypes.byref(_decode(pkg._lib, **kw)), None) == code
 
 
+def test_attn_workspace_of_few_rows(lib, pkg):
+    """Parts (a maximum, a sum and D values a row and split) only where few blocks
+    of rows share long keys, at most 512 blocks of them."""
+    size = lambda **kw: lib.gdn_attn_workspace_size(ctypes.byref(_attn(pkg._lib, **kw)))
+    few = dict(Tq=40, Tk=5000, window=5000)
+    assert size() == 0 and size(Tq=40, Tk=5000) == 0           # 100 keys; a short window
+    assert 0 < size(**few) <= 512 * 128 * (64 + 2) * 4 + 256
+    assert size(B=64, N=64, **few) == 0                        # enough blocks
+    assert size(cu_seqlens=FAKE, B=1, Tq=5000, Tk=5000, window=5000) == 0
+    assert size(D=96) == -1 and lib.gdn_attn_workspace_size(None) == -1
+    for kw in (dict(workspace=None), dict(workspace_bytes=100), dict(workspace=FAKE + 16)):
+        assert lib.gdn_attn_launch(ctypes.byref(_attn(pkg._lib, **few, **kw)), None) == 1006
+
+
 def test_decode_workspace(lib, pkg):
     size = lambda **kw: lib.gdn_attn_decode_workspace_size(ctypes.byref(_decode(pkg._lib, **kw)))
     assert size() > 0 and size(B=512) == 0          # enough sequences: no splits, no parts

@@ -485,3 +485,31 @@ def test_few_rows_over_long_keys(pkg, cuda, dtype, D, B, T, S, Hq, Hk, window, s
         none = ~seen.any(1)
         assert (o[:, none] == 0).all() and (l[:, none] == -math.inf).all()
         assert (l[:, ~none].double() - lse[:, ~none]).abs().max() <= 2.0 ** -18 * max(1.0, lse[:, ~none].abs().max().item())
+
+
+@pytest.mark.parametrize("dtype,D", [(torch.float16, 64), (torch.bfloat16, 128)])
+@pytest.mark.parametrize("T,lens", [(None, None), (7, None), (None, [0, 1, 0]), (None, [0, 0, 300])])
+@pytest.mark.parametrize("window,sinks", [(128, 1), (128, 4), (60, 130), (1024, 4)])
+@pytest.mark.parametrize("beyond", [127, 128, 129])
+def test_first_rows_beyond_a_blocks_window(pkg, cuda, dtype, D, T, lens, window, sinks, beyond):
+    """Keys about one block of 128 longer than the window: the last rows see the
+    first keys across it.  The scores put the rows' mass on the first keys, whose
+    gradients are compared by themselves: a row that is left out takes about
+    (window + 128)^-1/2 of them."""
+    S = window + beyond
+    T = S if T is None else T
+    if lens is not None:        # a whole sequence of S rows between others
+        lens = [S if n == 1 else n for n in lens] if 1 in lens else lens + [S]
+        T = S = sum(lens)
+    q, k, v, do = _inputs(cuda, 1, T, S, 2, 1, D, dtype, seed=window + beyond)
+    s0 = S - (window + beyond) if lens is not None else 0
+    u = torch.nn.functional.normalize(torch.randn(D, generator=torch.Generator().manual_seed(1)), dim=0).to(cuda)
+    q = (q.float() + 2 * D ** 0.25 * u).to(dtype)
+    k[:, s0:s0 + sinks] = (k[:, s0:s0 + sinks].float() + 2 * D ** 0.25 * u).to(dtype)
+    cu = None if lens is None else torch.tensor([0] + list(itertools.accumulate(lens)), device=cuda)
+    o, lse = pkg.window_attn(q, k, v, window, sinks, cu_seqlens=cu, return_lse=True)
+    _, dk, dv = pkg.window_attn_bwd(q, k, v, o, lse, do, window, sinks, cu_seqlens=cu)
+    q, do = (t[0, s0:] if lens is not None else t[0] for t in (q, do))
+    _, _, (_, wk, wv), (_, sk) = oracle(q, k[0, s0:], v[0, s0:], window, sinks, do=do)
+    _close(dv[0, s0:s0 + sinks], wv[:sinks], 2, 0.0, "dv")
+    _close(dk[0, s0:s0 + sinks], wk[:sinks], 4, sk, "dk")

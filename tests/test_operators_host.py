@@ -293,3 +293,18 @@ def test_decode_and_fp8_refuse_gradients(pkg):
 def test_norm_arguments(pkg, args, msg):
     with pytest.raises(ValueError, match=msg):
         pkg.add_rms_norm(*args)
+
+
+@pytest.mark.parametrize("window", [1, 60, 128, 1000])
+@pytest.mark.parametrize("sinks", [1, 4, 130])
+def test_attn_bwd_parts_of_the_first_rows(lib, pkg, window, sinks):
+    """The first block of 128 keys is in its window's reach of the positions up to
+    window + 126; from the next on its sinks' gradients have parts."""
+    def size(S, sinks, **kw):
+        kw = dict(dict(B=1, N=1, Tq=S, Tk=S, window=window, sinks=sinks, Hq=64, Hk=64, dtype=pkg._lib.DTYPE_BF16), **kw)
+        return lib.gdn_attn_bwd_workspace_size(ctypes.byref(_attn(pkg._lib, **kw)))
+    for S in range(window + 100, window + 160):
+        for kw in (dict(), dict(Tq=7), dict(cu_seqlens=FAKE)):
+            # (64 key heads of 3 blocks and more: one workgroup a block)
+            if 64 * -(-S // 128) >= 128:
+                assert (size(S, sinks, **kw) > size(S, 0, **kw)) == (S >= window + 128), (S, kw)

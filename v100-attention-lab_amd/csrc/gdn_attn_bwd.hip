@@ -714,11 +714,12 @@ __global__ __launch_bounds__(256, 2) void q_kernel(const BArgs a) {
 int64_t up256(int64_t n) { return (n + 255) & ~(int64_t)255; }
 
 // Blocks of first keys, rows a segment and segment slots of a call (none where
-// no row lies beyond the first block's window).
+// no row lies beyond the first block's window: its last key kKB - 1 is in reach
+// of positions up to kKB - 2 + window, and the last position is Tk - 1).
 void sink_plan(const GdnAttnParams& P, int& blocks, int& seg, int& slots) {
   blocks = seg = slots = 0;
   const int64_t sinks = std::min<int64_t>(P.sinks, P.Tk);
-  if (sinks == 0 || P.Tq == 0 || (int64_t)P.window + kKB >= P.Tk) return;
+  if (sinks == 0 || P.Tq == 0 || (int64_t)P.window + kKB > P.Tk) return;
   blocks = (int)((sinks + kKB - 1) / kKB);
   // half of a block's own tiles a segment, 16 at most (of all heads together),
   // and no more parts than rows of D floats for every query row, twice

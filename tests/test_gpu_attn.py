@@ -513,3 +513,29 @@ def test_first_rows_beyond_a_blocks_window(pkg, cuda, dtype, D, T, lens, window,
     _, _, (_, wk, wv), (_, sk) = oracle(q, k[0, s0:], v[0, s0:], window, sinks, do=do)
     _close(dv[0, s0:s0 + sinks], wv[:sinks], 2, 0.0, "dv")
     _close(dk[0, s0:s0 + sinks], wk[:sinks], 4, sk, "dk")
+
+
+@pytest.mark.parametrize("D,dtype", [(64, torch.float16), (128, torch.bfloat16)])
+def test_nan_scores_of_shared_keys(pkg, cuda, D, dtype):
+    """Keys of few rows, shared by workgroups: a NaN query row is NaN in o and
+    lse, and so is every row over a run of keys that are all NaN; other rows keep
+    their bits."""
+    q, k, v, _ = _inputs(cuda, 1, 3, 4096, 2, 1, D, dtype, seed=31)
+    o, lse = pkg.window_attn(q, k, v, return_lse=True)
+    q2 = q.clone()
+    q2[0, 1, 0, 3] = float("nan")
+    o2, lse2 = pkg.window_attn(q2, k, v, return_lse=True)
+    hit = torch.zeros_like(lse, dtype=torch.bool)
+    hit[0, 1, 0] = True
+    assert torch.isnan(o2[hit]).all() and torch.isnan(lse2[hit]).all()
+    assert torch.equal(o2[~hit], o[~hit]) and torch.equal(lse2[~hit], lse[~hit])
+    k2 = k.clone()
+    k2[:, 512:1024] = float("nan")      # whole workgroups' shares
+    o2, lse2 = pkg.window_attn(q, k2, v, return_lse=True)
+    assert torch.isnan(o2).all() and torch.isnan(lse2).all()
+    # rows that do not see them keep their values: the first of 3 rows ends before
+    k2 = k.clone()
+    k2[:, 4094] = float("nan")
+    o2, lse2 = pkg.window_attn(q, k2, v, return_lse=True)
+    assert torch.equal(o2[:, 0], o[:, 0]) and torch.equal(lse2[:, 0], lse[:, 0])
+    assert torch.isnan(o2[:, 1:]).all() and torch.isnan(lse2[:, 1:]).all()

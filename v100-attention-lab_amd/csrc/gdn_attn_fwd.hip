@@ -186,8 +186,10 @@ __global__ __launch_bounds__(kNT) void join_rows_kernel(const FArgs a) {
   for (int s = 0; s < a.splits; ++s) {
     const float2 ml = *reinterpret_cast<const float2*>(a.stat + 2 * (s * rows + at));
     const float4 x = *reinterpret_cast<const float4*>(a.part + (s * rows + at) * D + d);
-    if (ml.x == -__builtin_inff()) continue;      // this split saw no key
-    const float f = exp2_fast(ml.x - top);
+    // a split that saw no key adds nothing; one that saw only NaN has no maximum
+    // either, but its sum is NaN
+    if (ml.y == 0.f) continue;
+    const float f = ml.x == -__builtin_inff() ? 0.f : exp2_fast(ml.x - top);
     l += f * ml.y;
     o.x += f * x.x;
     o.y += f * x.y;

@@ -539,3 +539,36 @@ def test_nan_scores_of_shared_keys(pkg, cuda, D, dtype):
     o2, lse2 = pkg.window_attn(q, k2, v, return_lse=True)
     assert torch.equal(o2[:, 0], o[:, 0]) and torch.equal(lse2[:, 0], lse[:, 0])
     assert torch.isnan(o2[:, 1:]).all() and torch.isnan(lse2[:, 1:]).all()
+
+
+@pytest.mark.parametrize("D,dtype", [(64, torch.float16), (128, torch.bfloat16)])
+@pytest.mark.parametrize("T", [1, 3])
+def test_decode_nan_scores(pkg, cuda, D, dtype, T):
+    """Over a cache that several workgroups share, a NaN query row, keys of a
+    whole share that are NaN and an infinite value at a key of no weight are not
+    lost; other rows keep their bits."""
+    q, k, v, _ = _inputs(cuda, 2, T, 4096, 4, 2, D, dtype, seed=32)
+    lens = torch.tensor([4096, 3000], dtype=torch.int32, device=cuda)
+    o = pkg.window_attn_decode(q, k, v, lens)
+    q2 = q.clone()
+    q2[1, 0, 2, 3] = float("nan")
+    o2 = pkg.window_attn_decode(q2, k, v, lens)
+    hit = torch.zeros(o.shape[:3], dtype=torch.bool, device=cuda)
+    hit[1, 0, 2] = True
+    assert torch.isnan(o2[hit]).all() and torch.equal(o2[~hit], o[~hit])
+    k2 = k.clone()
+    k2[0, 1024:1536, 1] = float("nan")
+    o2 = pkg.window_attn_decode(q, k2, v, lens)
+    hit = torch.zeros_like(hit)
+    hit[0, :, 2:] = True
+    assert torch.isnan(o2[hit]).all() and torch.equal(o2[~hit], o[~hit])
+    # scores about 400 below the rest: the weight is 0 in 32 bits, and 0 inf is NaN
+    q2 = q.abs() + 1
+    k2 = k.abs()
+    k2[0, 1024:1536, 1] = -400.0 / D ** 0.5
+    v2 = v.clone()
+    v2[0, 1300, 1, 7] = float("inf")
+    o2 = pkg.window_attn_decode(q2, k2, v2, lens)
+    hit = torch.zeros_like(o, dtype=torch.bool)
+    hit[0, :, 2:, 7] = True
+    assert not torch.isfinite(o2[hit]).any() and torch.isfinite(o2[~hit]).all()

@@ -155,8 +155,7 @@ __global__ __launch_bounds__(64 * kDWaves) void decode_kernel(const DArgs a) {
   for (int e = 0; e < D / 8; ++e) {
     out[e] = 0.f;
 #pragma unroll
-    for (int w = 0; w < kDWaves; ++w)
-      if (f[w] != 0.f) out[e] += f[w] * so[(w * D + d0 + e) * 32 + c];
+    for (int w = 0; w < kDWaves; ++w) out[e] += f[w] * so[(w * D + d0 + e) * 32 + c];
   }
   if (a.splits > 1) {
     float* part = a.part + ((int64_t)unit * a.splits + split) * 32 * (D + 2);
@@ -194,15 +193,18 @@ __global__ __launch_bounds__(kJT) void join_kernel(const DArgs a) {
 #pragma unroll
   for (int s = 32; s >= 1; s >>= 1) top = fmaxf(top, __shfl_xor(top, s, 64));
   const float f = weight(m, top);
-  float l = f != 0.f ? f * ls : 0.f;
+  float l = f * ls;
 #pragma unroll
   for (int s = 32; s >= 1; s >>= 1) l += __shfl_xor(l, s, 64);
+  // a split that saw no key (-1) is not read; one that saw only NaN has no maximum
+  // either, but its sum is NaN, and what is not finite stays so at a weight of 0
+  const float use = ls == 0.f ? -1.f : f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
   for (int k = 0; k < kMaxSplits / kGroups; ++k) {
     const int s = k * kGroups + g;
-    const float fs = __shfl(f, s < a.splits ? s : 0, 64);
-    if (s < a.splits && fs != 0.f) {
+    const float fs = __shfl(use, s < a.splits ? s : 0, 64);
+    if (s < a.splits && !(fs < 0.f)) {
       const float4 x = *reinterpret_cast<const float4*>(part + s * step + 64 + c * D + 4 * d);
       o.x += fs * x.x;
       o.y += fs * x.y;

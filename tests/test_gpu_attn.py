@@ -572,3 +572,15 @@ def test_decode_nan_scores(pkg, cuda, D, dtype, T):
     hit = torch.zeros_like(o, dtype=torch.bool)
     hit[0, :, 2:, 7] = True
     assert not torch.isfinite(o2[hit]).any() and torch.isfinite(o2[~hit]).all()
+
+
+@pytest.mark.parametrize("Hk", [1, 3])
+@pytest.mark.parametrize("window,sinks", [(40, 4), (40, 150), (1, 128), (300, 20)])
+@pytest.mark.parametrize("lens", [[5] * 60 + [400, 0, 0, 50, 170, 168, 167, 1, 900, 0], [700] + [2] * 70 + [168, 429],
+                                  [429, 428, 427, 0, 129, 128, 168]])
+def test_first_keys_of_many_sequences(pkg, cuda, lens, window, sinks, Hk):
+    """Long sequences, whose later rows reach the first keys from beyond a block's
+    window, among many short and empty ones; and lengths where that begins."""
+    T = sum(lens)
+    q, k, v, do = _inputs(cuda, 1, T, T, 2 * Hk, Hk, 64, torch.float16 if Hk == 1 else torch.bfloat16, seed=T)
+    _check(pkg, q, k, v, do, window, sinks, lens=lens)

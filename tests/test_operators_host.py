@@ -308,3 +308,14 @@ def test_attn_bwd_parts_of_the_first_rows(lib, pkg, window, sinks):
             # (64 key heads of 3 blocks and more: one workgroup a block)
             if 64 * -(-S // 128) >= 128:
                 assert (size(S, sinks, **kw) > size(S, 0, **kw)) == (S >= window + 128), (S, kw)
+
+
+def test_attn_bwd_workspace_of_many_sequences(lib, pkg):
+    """Parts of the first keys only for sequences longer than the window and a
+    block: their number follows from the rows, not from the sequences."""
+    def size(N, sinks):
+        kw = dict(cu_seqlens=FAKE, B=1, N=N, Tq=65536, Tk=65536, Hq=32, Hk=8, D=128, window=1024, sinks=sinks,
+                  dtype=pkg._lib.DTYPE_BF16)
+        return lib.gdn_attn_bwd_workspace_size(ctypes.byref(_attn(pkg._lib, **kw)))
+    assert size(8, 4) <= size(56, 4) == size(2048, 4) <= 512 << 20      # 56 * 1152 rows are the most
+    assert size(2048, 0) < 17 << 20

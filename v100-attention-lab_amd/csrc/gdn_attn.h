@@ -269,6 +269,18 @@ __device__ __forceinline__ Seq get_seq(const SeqArgs& a, int i) {
   return s;
 }
 
+// The last of N packed sequences whose first(start row, sequence) is at most
+// `at` (it rises along the sequences).
+template <typename First>
+__device__ __forceinline__ int last_seq(const SeqArgs& a, int at, First first) {
+  int lo = 0, hi = a.N;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (first(clamp_row(a.cu[mid], 0, a.Tq), mid) <= at) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
 // Blocks of `rows` rows: a dense sequence has ceil(T / rows); packed sequence
 // i has its first at slot start / rows + i, which leaves each room for
 // ceil(len / rows) blocks.  Returns the sequence and the block in it (which
@@ -278,14 +290,10 @@ __device__ __forceinline__ int find_block(const SeqArgs& a, int slot, int rows, 
     block = slot % nblk;
     return slot / nblk;
   }
-  auto first = [&](int i) { return (int)(clamp_row(a.cu[i], 0, a.Tq) / rows) + i; };
-  int lo = 0, hi = a.N;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (first(mid) <= slot) lo = mid; else hi = mid;
-  }
-  block = slot - first(lo);
-  return lo;
+  auto first = [&](int64_t start, int i) { return (int)(start / rows) + i; };
+  const int i = last_seq(a, slot, first);
+  block = slot - first(clamp_row(a.cu[i], 0, a.Tq), i);
+  return i;
 }
 
 // Key tiles of TK keys that query positions [p0, p1] see: tiles [0, ns) of the

@@ -56,7 +56,7 @@ struct BArgs {
   float* stat;      // [Hq][rows][2]: lse in powers of 2, D
   float* rmax;      // [Hq][rows] largest |dO| (fp16)
   float* vmax;      // [units_k][kVParts] (fp16)
-  float* part;      // [units_k][sink blocks][segments][2][kKB][D]
+  float* part;      // [units_k][sink blocks][slots_s][2][kKB][D], then own_part's
   SeqArgs seq;
   int64_t qs[3], ks[3], vs[3], os[3], dos[3], dqs[3], dks[3], dvs[3];
   int64_t rows;     // B Tq
@@ -66,6 +66,7 @@ struct BArgs {
   int kv_halves;                // waves of a workgroup / 4 (kv)
   int splits;                   // workgroups a key block
   int sink_blocks, seg, slots_s;  // blocks of the first keys, rows a segment, segment slots
+  int longs, long_rows;           // places of long sequences (packed), rows of the shortest
   int window, sinks;
   float scale, scale_log2;
 };
@@ -170,12 +171,27 @@ __device__ __forceinline__ QRange seg_rows(const BArgs& a, const Seq& s, int k0,
   return q;
 }
 
+// Whether rows beyond a block of first keys' own see it: only then its sums are
+// parts.  Packed sequences that have such rows are at least window + kKB long,
+// so start / (window + kKB) numbers them without a place for the others; few
+// sequences are numbered as they are.
+__device__ __forceinline__ bool has_beyond(const BArgs& a, const Seq& s, int k0) { return own_rows(a, s, k0).r1 < s.nq; }
+__device__ __forceinline__ int long_place(const BArgs& a, int64_t start, int i) {
+  return a.longs == a.seq.N ? i : (int)((uint32_t)start / (uint32_t)a.long_rows);
+}
+// Slot of segment 0 of a packed long sequence (room for ceil(rows / seg)).
+__device__ __forceinline__ int first_seg(const BArgs& a, int64_t start, int i) {
+  return (int)((uint32_t)start / (uint32_t)a.seg) + long_place(a, start, i);
+}
+
 // Place of the part of a key block's own rows: with splits one for each slot
-// and split, else one for each block of first keys of each sequence.
-__device__ __forceinline__ int64_t own_part(const BArgs& a, int unit, int si, int block, int slot, int split) {
+// and split, else one for each block of first keys of each long sequence.
+__device__ __forceinline__ int64_t own_part(const BArgs& a, int unit, const Seq& sq, int si, int block, int slot,
+                                            int split) {
   const int64_t first = (int64_t)a.units_k * a.sink_blocks * a.slots_s;
   if (a.splits > 1) return first + ((int64_t)unit * a.slots_k + slot) * a.splits + split;
-  return first + ((int64_t)unit * (a.seq.cu == nullptr ? 1 : a.seq.N) + (a.seq.cu == nullptr ? 0 : si)) * a.sink_blocks + block;
+  const int64_t seq = a.seq.cu == nullptr ? unit : (int64_t)unit * a.longs + long_place(a, sq.q0, si);
+  return first + seq * a.sink_blocks + block;
 }
 
 // 4 bytes per lane from global memory to LDS at `at` + 4 * lane.
@@ -213,7 +229,9 @@ __global__ __launch_bounds__(256 * QH, D == 64 && QH == 1 ? 3 : 2) void kv_kerne
     hk = unit;
     if (extra) {
       block = item % a.sink_blocks;
-      si = find_block(a.seq, item / a.sink_blocks, a.seg, 0, seg);
+      const int slot = item / a.sink_blocks;
+      si = last_seq(a.seq, slot, [&](int64_t start, int i) { return first_seg(a, start, i); });
+      seg = slot - first_seg(a, clamp_row(a.seq.cu[si], 0, a.seq.Tq), si);
     } else {
       si = find_block(a.seq, item, kKB, 0, block);
     }
@@ -446,11 +464,11 @@ __global__ __launch_bounds__(256 * QH, D == 64 && QH == 1 ? 3 : 2) void kv_kerne
     }
   }
   if (qh == 1) return;
-  if (block < a.sink_blocks || a.splits > 1) {
+  if (extra || a.splits > 1 || (block < a.sink_blocks && has_beyond(a, sq, k0))) {
     // fp32 parts: of segments and, behind them, of the blocks' own rows
     if (extra && j0 >= a.sinks) return;
     const int64_t at = extra ? ((int64_t)unit * a.sink_blocks + block) * a.slots_s + item / a.sink_blocks
-                             : own_part(a, unit, si, block, item, split);
+                             : own_part(a, unit, sq, si, block, item, split);
     float* pk = a.part + at * (2 * kKB * D) + (kg * 32 + l32) * D;
     float* pv = pk + kKB * D;
 #pragma unroll
@@ -485,16 +503,19 @@ __global__ __launch_bounds__(256) void part_sum_kernel(const BArgs a, int blocks
       slot = e;
       si = find_block(a.seq, slot, kKB, 0, block);
     } else {
-      si = e / a.sink_blocks;
+      // the last sequence that starts at this place, if it is a long one
+      const int place = e / a.sink_blocks;
+      si = last_seq(a.seq, place, [&](int64_t start, int i) { return long_place(a, start, i); });
+      if (long_place(a, clamp_row(a.seq.cu[si], 0, a.seq.Tq), si) != place) return;
       block = e % a.sink_blocks;
     }
   }
   const Seq sq = get_seq(a.seq, si);
   const int k0 = block * kKB;
-  if (block < 0 || k0 >= sq.nk) return;
+  if (block < 0 || k0 >= sq.nk || (a.splits == 1 && !has_beyond(a, sq, k0))) return;
   const int64_t one = 2 * kKB * D;
-  const float* own = a.part + own_part(a, unit, si, block, slot, 0) * one;
-  const int first = a.seq.cu == nullptr || a.seg == 0 ? 0 : (int)(sq.q0 / a.seg) + si;
+  const float* own = a.part + own_part(a, unit, sq, si, block, slot, 0) * one;
+  const int first = a.seq.cu == nullptr || a.seg == 0 ? 0 : first_seg(a, sq.q0, si);
   const int nseg = block < a.sink_blocks ? (sq.nq + a.seg - 1) / a.seg : 0;
   // segments that end before the rows beyond the block's own have no part
   const QRange mine = own_rows(a, sq, k0);
@@ -713,6 +734,10 @@ __global__ __launch_bounds__(256, 2) void q_kernel(const BArgs a) {
 
 int64_t up256(int64_t n) { return (n + 255) & ~(int64_t)255; }
 
+// Packed sequences of window + kKB rows or more, at most.
+int64_t long_rows(const GdnAttnParams& P) { return (int64_t)P.window + kKB; }
+int long_seqs(const GdnAttnParams& P) { return (int)std::min<int64_t>(P.N, P.Tq / long_rows(P)); }
+
 // Blocks of first keys, rows a segment and segment slots of a call (none where
 // no row lies beyond the first block's window: its last key kKB - 1 is in reach
 // of positions up to kKB - 2 + window, and the last position is Tk - 1).
@@ -726,7 +751,7 @@ void sink_plan(const GdnAttnParams& P, int& blocks, int& seg, int& slots) {
   const int64_t group = P.Hq / P.Hk, own = ((int64_t)P.window + kKB) / kSegRows;
   const int64_t tiles = std::max<int64_t>(1, std::min<int64_t>(16 / group, own / 2));
   seg = (int)std::max<int64_t>(tiles * kSegRows, (int64_t)blocks * kKB);
-  slots = P.cu_seqlens == nullptr ? (P.Tq + seg - 1) / seg : P.Tq / seg + P.N;
+  slots = P.cu_seqlens == nullptr ? (P.Tq + seg - 1) / seg : P.Tq / seg + long_seqs(P);
 }
 
 // Key blocks (slots) of a call, and the workgroups that share one: where the
@@ -754,7 +779,7 @@ Space space(const GdnAttnParams& P) {
   s.vmax = s.rmax + (P.dtype == GDN_DTYPE_F16 ? up256(rows * P.Hq * 4) : 0);
   s.part = s.vmax + (P.dtype == GDN_DTYPE_F16 ? up256((int64_t)P.B * P.Hk * kVParts * 4) : 0);
   const int64_t units = key_units(P), splits = key_splits(P);
-  const int64_t own = splits > 1 ? key_slots(P) * splits : (int64_t)blocks * (P.cu_seqlens == nullptr ? 1 : P.N);
+  const int64_t own = splits > 1 ? key_slots(P) * splits : (int64_t)blocks * (P.cu_seqlens == nullptr ? 1 : long_seqs(P));
   s.total = s.part + up256(units * ((int64_t)blocks * slots + own) * 2 * kKB * P.D * 4);
   return s;
 }
@@ -772,7 +797,7 @@ int launch(const BArgs& a, hipStream_t s) {
     else hipLaunchKernelGGL((kv_kernel<T, D, 2>), dim3((uint32_t)kvb), dim3(512), 0, s, a);
   }
   if (a.sink_blocks > 0 || a.splits > 1) {
-    const int64_t blocks = a.splits > 1 ? a.slots_k : (int64_t)a.sink_blocks * (a.seq.cu == nullptr ? 1 : a.seq.N);
+    const int64_t blocks = a.splits > 1 ? a.slots_k : (int64_t)a.sink_blocks * (a.seq.cu == nullptr ? 1 : a.longs);
     const int64_t pb = a.units_k * blocks * (kKB / 8);
     if (pb > 0x7fffffffLL) return GDN_ERR_BAD_SHAPE;
     if (pb > 0) hipLaunchKernelGGL((part_sum_kernel<T, D>), dim3((uint32_t)pb), dim3(256), 0, s, a, (int)blocks);
@@ -853,6 +878,8 @@ int gdn_attn_bwd_launch(const GdnAttnParams* prm, void* stream) {
   // 602 and 581; 1040 blocks of D 64: 219 and 170)
   a.kv_halves = (int64_t)a.units_k * a.slots_k >= 512 ? 1 : 2;
   sink_plan(P, a.sink_blocks, a.seg, a.slots_s);
+  a.longs = long_seqs(P);
+  a.long_rows = (int)std::min<int64_t>(long_rows(P), 0x7fffffff);
   a.window = P.window;
   a.sinks = P.sinks;
   a.scale = P.scale;

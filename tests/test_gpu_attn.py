@@ -584,3 +584,26 @@ def test_first_keys_of_many_sequences(pkg, cuda, lens, window, sinks, Hk):
     T = sum(lens)
     q, k, v, do = _inputs(cuda, 1, T, T, 2 * Hk, Hk, 64, torch.float16 if Hk == 1 else torch.bfloat16, seed=T)
     _check(pkg, q, k, v, do, window, sinks, lens=lens)
+
+
+def test_fp16_gradients_of_packed_sequences_apart(pkg, cuda):
+    """A sequence's gradients do not depend on its neighbours' values, nor on
+    rows that no sequence holds: the same bits beside values 2^14 times as large,
+    and precise by their own size."""
+    lens, T = [130, 70, 200], 500
+    q, k, v, do = _inputs(cuda, 1, T, T, 2, 1, 64, torch.float16, seed=41)
+    cu = torch.tensor([0, 130, 200, 400], device=cuda)
+    v = v * 2.0 ** -4
+    v2 = v.clone()
+    v2[:, 130:200] *= 2.0 ** 14
+    v2[:, 400:] = 60000.0
+    got = []
+    for x in (v, v2):
+        o, lse = pkg.window_attn(q, k, x, 50, 2, cu_seqlens=cu, return_lse=True)
+        got.append(pkg.window_attn_bwd(q, k, x, o, lse, do, 50, 2, cu_seqlens=cu))
+    for s, e in ((0, 130), (200, 400)):
+        for a, b in zip(*got):
+            assert torch.equal(a[:, s:e], b[:, s:e])
+        _, _, want, sizes = oracle(q[0, s:e], k[0, s:e], v[0, s:e], 50, 2, do=do[0, s:e])
+        for g, w, n, name in zip(got[1], want, (*sizes, 0.0), ("dq", "dk", "dv")):
+            _close(g[0, s:e], w, 4, n, name)

@@ -290,7 +290,7 @@ __device__ __forceinline__ int find_block(const SeqArgs& a, int slot, int rows, 
     block = slot % nblk;
     return slot / nblk;
   }
-  auto first = [&](int64_t start, int i) { return (int)(start / rows) + i; };
+  auto first = [&](int64_t start, int i) { return (int)((uint32_t)start / (uint32_t)rows) + i; };
   const int i = last_seq(a, slot, first);
   block = slot - first(clamp_row(a.cu[i], 0, a.Tq), i);
   return i;

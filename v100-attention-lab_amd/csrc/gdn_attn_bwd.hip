@@ -15,9 +15,8 @@
 //
 // fp16 keeps P times 2^14 and dS in a unit of its own, 2^-7 of the product of
 // the largest |dO| (of the row, or of the tiles so far) and the largest |v| of
-// the head: |dS| <= 2 D of that product, so none overflows and small gradients
-// keep their precision.
-
+// the sequence's head: |dS| <= 2 D of that product, so none overflows and small
+// gradients keep their precision.  Neither looks beyond the sequence.
 //
 // Bound by the matrix cores and the operands' way through LDS: a wave's 32 keys
 // by 32 rows at head size 128 are 32 products (1024 cycles of a SIMD) and 40 KB
@@ -41,7 +40,7 @@ constexpr int kSegRows = 64;   // rows of segments come in multiples of it
 constexpr int kQB = 128;       // query rows a workgroup (q)
 constexpr int kKT = 64;        // keys a tile (q)
 constexpr int kFewTiles = 4;   // up to so many key tiles a block of rows sums D itself (q)
-constexpr int kVParts = 64;    // partial maxima of |v| a head
+constexpr int kVParts = 64;    // partial maxima of |v| a head of a sequence, at most
 
 struct BArgs {
   const uint16_t* q;
@@ -55,14 +54,15 @@ struct BArgs {
   uint16_t* dv;
   float* stat;      // [Hq][rows][2]: lse in powers of 2, D
   float* rmax;      // [Hq][rows] largest |dO| (fp16)
-  float* vmax;      // [units_k][kVParts] (fp16)
+  float* vmax;      // [units_k][v_slots] (fp16)
   float* part;      // [units_k][sink blocks][slots_s][2][kKB][D], then own_part's
   SeqArgs seq;
   int64_t qs[3], ks[3], vs[3], os[3], dos[3], dqs[3], dks[3], dvs[3];
   int64_t rows;     // B Tq
-  int Hq, Hk, G, B;
+  int Hq, Hk, G;
   int units_q, units_k;         // (batch and) heads of the q and kv grids
   int slots_q, slots_k;         // blocks of each
+  int v_rows, v_slots;          // rows of a partial maximum of |v|, slots of a unit's
   int kv_halves;                // waves of a workgroup / 4 (kv)
   int splits;                   // workgroups a key block
   int sink_blocks, seg, slots_s;  // blocks of the first keys, rows a segment, segment slots
@@ -105,17 +105,25 @@ __device__ __forceinline__ float finite_abs(float x) {
   return y < __builtin_inff() ? y : 0.f;
 }
 
-// One part of the keys of one head: the largest |v|.
+// v_rows keys of one head of a sequence: the largest |v|.
 template <int D>
 __global__ __launch_bounds__(256) void v_max_kernel(const BArgs a) {
   constexpr int L = D / 8, RPB = 256 / L;      // lanes a row, rows a workgroup
-  const int part = blockIdx.x % kVParts, unit = blockIdx.x / kVParts;
-  const int b = unit / a.Hk, hk = unit % a.Hk;
-  const int n = (a.seq.Tk + kVParts - 1) / kVParts, t0 = part * n, t1 = min(t0 + n, a.seq.Tk);
+  const int slot = blockIdx.x % a.v_slots, unit = blockIdx.x / a.v_slots;
+  int hk = unit, part;
+  const int si = find_block(a.seq, slot, a.v_rows, a.v_slots, part);
+  Seq sq = get_seq(a.seq, si);
+  if (a.seq.cu == nullptr) {
+    sq.b = unit / a.Hk;
+    hk = unit % a.Hk;
+  }
+  if (part < 0) return;
+  const int64_t t0 = (int64_t)part * a.v_rows;
+  const int t1 = (int)min(t0 + a.v_rows, (int64_t)sq.nk);
   float m = 0.f;
-  for (int t = t0 + threadIdx.x / L; t < t1; t += RPB) {
+  for (int64_t t = t0 + threadIdx.x / L; t < t1; t += RPB) {
     rowio::Pack<f16, 8> pv;
-    pv.load(reinterpret_cast<const f16*>(a.v) + b * a.vs[0] + (int64_t)t * a.vs[1] + hk * a.vs[2] + 8 * (threadIdx.x % L));
+    pv.load(reinterpret_cast<const f16*>(a.v) + sq.b * a.vs[0] + (sq.k0 + t) * a.vs[1] + hk * a.vs[2] + 8 * (threadIdx.x % L));
 #pragma unroll
     for (int i = 0; i < 8; ++i) m = fmaxf(m, finite_abs(pv.get(i)));
   }
@@ -124,12 +132,15 @@ __global__ __launch_bounds__(256) void v_max_kernel(const BArgs a) {
   __shared__ float sm[4];
   if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
   __syncthreads();
-  if (threadIdx.x == 0) a.vmax[unit * kVParts + part] = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+  if (threadIdx.x == 0) a.vmax[(int64_t)unit * a.v_slots + slot] = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
 }
 
-// The largest |v| of a head, as a power of 2.
-__device__ __forceinline__ float v_unit(const BArgs& a, int b, int hk, int lane) {
-  float m = a.vmax[(b * a.Hk + hk) * kVParts + lane];
+// The largest |v| of a head of a sequence, as a power of 2.
+__device__ __forceinline__ float v_unit(const BArgs& a, const Seq& sq, int si, int hk, int lane) {
+  const int n = ((uint32_t)sq.nk + (uint32_t)a.v_rows - 1) / (uint32_t)a.v_rows;    // kVParts at most
+  const int64_t first = a.seq.cu == nullptr ? ((int64_t)sq.b * a.Hk + hk) * a.v_slots
+                                            : (int64_t)hk * a.v_slots + (uint32_t)sq.k0 / (uint32_t)a.v_rows + si;
+  float m = lane < n ? a.vmax[first + lane] : 0.f;
 #pragma unroll
   for (int s = 32; s >= 1; s >>= 1) m = fmaxf(m, __shfl_xor(m, s, 64));
   return pow2_above(m);
@@ -267,7 +278,7 @@ __global__ __launch_bounds__(256 * QH, D == 64 && QH == 1 ? 3 : 2) void kv_kerne
   }
   float vu = 1.f;
   if constexpr (kScaled<T>)
-    if (n > 0) vu = v_unit(a, sq.b, hk, lane);
+    if (n > 0) vu = v_unit(a, sq, si, hk, lane);
   float unit_do = 0x1p-24f;                     // unit of dO so far (fp16)
   f32x16 dk[D / 32] = {}, dv[D / 32] = {};
 
@@ -676,7 +687,7 @@ __global__ __launch_bounds__(256, 2) void q_kernel(const BArgs a) {
   }
   float u = 1.f, sc = 1.f;
   if constexpr (kScaled<T>) {
-    u = pow2_above(dmax) * v_unit(a, sq.b, hk, lane);
+    u = pow2_above(dmax) * v_unit(a, sq, si, hk, lane);
     sc = 0x1p-7f * pow2_inverse(u);
   }
   const float lb = kPUp<T> - lse2, de = -dsum * sc;
@@ -766,6 +777,10 @@ int key_splits(const GdnAttnParams& P) {
   return (int)std::max<int64_t>(1, std::min<int64_t>(256 / blocks, tiles / 4));
 }
 
+// Partial maxima of |v|: rows of each (64 cover every sequence), slots a unit.
+int v_rows(const GdnAttnParams& P) { return std::max(1, (P.Tk + kVParts - 1) / kVParts); }
+int64_t v_slots(const GdnAttnParams& P) { return P.cu_seqlens == nullptr ? kVParts : P.Tk / v_rows(P) + P.N; }
+
 struct Space {
   int64_t stat, rmax, vmax, part, total;
 };
@@ -777,7 +792,7 @@ Space space(const GdnAttnParams& P) {
   s.stat = 0;
   s.rmax = s.stat + up256(rows * P.Hq * 8);
   s.vmax = s.rmax + (P.dtype == GDN_DTYPE_F16 ? up256(rows * P.Hq * 4) : 0);
-  s.part = s.vmax + (P.dtype == GDN_DTYPE_F16 ? up256((int64_t)P.B * P.Hk * kVParts * 4) : 0);
+  s.part = s.vmax + (P.dtype == GDN_DTYPE_F16 ? up256(key_units(P) * v_slots(P) * 4) : 0);
   const int64_t units = key_units(P), splits = key_splits(P);
   const int64_t own = splits > 1 ? key_slots(P) * splits : (int64_t)blocks * (P.cu_seqlens == nullptr ? 1 : long_seqs(P));
   s.total = s.part + up256(units * ((int64_t)blocks * slots + own) * 2 * kKB * P.D * 4);
@@ -786,7 +801,7 @@ Space space(const GdnAttnParams& P) {
 
 template <typename T, int D>
 int launch(const BArgs& a, hipStream_t s) {
-  const int64_t vb = kScaled<T> && a.rows > 0 ? (int64_t)a.B * a.Hk * kVParts : 0;
+  const int64_t vb = kScaled<T> && a.rows > 0 ? (int64_t)a.units_k * a.v_slots : 0;
   const int64_t kvb = (int64_t)a.units_k * ((int64_t)a.slots_k * a.splits + (int64_t)a.sink_blocks * a.slots_s);
   const int64_t qb = (int64_t)a.units_q * a.slots_q;
   if (vb > 0x7fffffffLL || kvb > 0x7fffffffLL || qb > 0x7fffffffLL) return GDN_ERR_BAD_SHAPE;
@@ -862,7 +877,6 @@ int gdn_attn_bwd_launch(const GdnAttnParams* prm, void* stream) {
     a.dvs[d] = P.dv_stride[d];
   }
   a.rows = (int64_t)P.B * P.Tq;
-  a.B = P.B;
   a.Hq = P.Hq;
   a.Hk = P.Hk;
   a.G = P.Hq / P.Hk;
@@ -878,6 +892,8 @@ int gdn_attn_bwd_launch(const GdnAttnParams* prm, void* stream) {
   // 602 and 581; 1040 blocks of D 64: 219 and 170)
   a.kv_halves = (int64_t)a.units_k * a.slots_k >= 512 ? 1 : 2;
   sink_plan(P, a.sink_blocks, a.seg, a.slots_s);
+  a.v_rows = v_rows(P);
+  a.v_slots = (int)v_slots(P);
   a.longs = long_seqs(P);
   a.long_rows = (int)std::min<int64_t>(long_rows(P), 0x7fffffff);
   a.window = P.window;

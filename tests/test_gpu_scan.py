@@ -215,3 +215,47 @@ def test_repeatable(pkg, cuda):
     runs = [(*pkg.gated_scan(x, g, h0), *pkg.gated_scan_bwd(x, g, h0, dy, df)) for _ in range(3)]
     for r in runs[1:]:
         assert all(torch.equal(a, b) for a, b in zip(r, runs[0]))
+
+
+@pytest.mark.parametrize("gate", [0.3, 2.0, 8.0])
+@pytest.mark.parametrize("xd,gd", TYPES)
+def test_infinite_states_stay(pkg, cuda, xd, gd, gate):
+    """An infinite state stays infinite under finite gates however many rows it
+    lives through, forward and backward, and a gate of -inf makes it NaN as
+    0 inf is; other channels keep their bits."""
+    T = 2500
+    x, g, h0, dy, df = _inputs(cuda, 2, T, 66, xd, gd, 2, seed=51, gate=gate)
+    y, fs, st = pkg.gated_scan(x, g, h0, return_states=True)
+    dx, dg, dh0 = pkg.gated_scan_bwd(x, g, h0, dy, df, states=st)
+    x2, h2, df2, dy2 = x.clone(), h0.clone(), df.clone(), dy.clone()
+    inf = float("inf")
+    h2[0, 7], h2[1, 8], x2[0, 300, 9] = inf, -inf, inf
+    df2[0, 20], dy2[1, 2000, 21] = -inf, inf
+    y2, fs2, st2 = pkg.gated_scan(x2, g, h2, return_states=True)
+    assert (y2[0, :, 7] == inf).all() and (y2[1, :, 8] == -inf).all() and (y2[0, 300:, 9] == inf).all()
+    assert fs2[0, 7] == inf and fs2[1, 8] == -inf and fs2[0, 9] == inf
+    hit = torch.zeros_like(y2, dtype=torch.bool)
+    hit[0, :, 7] = hit[1, :, 8] = hit[0, 300:, 9] = True
+    assert torch.equal(y2[~hit], y[~hit])
+    for states in (st, None):
+        dx2, _, dh2 = pkg.gated_scan_bwd(x, g, h0, dy2, df2, states=states)
+        assert (dx2[0, :, 20] == -inf).all() and (dx2[1, :2001, 21] == inf).all()
+        assert dh2[0, 20] == -inf and dh2[1, 21] == inf
+        hit = torch.zeros_like(dx2, dtype=torch.bool)
+        hit[0, :, 20] = hit[1, :2001, 21] = True
+        assert torch.equal(dx2[~hit], dx[~hit])
+    g2 = g.clone()
+    g2[0, 900, 7] = -inf
+    y2, _ = pkg.gated_scan(x2, g2, h2)
+    assert (y2[0, :900, 7] == inf).all() and torch.isnan(y2[0, 900:, 7]).all()
+
+
+def test_growing_gates_before_any_state(pkg, cuda):
+    """Gates above 0 over rows whose state is still zero: e^G of many rows leaves
+    the range of floats, the rows' own states do not."""
+    x, g, _, dy, _ = _inputs(cuda, 1, 2600, 64, torch.float32, torch.float32, 1, seed=52)
+    g[:, :2200] = 0.5
+    x[:, :2200] = 0.0
+    y, fs = pkg.gated_scan(x, g)
+    want = oracle(x, g, None, dy, None, None)
+    assert _err(y, want[0]) <= F32 and _err(fs, want[1]) <= F32

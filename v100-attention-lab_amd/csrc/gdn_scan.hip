@@ -145,6 +145,38 @@ __device__ __forceinline__ float step(float t, float h, float x) {
   return __builtin_fmaf(t, near1 ? __builtin_amdgcn_fmed3f(h, -top, top) : h, near1 ? h + x : x);
 }
 
+// e^G h + H for rows together, G the sum of their g.
+struct Plain {
+  __device__ __forceinline__ float operator()(float G, float h, float H) const { return step(decay(G), h, H); }
+};
+// The same where e^G leaves the range of floats and the rows' own gates do not:
+// of a state 0 it stays 0, and an infinite one stays infinite (but under a gate of
+// -inf, where it becomes NaN as 0 inf does for a row).
+struct Careful {
+  __device__ __forceinline__ float operator()(float G, float h, float H) const {
+    const bool inf = fabsf(h) == __builtin_inff() && G > -__builtin_inff();
+    return step(h == 0.f || inf ? 1.f : decay(G), h, H);
+  }
+};
+// walk(join, h): a chain of joins from h on.  0 inf shows as NaN at its end: only
+// then the chain is taken again, carefully (taken so at once, B4 T4096 D2048 takes
+// 200 us forward and backward instead of 188).
+template <int V, typename Walk>
+__device__ __forceinline__ void chain(float (&h)[V], Walk walk) {
+  float first[V];
+  bool odd = false;
+#pragma unroll
+  for (int e = 0; e < V; ++e) first[e] = h[e];
+  walk(Plain{}, h);
+#pragma unroll
+  for (int e = 0; e < V; ++e) odd |= h[e] != h[e];
+  if (__any(odd)) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) h[e] = first[e];
+    walk(Careful{}, h);
+  }
+}
+
 template <typename TX, typename TG, int V>
 __device__ __forceinline__ void load_rows(const TX* x, const TG* g, int64_t xs, int64_t gs, int n, bool ok,
                                           Pack<TX, V> (&xr)[kRows], Pack<TG, V> (&gr)[kRows]) {
@@ -208,37 +240,44 @@ template <int V, bool REV>
 __device__ __forceinline__ void leave(const Args& p, const Join<V>& sh, uint32_t u, int c0) {
   const int ch = threadIdx.x, c = c0 + ch;
   if (ch >= 64 * V || c >= p.D) return;
-  float g = 0.f, h = 0.f;
+  float g = 0.f, h[1] = {0.f};
 #pragma unroll
-  for (int s = 0; s < kWaves; ++s) {
-    const int i = REV ? kWaves - 1 - s : s;
-    h = step(decay(sh.g[i][ch]), h, sh.h[i][ch]);
-    g += sh.g[i][ch];
-  }
-  leave_pair(p.agg + (int64_t)u * p.D + c, g, h);
+  for (int i = 0; i < kWaves; ++i) g += sh.g[i][ch];
+  chain<1>(h, [&](auto join, float (&h)[1]) {
+#pragma unroll
+    for (int s = 0; s < kWaves; ++s) {
+      const int i = REV ? kWaves - 1 - s : s;
+      h[0] = join(sh.g[i][ch], h[0], sh.h[i][ch]);
+    }
+  });
+  leave_pair(p.agg + (int64_t)u * p.D + c, g, h[0]);
   if (u % kSet != kSet - 1) return;
   const uint64_t* first = p.agg + (int64_t)(u - (kSet - 1)) * p.D + c;
   constexpr int kBatch = 5;
   static_assert((kSet - 1) % kBatch == 0, "whole batches");
-  float gs = 0.f, hs = 0.f;
+  float gs = 0.f, hs[1] = {0.f};
+  chain<1>(hs, [&](auto join, float (&hs)[1]) {
+    gs = 0.f;
 #pragma unroll 1
-  for (int k = 0; k < kSet - 1; k += kBatch) {
-    uint64_t v[kBatch];
-    bool all;
-    do {
-      all = true;
+    for (int k = 0; k < kSet - 1; k += kBatch) {
+      uint64_t v[kBatch];
+      bool all;
+      do {
+        all = true;
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) v[i] = look(first + (int64_t)(k + i) * p.D);
+        for (int i = 0; i < kBatch; ++i) v[i] = look(first + (int64_t)(k + i) * p.D);
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) all &= v[i] != kAbsent;
-    } while (!all);
+        for (int i = 0; i < kBatch; ++i) all &= v[i] != kAbsent;
+      } while (!all);
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      hs = step(decay(pair_g(v[i])), hs, pair_h(v[i]));
-      gs += pair_g(v[i]);
+      for (int i = 0; i < kBatch; ++i) {
+        hs[0] = join(pair_g(v[i]), hs[0], pair_h(v[i]));
+        gs += pair_g(v[i]);
+      }
     }
-  }
-  leave_pair(p.agg16 + (int64_t)(u / kSet) * p.D + c, gs + g, step(decay(g), hs, h));
+    hs[0] = join(g, hs[0], h[0]);
+  });
+  leave_pair(p.agg16 + (int64_t)(u / kSet) * p.D + c, gs + g, hs[0]);
 }
 
 // The state h (of this lane's V channels) behind the places first .. u - 1, in
@@ -287,9 +326,22 @@ __device__ __forceinline__ void carry(const Args& p, Join<V>& sh, uint32_t first
         if (k + i < k1) {
 #pragma unroll
           for (int e = 0; e < V; ++e) {
-            H[e] = step(decay(pair_g(v[i][e])), H[e], pair_h(v[i][e]));
+            H[e] = Plain{}(pair_g(v[i][e]), H[e], pair_h(v[i][e]));
             G[e] += pair_g(v[i][e]);
           }
+        }
+      }
+    }
+    // (see chain; here a loop of its own over pairs that are all there: as a chain
+    // the loop above made the fp32 backward of 50001 rows of 640 143 us, not 135)
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      if (H[e] != H[e]) {
+        H[e] = 0.f;
+#pragma unroll 1
+        for (int k = k0; k < k1; ++k) {
+          const uint64_t v = look(at(k) + e);
+          H[e] = Careful{}(pair_g(v), H[e], pair_h(v));
         }
       }
     }
@@ -300,10 +352,12 @@ __device__ __forceinline__ void carry(const Args& p, Join<V>& sh, uint32_t first
     sh.h[w][lane * V + e] = H[e];
   }
   __syncthreads();
-  for (int i = 0; i < kWaves && i * share < n; ++i) {
+  chain<V>(h, [&](auto join, float (&h)[V]) {
+    for (int i = 0; i < kWaves && i * share < n; ++i) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) h[e] = step(decay(sh.g[i][lane * V + e]), h[e], sh.h[i][lane * V + e]);
-  }
+      for (int e = 0; e < V; ++e) h[e] = join(sh.g[i][lane * V + e], h[e], sh.h[i][lane * V + e]);
+    }
+  });
 }
 
 // ---------------------------------------------------------------------------
@@ -375,10 +429,12 @@ __global__ __launch_bounds__(kThreads, (kMore<TX, TG> ? 6 : 4)) void fwd_kernel(
   }
   if constexpr (ONLY_STATES) return;
   TX* y = static_cast<TX*>(p.y) + j.b * p.ys[0] + (j.row + r0) * p.ys[1] + c;
-  for (int i = 0; i < w; ++i) {
+  chain<V>(h, [&](auto join, float (&h)[V]) {
+    for (int i = 0; i < w; ++i) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) h[e] = step(decay(waves.g[i][lane * V + e]), h[e], waves.h[i][lane * V + e]);
-  }
+      for (int e = 0; e < V; ++e) h[e] = join(waves.g[i][lane * V + e], h[e], waves.h[i][lane * V + e]);
+    }
+  });
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
     if (i < n) {
@@ -429,13 +485,14 @@ __global__ __launch_bounds__(kThreads, 4) void bwd_kernel(const Args p, bool sin
     if (i < n && ok) dr[i].load(dy + i * p.dys[1]);
   }
   float h[V], d[V];
+  auto start = [&](int e) {
+    if (!ok || j.chunk < 0) return 0.f;
+    if (!single && j.len > 0) return p.states[(int64_t)slot * p.D + c + e];
+    return p.h0 != nullptr ? p.h0[j.seq * p.h0s + c + e] : 0.f;
+  };
 #pragma unroll
   for (int e = 0; e < V; ++e) {
-    h[e] = 0.f;
-    if (ok && j.chunk >= 0) {
-      if (!single && j.len > 0) h[e] = p.states[(int64_t)slot * p.D + c + e];
-      else if (p.h0 != nullptr) h[e] = p.h0[j.seq * p.h0s + c + e];
-    }
+    h[e] = start(e);
     d[e] = ok && p.dfinal != nullptr ? p.dfinal[j.seq * p.dfs + c + e] : 0.f;
   }
   float a[kRows][V], G[V], H[V], R[V];
@@ -478,14 +535,18 @@ __global__ __launch_bounds__(kThreads, 4) void bwd_kernel(const Args p, bool sin
   if (j.chunk < 0 || !ok) return;
   TX* dx = static_cast<TX*>(p.dx) + j.b * p.dxs[0] + row * p.dxs[1] + c;
   TG* dg = static_cast<TG*>(p.dg) + j.b * p.dgs[0] + row * p.dgs[1] + c;
-  for (int i = 0; i < w; ++i) {
+  chain<V>(h, [&](auto join, float (&h)[V]) {
+    for (int i = 0; i < w; ++i) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) h[e] = step(decay(waves.g[i][lane * V + e]), h[e], sh_h[i][lane * V + e]);
-  }
-  for (int i = kWaves - 1; i > w; --i) {
+      for (int e = 0; e < V; ++e) h[e] = join(waves.g[i][lane * V + e], h[e], sh_h[i][lane * V + e]);
+    }
+  });
+  chain<V>(d, [&](auto join, float (&d)[V]) {
+    for (int i = kWaves - 1; i > w; --i) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) d[e] = step(decay(waves.g[i][lane * V + e]), d[e], waves.h[i][lane * V + e]);
-  }
+      for (int e = 0; e < V; ++e) d[e] = join(waves.g[i][lane * V + e], d[e], waves.h[i][lane * V + e]);
+    }
+  });
   float ah[kRows][V];   // e^{g_t} h_{t-1}
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {

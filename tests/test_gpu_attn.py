@@ -607,3 +607,24 @@ def test_fp16_gradients_of_packed_sequences_apart(pkg, cuda):
         _, _, want, sizes = oracle(q[0, s:e], k[0, s:e], v[0, s:e], 50, 2, do=do[0, s:e])
         for g, w, n, name in zip(got[1], want, (*sizes, 0.0), ("dq", "dk", "dv")):
             _close(g[0, s:e], w, 4, n, name)
+
+
+def test_scale_changed_in_place(pkg, cuda):
+    """A scale that comes as a tensor counts by its value at the call."""
+    q, k, v, do = _inputs(cuda, 1, 100, 100, 2, 1, 64, torch.bfloat16, seed=61)
+    lens = torch.tensor([100], dtype=torch.int32, device=cuda)
+    scale = torch.tensor(0.1)
+    for value in (0.1, 0.4):
+        scale.fill_(value)
+        o, lse = pkg.window_attn(q, k, v, 30, 2, scale, return_lse=True)
+        want = pkg.window_attn(q, k, v, 30, 2, value, return_lse=True)
+        assert torch.equal(o, want[0]) and torch.equal(lse, want[1])
+        got = pkg.window_attn_bwd(q, k, v, o, lse, do, 30, 2, scale)
+        assert all(torch.equal(a, b) for a, b in zip(got, pkg.window_attn_bwd(q, k, v, o, lse, do, 30, 2, value)))
+        assert torch.equal(pkg.window_attn_decode(q[:, -1:], k, v, lens, 30, 2, scale),
+                           pkg.window_attn_decode(q[:, -1:], k, v, lens, 30, 2, value))
+    a = q.clone().requires_grad_()
+    o = pkg.window_attn(a, k, v, 30, 2, scale)
+    scale.fill_(0.1)
+    o.backward(do)
+    assert torch.equal(a.grad, got[0])

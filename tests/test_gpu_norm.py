@@ -234,3 +234,21 @@ def test_other_stream_and_repeat(pkg, cuda):
         again = (*pkg.add_rms_norm(x, w, res), *pkg.add_rms_norm_bwd(res, w, dy, dr))
     torch.cuda.current_stream().wait_stream(s)
     assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+def test_eps_changed_in_place(pkg, cuda):
+    """An eps that comes as a tensor counts by its value at the call, in the
+    backward too."""
+    gen = torch.Generator(device=cuda).manual_seed(71)
+    x, dy = (torch.randn(6, 64, generator=gen, device=cuda) for _ in range(2))
+    w = torch.ones(64, device=cuda)
+    grads = []
+    for change in (False, True):
+        eps = torch.tensor(0.5)
+        a = x.clone().requires_grad_()
+        y, _ = pkg.add_rms_norm(a, w, None, eps)
+        if change:
+            eps.fill_(5.0)
+        y.backward(dy)
+        grads.append(a.grad)
+    assert torch.equal(*grads)

@@ -30,6 +30,12 @@ def _check_window(window, sinks):
     return min(window, _INT_MAX), min(sinks, _INT_MAX)
 
 
+def _number(scale):
+    """scale as a float (or None): plans and the backward keep its value, not a
+    tensor that may change."""
+    return None if scale is None else float(scale)
+
+
 def _check_rows(t, name):
     """Rows are read 16 bytes at a time; strides of single indexes do not count."""
     if t.numel() == 0:
@@ -84,7 +90,7 @@ def _params(q, k, v, B, T, S, Hq, Hk, D, n_seq, window, sinks, scale):
     P.B, P.Tq, P.Tk, P.N = B, T, S, B if n_seq is None else n_seq
     P.Hq, P.Hk, P.D = Hq, Hk, D
     P.window, P.sinks = window, sinks
-    P.scale = D ** -0.5 if scale is None else float(scale)
+    P.scale = D ** -0.5 if scale is None else scale
     P.dtype = _DTYPE_CODE[q.dtype]
     P.q_stride[:], P.k_stride[:], P.v_stride[:] = q.stride()[:3], k.stride()[:3], v.stride()[:3]
     P.o_stride[:] = (T * Hq * D, Hq * D, D)
@@ -164,6 +170,7 @@ def window_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: Optio
     is differentiable (``lse`` is not).
     """
     cu, n_seq = _seqs(q, cu_seqlens)
+    scale = _number(scale)
     if _needs_grad(q, k, v):
         o, lse = _AttnFunction.apply(q, k, v, window, sinks, scale, cu, n_seq)
     else:
@@ -236,7 +243,7 @@ def window_attn_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.
     head's gradient is the sum over the query heads that share it, in a fixed
     order: repeated calls give the same bits."""
     cu, n_seq = _seqs(q, cu_seqlens)
-    return _run_bwd(q, k, v, o, lse, do, window, sinks, scale, cu, n_seq)
+    return _run_bwd(q, k, v, o, lse, do, window, sinks, _number(scale), cu, n_seq)
 
 
 class _AttnFunction(torch.autograd.Function):
@@ -271,7 +278,7 @@ def _decode_plan(q, k_cache, v_cache, lens, window, sinks, scale):
     P = _lib.GdnAttnDecodeParams()
     P.B, P.T, P.S, P.Hq, P.Hk, P.D = B, T, S, Hq, Hk, D
     P.window, P.sinks = w, s
-    P.scale = D ** -0.5 if scale is None else float(scale)
+    P.scale = D ** -0.5 if scale is None else scale
     P.dtype = _DTYPE_CODE[q.dtype]
     P.q_stride[:], P.k_stride[:], P.v_stride[:] = q.stride()[:3], k_cache.stride()[:3], v_cache.stride()[:3]
     P.o_stride[:] = (T * Hq * D, Hq * D, D)
@@ -299,6 +306,7 @@ def window_attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
     """
     if _needs_grad(q, k_cache, v_cache):
         raise NotImplementedError("window_attn_decode has no gradient: use window_attn in training")
+    scale = _number(scale)
     try:
         key = (_sig(q), _sig(k_cache), _sig(v_cache), _sig(cache_seqlens), window, sinks, scale)
         plan = _DECODE_PLANS.get(key)

@@ -131,6 +131,7 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch
       input requires grad.
     """
     if _needs_grad(x, weight, residual):
+        eps = float(eps)        # (kept for the backward)
         if residual is None:
             return _NormFunction.apply(x, weight, None, eps), x
         return _NormFunction.apply(x, weight, residual, eps)

@@ -252,3 +252,14 @@ def test_eps_changed_in_place(pkg, cuda):
         y.backward(dy)
         grads.append(a.grad)
     assert torch.equal(*grads)
+
+
+def test_no_rows_of_many_dimensions(pkg, cuda):
+    x = torch.zeros(2, 3, 0, 8, device=cuda)
+    w = torch.ones(8, device=cuda)
+    y, r = pkg.add_rms_norm(x, w, x)
+    assert y.shape == r.shape == x.shape
+    dr, dw = pkg.add_rms_norm_bwd(r, w, y)
+    assert dr.shape == x.shape and (dw == 0).all()
+    y, scale, _ = pkg.add_rms_norm_fp8(x, w)
+    assert y.shape == x.shape and scale.shape == (2, 3, 0, 1)

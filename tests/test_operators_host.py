@@ -319,3 +319,15 @@ def test_attn_bwd_workspace_of_many_sequences(lib, pkg):
         return lib.gdn_attn_bwd_workspace_size(ctypes.byref(_attn(pkg._lib, **kw)))
     assert size(8, 4) <= size(56, 4) == size(2048, 4) <= 512 << 20      # 56 * 1152 rows are the most
     assert size(2048, 0) < 17 << 20
+
+
+@pytest.mark.parametrize("shape", [(2, 3, 0, 8), (0, 2, 4, 8), (2, 0, 0, 8), (3, 2, 4, 0)])
+def test_norm_no_rows_of_many_dimensions(pkg, shape):
+    """Leading dimensions without rows are joined like others (the refusal here is
+    of the CPU, or of rows without columns)."""
+    x, w = torch.zeros(shape), torch.ones(shape[-1])
+    msg = "GPU" if shape[-1] else "must be a"
+    for call in (lambda: pkg.add_rms_norm(x, w), lambda: pkg.add_rms_norm(x, w, x), lambda: pkg.add_rms_norm_fp8(x, w),
+                 lambda: pkg.add_rms_norm_bwd(x, w, x)):
+        with pytest.raises(ValueError, match=msg):
+            call()

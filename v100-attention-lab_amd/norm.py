@@ -28,7 +28,7 @@ def _rows(t):
 def _at_most_3d(t):
     """t with its leading dimensions but the last joined (a copy only where its
     strides need one)."""
-    return t.reshape(-1, t.shape[-2], t.shape[-1]) if isinstance(t, torch.Tensor) and t.dim() > 3 else t
+    return t.flatten(0, -3) if isinstance(t, torch.Tensor) and t.dim() > 3 else t
 
 
 def _check_x(x, name, weight):

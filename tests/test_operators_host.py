@@ -331,3 +331,43 @@ def test_norm_no_rows_of_many_dimensions(pkg, shape):
                  lambda: pkg.add_rms_norm_bwd(x, w, x)):
         with pytest.raises(ValueError, match=msg):
             call()
+
+
+def _once(pkg, monkeypatch, name):
+    """(call, inputs): a differentiable operator with its two launches replaced by
+    results of the right shapes."""
+    mod = {"gdn_fwd": pkg.ops, "gated_scan": pkg.scan, "window_attn": pkg.attn, "add_rms_norm": pkg.norm}[name]
+    x = torch.randn(1, 4, 8)
+    q = torch.randn(1, 4, 2, 64)
+    gate = torch.randn(1, 4, 2)
+    case = {
+        "gdn_fwd": ((q, q, q, gate, gate), lambda *a: (torch.ones_like(q), torch.ones(1, 2, 64, 64)),
+                    lambda *a: (torch.ones_like(q),) * 3 + (torch.ones_like(gate),) * 2 + (None,)),
+        "gated_scan": ((x, x), lambda *a: (torch.ones_like(x), torch.ones(1, 8), torch.ones(1, 8)),
+                       lambda *a: (torch.ones_like(x), torch.ones_like(x), None)),
+        "window_attn": ((q, q, q), lambda *a: (torch.ones_like(q), torch.ones(1, 4, 2)),
+                        lambda *a: (torch.ones_like(q),) * 3),
+        "add_rms_norm": ((x, torch.ones(8)), lambda *a: (torch.ones_like(x), None, x),
+                         lambda *a: (torch.ones_like(x), None, torch.ones(8))),
+    }
+    inputs, fwd, bwd = case[name]
+    monkeypatch.setattr(mod, "_run", fwd)
+    monkeypatch.setattr(mod, "_run_bwd", bwd)
+    return getattr(pkg, name), [t.clone().requires_grad_() for t in inputs]
+
+
+@pytest.mark.parametrize("name", ["gdn_fwd", "gated_scan", "window_attn", "add_rms_norm"])
+def test_second_derivatives_are_refused(pkg, monkeypatch, name):
+    """The kernels' gradients have no graph: a gradient of theirs raises instead
+    of leaving out its terms."""
+    call, inputs = _once(pkg, monkeypatch, name)
+    out = call(*inputs)
+    out = out[0] if isinstance(out, tuple) else out
+    grad, = torch.autograd.grad(out.sum(), inputs[0], create_graph=True)
+    assert grad.requires_grad
+    with pytest.raises(RuntimeError, match="second derivatives"):
+        grad.square().sum().backward()
+    call(*inputs)
+    out = call(*inputs)
+    (out[0] if isinstance(out, tuple) else out).sum().backward()       # first ones as before
+    assert inputs[0].grad is not None

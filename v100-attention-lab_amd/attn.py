@@ -10,7 +10,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .ops import _DTYPE_CODE, _PLANS_MAX, _check_devices, _launch, _needs_grad, _offsets
+from .ops import _DTYPE_CODE, _PLANS_MAX, _check_devices, _first_order, _launch, _needs_grad, _offsets
 from .scan import _failed, _like, _sig
 
 SUPPORTED_D = (64, 128)
@@ -256,6 +256,7 @@ class _AttnFunction(torch.autograd.Function):
         return o, lse
 
     @staticmethod
+    @_first_order
     def backward(ctx, do, _):
         q, k, v, o, lse, cu = ctx.saved_tensors
         n_seq = None

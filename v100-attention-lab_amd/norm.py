@@ -9,7 +9,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .ops import _DTYPE_CODE, _PLANS_MAX, _check_devices, _code, _launch, _needs_grad
+from .ops import _DTYPE_CODE, _PLANS_MAX, _check_devices, _code, _first_order, _launch, _needs_grad
 from .scan import _check_columns, _failed, _like, _sig
 
 _FWD_PLANS = {}
@@ -241,6 +241,7 @@ class _NormFunction(torch.autograd.Function):
         return (y, r) if residual is not None else y
 
     @staticmethod
+    @_first_order
     def backward(ctx, dy, dr=None):
         r, weight = ctx.saved_tensors
         if dy is None:

@@ -15,6 +15,7 @@ fallback: without the HIP library or a ROCm device they raise.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional, Tuple
 
 import torch
@@ -676,6 +677,39 @@ def _run_bwd(q, k, v, g, beta, h0, do, dfinal, scale, cu, n_seq, need_dh0, max_s
     return dq, dk, dv, dg, dbeta, dh0
 
 
+class _NoSecond(torch.autograd.Function):
+    """Passes gradients on; theirs raises."""
+
+    @staticmethod
+    def forward(ctx, anchor, *grads):
+        return tuple(t.view_as(t) for t in grads)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("these operators have no second derivatives: a gradient taken with "
+                           "create_graph=True cannot be differentiated through them")
+
+
+def _first_order(backward):
+    """Decorator of an autograd backward that runs kernels: its results carry no
+    graph, so under create_graph (the only backward with grad mode on) their own
+    gradient raises where it would be taken for zero."""
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        create_graph = torch.is_grad_enabled()
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        if not create_graph:
+            return out
+        at = [i for i, t in enumerate(out) if t is not None]
+        kept = _NoSecond.apply(torch.zeros((), requires_grad=True), *(out[i] for i in at))
+        out = list(out)
+        for i, t in zip(at, kept):
+            out[i] = t
+        return tuple(out)
+    return run
+
+
 class _GdnFunction(torch.autograd.Function):
     """``_run`` with the HIP backward: o, final_state differentiable in
     q, k, v, g, beta and h0."""
@@ -690,6 +724,7 @@ class _GdnFunction(torch.autograd.Function):
         return o, fs
 
     @staticmethod
+    @_first_order
     def backward(ctx, do, dfs):
         q, k, v, g, beta, h0, cu = ctx.saved_tensors
         if do is None:

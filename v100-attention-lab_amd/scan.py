@@ -10,7 +10,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .ops import (_DTYPE_CODE, _PLANS_MAX, _check_devices, _code, _launch, _needs_grad, _offsets)
+from .ops import _DTYPE_CODE, _PLANS_MAX, _check_devices, _code, _first_order, _launch, _needs_grad, _offsets
 
 _FWD_PLANS = {}
 _BWD_PLANS = {}
@@ -259,6 +259,7 @@ class _ScanFunction(torch.autograd.Function):
         return y, fs, states
 
     @staticmethod
+    @_first_order
     def backward(ctx, dy, dfs, _):
         x, g, h0, cu, states = ctx.saved_tensors
         n_seq = None

@@ -371,3 +371,34 @@ def test_second_derivatives_are_refused(pkg, monkeypatch, name):
     out = call(*inputs)
     (out[0] if isinstance(out, tuple) else out).sum().backward()       # first ones as before
     assert inputs[0].grad is not None
+
+
+def _calls(pkg):
+    x, w = torch.randn(1, 4, 64), torch.ones(64)
+    q, gate = torch.randn(1, 4, 2, 64).half(), torch.randn(1, 4, 2)
+    lens = torch.ones(1, dtype=torch.int32)
+    return {
+        "gdn_fwd": (pkg.gdn_fwd, (q, q, q, gate, gate)), "gdn_chunk_fwd": (pkg.gdn_chunk_fwd, (q, q, q, gate, gate)),
+        "chunk_gated_delta_rule": (pkg.chunk_gated_delta_rule, (q, q, q, gate, gate)),
+        "gated_scan": (pkg.gated_scan, (x, x)), "window_attn": (pkg.window_attn, (q, q, q)),
+        "window_attn_decode": (pkg.window_attn_decode, (q, q, q, lens)),
+        "add_rms_norm": (pkg.add_rms_norm, (x, w, x)), "add_rms_norm_fp8": (pkg.add_rms_norm_fp8, (x, w, x)),
+    }
+
+
+@pytest.mark.parametrize("name", ["gdn_fwd", "gdn_chunk_fwd", "chunk_gated_delta_rule", "gated_scan", "window_attn",
+                                  "window_attn_decode", "add_rms_norm", "add_rms_norm_fp8"])
+def test_forward_mode_is_refused(pkg, name):
+    """Dual tensors: an error instead of a result without its tangent, whether or
+    not they require grad."""
+    from torch.autograd import forward_ad
+    call, args = _calls(pkg)[name]
+    for i in range(2):
+        for grad in (False, True):
+            with forward_ad.dual_level():
+                dual = list(args)
+                dual[i] = forward_ad.make_dual(args[i].clone().requires_grad_(grad), torch.ones_like(args[i]))
+                with pytest.raises(NotImplementedError, match="forward mode"):
+                    call(*dual)
+                with pytest.raises(ValueError, match="GPU"):        # other tensors beside it pass on
+                    call(*args)

@@ -19,6 +19,7 @@ import functools
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -747,5 +748,10 @@ class _GdnFunction(torch.autograd.Function):
 
 
 def _needs_grad(*ts) -> bool:
+    """Whether the call goes through autograd; refuses tangents, which only dual
+    tensors inside a dual_level() have."""
+    if forward_ad._current_level >= 0 and any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None
+                                              for t in ts):
+        raise NotImplementedError("forward mode (tangents of dual tensors) is not supported")
     return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad
                                            for t in ts)

@@ -402,3 +402,17 @@ def test_forward_mode_is_refused(pkg, name):
                     call(*dual)
                 with pytest.raises(ValueError, match="GPU"):        # other tensors beside it pass on
                     call(*args)
+
+
+def test_scale_without_gradient_is_refused(pkg):
+    """A scale that requires grad would get none."""
+    q = torch.zeros(1, 4, 2, 64, dtype=torch.float16)
+    s = torch.tensor(0.1, requires_grad=True)
+    lens = torch.ones(1, dtype=torch.int32)
+    for call in (lambda: pkg.window_attn(q, q, q, scale=s), lambda: pkg.window_attn_decode(q, q, q, lens, scale=s)):
+        with pytest.raises(NotImplementedError, match="scale"):
+            call()
+        with torch.no_grad(), pytest.raises(ValueError, match="GPU"):
+            call()
+    with pytest.raises(ValueError, match="GPU"):
+        pkg.window_attn(q, q, q, scale=s.detach())

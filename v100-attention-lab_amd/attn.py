@@ -33,6 +33,8 @@ def _check_window(window, sinks):
 def _number(scale):
     """scale as a float (or None): plans and the backward keep its value, not a
     tensor that may change."""
+    if _needs_grad(scale):
+        raise NotImplementedError("scale has no gradient: multiply q by it instead")
     return None if scale is None else float(scale)
 
 
@@ -158,7 +160,7 @@ def window_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: Optio
         {64, 128}, 16-byte aligned rows, any other strides.
       window: keys in reach, the row's own among them; None: all earlier ones.
       sinks: first keys that every later row sees.
-      scale: of the scores, default ``D ** -0.5``.
+      scale: of the scores, a number, default ``D ** -0.5``.
       cu_seqlens: optional int64 ``[N + 1]`` offsets of N sequences packed
         along t (B = 1, S = T), rising from 0 to T.  They are not read on the
         host; the kernels clamp them to ``[0, T]``, and rows outside every

@@ -416,3 +416,17 @@ def test_scale_without_gradient_is_refused(pkg):
             call()
     with pytest.raises(ValueError, match="GPU"):
         pkg.window_attn(q, q, q, scale=s.detach())
+
+
+def test_inline_assembly_names_m0():
+    """Assembly that sets m0 says so to the compiler."""
+    import glob
+    import re
+    found = 0
+    for path in glob.glob(os.path.join(REPO, "v100-attention-lab_amd", "csrc", "*")):
+        with open(path) as f:
+            for asm in re.findall(r"asm volatile\((.*?)\);", f.read(), re.S):
+                if re.search(r"_b32 m0,", asm):
+                    found += 1
+                    assert '"m0"' in asm.split("::")[1], (path, asm)
+    assert found >= 3

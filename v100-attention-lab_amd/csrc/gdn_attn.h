@@ -119,16 +119,15 @@ __device__ __forceinline__ uint32_t lds_addr(const void* p) { return (uint32_t)(
 // uniform).  Written out, so that the compiler does not take every LDS read
 // that follows for a reader of these bytes and wait for them there: a buffer
 // is read only after dma_wait() in every wave that filled it and a barrier.
-// (m0 holds nothing else: the compiler sets it right before each use.)
 // The instruction has no result registers, and a count of outstanding loads
 // that the compiler waits for is only met later for it, never earlier.
 __device__ __forceinline__ void dma16(const void* src, uint32_t at) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(at) : "memory");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(at) : "memory", "m0");
 }
 // the same from a uniform base and a byte offset per lane
 __device__ __forceinline__ void dma16(const void* base, uint32_t ofs, uint32_t at) {
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(ofs), "s"(base), "s"(at)
-               : "memory");
+               : "memory", "m0");
 }
 // Every load of this wave so far, from memory and from LDS, is done.
 __device__ __forceinline__ void dma_wait() {

@@ -208,7 +208,7 @@ __device__ __forceinline__ int64_t own_part(const BArgs& a, int unit, const Seq&
 // 4 bytes per lane from global memory to LDS at `at` + 4 * lane.
 __device__ __forceinline__ void dma4(const void* src, uint32_t at) {
   at = __builtin_amdgcn_readfirstlane(at);
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(at) : "memory");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(at) : "memory", "m0");
 }
 
 template <typename T, int D, int QH>

@@ -263,3 +263,16 @@ def test_no_rows_of_many_dimensions(pkg, cuda):
     assert dr.shape == x.shape and (dw == 0).all()
     y, scale, _ = pkg.add_rms_norm_fp8(x, w)
     assert y.shape == x.shape and scale.shape == (2, 3, 0, 1)
+
+
+def test_more_rows_than_a_launch_holds(pkg, cuda):
+    """2^29 rows of 8 threads each are more than 32 bits of threads."""
+    rows, D = 2 ** 29 + 3, 8
+    gen = torch.Generator(device=cuda).manual_seed(81)
+    row = torch.randn(1, D, generator=gen, device=cuda).to(torch.bfloat16)
+    w = torch.randn(D, generator=gen, device=cuda).to(torch.bfloat16)
+    y, r = pkg.add_rms_norm(row.expand(rows, D), w)
+    want, _ = pkg.add_rms_norm(row, w)
+    words, want = y.view(torch.int64), want.view(torch.int64)       # a row is two
+    for i in range(0, rows, 2 ** 26):
+        assert (words[i:i + 2 ** 26] == want).all(), i

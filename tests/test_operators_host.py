@@ -430,3 +430,27 @@ def test_inline_assembly_names_m0():
                     found += 1
                     assert '"m0"' in asm.split("::")[1], (path, asm)
     assert found >= 3
+
+
+@pytest.mark.parametrize("name,make,kw", [
+    ("gdn_scan_launch", _scan, dict(B=1 << 17, N=1 << 17, T=9, D=8192)),
+    ("gdn_scan_launch", _scan, dict(B=1 << 23, N=1 << 23, T=2, D=1024)),
+    ("gdn_scan_launch", _scan, dict(B=1, N=1 << 23, cu_seqlens=FAKE, T=100, D=64)),
+    ("gdn_scan_launch", _scan, dict(B=1, N=1, T=1, D=2 ** 31 - 1)),
+    ("gdn_scan_launch", _scan, dict(B=1, N=1, T=2 ** 31 - 1, D=1)),
+    ("gdn_scan_bwd_launch", _scan, dict(B=1 << 20, N=1 << 20, T=2, D=2048)),
+    ("gdn_norm_launch", _norm, dict(D=2 ** 31 - 1)),
+    ("gdn_norm_bwd_launch", _norm, dict(D=1 << 28)),
+    ("gdn_attn_launch", _attn, dict(B=1, cu_seqlens=FAKE, N=1 << 22, Tq=1 << 22, Tk=1 << 22, Hq=4, Hk=4)),
+    ("gdn_attn_launch", _attn, dict(B=1 << 20, N=1 << 20, Tq=1, Tk=1, Hq=16, Hk=16)),
+    ("gdn_attn_launch", _attn, dict(B=1 << 20, N=1 << 20, Hq=1 << 12, Hk=1 << 12)),
+    ("gdn_attn_bwd_launch", _attn, dict(B=1, cu_seqlens=FAKE, N=1 << 21, Tq=1 << 21, Tk=1 << 21, Hq=8, Hk=8)),
+    ("gdn_attn_bwd_launch", _attn, dict(B=1 << 20, N=1 << 20, Hq=1 << 12, Hk=1 << 12)),
+    ("gdn_attn_decode_launch", _decode, dict(B=1 << 20, Hq=16, Hk=16)),
+    ("gdn_attn_decode_launch", _decode, dict(B=1, Hq=1 << 28, Hk=1, T=16)),
+])
+def test_more_workgroups_than_a_launch_holds(lib, pkg, name, make, kw):
+    """A launch counts its threads in 32 bits and runs what is left of more: such
+    calls are refused before any kernel (the norm's forward takes several launches)."""
+    P = make(pkg._lib, **dict(dict(workspace_bytes=1 << 62), **kw))
+    assert getattr(lib, name)(ctypes.byref(P), None) == 1002

@@ -804,19 +804,17 @@ int launch(const BArgs& a, hipStream_t s) {
   const int64_t vb = kScaled<T> && a.rows > 0 ? (int64_t)a.units_k * a.v_slots : 0;
   const int64_t kvb = (int64_t)a.units_k * ((int64_t)a.slots_k * a.splits + (int64_t)a.sink_blocks * a.slots_s);
   const int64_t qb = (int64_t)a.units_q * a.slots_q;
-  if (vb > 0x7fffffffLL || kvb > 0x7fffffffLL || qb > 0x7fffffffLL) return GDN_ERR_BAD_SHAPE;
+  const int64_t blocks = a.splits > 1 ? a.slots_k : (int64_t)a.sink_blocks * (a.seq.cu == nullptr ? 1 : a.longs);
+  const int64_t pb = a.sink_blocks > 0 || a.splits > 1 ? a.units_k * blocks * (kKB / 8) : 0;
+  if (!grid_fits(vb, 256) || !grid_fits(kvb, 256 * a.kv_halves) || !grid_fits(qb, 256) || !grid_fits(pb, 256))
+    return GDN_ERR_BAD_SHAPE;
   if (vb > 0) hipLaunchKernelGGL((v_max_kernel<D>), dim3((uint32_t)vb), dim3(256), 0, s, a);
   if (qb > 0) hipLaunchKernelGGL((q_kernel<T, D>), dim3((uint32_t)qb), dim3(256), 0, s, a);
   if (kvb > 0) {
     if (a.kv_halves == 1) hipLaunchKernelGGL((kv_kernel<T, D, 1>), dim3((uint32_t)kvb), dim3(256), 0, s, a);
     else hipLaunchKernelGGL((kv_kernel<T, D, 2>), dim3((uint32_t)kvb), dim3(512), 0, s, a);
   }
-  if (a.sink_blocks > 0 || a.splits > 1) {
-    const int64_t blocks = a.splits > 1 ? a.slots_k : (int64_t)a.sink_blocks * (a.seq.cu == nullptr ? 1 : a.longs);
-    const int64_t pb = a.units_k * blocks * (kKB / 8);
-    if (pb > 0x7fffffffLL) return GDN_ERR_BAD_SHAPE;
-    if (pb > 0) hipLaunchKernelGGL((part_sum_kernel<T, D>), dim3((uint32_t)pb), dim3(256), 0, s, a, (int)blocks);
-  }
+  if (pb > 0) hipLaunchKernelGGL((part_sum_kernel<T, D>), dim3((uint32_t)pb), dim3(256), 0, s, a, (int)blocks);
   return (int)hipGetLastError();
 }
 

@@ -233,6 +233,7 @@ __global__ __launch_bounds__(kJT) void join_kernel(const DArgs a) {
 int check(const GdnAttnDecodeParams& P) {
   if (P.B <= 0 || P.T < 1 || P.T > kMaxT || P.S <= 0 || P.Hq <= 0 || P.Hk <= 0 || P.Hq % P.Hk != 0) return GDN_ERR_BAD_SHAPE;
   if (P.window < 1 || P.sinks < 0 || P.S > 0x3fffffff) return GDN_ERR_BAD_SHAPE;
+  if ((int64_t)P.B * P.Hq > 0x7fffffff / (2 * kMaxT)) return GDN_ERR_BAD_SHAPE;   // rows are 32-bit
   if (P.D != 64 && P.D != 128) return GDN_ERR_UNSUPPORTED;
   if (P.dtype != GDN_DTYPE_F16 && P.dtype != GDN_DTYPE_BF16) return GDN_ERR_BAD_DTYPE;
   return GDN_OK;
@@ -287,7 +288,9 @@ int gdn_attn_decode_launch(const GdnAttnDecodeParams* prm, void* stream) {
   if (!rows16(P.q, P.q_stride, P.B, P.T, P.Hq) || !rows16(P.o, P.o_stride, P.B, P.T, P.Hq) ||
       !rows16(P.k, P.k_stride, P.B, P.S, P.Hk) || !rows16(P.v, P.v_stride, P.B, P.S, P.Hk))
     return GDN_ERR_MISALIGNED;
-  if ((int64_t)P.B * P.Hk * row_tiles(P) * kMaxSplits > 0x7fffffffLL) return GDN_ERR_BAD_SHAPE;
+  if (!grid_fits((int64_t)P.B * P.Hk * row_tiles(P) * splits_of(P), 64 * kDWaves) ||
+      (splits_of(P) > 1 && !grid_fits((int64_t)P.B * P.Hq * P.T, kJT)))
+    return GDN_ERR_BAD_SHAPE;
   const int64_t need = gdn_attn_decode_workspace_size(prm);
   if (need > 0 && (P.workspace == nullptr || P.workspace_bytes < need ||
                    reinterpret_cast<uintptr_t>(P.workspace) % 256 != 0))

@@ -211,8 +211,8 @@ int check_attn(const GdnAttnParams& P) {
   if (P.window < 1 || P.sinks < 0) return GDN_ERR_BAD_SHAPE;
   if (P.D != 64 && P.D != 128) return GDN_ERR_UNSUPPORTED;
   if (P.dtype != GDN_DTYPE_F16 && P.dtype != GDN_DTYPE_BF16) return GDN_ERR_BAD_DTYPE;
-  // positions are 32-bit
-  if ((int64_t)P.Tq + P.Tk > 0x3fffffffLL) return GDN_ERR_BAD_SHAPE;
+  // positions and (batch, head) are 32-bit
+  if ((int64_t)P.B * P.Hq > 0x7fffffffLL || (int64_t)P.Tq + P.Tk > 0x3fffffffLL) return GDN_ERR_BAD_SHAPE;
   return GDN_OK;
 }
 
@@ -297,7 +297,7 @@ int gdn_attn_launch(const GdnAttnParams* prm, void* stream) {
   } else {
     slots = P.Tq / kBM + P.N;
   }
-  if (units * slots > 0x7fffffffLL) return GDN_ERR_BAD_SHAPE;
+  if (!grid_fits(units * slots * splits_of(P), kNT)) return GDN_ERR_BAD_SHAPE;
   a.units = (int)units;
   a.slots = (int)slots;
   a.splits = splits_of(P);

@@ -44,7 +44,7 @@ struct Args {
   float* part;      // [parts, D] partial sums of dw
   float* rstd;      // [rows] (long rows' backward)
   int64_t xs[2], ress[2], ys[2], ros[2], rs[2], dys[2], dris[2], drs[2], dxs[2];
-  uint32_t rows, n_inner;
+  uint32_t rows, n_inner, row0;   // row0: first row of a launch (forward, long rows' backward)
   int D, group, parts;
   float eps;
   int w_f32;
@@ -140,7 +140,7 @@ template <typename TX, typename TR, int V, int P, int TEAM, int FP8>
 __global__ __launch_bounds__(kBlock) void fwd_kernel(const Args p) {
   constexpr int ROWS = kBlock / TEAM;
   const int t = threadIdx.x % TEAM;
-  const uint32_t row = blockIdx.x * ROWS + threadIdx.x / TEAM;
+  const uint32_t row = p.row0 + blockIdx.x * ROWS + threadIdx.x / TEAM;
   if (TEAM <= 64 && row >= p.rows) return;   // no barrier below for these
   const TX* x = static_cast<const TX*>(p.x) + row_at(p, row, p.xs);
   Pack<TX, V> xr[P];
@@ -231,7 +231,7 @@ __global__ __launch_bounds__(kBlock) void fwd_kernel(const Args p) {
 // Forward of any row: one workgroup a row, the row read again for each step.
 template <typename TX, typename TR, int FP8>
 __global__ __launch_bounds__(kBlock) void fwd_long_kernel(const Args p) {
-  const uint32_t row = blockIdx.x;
+  const uint32_t row = p.row0 + blockIdx.x;
   const int t = threadIdx.x;
   const bool has_res = p.res != nullptr;
   const TX* x = static_cast<const TX*>(p.x) + row_at(p, row, p.xs);
@@ -425,7 +425,7 @@ __global__ __launch_bounds__(kBlock) void bwd_kernel(const Args p) {
 // Backward of any row: dr (and dx), and rstd for the columns' kernel.
 template <typename TX, typename TR>
 __global__ __launch_bounds__(kBlock) void bwd_long_kernel(const Args p) {
-  const uint32_t row = blockIdx.x;
+  const uint32_t row = p.row0 + blockIdx.x;
   const int t = threadIdx.x;
   const TR* r = static_cast<const TR*>(p.r) + row_at(p, row, p.rs);
   const TX* dy = static_cast<const TX*>(p.dy) + row_at(p, row, p.dys);
@@ -529,13 +529,26 @@ Shape shape_of(int D, bool wide) {
   return {0, 0, 0};
 }
 
+// launch(args, grid) for all rows, `per` a workgroup, as many launches as they take.
+template <typename F>
+int by_rows(Args a, uint32_t per, F launch) {
+  constexpr uint32_t kMost = 1 << 23;
+  static_assert(kMost <= 0xffffffffu / kBlock, "one launch holds them (see grid_fits)");
+  for (; a.row0 < a.rows; a.row0 += kMost * per) {
+    launch(a, dim3((uint32_t)std::min<uint64_t>(kMost, ((uint64_t)a.rows - a.row0 + per - 1) / per)));
+    const int st = (int)hipGetLastError();
+    if (st != 0) return st;
+  }
+  return 0;
+}
+
 template <typename TX, typename TR, int V, int P, int TEAM>
 int fwd_shape(const Args& a, hipStream_t s) {
-  const dim3 grid((a.rows + kBlock / TEAM - 1) / (kBlock / TEAM));
-  if (a.scale == nullptr) hipLaunchKernelGGL((fwd_kernel<TX, TR, V, P, TEAM, 0>), grid, dim3(kBlock), 0, s, a);
-  else if (a.group == 0) hipLaunchKernelGGL((fwd_kernel<TX, TR, V, P, TEAM, 1>), grid, dim3(kBlock), 0, s, a);
-  else if constexpr (V == 8 && TEAM >= 16) hipLaunchKernelGGL((fwd_kernel<TX, TR, V, P, TEAM, 2>), grid, dim3(kBlock), 0, s, a);
-  return (int)hipGetLastError();
+  return by_rows(a, kBlock / TEAM, [&](const Args& b, dim3 grid) {
+    if (b.scale == nullptr) hipLaunchKernelGGL((fwd_kernel<TX, TR, V, P, TEAM, 0>), grid, dim3(kBlock), 0, s, b);
+    else if (b.group == 0) hipLaunchKernelGGL((fwd_kernel<TX, TR, V, P, TEAM, 1>), grid, dim3(kBlock), 0, s, b);
+    else if constexpr (V == 8 && TEAM >= 16) hipLaunchKernelGGL((fwd_kernel<TX, TR, V, P, TEAM, 2>), grid, dim3(kBlock), 0, s, b);
+  });
 }
 
 template <typename TX, typename TR>
@@ -560,11 +573,11 @@ int fwd_typed(const Args& a, bool wide, hipStream_t s) {
     case 32256: return fwd_shape<TX, TR, 1, 32, 256>(a, s);
     default: break;
   }
-  const dim3 grid(a.rows);
-  if (a.scale == nullptr) hipLaunchKernelGGL((fwd_long_kernel<TX, TR, 0>), grid, dim3(kBlock), 0, s, a);
-  else if (a.group == 0) hipLaunchKernelGGL((fwd_long_kernel<TX, TR, 1>), grid, dim3(kBlock), 0, s, a);
-  else hipLaunchKernelGGL((fwd_long_kernel<TX, TR, 2>), grid, dim3(kBlock), 0, s, a);
-  return (int)hipGetLastError();
+  return by_rows(a, 1, [&](const Args& b, dim3 grid) {
+    if (b.scale == nullptr) hipLaunchKernelGGL((fwd_long_kernel<TX, TR, 0>), grid, dim3(kBlock), 0, s, b);
+    else if (b.group == 0) hipLaunchKernelGGL((fwd_long_kernel<TX, TR, 1>), grid, dim3(kBlock), 0, s, b);
+    else hipLaunchKernelGGL((fwd_long_kernel<TX, TR, 2>), grid, dim3(kBlock), 0, s, b);
+  });
 }
 
 template <typename TX, typename TR, int V, int P, int TEAM>
@@ -592,7 +605,9 @@ int bwd_typed(const Args& a, bool wide, hipStream_t s) {
     case 16256: bwd_shape<TX, TR, 1, 16, 256>(a, s); break;
     case 32256: bwd_shape<TX, TR, 1, 32, 256>(a, s); break;
     default:
-      if (a.rows > 0) hipLaunchKernelGGL((bwd_long_kernel<TX, TR>), dim3(a.rows), dim3(kBlock), 0, s, a);
+      by_rows(a, 1, [&](const Args& b, dim3 grid) {
+        hipLaunchKernelGGL((bwd_long_kernel<TX, TR>), grid, dim3(kBlock), 0, s, b);
+      });
       hipLaunchKernelGGL((dw_cols_kernel<TX, TR>), dim3((a.D + kBlock - 1) / kBlock, a.parts), dim3(kBlock), 0, s, a);
   }
   hipLaunchKernelGGL((dw_sum_kernel<TX>), dim3((a.D + 63) / 64), dim3(1024), 0, s, a);
@@ -626,11 +641,20 @@ struct Bwd {
 };
 
 int check(const GdnNormParams& P) {
-  if (P.n_outer < 0 || P.n_inner < 0 || P.D <= 0 || (int64_t)P.n_outer * P.n_inner > 0x3fffffffLL) return GDN_ERR_BAD_SHAPE;
+  // (columns are counted in 32 bits, a workgroup's past the last)
+  if (P.n_outer < 0 || P.n_inner < 0 || P.D <= 0 || P.D > 0x7fffffff - 1024 ||
+      (int64_t)P.n_outer * P.n_inner > 0x3fffffffLL)
+    return GDN_ERR_BAD_SHAPE;
   if (!scan_dtype_ok(P.x_dtype) || !(P.r_dtype == P.x_dtype || P.r_dtype == GDN_DTYPE_F32) ||
       !(P.w_dtype == P.x_dtype || P.w_dtype == GDN_DTYPE_F32))
     return GDN_ERR_BAD_DTYPE;
   return GDN_OK;
+}
+
+// The gradient's too: dw's sum takes 1024 threads for 64 columns.
+int check_bwd(const GdnNormParams& P) {
+  const int st = check(P);
+  return st == GDN_OK && !grid_fits((P.D + 63) / 64, 1024) ? GDN_ERR_BAD_SHAPE : st;
 }
 
 // Whether 8 columns at a time fit these rows: 16-byte aligned (8 for e4m3).
@@ -697,7 +721,7 @@ int gdn_norm_launch(const GdnNormParams* prm, void* stream) {
 }
 
 int64_t gdn_norm_bwd_workspace_size(const GdnNormParams* prm) {
-  if (prm == nullptr || check(*prm) != GDN_OK) return -1;
+  if (prm == nullptr || check_bwd(*prm) != GDN_OK) return -1;
   const int64_t rows = (int64_t)prm->n_outer * prm->n_inner;
   // partial rows of dw, and a float a row for rows that do not fit registers
   const int parts = std::max(parts_of(rows, prm->D, true), parts_of(rows, prm->D, false));
@@ -707,7 +731,7 @@ int64_t gdn_norm_bwd_workspace_size(const GdnNormParams* prm) {
 int gdn_norm_bwd_launch(const GdnNormParams* prm, void* stream) {
   if (prm == nullptr) return GDN_ERR_NULL_POINTER;
   const GdnNormParams& P = *prm;
-  const int st = check(P);
+  const int st = check_bwd(P);
   if (st != GDN_OK) return st;
   const int64_t rows = (int64_t)P.n_outer * P.n_inner;
   if (P.dw == nullptr || P.w == nullptr || (rows > 0 && (P.r == nullptr || P.dy == nullptr || P.dr == nullptr)))

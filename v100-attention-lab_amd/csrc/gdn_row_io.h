@@ -97,6 +97,9 @@ struct Pack {
 
 // gdn_fwd_kernel.h's dtype codes on the host.
 inline bool scan_dtype_ok(int dt) { return dt == GDN_DTYPE_F32 || dt == GDN_DTYPE_F16 || dt == GDN_DTYPE_BF16; }
+// Whether one launch holds that many workgroups: its threads are counted in 32
+// bits, and a launch of more runs what is left of them without an error.
+inline bool grid_fits(int64_t blocks, int threads) { return blocks * threads <= 0xffffffffLL; }
 inline int dtype_bytes(int dt) { return dt == GDN_DTYPE_F32 ? 4 : 2; }
 
 }  // namespace gdn

@@ -644,9 +644,11 @@ template <typename TX, typename TG, int V>
 int run_fwd(Args& a, bool single, hipStream_t s) {
   a.nblk = (a.D + 64 * V - 1) / (64 * V);
   if (a.cu == nullptr && a.T <= kShort) {
+    if (!grid_fits((int64_t)a.N * a.nblk, 64)) return GDN_ERR_BAD_SHAPE;
     hipLaunchKernelGGL((short_kernel<TX, TG, V>), dim3((uint32_t)a.N * a.nblk), dim3(64), 0, s, a);
     return (int)hipGetLastError();
   }
+  if (!grid_fits((int64_t)a.slots * a.nblk, kThreads)) return GDN_ERR_BAD_SHAPE;
   if (!single) clear(a, s);
   hipLaunchKernelGGL((fwd_kernel<TX, TG, V, false>), dim3(a.slots * a.nblk), dim3(kThreads), 0, s, a, single);
   return (int)hipGetLastError();
@@ -655,6 +657,7 @@ int run_fwd(Args& a, bool single, hipStream_t s) {
 template <typename TX, typename TG, int V>
 int run_bwd(Args& a, bool single, bool have_states, hipStream_t s) {
   a.nblk = (a.D + 64 * V - 1) / (64 * V);
+  if (!grid_fits((int64_t)a.slots * a.nblk, kThreads)) return GDN_ERR_BAD_SHAPE;
   const dim3 grid(a.slots * a.nblk);
   if (!single) {
     clear(a, s);
@@ -668,7 +671,9 @@ int run_bwd(Args& a, bool single, bool have_states, hipStream_t s) {
 }
 
 int check(const GdnScanParams& P) {
-  if (P.B <= 0 || P.T < 0 || P.D <= 0 || P.N <= 0) return GDN_ERR_BAD_SHAPE;
+  // (rows and channels are counted in 32 bits, a workgroup's past the last)
+  if (P.B <= 0 || P.T < 0 || P.D <= 0 || P.N <= 0 || P.T > 0x7fffffff - 1024 || P.D > 0x7fffffff - 1024)
+    return GDN_ERR_BAD_SHAPE;
   if (P.cu_seqlens == nullptr ? P.N != P.B : P.B != 1) return GDN_ERR_BAD_SHAPE;
   if (!scan_dtype_ok(P.x_dtype) || !(P.g_dtype == P.x_dtype || P.g_dtype == GDN_DTYPE_F32)) return GDN_ERR_BAD_DTYPE;
   // one workgroup a slot and 64 channels, and one a sequence and 64 channels

@@ -259,3 +259,11 @@ def test_growing_gates_before_any_state(pkg, cuda):
     y, fs = pkg.gated_scan(x, g)
     want = oracle(x, g, None, dy, None, None)
     assert _err(y, want[0]) <= F32 and _err(fs, want[1]) <= F32
+
+
+def test_states_of_another_call_are_refused(pkg, cuda):
+    x, g, h0, dy, df = _inputs(cuda, 1, 300, 64, torch.float32, torch.float32, 1, seed=9)
+    _, _, st = pkg.gated_scan(x, g, h0, return_states=True)
+    for bad in ("states", 3, st[:-1], st.double(), st.t().contiguous().t(), st.cpu()):
+        with pytest.raises(ValueError):
+            pkg.gated_scan_bwd(x, g, h0, dy, df, states=bad)

@@ -174,6 +174,8 @@ def _bwd_plan(x, g, h0, dy, dfinal, states, n_seq, need_dh0):
         raise ValueError(f"dy must have x's shape {tuple(x.shape)} and dtype {x.dtype}")
     _check_columns(dy, "dy")
     _check_state(dfinal, "dfinal", N, D)
+    if states is not None and not isinstance(states, torch.Tensor):
+        raise ValueError("states must be the tensor that gated_scan returned")
     _check_devices(x, dy, dfinal, states)
     P = _params(x, g, h0, B, T, D, N)
     P.dy_stride[:] = dy.stride()[:2]

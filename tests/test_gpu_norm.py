@@ -276,3 +276,15 @@ def test_more_rows_than_a_launch_holds(pkg, cuda):
     words, want = y.view(torch.int64), want.view(torch.int64)       # a row is two
     for i in range(0, rows, 2 ** 26):
         assert (words[i:i + 2 ** 26] == want).all(), i
+
+
+@pytest.mark.parametrize("rows,D,group", [(700, 2048, None), (300, 4096, 128), (900, 1001, None), (50, 20000, None),
+                                          (60, 16512, 128)])
+def test_fp8_is_the_output_over_its_scale(pkg, cuda, rows, D, group):
+    """fp32 rows: the bytes are the 32-bit output divided by the scale that is
+    returned, rounded to the nearest (ties to even), bit for bit."""
+    x, res, w, _, _ = _inputs(cuda, (rows, D), torch.float32, torch.float32, torch.float32, seed=rows)
+    y, _ = pkg.add_rms_norm(x, w, res)
+    q, s, _ = pkg.add_rms_norm_fp8(x, w, res, group=group)
+    want = (y.unflatten(-1, (-1, group or D)) / s[..., None]).flatten(-2).clamp(-448, 448).cpu().to(torch.float8_e4m3fn)
+    assert torch.equal(q.cpu().view(torch.uint8), want.view(torch.uint8))

@@ -123,15 +123,22 @@ __device__ __forceinline__ void store_fp8(uint8_t* q, const float (&v)[V]) {
     *q = (uint8_t)(pack_fp8(v[0], 0.f, 0.f, 0.f) & 0xffu);
   }
 }
-// y / scale for scale = amax / 448, as y * up * inv: `up` keeps 448 / amax
-// finite for the smallest rows.  A group of zeros gives zeros, NaN gives NaN.
+// y / scale, rounded once, by the scale that is stored: the product with 1 / scale
+// (one unit off at most), corrected by its remainder.  `up` keeps 1 / scale finite
+// for the smallest scales.  A scale of 0 (a group of zeros) gives zeros, of infinity
+// zeros and inf / inf.
 struct Quant {
-  float up, inv;
-  __device__ __forceinline__ explicit Quant(float amax) {
-    up = amax < 1e-30f ? 0x1p100f : 1.f;
-    inv = amax == 0.f ? 0.f : kFp8Max / (amax * up);
+  float up, s, inv;
+  __device__ __forceinline__ explicit Quant(float scale) {
+    up = scale < 0x1p-100f ? 0x1p100f : 1.f;
+    s = scale < __builtin_inff() ? scale * up : 0.f;
+    inv = scale == 0.f ? 0.f : __builtin_amdgcn_rcpf(scale * up);
   }
-  __device__ __forceinline__ float operator()(float y) const { return y * up * inv; }
+  __device__ __forceinline__ float operator()(float y) const {
+    y *= up;
+    const float q = y * inv;
+    return __builtin_fmaf(__builtin_fmaf(-q, s, y), inv, q);
+  }
 };
 
 // Forward, the row in registers.  FP8: 0 none, 1 a scale per row, 2 per 128
@@ -205,8 +212,8 @@ __global__ __launch_bounds__(kBlock) void fwd_kernel(const Args p) {
   } else {
     uint8_t* y = static_cast<uint8_t*>(p.y) + row_at(p, row, p.ys);
     if constexpr (FP8 == 1) {
-      amax = team_reduce<TEAM, true>(amax, slots[1]);
-      if (t == 0) p.scale[row] = amax / kFp8Max;
+      amax = team_reduce<TEAM, true>(amax, slots[1]) / kFp8Max;
+      if (t == 0) p.scale[row] = amax;
     }
 #pragma unroll
     for (int i = 0; i < P; ++i) {
@@ -216,10 +223,10 @@ __global__ __launch_bounds__(kBlock) void fwd_kernel(const Args p) {
         m = 0.f;
 #pragma unroll
         for (int e = 0; e < V; ++e) m = nan_max(m, fabsf(r[i][e]));
-        m = lanes_max<16>(m);
-        if (c < p.D && (c & 127) == 0) p.scale[(int64_t)row * (p.D / 128) + c / 128] = m / kFp8Max;
+        m = lanes_max<16>(m) / kFp8Max;
+        if (c < p.D && (c & 127) == 0) p.scale[(int64_t)row * (p.D / 128) + c / 128] = m;
       }
-      const Quant quant(m);
+      const Quant quant(m);      // (amax, m: the scale by now)
       float q[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) q[e] = quant(r[i][e]);
@@ -264,9 +271,9 @@ __global__ __launch_bounds__(kBlock) void fwd_long_kernel(const Args p) {
         const float v = value(c) * rstd * weight(c);
         amax = nan_max(amax, fabsf(v));
       }
-      amax = team_reduce<kBlock, true>(amax, slots[1]);
-      if (t == 0) p.scale[row] = amax / kFp8Max;
-      const Quant quant(amax);
+      const float scale = team_reduce<kBlock, true>(amax, slots[1]) / kFp8Max;
+      if (t == 0) p.scale[row] = scale;
+      const Quant quant(scale);
       for (int c = t; c < p.D; c += kBlock) {
         const float v = value(c);
         if (has_res) ro[c] = from_f32<TR>(v);
@@ -286,8 +293,8 @@ __global__ __launch_bounds__(kBlock) void fwd_long_kernel(const Args p) {
           v[e] = v[e] * rstd * weight(c);
           m = nan_max(m, fabsf(v[e]));
         }
-        m = lanes_max<64>(m);
-        if (lane == 0) p.scale[(int64_t)row * (p.D / 128) + g] = m / kFp8Max;
+        m = lanes_max<64>(m) / kFp8Max;
+        if (lane == 0) p.scale[(int64_t)row * (p.D / 128) + g] = m;
         const Quant quant(m);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {

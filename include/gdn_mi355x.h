@@ -344,7 +344,10 @@ int gdn_bwd_launch(const GdnBwdParams* params, void* stream);
  * h in fp32.  Dense [B,T,D] (cu_seqlens NULL), or N sequences packed along t
  * of batch 0 with offsets cu_seqlens as in GdnFwdParams (device memory, not
  * read on the host, clamped to [0, T] by the kernels; rows that no sequence
- * holds are not written).
+ * holds are not written).  States of 0 and of infinity stay what they are under
+ * finite gates; a gate of -inf makes an infinite one NaN.  GDN_ERR_BAD_SHAPE from
+ * 2^32 threads a launch on: 512 for each chunk of gdn_scan_chunk() rows and 64 or
+ * 128 channels (forward of up to 8 rows: 64).
  *   - x, y (and dy, dx): x_dtype; g (and dg): g_dtype, x_dtype or fp32.  The
  *     channel dimension is contiguous, (b, t) strides in elements are any;
  *     with an even D, 4-byte aligned pointers (8-byte for fp32) and even
@@ -399,11 +402,12 @@ int gdn_scan_bwd_launch(const GdnScanParams* params, void* stream);
  * gradient at the stored r:
  *     dr = dr_in + rstd (w dy - n mean(w dy n)),  dw = sum_rows dy n,
  *     n = r rstd.
- * Rows are (n_outer, n_inner) with a stride for each; the columns are
- * contiguous.
+ * Rows are (n_outer, n_inner) with a stride for each, 2^30 - 1 at most; the
+ * columns are contiguous, below 2^28 of them in the backward.
  *   - res nullable: r = x, r_out is not written and r_dtype is x_dtype.
- *   - y: x_dtype, or e4m3 bytes when `scale` is set: y / scale rounded to the
- *     nearest, scale = max|y| / 448 over the row (group 0) or over each 128
+ *   - y: x_dtype, or e4m3 bytes when `scale` is set: y / scale (in fp32, by the
+ *     scale that is stored) rounded to the nearest, scale = max|y| / 448 over the
+ *     row (group 0) or over each 128
  *     columns (group 128, D a multiple of it); scale is dense
  *     [rows, D / group] (or [rows, 1]); a group of zeros has scale 0.
  *   - backward: r, dy (x_dtype), dr_in (nullable, r_dtype); dr (r_dtype), dx
@@ -452,7 +456,11 @@ int gdn_norm_bwd_launch(const GdnNormParams* params, void* stream);
  * share Hk key heads (Hq a multiple of Hk), head h reads key head h / (Hq/Hk).
  *     P = softmax(scale q k^T) over the visible keys, o = P v,
  *     lse = log sum e^{scale q k^T}
- * A row that sees no key has o = 0, lse = -inf and no gradients.
+ * A row that sees no key has o = 0, lse = -inf and no gradients; a NaN score makes
+ * its row NaN in o and lse.  P, and dS in the backward, are rounded to dtype before
+ * their products; fp16 keeps dS in a unit from the largest |dO| and the largest |v|
+ * of the sequence's head.  GDN_ERR_BAD_SHAPE from 2^32 threads a launch on: 256 for
+ * each 128 query rows of a sequence and head, 256 or 512 for each 128 key rows.
  *   - q, o, dO, dq [B,Tq,Hq,D], k, v, dk, dv [B,Tk,Hk,D]: one 16-bit dtype;
  *     D in {64, 128}, contiguous; pointers and (b, t, h) strides give
  *     16-byte aligned rows.  lse [B,Tq,Hq] fp32, dense.

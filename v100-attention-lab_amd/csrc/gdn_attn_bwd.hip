@@ -22,11 +22,14 @@
 // by 32 rows at head size 128 are 32 products (1024 cycles of a SIMD) and 40 KB
 // of LDS reads (320 cycles of the CU's 128 bytes a cycle, for each of 8 waves),
 // and the accumulators of dk and dv with the keys take all registers of two
-// waves a SIMD.  B2 Hq16 Hk4 T4096 D128 window 1024 bf16: kv 186 us (645
-// TFLOP/s of visible pairs), q 127 us (710), parts 5 us.  At head size 64 the
-// VALU is the bound (8192 packed rows of 16 heads, window 512, fp16: kv 86 us,
-// q 57, parts 8, the largest |v| 5).  One kernel for dq, dk and dv would save
-// two of seven products, but its dq needs atomics, whose order changes results.
+// waves a SIMD.  B2 Hq16 Hk4 T4096 D128 window 1024 bf16: kv 183 us (656
+// TFLOP/s of visible pairs), q 126 us (716), parts 6 us; a matrix instruction runs
+// in 30 and 34 % of the SIMD-cycles.  At head size 64 a tile's chain of reads,
+// products and exponentials is short and its steps wait for one another (8192
+// packed rows of 16 heads, window 512, fp16: kv 86 us, q 57, parts 9, the largest
+// |v| 6; matrix instructions 15 to 18 %, all vector instructions 29 to 33 %, waves
+// waiting 36 to 46 % of their time).  One kernel for dq, dk and dv would save two of
+// seven products, but its dq needs atomics, whose order changes results.
 
 #include <algorithm>
 

@@ -9,8 +9,8 @@
 //
 // Bound by reading the cache rows once (32 sequences, 4 key heads of 128, 4100
 // visible keys, bf16: 51 us with the call, 5.3 TB/s), and for few sequences by the
-// chain of one workgroup and the join (one sequence of the same: 8 us and 4 us
-// for 8.4 MB).
+// chain of one workgroup and the join (one sequence of the same: 6 to 8 us and
+// 4 us for 8.4 MB).
 
 #include <algorithm>
 

@@ -14,8 +14,9 @@
 // chunk's pair in the workspace, takes the pairs of the chunks before it (in
 // the backward, after it) and walks its rows from the state that they give: x,
 // g and y pass through memory once.  Every 16th workgroup also leaves the pair
-// of its 16 chunks, so that a chunk reads at most 30 pairs and one for each 16
-// chunks between.  All sums have a fixed order.
+// of its 16 chunks, so that a chunk reads at most 46 pairs (15 before the first
+// set, 31 behind the last) and one for each 16 chunks between.  All sums have a
+// fixed order.
 //
 // Waiting: a channel block's chunks are dealt by its counter in the order of
 // the walk, so whatever a workgroup waits for is left by workgroups that already
@@ -27,10 +28,10 @@
 //
 // Bound by memory, and by the walk's phases (rows in, pairs out and back, rows
 // out), which the workgroups of a CU pass through side by side.  B4 T4096 D2048,
-// bf16 with fp32 gates: forward 84 us (268 MB, 3.2 TB/s), backward from the
-// forward's states 104 us (470 MB, 4.5 TB/s), a large copy 4.9 TB/s.  Chunks of
-// 128 rows by 8 waves: forward and backward 188 us; by 4 waves 224 (more pairs),
-// 256 rows by 16 waves 215 (one workgroup a CU).
+// bf16 with fp32 gates: forward 80 us (268 MB, 3.4 TB/s), backward from the
+// forward's states 107 us (470 MB, 4.4 TB/s), a large copy 4.9 TB/s.  Chunks of
+// 128 rows by 8 waves; of 64 by 4 waves (more pairs) forward and backward took 19 %
+// more, of 256 by 16 waves (one workgroup a CU) 14 %.
 
 #include <algorithm>
 
@@ -365,8 +366,8 @@ __device__ __forceinline__ void carry(const Args& p, Join<V>& sh, uint32_t first
 // ---------------------------------------------------------------------------
 
 // 16-bit gates: e^g is formed again in the second walk instead of held, which
-// leaves room for 6 waves a SIMD (B4 T4096 D2048 bf16: 67.3 us; held, 4 waves,
-// 73.5).  32-bit gates hold it: 6 waves would spill (90 us; 4 waves 75.5).
+// leaves room for 6 waves a SIMD (B4 T4096 D2048 bf16: 69 us, held with 4 waves 9 %
+// more).  32-bit gates hold it: 6 waves would spill (19 % more than the 80 us).
 template <typename TX, typename TG>
 constexpr bool kMore = sizeof(TX) == 2 && sizeof(TG) == 2;
 

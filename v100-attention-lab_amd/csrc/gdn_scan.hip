@@ -171,7 +171,7 @@ __device__ __forceinline__ void chain(float (&h)[V], Walk walk) {
   walk(Plain{}, h);
 #pragma unroll
   for (int e = 0; e < V; ++e) odd |= h[e] != h[e];
-  if (__any(odd)) {
+  if (__builtin_expect(__any(odd), 0)) {
 #pragma unroll
     for (int e = 0; e < V; ++e) h[e] = first[e];
     walk(Careful{}, h);
@@ -337,7 +337,7 @@ __device__ __forceinline__ void carry(const Args& p, Join<V>& sh, uint32_t first
     // the loop above made the fp32 backward of 50001 rows of 640 143 us, not 135)
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      if (H[e] != H[e]) {
+      if (__builtin_expect(H[e] != H[e], 0)) {
         H[e] = 0.f;
 #pragma unroll 1
         for (int k = k0; k < k1; ++k) {

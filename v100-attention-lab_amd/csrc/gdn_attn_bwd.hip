@@ -43,7 +43,7 @@ constexpr int kSegRows = 64;   // rows of segments come in multiples of it
 constexpr int kQB = 128;       // query rows a workgroup (q)
 constexpr int kKT = 64;        // keys a tile (q)
 constexpr int kFewTiles = 4;   // up to so many key tiles a block of rows sums D itself (q)
-constexpr int kVParts = 64;    // partial maxima of |v| a head of a sequence, at most
+constexpr int kVParts = 128;   // partial maxima of |v| a head of a sequence, at most (two a lane)
 
 struct BArgs {
   const uint16_t* q;
@@ -65,7 +65,7 @@ struct BArgs {
   int Hq, Hk, G;
   int units_q, units_k;         // (batch and) heads of the q and kv grids
   int slots_q, slots_k;         // blocks of each
-  int v_rows, v_slots;          // rows of a partial maximum of |v|, slots of a unit's
+  int v_shift, v_slots;         // rows of a partial maximum of |v| (2^v_shift), slots of a unit's
   int kv_halves;                // waves of a workgroup / 4 (kv)
   int splits;                   // workgroups a key block
   int sink_blocks, seg, slots_s;  // blocks of the first keys, rows a segment, segment slots
@@ -108,21 +108,21 @@ __device__ __forceinline__ float finite_abs(float x) {
   return y < __builtin_inff() ? y : 0.f;
 }
 
-// v_rows keys of one head of a sequence: the largest |v|.
+// 2^v_shift keys of one head of a sequence: the largest |v|.
 template <int D>
 __global__ __launch_bounds__(256) void v_max_kernel(const BArgs a) {
   constexpr int L = D / 8, RPB = 256 / L;      // lanes a row, rows a workgroup
   const int slot = blockIdx.x % a.v_slots, unit = blockIdx.x / a.v_slots;
   int hk = unit, part;
-  const int si = find_block(a.seq, slot, a.v_rows, a.v_slots, part);
+  const int si = find_block(a.seq, slot, 1 << a.v_shift, a.v_slots, part);
   Seq sq = get_seq(a.seq, si);
   if (a.seq.cu == nullptr) {
     sq.b = unit / a.Hk;
     hk = unit % a.Hk;
   }
   if (part < 0) return;
-  const int64_t t0 = (int64_t)part * a.v_rows;
-  const int t1 = (int)min(t0 + a.v_rows, (int64_t)sq.nk);
+  const int64_t t0 = (int64_t)part << a.v_shift;
+  const int t1 = (int)min(t0 + (1 << a.v_shift), (int64_t)sq.nk);
   float m = 0.f;
   for (int64_t t = t0 + threadIdx.x / L; t < t1; t += RPB) {
     rowio::Pack<f16, 8> pv;
@@ -140,10 +140,12 @@ __global__ __launch_bounds__(256) void v_max_kernel(const BArgs a) {
 
 // The largest |v| of a head of a sequence, as a power of 2.
 __device__ __forceinline__ float v_unit(const BArgs& a, const Seq& sq, int si, int hk, int lane) {
-  const int n = ((uint32_t)sq.nk + (uint32_t)a.v_rows - 1) / (uint32_t)a.v_rows;    // kVParts at most
+  const int n = (int)((uint32_t)(sq.nk + (1 << a.v_shift) - 1) >> a.v_shift);    // kVParts at most
   const int64_t first = a.seq.cu == nullptr ? ((int64_t)sq.b * a.Hk + hk) * a.v_slots
-                                            : (int64_t)hk * a.v_slots + (uint32_t)sq.k0 / (uint32_t)a.v_rows + si;
-  float m = lane < n ? a.vmax[first + lane] : 0.f;
+                                            : (int64_t)hk * a.v_slots + (sq.k0 >> a.v_shift) + si;
+  float m = 0.f;
+  if (lane < n) m = a.vmax[first + lane];
+  if (lane + 64 < n) m = fmaxf(m, a.vmax[first + lane + 64]);
 #pragma unroll
   for (int s = 32; s >= 1; s >>= 1) m = fmaxf(m, __shfl_xor(m, s, 64));
   return pow2_above(m);
@@ -780,9 +782,16 @@ int key_splits(const GdnAttnParams& P) {
   return (int)std::max<int64_t>(1, std::min<int64_t>(256 / blocks, tiles / 4));
 }
 
-// Partial maxima of |v|: rows of each (64 cover every sequence), slots a unit.
-int v_rows(const GdnAttnParams& P) { return std::max(1, (P.Tk + kVParts - 1) / kVParts); }
-int64_t v_slots(const GdnAttnParams& P) { return P.cu_seqlens == nullptr ? kVParts : P.Tk / v_rows(P) + P.N; }
+// Partial maxima of |v|: rows of each (kVParts cover every sequence), slots a unit.
+int v_shift(const GdnAttnParams& P) {
+  int shift = 5;
+  while (((int64_t)kVParts << shift) < P.Tk) ++shift;
+  return shift;
+}
+int64_t v_slots(const GdnAttnParams& P) {
+  const int shift = v_shift(P);
+  return P.cu_seqlens == nullptr ? ((int64_t)P.Tk + (1 << shift) - 1) >> shift : (P.Tk >> shift) + (int64_t)P.N;
+}
 
 struct Space {
   int64_t stat, rmax, vmax, part, total;
@@ -893,7 +902,7 @@ int gdn_attn_bwd_launch(const GdnAttnParams* prm, void* stream) {
   // 602 and 581; 1040 blocks of D 64: 219 and 170)
   a.kv_halves = (int64_t)a.units_k * a.slots_k >= 512 ? 1 : 2;
   sink_plan(P, a.sink_blocks, a.seg, a.slots_s);
-  a.v_rows = v_rows(P);
+  a.v_shift = v_shift(P);
   a.v_slots = (int)v_slots(P);
   a.longs = long_seqs(P);
   a.long_rows = (int)std::min<int64_t>(long_rows(P), 0x7fffffff);

@@ -347,7 +347,7 @@ def _once(pkg, monkeypatch, name):
                        lambda *a: (torch.ones_like(x), torch.ones_like(x), None)),
         "window_attn": ((q, q, q), lambda *a: (torch.ones_like(q), torch.ones(1, 4, 2)),
                         lambda *a: (torch.ones_like(q),) * 3),
-        "add_rms_norm": ((x, torch.ones(8)), lambda *a: (torch.ones_like(x), None, x),
+        "add_rms_norm": ((x, torch.ones(8)), lambda *a: (torch.ones_like(x), None, a[0]),      # (r is x)
                          lambda *a: (torch.ones_like(x), None, torch.ones(8))),
     }
     inputs, fwd, bwd = case[name]
@@ -454,3 +454,18 @@ def test_more_workgroups_than_a_launch_holds(lib, pkg, name, make, kw):
     calls are refused before any kernel (the norm's forward takes several launches)."""
     P = make(pkg._lib, **dict(dict(workspace_bytes=1 << 62), **kw))
     assert getattr(lib, name)(ctypes.byref(P), None) == 1002
+
+
+@pytest.mark.parametrize("name", ["gdn_fwd", "gated_scan", "window_attn", "add_rms_norm"])
+def test_second_derivatives_are_refused_beside_others(pkg, monkeypatch, name):
+    """The same where the engine is asked for some inputs alone, which other paths
+    of the graph reach as well, and for the gradient that came in."""
+    call, inputs = _once(pkg, monkeypatch, name)
+    out = call(*inputs)
+    out = out[0] if isinstance(out, tuple) else out
+    weight = torch.ones_like(out, requires_grad=True)
+    for want in (inputs[0], weight):
+        loss = (out * weight).sum() + inputs[0].pow(3).sum()
+        grad, = torch.autograd.grad(loss, inputs[0], create_graph=True)
+        with pytest.raises(RuntimeError, match="second derivatives"):
+            torch.autograd.grad(grad.square().sum(), want, allow_unused=True)

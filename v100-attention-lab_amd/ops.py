@@ -679,11 +679,11 @@ def _run_bwd(q, k, v, g, beta, h0, do, dfinal, scale, cu, n_seq, need_dh0, max_s
 
 
 class _NoSecond(torch.autograd.Function):
-    """Passes gradients on; theirs raises."""
+    """Makes gradients (a list) functions of tensors; their own gradient raises."""
 
     @staticmethod
-    def forward(ctx, anchor, *grads):
-        return tuple(t.view_as(t) for t in grads)
+    def forward(ctx, grads, *of):
+        return tuple(grads)
 
     @staticmethod
     def backward(ctx, *_):
@@ -693,8 +693,9 @@ class _NoSecond(torch.autograd.Function):
 
 def _first_order(backward):
     """Decorator of an autograd backward that runs kernels: its results carry no
-    graph, so under create_graph (the only backward with grad mode on) their own
-    gradient raises where it would be taken for zero."""
+    graph, so under create_graph (the only backward with grad mode on) they are
+    made functions of what they depend on, and their own gradient raises where it
+    would be taken for zero."""
     @functools.wraps(backward)
     def run(ctx, *grads):
         create_graph = torch.is_grad_enabled()
@@ -702,10 +703,10 @@ def _first_order(backward):
             out = backward(ctx, *grads)
         if not create_graph:
             return out
+        of = [t for t in (*grads, *ctx.saved_tensors) if t is not None and t.requires_grad]
         at = [i for i, t in enumerate(out) if t is not None]
-        kept = _NoSecond.apply(torch.zeros((), requires_grad=True), *(out[i] for i in at))
         out = list(out)
-        for i, t in zip(at, kept):
+        for i, t in zip(at, _NoSecond.apply([out[i] for i in at], *of)):
             out[i] = t
         return tuple(out)
     return run

@@ -628,3 +628,34 @@ def test_scale_changed_in_place(pkg, cuda):
     scale.fill_(0.1)
     o.backward(do)
     assert torch.equal(a.grad, got[0])
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 3), (60, 0), (60, 4), (60, 130), (128, 1), (200, 33), (300, 140)])
+def test_every_visible_pair_counts_once(pkg, cuda, window, sinks):
+    """Scores of 0 give a row of n visible keys P = 1 / n each: with dO = n, dv of a
+    key is the number of rows that see it.  Every length about the places where
+    blocks, windows and segments end; fewer rows than keys; packed.  (P is within
+    2^-11 of itself and n exact, so counts, of 560 at most, are within 0.28, and dv's
+    rounding to 11 bits adds at most 0.25.)"""
+    def check(T, S, lens=None):
+        q = torch.zeros(1, T, 1, 64, dtype=torch.float16, device=cuda)
+        k = torch.zeros(1, S, 1, 64, dtype=torch.float16, device=cuda)
+        spans = [(0, T, 0, S)] if lens is None else \
+            [(s, s + n, s, s + n) for s, n in zip(itertools.accumulate([0] + lens[:-1]), lens)]
+        cu = None if lens is None else torch.tensor([0] + list(itertools.accumulate(lens)), device=cuda)
+        want = torch.zeros(S, device=cuda)
+        do = torch.zeros_like(q)
+        for a, b, c, d in spans:
+            m = visible(b - a, d - c, window, sinks, cuda)
+            do[0, a:b] = m.sum(1)[:, None, None].to(do.dtype)
+            want[c:d] = m.sum(0)
+        o, lse = pkg.window_attn(q, k, k, window, sinks, cu_seqlens=cu, return_lse=True)
+        dv = pkg.window_attn_bwd(q, k, k, o, lse, do, window, sinks, cu_seqlens=cu)[2]
+        assert ((dv[0, :, 0].float() - want[:, None]).abs() <= 0.65).all(), (T, S, lens)
+
+    for S in sorted({n for e in (window, window + 128, window + 256) for n in range(max(1, e - 2), e + 3)}):
+        check(S, S)
+        check(min(S, 70), S)
+        check(S, S, [S])
+        check(2 * S + 9, 2 * S + 9, [0, S, 7, 0, S, 2])
+        check(S + 60, S + 60, [1] * 60 + [S])

@@ -528,6 +528,42 @@ typedef struct GdnAttnDecodeParams {
 int64_t gdn_attn_decode_workspace_size(const GdnAttnDecodeParams* params);
 int gdn_attn_decode_launch(const GdnAttnDecodeParams* params, void* stream);
 
+/* Softmax cross entropy of a linear head, N rows of D against V weights, the
+ * logits l = x w^T (in fp32) made in pieces of the vocabulary and never kept:
+ *     lse_n = log sum_v e^{l_nv},   loss_n = lse_n - l_{n, target_n}
+ *     G = dloss_n (e^{l - lse} - [v = target_n]),  dx = G w,  dw = G^T x
+ * A row whose target is outside [0, V) does not count: loss and lse 0, dx 0,
+ * nothing in dw, whatever the row holds.  G is rounded once to dtype (fp16: in a
+ * unit from the largest |dloss|); sums are fp32, in a fixed order.
+ *   - x [N,D], w [V,D]: fp16 or bf16, rows contiguous and 16-byte aligned, D a
+ *     multiple of 8 (at least 8); strides at most 2^22 elements.  target: int64.
+ *   - lse: written by the forward, read by the backward; dloss: fp32 with a
+ *     stride (0: one value for all rows); dx, dw: dense, dtype.
+ *   - N, V up to 2^28; workspaces of gdn_xent[_bwd]_workspace_size() bytes,
+ *     256-byte aligned. */
+typedef struct GdnXentParams {
+  const void* x;
+  const void* w;
+  const int64_t* target;
+  float* loss;              /* forward only */
+  float* lse;
+  const float* dloss;       /* backward only, like dx and dw */
+  void* dx;
+  void* dw;
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t x_stride;         /* rows, in elements */
+  int64_t w_stride;
+  int64_t dloss_stride;
+  int32_t N, D, V;
+  int32_t dtype;
+} GdnXentParams;
+
+int64_t gdn_xent_workspace_size(const GdnXentParams* params);
+int gdn_xent_launch(const GdnXentParams* params, void* stream);
+int64_t gdn_xent_bwd_workspace_size(const GdnXentParams* params);
+int gdn_xent_bwd_launch(const GdnXentParams* params, void* stream);
+
 /* Human-readable text for a status code. */
 const char* gdn_fwd_status_string(int status);
 

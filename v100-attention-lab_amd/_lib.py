@@ -59,6 +59,10 @@ EXPORTED_SYMBOLS = (
     "gdn_attn_bwd_launch",
     "gdn_attn_decode_workspace_size",
     "gdn_attn_decode_launch",
+    "gdn_xent_workspace_size",
+    "gdn_xent_launch",
+    "gdn_xent_bwd_workspace_size",
+    "gdn_xent_bwd_launch",
 )
 
 _I64x2 = ctypes.c_int64 * 2
@@ -206,6 +210,15 @@ class GdnAttnDecodeParams(ctypes.Structure):
         ("dtype", ctypes.c_int32))
 
 
+class GdnXentParams(ctypes.Structure):
+    """Mirror of ``GdnXentParams`` in include/gdn_mi355x.h."""
+
+    _fields_ = _fields(
+        ("x w target loss lse dloss dx dw workspace", ctypes.c_void_p),
+        ("workspace_bytes x_stride w_stride dloss_stride", ctypes.c_int64),
+        ("N D V dtype", ctypes.c_int32))
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -249,7 +262,8 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
         lib.gdn_bwd_segment_workspace_size.restype = ctypes.c_int64
         for name, struct in (("scan", GdnScanParams), ("scan_bwd", GdnScanParams), ("norm", GdnNormParams),
                              ("norm_bwd", GdnNormParams), ("attn", GdnAttnParams), ("attn_bwd", GdnAttnParams),
-                             ("attn_decode", GdnAttnDecodeParams)):
+                             ("attn_decode", GdnAttnDecodeParams), ("xent", GdnXentParams),
+                             ("xent_bwd", GdnXentParams)):
             if f"gdn_{name}_workspace_size" in EXPORTED_SYMBOLS:
                 size = getattr(lib, f"gdn_{name}_workspace_size")
                 size.argtypes, size.restype = [ctypes.POINTER(struct)], ctypes.c_int64

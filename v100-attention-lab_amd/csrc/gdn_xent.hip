@@ -1,0 +1,589 @@
+// Softmax cross entropy of a linear head, logits made in pieces and never kept:
+//     l = X W^T,  lse_n = log sum_v e^{l_nv},  loss_n = lse_n - l_{n, t_n}
+//     G = dloss_n (e^{l - lse} - [v = t_n]),  dX = G W,  dW = G^T X
+//
+// Forward: tiles of logits (vocabulary x rows) on matrix instructions; each
+// leaves the maximum and the sum of exponentials of its vocabulary for its rows,
+// and a second kernel joins them in order.
+// Backward: piece by piece of the vocabulary the logits are made again by the
+// same loop (so that e^{l - lse} fits its lse), G of the piece is rounded once to
+// the operands' type into the workspace, dW of the piece is one product over all
+// rows and dX a sum over the pieces, kept in fp32 in the order of the
+// accumulators.  Where dX has few tiles the piece's vocabulary is cut into parts
+// that have sums of their own, joined in order at the end.
+//
+// fp16 keeps G in a unit: the power of 2 that brings the largest |dloss| to 2^13,
+// so that probabilities of a large vocabulary over many rows stay normal numbers;
+// bf16 has the range without.
+#include <algorithm>
+
+#include "gdn_gemm.h"
+
+namespace gdn {
+namespace xent {
+
+using namespace gemm;
+using attn::exp2_fast;
+using attn::kLn2;
+using attn::kLog2e;
+using attn::max_halves;
+using attn::Ops;
+using attn::swap_halves;
+
+typedef Shape<4, 2, 2, 4> Big;      // 256 x 256, one workgroup a CU
+typedef Shape<2, 2, 2, 2> Mid;      // 128 x 128, two
+typedef Shape<2, 1, 2, 2> Narrow;   // 128 x 64 (vocabulary x rows)
+
+struct Row {
+  float lse2, g;      // lse log2 e; dloss in the unit of G, 0 for rows that do not count
+};
+
+struct Args {
+  const void* x;
+  const void* w;
+  const int64_t* target;
+  float* loss;
+  float* lse;              // written by the forward, read by the backward
+  const float* dloss;
+  void* dx;
+  void* dw;
+  int64_t xld, wld;        // bytes between rows
+  int64_t dloss_step;
+  int N, D, V;
+  // workspace
+  float2* part;            // forward: (maximum, sum) [tiles of V][N]
+  float* hit;              // the target's logit [N]
+  Row* rows;               // backward: [N up to 256]
+  int32_t* tgt;            // the row's target, -1 without
+  uint64_t* live;          // a bit for each row that counts
+  float* unit;             // 1 / unit of G
+  uint16_t* g;             // [N up to 256][ldg]
+  float4* dxp;             // sums of dX, in the order of the accumulators
+  int ldg;
+  int v0, vn;              // the piece: first of V, how many
+  int tm, tn, splits, first, last;
+};
+
+// ---------------------------------------------------------------------------
+// logits
+// ---------------------------------------------------------------------------
+
+// Tile of logits: M the vocabulary, N the rows.
+template <typename T, typename S>
+__device__ __forceinline__ void logits(const Args& a, f32x16 (&acc)[S::MT][S::NT], const TileAt& t, uint32_t lds, int wm,
+                                       int wn) {
+  const int lane = threadIdx.x & 63;
+  const PlainCopy<S::BM, S::kWaves> ca((const uint8_t*)a.w + (int64_t)a.v0 * a.wld, a.wld, t.m * S::BM, a.vn, 2 * a.D);
+  const PlainCopy<S::BN, S::kWaves> cb(a.x, a.xld, t.n * S::BN, a.N, 2 * a.D);
+  const PlainRead ra(lane, 32 * S::MT * wm), rb(lane, 32 * S::NT * wn);
+  product16<T, S>(acc, (a.D + 63) / 64, lds, ra, rb, [&](int k, uint32_t at) {
+    ca.copy(k, at);
+    cb.copy(k, at + S::kA);
+  });
+}
+
+template <typename T, typename S>
+__global__ __launch_bounds__(S::kThreads) void fwd_kernel(const Args a) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[S::kLds];
+  const TileAt t(blockIdx.x, a.tm, a.tn);
+  const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wv % S::WM, wn = wv / S::WM;
+  f32x16 acc[S::MT][S::NT] = {};
+  logits<T, S>(a, acc, t, lds_addr(lds), wm, wn);
+
+  const int v0 = t.m * S::BM + 32 * S::MT * wm, left = a.V - v0;     // of the wave's vocabulary
+  float* sm = reinterpret_cast<float*>(lds);                        // [WM][BN]
+  float* ss = sm + S::WM * S::BN;
+#pragma unroll
+  for (int j = 0; j < S::NT; ++j) {
+    const int c = 32 * (S::NT * wn + j) + l32, n = t.n * S::BN + c;
+    const int64_t hit = n < a.N ? a.target[n] - v0 : -1;
+    const bool here = hit >= 0 && hit < min(32 * S::MT, left);
+    if (__any(here)) {
+#pragma unroll
+      for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (here && hit == 32 * i + attn::acc_row(r, half)) a.hit[n] = acc[i][j][r];
+    }
+    if (left < 32 * S::MT) {
+#pragma unroll
+      for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          acc[i][j][r] = 32 * i + attn::acc_row(r, half) < left ? acc[i][j][r] : -__builtin_inff();
+    }
+    float m = acc[0][j][0];
+#pragma unroll
+    for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) m = fmaxf(m, acc[i][j][r]);
+    m = max_halves(m) * kLog2e;
+    const float mb = m == -__builtin_inff() ? 0.f : -m;
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s += exp2_fast(__builtin_fmaf(acc[i][j][r], kLog2e, mb));
+    s += swap_halves(s);
+    if (half == 0) {
+      sm[wm * S::BN + c] = m;
+      ss[wm * S::BN + c] = s;
+    }
+  }
+  __syncthreads();
+  const int c = threadIdx.x, n = t.n * S::BN + c;
+  if (c >= S::BN || n >= a.N) return;
+  float m = sm[c], s = 0.f;
+#pragma unroll
+  for (int w = 1; w < S::WM; ++w) m = fmaxf(m, sm[w * S::BN + c]);
+#pragma unroll
+  for (int w = 0; w < S::WM; ++w) {
+    const float x = sm[w * S::BN + c];
+    s += ss[w * S::BN + c] * (x == m ? 1.f : exp2_fast(x - m));
+  }
+  a.part[(int64_t)t.m * a.N + n] = make_float2(m, s);
+}
+
+// lse and loss: 16 rows a workgroup, 16 threads a row.
+constexpr int kJoin = 256;
+__global__ __launch_bounds__(kJoin) void join_kernel(const Args a) {
+  const int c = threadIdx.x & 15, g = threadIdx.x >> 4;
+  const int n = blockIdx.x * 16 + c;
+  float m = -__builtin_inff(), s = 0.f;
+  auto add = [&](float2 p) {
+    // a part's sum is 0 only where all its logits are -inf
+    const float top = fmaxf(m, p.x);
+    if (top == -__builtin_inff()) {
+      s += p.y;      // (0, or NaN)
+      return;
+    }
+    s = s * (m == top ? 1.f : exp2_fast(m - top)) + p.y * (p.x == top ? 1.f : exp2_fast(p.x - top));
+    m = top;
+  };
+  if (n < a.N) {
+#pragma unroll 4
+    for (int t = g; t < a.tm; t += 16) add(a.part[(int64_t)t * a.N + n]);
+  }
+  __shared__ float2 all[16][16];
+  all[g][c] = make_float2(m, s);
+  __syncthreads();
+  if (g != 0 || n >= a.N) return;
+#pragma unroll
+  for (int k = 1; k < 16; ++k) add(all[k][c]);
+  const int64_t t = a.target[n];
+  const bool counts = t >= 0 && t < a.V;
+  const float lse = (m + __builtin_amdgcn_logf(s)) * kLn2;
+  a.lse[n] = counts ? lse : 0.f;
+  if (counts) a.loss[n] = lse - a.hit[n];
+  else a.loss[n] = 0.f;
+}
+
+// ---------------------------------------------------------------------------
+// backward
+// ---------------------------------------------------------------------------
+
+__device__ __forceinline__ bool row_counts(const Args& a, int n) {
+  const int64_t t = n < a.N ? a.target[n] : -1;
+  return t >= 0 && t < a.V;
+}
+
+// What the pieces need of each row, and the unit of G (every workgroup finds it
+// for itself).
+template <bool UNIT>
+__global__ __launch_bounds__(kJoin) void rows_kernel(const Args a) {
+  float unit = 1.f;
+  if constexpr (UNIT) {
+    float top = 0.f;
+    for (int n = threadIdx.x; n < a.N; n += kJoin)
+      if (row_counts(a, n)) top = fmaxf(top, fabsf(a.dloss[n * a.dloss_step]));
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    __shared__ float tops[kJoin / 64];
+    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kJoin / 64; ++w) top = fmaxf(top, tops[w]);
+    if (top > 0.f && top < __builtin_inff()) unit = ldexpf(1.f, max(-100, min(100, 13 - ilogbf(top))));
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.unit = 1.f / unit;
+  const int all = (a.N + 255) / 256 * 256;
+  for (int n = blockIdx.x * kJoin + threadIdx.x; n < all; n += gridDim.x * kJoin) {
+    const bool c = row_counts(a, n);
+    Row r = {0.f, 0.f};
+    if (c) r = Row{a.lse[n] * kLog2e, a.dloss[n * a.dloss_step] * unit};
+    a.rows[n] = r;
+    a.tgt[n] = c ? (int32_t)a.target[n] : -1;
+    const uint64_t m = __ballot(c);
+    if ((threadIdx.x & 63) == 0) a.live[n / 64] = m;
+  }
+}
+
+// G of a tile of the piece.
+template <typename T, typename S>
+__global__ __launch_bounds__(S::kThreads) void grad_kernel(const Args a) {
+  using O = Ops<T>;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[S::kLds];
+  const TileAt t(blockIdx.x, a.tm, a.tn);
+  const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wv % S::WM, wn = wv / S::WM;
+  f32x16 acc[S::MT][S::NT] = {};
+  logits<T, S>(a, acc, t, lds_addr(lds), wm, wn);
+
+  const int v0 = t.m * S::BM + 32 * S::MT * wm, left = a.vn - v0;    // in the piece
+#pragma unroll
+  for (int j = 0; j < S::NT; ++j) {
+    const int n = t.n * S::BN + 32 * (S::NT * wn + j) + l32;
+    const Row row = a.rows[n];
+    const int hit = a.tgt[n] - a.v0 - v0;
+    const bool counts = a.tgt[n] >= 0;
+#pragma unroll
+    for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float p = exp2_fast(__builtin_fmaf(acc[i][j][r], kLog2e, -row.lse2)) * row.g;
+        acc[i][j][r] = counts ? p : 0.f;
+      }
+    if (__any(counts && hit >= 0 && hit < 32 * S::MT)) {
+#pragma unroll
+      for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (counts && hit == 32 * i + attn::acc_row(r, half)) acc[i][j][r] -= row.g;
+    }
+    if (left < 32 * S::MT) {
+#pragma unroll
+      for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][j][r] = 32 * i + attn::acc_row(r, half) < left ? acc[i][j][r] : 0.f;
+    }
+    uint16_t* g = a.g + (int64_t)n * a.ldg + v0 + 4 * half;
+#pragma unroll
+    for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<uint2*>(g + 32 * i + 8 * q) =
+            make_uint2(O::pack(acc[i][j][4 * q], acc[i][j][4 * q + 1]), O::pack(acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]));
+  }
+}
+
+// 4 neighbouring columns from 4 sums.
+template <typename T>
+__device__ __forceinline__ void store4(uint16_t* row, int col, int cols, float4 v, float f) {
+  if (col < cols)      // (cols: a multiple of 8)
+    *reinterpret_cast<uint2*>(row + col) = make_uint2(Ops<T>::pack(v.x * f, v.y * f), Ops<T>::pack(v.z * f, v.w * f));
+}
+
+// dX += G W over the piece, M the columns of X.
+template <typename T, typename S>
+__global__ __launch_bounds__(S::kThreads) void dx_kernel(const Args a) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[S::kLds];
+  const uint32_t tiles = a.tm * a.tn, split = blockIdx.x / tiles;
+  const TileAt t(blockIdx.x % tiles, a.tm, a.tn);
+  const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wv % S::WM, wn = wv / S::WM;
+  const int slabs = (a.vn + 63) / 64, per = (slabs + a.splits - 1) / a.splits;
+  const int s0 = min((int)split * per, slabs), s1 = min(s0 + per, slabs);
+  f32x16 acc[S::MT][S::NT] = {};
+  {
+    const TurnedCopy<S::BM, S::kWaves> ca((const uint8_t*)a.w + (int64_t)a.v0 * a.wld, a.wld, t.m * S::BM, a.D);
+    const PlainCopy<S::BN, S::kWaves> cb(a.g, 2 * (int64_t)a.ldg, t.n * S::BN, (a.N + 255) / 256 * 256, 2 * a.ldg);
+    const TurnedRead<S::BM> ra(lane, 32 * S::MT * wm);
+    const PlainRead rb(lane, 32 * S::NT * wn);
+    product16<T, S>(acc, s1 - s0, lds_addr(lds), ra, rb, [&](int k, uint32_t at) {
+      ca.copy(s0 + k, at, rows_left(s0 + k, a.vn));
+      cb.copy(s0 + k, at + S::kA);
+    });
+  }
+  const bool whole = a.last && a.splits == 1;
+  const float f = whole ? *a.unit : 1.f;
+  float4* sums = a.dxp + (int64_t)(blockIdx.x / tiles * tiles + t.m * a.tn + t.n) * (S::BM * S::BN / 4) + threadIdx.x;
+#pragma unroll
+  for (int j = 0; j < S::NT; ++j) {
+    const int n = t.n * S::BN + 32 * (S::NT * wn + j) + l32;
+    uint16_t* row = (uint16_t*)a.dx + (int64_t)n * a.D;
+#pragma unroll
+    for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float4 v = make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
+        float4* at = sums + ((j * S::MT + i) * 4 + q) * S::kThreads;
+        if (!a.first) {
+          const float4 o = *at;
+          v = make_float4(v.x + o.x, v.y + o.y, v.z + o.z, v.w + o.w);
+        }
+        if (!whole) *at = v;
+        else if (n < a.N) store4<T>(row, t.m * S::BM + 32 * (S::MT * wm + i) + 8 * q + 4 * half, a.D, v, f);
+      }
+  }
+}
+
+// The parts of dX, added in order.
+template <typename T, typename S>
+__global__ __launch_bounds__(S::kThreads) void dx_join_kernel(const Args a) {
+  constexpr int kPer = S::MT * S::NT * 4;
+  const uint32_t tile = blockIdx.x / kPer, e = blockIdx.x % kPer, tiles = a.tm * a.tn;
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, wm = wv % S::WM, wn = wv / S::WM;
+  const int q = e % 4, i = e / 4 % S::MT, j = e / 4 / S::MT;
+  const int m = tile / a.tn * S::BM + 32 * (S::MT * wm + i) + 8 * q + 4 * (lane >> 5);
+  const int n = tile % a.tn * S::BN + 32 * (S::NT * wn + j) + (lane & 31);
+  const float4* p = a.dxp + ((int64_t)tile * kPer + e) * S::kThreads + threadIdx.x;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int s = 0; s < a.splits; ++s) {
+    const float4 o = p[(int64_t)s * tiles * kPer * S::kThreads];
+    v = make_float4(v.x + o.x, v.y + o.y, v.z + o.z, v.w + o.w);
+  }
+  if (n < a.N) store4<T>((uint16_t*)a.dx + (int64_t)n * a.D, m, a.D, v, *a.unit);
+}
+
+// dW of the piece = G^T X, M the columns of X, N the vocabulary.
+template <typename T, typename S>
+__global__ __launch_bounds__(S::kThreads) void dw_kernel(const Args a) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[S::kLds];
+  const TileAt t(blockIdx.x, a.tm, a.tn);
+  const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wv % S::WM, wn = wv / S::WM;
+  f32x16 acc[S::MT][S::NT] = {};
+  {
+    const TurnedCopy<S::BM, S::kWaves> ca(a.x, a.xld, t.m * S::BM, a.D);
+    const TurnedCopy<S::BN, S::kWaves> cb(a.g, 2 * (int64_t)a.ldg, t.n * S::BN, a.ldg);
+    const TurnedRead<S::BM> ra(lane, 32 * S::MT * wm);
+    const TurnedRead<S::BN> rb(lane, 32 * S::NT * wn);
+    // a row that does not count may hold anything; which do is read a slab ahead
+    const auto* live = (const __attribute__((address_space(4))) uint64_t*)(uintptr_t)uniform64((int64_t)(uintptr_t)a.live);
+    const int slabs = (a.N + 63) / 64;
+    uint64_t now = live[0];
+    product16<T, S>(acc, slabs, lds_addr(lds), ra, rb, [&](int k, uint32_t at) {
+      const uint64_t rows = now;
+      now = live[min(k + 1, slabs - 1)];
+      ca.copy(k, at, rows);
+      cb.copy(k, at + S::kA, ~0ull);
+    });
+  }
+  const float f = *a.unit;
+#pragma unroll
+  for (int j = 0; j < S::NT; ++j) {
+    const int v = t.n * S::BN + 32 * (S::NT * wn + j) + l32;
+    uint16_t* row = (uint16_t*)a.dw + (int64_t)(a.v0 + v) * a.D;
+    if (v < a.vn)
+#pragma unroll
+      for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          store4<T>(row, t.m * S::BM + 32 * (S::MT * wm + i) + 8 * q + 4 * half, a.D,
+                    make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]), f);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+
+inline int64_t ceil_to(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+inline int64_t tiles_of(int64_t m, int64_t n, int bm, int bn) { return (m + bm - 1) / bm * ((n + bn - 1) / bn); }
+
+int check(const GdnXentParams& P) {
+  if (P.N < 0 || P.D < 8 || P.V < 1) return GDN_ERR_BAD_SHAPE;
+  if (P.D % 8 != 0) return GDN_ERR_UNSUPPORTED;
+  if (P.dtype != GDN_DTYPE_F16 && P.dtype != GDN_DTYPE_BF16) return GDN_ERR_BAD_DTYPE;
+  // rows of a tile lie within 31 bits
+  if ((P.N > 1 && (P.x_stride < 0 || P.x_stride > 1 << 22)) || (P.V > 1 && (P.w_stride < 0 || P.w_stride > 1 << 22)) ||
+      P.D > 1 << 22)
+    return GDN_ERR_UNSUPPORTED;
+  if (P.N > 1 << 28 || P.V > 1 << 28) return GDN_ERR_BAD_SHAPE;
+  return GDN_OK;
+}
+
+// Tiles of 256 x 256 where they fill the card, else smaller ones, two or more a CU.
+enum Kind { kBig, kMid, kNarrow };
+Kind kind_of(int64_t m, int64_t n, bool narrow) {
+  if (narrow && n <= 64) return kNarrow;
+  return tiles_of(m, n, 256, 256) >= 192 ? kBig : kMid;
+}
+
+// Vocabulary of a piece: G takes about 128 MiB.
+int piece_of(const GdnXentParams& P) {
+  const int64_t rows = ceil_to(std::max(P.N, 1), 256);
+  const int64_t most = std::max<int64_t>((128ll << 20) / (2 * rows) / 256 * 256, 256);
+  return (int)std::min(most, ceil_to(P.V, 256));
+}
+
+// Parts of a piece's vocabulary for dX.
+struct DxPlan {
+  Kind kind;
+  int splits;
+  int64_t tiles, floats;
+};
+DxPlan dx_plan(const GdnXentParams& P) {
+  DxPlan d;
+  d.kind = kind_of(P.D, P.N, false);
+  const int b = d.kind == kBig ? 256 : 128;
+  d.tiles = tiles_of(P.D, P.N, b, b);
+  const int64_t slabs = piece_of(P) / 64, places = d.kind == kBig ? 256 : 512;
+  d.splits = (int)std::max<int64_t>(1, std::min(places / d.tiles, slabs / 8));
+  const bool kept = d.splits > 1 || piece_of(P) < P.V;
+  d.floats = kept ? d.tiles * d.splits * b * b : 0;
+  return d;
+}
+
+struct BwdLayout {
+  int64_t rows, tgt, live, unit, g, dx, bytes;
+  explicit BwdLayout(const GdnXentParams& P) {
+    const int64_t n = ceil_to(std::max(P.N, 1), 256);
+    rows = 0;
+    tgt = rows + n * (int64_t)sizeof(Row);
+    live = tgt + n * 4;
+    unit = ceil_to(live + n / 8, 256);
+    g = unit + 256;
+    dx = g + n * piece_of(P) * 2;
+    bytes = dx + dx_plan(P).floats * 4;
+  }
+};
+
+Kind fwd_kind(const GdnXentParams& P) { return kind_of(P.V, P.N, true); }
+int64_t fwd_tiles(const GdnXentParams& P) { return (P.V + 127) / 128; }
+
+Args args_of(const GdnXentParams& P) {
+  Args a = {};
+  a.x = P.x;
+  a.w = P.w;
+  a.target = P.target;
+  a.loss = P.loss;
+  a.lse = P.lse;
+  a.dloss = P.dloss;
+  a.dx = P.dx;
+  a.dw = P.dw;
+  a.xld = 2 * (P.N > 1 ? P.x_stride : (int64_t)P.D);
+  a.wld = 2 * (P.V > 1 ? P.w_stride : (int64_t)P.D);
+  a.dloss_step = P.dloss_stride;
+  a.N = P.N;
+  a.D = P.D;
+  a.V = P.V;
+  return a;
+}
+
+// K<T, S>(args, stream), S by kind.
+#define GDN_XENT_BY_KIND(kernel, T, kind, grid, s, a)                                                        \
+  switch (kind) {                                                                                            \
+    case kBig: hipLaunchKernelGGL((kernel<T, Big>), dim3(grid), dim3(Big::kThreads), 0, s, a); break;        \
+    default: hipLaunchKernelGGL((kernel<T, Mid>), dim3(grid), dim3(Mid::kThreads), 0, s, a); break;          \
+  }
+
+void set_tiles(Args& a, Kind k, int64_t m, int64_t n) {
+  const int bm = k == kBig ? 256 : 128, bn = k == kBig ? 256 : k == kMid ? 128 : 64;
+  a.tm = (int)((m + bm - 1) / bm);
+  a.tn = (int)((n + bn - 1) / bn);
+}
+
+template <typename T>
+int launch_fwd(Args a, Kind kind, hipStream_t s) {
+  a.v0 = 0;
+  a.vn = a.V;
+  set_tiles(a, kind, a.V, a.N);
+  const uint32_t grid = (uint32_t)a.tm * a.tn;
+  if (kind == kNarrow) hipLaunchKernelGGL((fwd_kernel<T, Narrow>), dim3(grid), dim3(Narrow::kThreads), 0, s, a);
+  else GDN_XENT_BY_KIND(fwd_kernel, T, kind, grid, s, a);
+  hipLaunchKernelGGL(join_kernel, dim3((a.N + 15) / 16), dim3(kJoin), 0, s, a);
+  return (int)hipGetLastError();
+}
+
+template <typename T>
+int launch_bwd(Args a, const GdnXentParams& P, hipStream_t s) {
+  const DxPlan d = dx_plan(P);
+  const int piece = piece_of(P);
+  a.ldg = piece;
+  const int blocks = std::min<int>((a.N + kJoin - 1) / kJoin, 256);
+  hipLaunchKernelGGL((rows_kernel<std::is_same<T, f16>::value>), dim3(blocks), dim3(kJoin), 0, s, a);
+  for (int v = 0; v < a.V; v += piece) {
+    a.v0 = v;
+    a.vn = std::min(piece, a.V - v);
+    a.first = v == 0;
+    a.last = v + piece >= a.V;
+    a.splits = 1;
+    const Kind kl = kind_of(a.vn, a.N, true);
+    set_tiles(a, kl, a.vn, a.N);
+    const uint32_t grid = (uint32_t)a.tm * a.tn;
+    if (kl == kNarrow) hipLaunchKernelGGL((grad_kernel<T, Narrow>), dim3(grid), dim3(Narrow::kThreads), 0, s, a);
+    else GDN_XENT_BY_KIND(grad_kernel, T, kl, grid, s, a);
+    const Kind kw = kind_of(a.D, a.vn, false);
+    set_tiles(a, kw, a.D, a.vn);
+    GDN_XENT_BY_KIND(dw_kernel, T, kw, (uint32_t)a.tm * a.tn, s, a);
+    set_tiles(a, d.kind, a.D, a.N);
+    a.splits = d.splits;
+    GDN_XENT_BY_KIND(dx_kernel, T, d.kind, (uint32_t)(d.tiles * d.splits), s, a);
+  }
+  if (d.splits > 1) GDN_XENT_BY_KIND(dx_join_kernel, T, d.kind, (uint32_t)(d.tiles * (d.kind == kBig ? 32 : 16)), s, a);
+  return (int)hipGetLastError();
+}
+
+bool rows_ok(const void* p, int64_t stride, int64_t n) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (n <= 1 || stride % 8 == 0);
+}
+
+}  // namespace xent
+}  // namespace gdn
+
+using namespace gdn;
+using namespace gdn::xent;
+
+extern "C" {
+
+int64_t gdn_xent_workspace_size(const GdnXentParams* prm) {
+  if (prm == nullptr || check(*prm) != GDN_OK) return -1;
+  return (int64_t)prm->N * (fwd_tiles(*prm) * 8 + 4);
+}
+
+int64_t gdn_xent_bwd_workspace_size(const GdnXentParams* prm) {
+  if (prm == nullptr || check(*prm) != GDN_OK) return -1;
+  return BwdLayout(*prm).bytes;
+}
+
+static int check_call(const GdnXentParams& P, int64_t need) {
+  const int st = check(P);
+  if (st != GDN_OK) return st;
+  if ((P.N > 0 && (P.x == nullptr || P.target == nullptr || P.lse == nullptr)) || P.w == nullptr) return GDN_ERR_NULL_POINTER;
+  if (!rows_ok(P.x, P.x_stride, P.N) || !rows_ok(P.w, P.w_stride, P.V)) return GDN_ERR_MISALIGNED;
+  // workgroups of the smallest tiles
+  if (!grid_fits(tiles_of(P.V, P.N, 128, 64), 256) || !grid_fits(tiles_of(P.D, std::max(P.N, P.V), 128, 128), 256))
+    return GDN_ERR_BAD_SHAPE;
+  if (need > 0 && (P.workspace == nullptr || P.workspace_bytes < need ||
+                   reinterpret_cast<uintptr_t>(P.workspace) % 256 != 0))
+    return GDN_ERR_WORKSPACE;
+  return GDN_OK;
+}
+
+int gdn_xent_launch(const GdnXentParams* prm, void* stream) {
+  if (prm == nullptr) return GDN_ERR_NULL_POINTER;
+  const GdnXentParams& P = *prm;
+  if (const int st = check_call(P, gdn_xent_workspace_size(prm))) return st;
+  if (P.N == 0) return GDN_OK;
+  if (P.loss == nullptr) return GDN_ERR_NULL_POINTER;
+  Args a = args_of(P);
+  a.part = static_cast<float2*>(P.workspace);
+  a.hit = reinterpret_cast<float*>(a.part + fwd_tiles(P) * P.N);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  return P.dtype == GDN_DTYPE_F16 ? launch_fwd<f16>(a, fwd_kind(P), s) : launch_fwd<bf16_t>(a, fwd_kind(P), s);
+}
+
+int gdn_xent_bwd_launch(const GdnXentParams* prm, void* stream) {
+  if (prm == nullptr) return GDN_ERR_NULL_POINTER;
+  const GdnXentParams& P = *prm;
+  if (const int st = check_call(P, gdn_xent_bwd_workspace_size(prm))) return st;
+  if (P.N < 1) return GDN_ERR_BAD_SHAPE;
+  if (P.dloss == nullptr || P.dx == nullptr || P.dw == nullptr) return GDN_ERR_NULL_POINTER;
+  if (!rows_ok(P.dx, 0, 1) || !rows_ok(P.dw, 0, 1)) return GDN_ERR_MISALIGNED;
+  const BwdLayout l(P);
+  Args a = args_of(P);
+  char* ws = static_cast<char*>(P.workspace);
+  a.rows = reinterpret_cast<Row*>(ws + l.rows);
+  a.tgt = reinterpret_cast<int32_t*>(ws + l.tgt);
+  a.live = reinterpret_cast<uint64_t*>(ws + l.live);
+  a.unit = reinterpret_cast<float*>(ws + l.unit);
+  a.g = reinterpret_cast<uint16_t*>(ws + l.g);
+  a.dxp = reinterpret_cast<float4*>(ws + l.dx);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  return P.dtype == GDN_DTYPE_F16 ? launch_bwd<f16>(a, P, s) : launch_bwd<bf16_t>(a, P, s);
+}
+
+}  // extern "C"

@@ -564,6 +564,49 @@ int gdn_xent_launch(const GdnXentParams* params, void* stream);
 int64_t gdn_xent_bwd_workspace_size(const GdnXentParams* params);
 int gdn_xent_bwd_launch(const GdnXentParams* params, void* stream);
 
+/* e4m3 with scales: scale = max|x| / 448, q = x / scale (in fp32, by the scale
+ * that is stored) rounded to the nearest; a group of zeros has scale 0, one with a
+ * NaN is NaN.  A group is 128 columns of a row (scale [rows, D / 128]), a row
+ * ([rows]) or a block of 128 x 128 ([ceil(rows / 128), D / 128]).
+ *   - x: any dtype, rows contiguous and 16-byte aligned, D a multiple of 128;
+ *     q [rows, D] and scale dense. */
+enum GdnFp8Mode { GDN_FP8_GROUPS = 0, GDN_FP8_ROWS = 1, GDN_FP8_BLOCKS = 2 };
+
+typedef struct GdnFp8QuantParams {
+  const void* x;
+  void* q;
+  float* scale;
+  int64_t x_stride;         /* rows, in elements */
+  int32_t rows, D;
+  int32_t x_dtype;
+  int32_t mode;
+} GdnFp8QuantParams;
+
+int gdn_fp8_quant_launch(const GdnFp8QuantParams* params, void* stream);
+
+/* Product of e4m3 rows with an e4m3 weight, b the blocks of 128 columns:
+ *     y_mn = sum_b x_scale_mb w_scale_{n/128, b} sum_{k in b} x_mk w_nk
+ * (sums in fp32, y rounded once).
+ *   - x [M,K], w [N,K]: rows contiguous and 16-byte aligned, at most 2^23 bytes
+ *     apart, K a multiple of 128; y [M,N] dense, 16-byte aligned, any dtype.
+ *   - x_scale dense [M, K / 128] (group 128) or [M] (group 0); w_scale dense
+ *     [ceil(N / 128), K / 128].
+ *   - M, N up to 2^28. */
+typedef struct GdnFp8LinearParams {
+  const void* x;
+  const float* x_scale;
+  const void* w;
+  const float* w_scale;
+  void* y;
+  int64_t x_stride;         /* rows, in elements */
+  int64_t w_stride;
+  int32_t M, N, K;
+  int32_t group;            /* 0 or 128 */
+  int32_t y_dtype;
+} GdnFp8LinearParams;
+
+int gdn_fp8_linear_launch(const GdnFp8LinearParams* params, void* stream);
+
 /* Human-readable text for a status code. */
 const char* gdn_fwd_status_string(int status);
 

@@ -26,6 +26,11 @@ GDN_ERR_BAD_DTYPE = 1005
 GDN_ERR_WORKSPACE = 1006
 GDN_ERR_SCRATCH_LIMIT = 1007
 
+# enum GdnFp8Mode
+FP8_GROUPS = 0
+FP8_ROWS = 1
+FP8_BLOCKS = 2
+
 # enum GdnFlags
 FLAG_PHASED_KERNEL = 1
 FLAG_FUSED_KERNEL = 2
@@ -63,6 +68,8 @@ EXPORTED_SYMBOLS = (
     "gdn_xent_launch",
     "gdn_xent_bwd_workspace_size",
     "gdn_xent_bwd_launch",
+    "gdn_fp8_quant_launch",
+    "gdn_fp8_linear_launch",
 )
 
 _I64x2 = ctypes.c_int64 * 2
@@ -219,6 +226,24 @@ class GdnXentParams(ctypes.Structure):
         ("N D V dtype", ctypes.c_int32))
 
 
+class GdnFp8QuantParams(ctypes.Structure):
+    """Mirror of ``GdnFp8QuantParams`` in include/gdn_mi355x.h."""
+
+    _fields_ = _fields(
+        ("x q scale", ctypes.c_void_p),
+        ("x_stride", ctypes.c_int64),
+        ("rows D x_dtype mode", ctypes.c_int32))
+
+
+class GdnFp8LinearParams(ctypes.Structure):
+    """Mirror of ``GdnFp8LinearParams`` in include/gdn_mi355x.h."""
+
+    _fields_ = _fields(
+        ("x x_scale w w_scale y", ctypes.c_void_p),
+        ("x_stride w_stride", ctypes.c_int64),
+        ("M N K group y_dtype", ctypes.c_int32))
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -263,7 +288,8 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
         for name, struct in (("scan", GdnScanParams), ("scan_bwd", GdnScanParams), ("norm", GdnNormParams),
                              ("norm_bwd", GdnNormParams), ("attn", GdnAttnParams), ("attn_bwd", GdnAttnParams),
                              ("attn_decode", GdnAttnDecodeParams), ("xent", GdnXentParams),
-                             ("xent_bwd", GdnXentParams)):
+                             ("xent_bwd", GdnXentParams), ("fp8_quant", GdnFp8QuantParams),
+                             ("fp8_linear", GdnFp8LinearParams)):
             if f"gdn_{name}_workspace_size" in EXPORTED_SYMBOLS:
                 size = getattr(lib, f"gdn_{name}_workspace_size")
                 size.argtypes, size.restype = [ctypes.POINTER(struct)], ctypes.c_int64

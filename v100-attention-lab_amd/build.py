@@ -21,7 +21,7 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 # compiled in parallel.
 SOURCES = ["gdn_fwd_api.hip", "gdn_fwd_f16.hip", "gdn_fwd_bf16.hip", "gdn_fwd_f32.hip",
            "gdn_fwd_f32_batch.hip", "gdn_fwd_c64.hip", "gdn_fwd_scan32.hip", "gdn_prep.hip", "gdn_bwd.hip",
-           "gdn_scan.hip", "gdn_norm.hip", "gdn_attn_fwd.hip", "gdn_attn_bwd.hip", "gdn_attn_decode.hip", "gdn_xent.hip"]
+           "gdn_scan.hip", "gdn_norm.hip", "gdn_attn_fwd.hip", "gdn_attn_bwd.hip", "gdn_attn_decode.hip", "gdn_xent.hip", "gdn_fp8_linear.hip"]
 OBJ_DIR = os.path.join(PKG_DIR, "_build")
 INCLUDE = os.path.join(REPO_DIR, "include")
 LIB_DIR = os.path.join(PKG_DIR, "lib")
@@ -51,6 +51,8 @@ HIPCC_FLAGS = [
 SOURCE_FLAGS = {
     "gdn_fwd_scan32.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "gdn_fwd_f32_batch.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    # every product goes through the vector unit to meet its scales
+    "gdn_fp8_linear.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

@@ -1,0 +1,511 @@
+// Product of e4m3 rows with an e4m3 weight, with scales along the contraction,
+// and the quantisers that make its operands:
+//     y_mn = sum_b xs_mb ws_{n / 128, b} sum_{k in block b} x_mk w_nk
+// (blocks of 128 columns; a row's scale may also be one for all blocks).
+//
+// Matrix instructions take 128 products deep blocks at a time; each block's sums
+// start at zero and enter the result times their scales, in fp32, which costs
+// one multiply-add for every 32 multiply-adds' time of the matrix unit and runs
+// beside it.  The matrix unit adds 8-bit products in groups of 8, each cut (towards
+// zero) at 2^-13 of the largest of its group (found by products of chosen sizes):
+// about 1.4e-5 of a result of normally distributed terms, under what 16-bit results
+// show and far under e4m3's own steps.  fp32 results are made of the same bytes as
+// fp16 operands instead, whose products are summed in fp32, at less than half the rate.
+//   - up to 64 rows: the weight is read once from memory straight into the
+//     operands' registers, the contraction dealt to the waves of a workgroup,
+//     whose sums are joined in LDS in order;
+//   - more: tiles through LDS (gdn_gemm.h), a slab being one block of 128.
+#include <algorithm>
+
+#include "gdn_fp8.h"
+#include "gdn_gemm.h"
+
+namespace gdn {
+namespace fp8 {
+
+using namespace gemm;
+using rowio::Pack;
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+struct LArgs {
+  const uint8_t* x;
+  const float* xs;
+  const uint8_t* w;
+  const float* ws;
+  void* y;
+  int64_t xld, wld, xsld, wsld;   // bytes; scales a row
+  int M, N, K;
+  int xstep;                      // 1: a scale a block, 0: a scale a row
+  int y_dtype;
+  int tm, tn;
+};
+
+// 8 e4m3 numbers as fp16 (exact).
+__device__ __forceinline__ f16x8 widen(int lo, int hi) {
+  typedef f16 f16x2 __attribute__((ext_vector_type(2)));
+  const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, false);
+  const f16x2 b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, true);
+  const f16x2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, false);
+  const f16x2 d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, true);
+  return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// Products of a block of 128.  EXACT: summed in fp32.
+template <bool EXACT>
+__device__ __forceinline__ f32x4 mfma128(const i32x8& a, const i32x8& b) {
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  if constexpr (EXACT) {
+#pragma unroll
+    for (int s = 0; s < 8; s += 2)
+      sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen(a[s], a[s + 1]), widen(b[s], b[s + 1]), sum, 0, 0, 0);
+    return sum;
+  } else {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, sum, 0, 0, 0, 0, 0, 0);
+  }
+}
+__device__ __forceinline__ i32x8 join16(const uint4& a, const uint4& b) {
+  return i32x8{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w};
+}
+
+// 4 neighbouring outputs n .. n + 3 of a row of N.
+__device__ __forceinline__ void store_y(const LArgs& a, int64_t m, int n, const f32x4& v) {
+  const int64_t at = m * a.N + n;
+  if (a.N % 4 == 0) {
+    if (n >= a.N) return;
+    if (a.y_dtype == GDN_DTYPE_F32) {
+      *reinterpret_cast<f32x4*>(static_cast<float*>(a.y) + at) = v;
+    } else {
+      const bool h = a.y_dtype == GDN_DTYPE_F16;
+      uint2 p;
+      p.x = h ? attn::Ops<f16>::pack(v[0], v[1]) : attn::Ops<bf16_t>::pack(v[0], v[1]);
+      p.y = h ? attn::Ops<f16>::pack(v[2], v[3]) : attn::Ops<bf16_t>::pack(v[2], v[3]);
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.y) + at) = p;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (n + e < a.N) store_scalar(a.y, at + e, a.y_dtype, v[e]);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// few rows
+// ---------------------------------------------------------------------------
+
+constexpr int kFewWaves = 8;
+
+// 16 NA outputs of up to 16 NB rows; wave w takes blocks w, w + 8, ...  Lane l
+// holds row l % 16 of an operand, bytes 32 (l / 16) .. + 31 of the block.
+template <int NA, int NB, bool EXACT>
+__global__ __launch_bounds__(64 * kFewWaves) void few_kernel(const LArgs a) {
+  const int lane = threadIdx.x & 63, l16 = lane & 15, part = lane >> 4;
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n0 = blockIdx.x * 16 * NA, m0 = blockIdx.y * 16 * NB;
+  const uint8_t *w[NA], *x[NB];
+  const float* xs[NB];
+#pragma unroll
+  for (int i = 0; i < NA; ++i) w[i] = a.w + (int64_t)min(n0 + 16 * i + l16, a.N - 1) * a.wld + 32 * part;
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    const int64_t m = min(m0 + 16 * j + l16, a.M - 1);
+    x[j] = a.x + m * a.xld + 32 * part;
+    xs[j] = a.xs + m * a.xsld;
+  }
+  const float* ws = a.ws + (int64_t)(n0 / 128) * a.wsld;
+  f32x4 acc[NA][NB] = {};
+  const int blocks = a.K / 128;
+  struct Block {
+    uint4 w[NA][2], x[NB][2];
+    float xs[NB], ws;
+  };
+  auto load = [&](Block& f, int b) {
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) f.w[i][h] = *reinterpret_cast<const uint4*>(w[i] + (int64_t)b * 128 + 16 * h);
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) f.x[j][h] = *reinterpret_cast<const uint4*>(x[j] + (int64_t)b * 128 + 16 * h);
+      f.xs[j] = xs[j][b * a.xstep];
+    }
+    f.ws = ws[b];
+  };
+  auto use = [&](const Block& f) {
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      const float s = f.xs[j] * f.ws;
+#pragma unroll
+      for (int i = 0; i < NA; ++i) {
+        const f32x4 p = mfma128<EXACT>(join16(f.w[i][0], f.w[i][1]), join16(f.x[j][0], f.x[j][1]));
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(p[r], s, acc[i][j][r]);
+      }
+    }
+  };
+  for (int b = wv; b < blocks; b += 2 * kFewWaves) {
+    Block f[2];
+    load(f[0], b);
+    const bool two = b + kFewWaves < blocks;
+    if (two) load(f[1], b + kFewWaves);
+    use(f[0]);
+    if (two) use(f[1]);
+  }
+  __shared__ f32x4 sums[kFewWaves][NA * NB][64];
+#pragma unroll
+  for (int i = 0; i < NA; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j) sums[wv][i * NB + j][lane] = acc[i][j];
+  __syncthreads();
+  for (int e = wv; e < NA * NB; e += kFewWaves) {
+    f32x4 v = sums[0][e][lane];
+#pragma unroll
+    for (int k = 1; k < kFewWaves; ++k) v += sums[k][e][lane];
+    const int m = m0 + 16 * (e % NB) + l16;
+    if (m < a.M) store_y(a, m, n0 + 16 * (e / NB) + 4 * part, v);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// tiles
+// ---------------------------------------------------------------------------
+
+// MT x NT products of 16 x 16 a wave, WM x WN waves.
+template <int MT_, int NT_, int WM_, int WN_>
+struct Shape8 {
+  static constexpr int MT = MT_, NT = NT_, WM = WM_, WN = WN_;
+  static constexpr int BM = 16 * MT * WM, BN = 16 * NT * WN, kWaves = WM * WN, kThreads = 64 * kWaves;
+  static constexpr uint32_t kA = kSlab * BM, kB = kSlab * BN, kStage = kA + kB, kLds = 2 * kStage;
+};
+typedef Shape8<8, 4, 2, 4> Big8;     // 256 outputs x 256 rows, one workgroup a CU
+typedef Shape8<4, 4, 2, 2> Mid8;     // 128 x 128, two
+typedef Shape8<4, 2, 2, 2> Low8;     // 128 x 64, three
+
+// Operand of a block: row 16 i + l % 16 from the wave's first, 32 bytes that lane
+// part l / 16 of both operands agrees on.
+struct Read8 {
+  uint32_t ofs;
+  __device__ __forceinline__ Read8(int lane, int first) {
+    const int r = lane & 15;      // (first: a multiple of 16)
+    ofs = (uint32_t)(first + r) * kSlab + 16 * ((2 * (lane >> 4)) ^ ((r >> 1) & 7));
+  }
+  __device__ __forceinline__ i32x8 operator()(uint32_t tile, int i) const {
+    const u32x4 a = *(const lds_u32x4*)(tile + ofs + 16 * kSlab * i);
+    const u32x4 b = *(const lds_u32x4*)(tile + (ofs ^ 16) + 16 * kSlab * i);
+    return i32x8{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
+  }
+};
+
+template <typename S, bool EXACT>
+__global__ __launch_bounds__(S::kThreads) void tile_kernel(const LArgs a) {
+  __shared__ __attribute__((aligned(1024))) uint8_t mem[S::kLds];
+  constexpr int MT = S::MT, NT = S::NT;
+  const TileAt t(blockIdx.x, a.tm, a.tn);
+  const int lane = threadIdx.x & 63, l16 = lane & 15;
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wv % S::WM, wn = wv / S::WM;
+  const uint32_t lds = lds_addr(mem);
+  const PlainCopy<S::BM, S::kWaves> ca(a.w, a.wld, t.m * S::BM, a.N, a.K);
+  const PlainCopy<S::BN, S::kWaves> cb(a.x, a.xld, t.n * S::BN, a.M, a.K);
+  const Read8 ra(lane, 16 * MT * wm), rb(lane, 16 * NT * wn);
+  auto copy = [&](int k, uint32_t at) {
+    ca.copy(k, at);
+    cb.copy(k, at + S::kA);
+  };
+  // scales: the lane's rows, and (the same for the wave) its 128 outputs
+  const auto* xs = (const __attribute__((address_space(1))) float*)(uintptr_t)uniform64(
+      (int64_t)(uintptr_t)(a.xs + (int64_t)t.n * S::BN * a.xsld));
+  uint32_t xofs[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+    xofs[j] = (uint32_t)min(16 * (NT * wn + j) + l16, a.M - 1 - t.n * S::BN) * (uint32_t)a.xsld;
+  const auto* ws = (const __attribute__((address_space(4))) float*)(uintptr_t)uniform64(
+      (int64_t)(uintptr_t)(a.ws + (int64_t)min((t.m * S::BM + 16 * MT * wm) / 128, (a.N - 1) / 128) * a.wsld));
+  const int slabs = a.K / 128;
+  f32x4 acc[MT][NT] = {};
+  float sx[NT], nx[NT], sw = ws[0], nw = 0.f;
+#pragma unroll
+  for (int j = 0; j < NT; ++j) sx[j] = xs[xofs[j]];
+  copy(0, lds);
+  dma_wait();
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  auto next_scales = [&](int k) {
+    const int b = min(k, slabs - 1);
+    nw = ws[b];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) nx[j] = (xs + b * a.xstep)[xofs[j]];
+  };
+  next_scales(1);
+  if (slabs > 1) copy(1, lds + S::kStage);
+  i32x8 fb[NT], fa[2];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) fb[j] = rb(lds + S::kA, j);
+  fa[0] = ra(lds, 0);
+  for (int k = 0; k < slabs; ++k) {
+    const uint32_t here = lds + (k & 1) * S::kStage, other = lds + ((k & 1) ^ 1) * S::kStage;
+    float f[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) f[j] = sx[j] * sw;
+    // a product enters its sum right before the next one of its column starts
+    f32x4 p[NT];
+    auto add = [&](int i, int j) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(p[j][r], f[j], acc[i][j][r]);
+      asm volatile("" : "+v"(acc[i][j]));     // (here, not at the slab's end with all products kept)
+    };
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      if (i + 1 < MT) fa[(i + 1) & 1] = ra(here, i + 1);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        if (i > 0) add(i - 1, j);
+        p[j] = mfma128<EXACT>(fa[i & 1], fb[j]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    // every operand of this slab is in registers, and the next slab in LDS
+    dma_wait();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < NT; ++j) sx[j] = nx[j];
+    sw = nw;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) asm volatile("" : "+v"(sx[j]));
+    next_scales(k + 2);
+    if (k + 2 < slabs) copy(k + 2, here);
+    // (behind the last slab from the other stage, for nobody)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) fb[j] = rb(other + S::kA, j);
+    fa[0] = ra(other, 0);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) add(MT - 1, j);
+  }
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const int m = t.n * S::BN + 16 * (NT * wn + j) + l16;
+    if (m < a.M)
+#pragma unroll
+      for (int i = 0; i < MT; ++i) store_y(a, m, t.m * S::BM + 16 * (MT * wm + i) + 4 * (lane >> 4), acc[i][j]);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// quantisers
+// ---------------------------------------------------------------------------
+
+struct QArgs {
+  const void* x;
+  uint8_t* q;
+  float* scale;
+  int64_t ld;        // elements between rows
+  int rows, D;
+  uint32_t groups;   // of all rows
+};
+
+constexpr int kQ = 256;
+
+// A group of 128 columns: 16 lanes.
+template <typename T>
+__global__ __launch_bounds__(kQ) void quant_groups_kernel(const QArgs a) {
+  const uint32_t g = blockIdx.x * (kQ / 16) + threadIdx.x / 16, per = a.D / 128;
+  const bool ok = g < a.groups;
+  const uint32_t row = ok ? g / per : 0, c = (ok ? g - row * per : 0) * 128 + threadIdx.x % 16 * 8;
+  Pack<T, 8> x;
+  x.load(static_cast<const T*>(a.x) + (int64_t)row * a.ld + c);
+  float v[8], m = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    v[e] = x.get(e);
+    m = nan_max(m, fabsf(v[e]));
+  }
+  m = lanes_max<16>(m) / kFp8Max;
+  if (!ok) return;
+  if (threadIdx.x % 16 == 0) a.scale[g] = m;
+  const Quant quant(m);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = quant(v[e]);
+  store_fp8<8>(a.q + (int64_t)row * a.D + c, v);
+}
+
+// A whole row, read twice: a workgroup.
+template <typename T>
+__global__ __launch_bounds__(kQ) void quant_rows_kernel(const QArgs a) {
+  const int64_t row = blockIdx.x;
+  const T* x = static_cast<const T*>(a.x) + row * a.ld;
+  float m = 0.f;
+  for (int c = threadIdx.x * 8; c < a.D; c += kQ * 8) {
+    Pack<T, 8> p;
+    p.load(x + c);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = nan_max(m, fabsf(p.get(e)));
+  }
+  __shared__ float slots[kQ / 64];
+  m = lanes_max<64>(m);
+  if ((threadIdx.x & 63) == 0) slots[threadIdx.x >> 6] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kQ / 64; ++w) m = nan_max(m, slots[w]);
+  m = m / kFp8Max;
+  if (threadIdx.x == 0) a.scale[row] = m;
+  const Quant quant(m);
+  for (int c = threadIdx.x * 8; c < a.D; c += kQ * 8) {
+    Pack<T, 8> p;
+    p.load(x + c);
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = quant(p.get(e));
+    store_fp8<8>(a.q + row * a.D + c, v);
+  }
+}
+
+// A block of 128 x 128 of a weight: 16 lanes a row, 8 rows a thread.
+template <typename T>
+__global__ __launch_bounds__(kQ) void quant_blocks_kernel(const QArgs a) {
+  const uint32_t per = a.D / 128, br = blockIdx.x / per, bc = blockIdx.x - br * per;
+  const int c = bc * 128 + threadIdx.x % 16 * 8, r0 = br * 128 + threadIdx.x / 16;
+  Pack<T, 8> x[8];
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    x[i].zero();
+    if (r0 + 16 * i < a.rows) x[i].load(static_cast<const T*>(a.x) + (int64_t)(r0 + 16 * i) * a.ld + c);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = nan_max(m, fabsf(x[i].get(e)));
+  }
+  __shared__ float slots[kQ / 64];
+  m = lanes_max<64>(m);
+  if ((threadIdx.x & 63) == 0) slots[threadIdx.x >> 6] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kQ / 64; ++w) m = nan_max(m, slots[w]);
+  m = m / kFp8Max;
+  if (threadIdx.x == 0) a.scale[blockIdx.x] = m;
+  const Quant quant(m);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = quant(x[i].get(e));
+    if (r0 + 16 * i < a.rows) store_fp8<8>(a.q + (int64_t)(r0 + 16 * i) * a.D + c, v);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+
+inline int64_t tiles_of(int64_t m, int64_t n, int bm, int bn) { return (m + bm - 1) / bm * ((n + bn - 1) / bn); }
+
+template <typename S, bool EXACT>
+void launch_tiles(LArgs& a, hipStream_t s) {
+  a.tm = (a.N + S::BM - 1) / S::BM;
+  a.tn = (a.M + S::BN - 1) / S::BN;
+  hipLaunchKernelGGL((tile_kernel<S, EXACT>), dim3((uint32_t)a.tm * a.tn), dim3(S::kThreads), 0, s, a);
+}
+template <int NA, int NB, bool EXACT>
+void launch_few(const LArgs& a, hipStream_t s) {
+  hipLaunchKernelGGL((few_kernel<NA, NB, EXACT>), dim3((a.N + 16 * NA - 1) / (16 * NA), (a.M + 16 * NB - 1) / (16 * NB)),
+                     dim3(64 * kFewWaves), 0, s, a);
+}
+
+template <bool EXACT>
+void launch_linear(LArgs& a, hipStream_t s) {
+  if (a.M <= 16) return launch_few<1, 1, EXACT>(a, s);
+  if (a.M <= 32) return launch_few<1, 2, EXACT>(a, s);
+  if (a.M <= 64) return launch_few<2, 4, EXACT>(a, s);
+  if constexpr (!EXACT) {
+    if (tiles_of(a.N, a.M, 256, 256) >= 192) return launch_tiles<Big8, EXACT>(a, s);
+  }
+  if (tiles_of(a.N, a.M, 128, 128) >= 256) return launch_tiles<Mid8, EXACT>(a, s);
+  launch_tiles<Low8, EXACT>(a, s);
+}
+
+template <typename T>
+void launch_quant(const QArgs& a, int mode, hipStream_t s) {
+  if (mode == GDN_FP8_GROUPS)
+    hipLaunchKernelGGL((quant_groups_kernel<T>), dim3((a.groups + kQ / 16 - 1) / (kQ / 16)), dim3(kQ), 0, s, a);
+  else if (mode == GDN_FP8_ROWS)
+    hipLaunchKernelGGL((quant_rows_kernel<T>), dim3(a.rows), dim3(kQ), 0, s, a);
+  else
+    hipLaunchKernelGGL((quant_blocks_kernel<T>), dim3((uint32_t)((a.rows + 127) / 128) * (a.D / 128)), dim3(kQ), 0, s, a);
+}
+
+}  // namespace fp8
+}  // namespace gdn
+
+using namespace gdn;
+using namespace gdn::fp8;
+
+extern "C" {
+
+int gdn_fp8_quant_launch(const GdnFp8QuantParams* prm, void* stream) {
+  if (prm == nullptr) return GDN_ERR_NULL_POINTER;
+  const GdnFp8QuantParams& P = *prm;
+  if (P.rows < 0 || P.D < 128 || P.x_stride < 0) return GDN_ERR_BAD_SHAPE;
+  if (P.D % 128 != 0 || P.mode < GDN_FP8_GROUPS || P.mode > GDN_FP8_BLOCKS) return GDN_ERR_UNSUPPORTED;
+  if (!scan_dtype_ok(P.x_dtype)) return GDN_ERR_BAD_DTYPE;
+  if (P.rows == 0) return GDN_OK;
+  if (P.x == nullptr || P.q == nullptr || P.scale == nullptr) return GDN_ERR_NULL_POINTER;
+  if (reinterpret_cast<uintptr_t>(P.x) % 16 != 0 || (P.rows > 1 && P.x_stride * dtype_bytes(P.x_dtype) % 16 != 0) ||
+      reinterpret_cast<uintptr_t>(P.q) % 8 != 0)
+    return GDN_ERR_MISALIGNED;
+  const int64_t groups = (int64_t)P.rows * (P.D / 128);
+  if (!grid_fits(groups, 16) || !grid_fits(P.rows, kQ)) return GDN_ERR_BAD_SHAPE;
+  QArgs a = {};
+  a.x = P.x;
+  a.q = static_cast<uint8_t*>(P.q);
+  a.scale = P.scale;
+  a.ld = P.rows > 1 ? P.x_stride : 0;
+  a.rows = P.rows;
+  a.D = P.D;
+  a.groups = (uint32_t)groups;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (P.x_dtype == GDN_DTYPE_F16) launch_quant<f16>(a, P.mode, s);
+  else if (P.x_dtype == GDN_DTYPE_BF16) launch_quant<bf16_t>(a, P.mode, s);
+  else launch_quant<float>(a, P.mode, s);
+  return (int)hipGetLastError();
+}
+
+int gdn_fp8_linear_launch(const GdnFp8LinearParams* prm, void* stream) {
+  if (prm == nullptr) return GDN_ERR_NULL_POINTER;
+  const GdnFp8LinearParams& P = *prm;
+  if (P.M < 0 || P.N < 1 || P.K < 128) return GDN_ERR_BAD_SHAPE;
+  if (P.K % 128 != 0 || (P.group != 0 && P.group != 128)) return GDN_ERR_UNSUPPORTED;
+  if (!scan_dtype_ok(P.y_dtype)) return GDN_ERR_BAD_DTYPE;
+  if (P.M > 1 << 28 || P.N > 1 << 28) return GDN_ERR_BAD_SHAPE;
+  // rows of a tile lie within 31 bits
+  if ((P.M > 1 && (P.x_stride < 0 || P.x_stride > 1 << 23)) || (P.N > 1 && (P.w_stride < 0 || P.w_stride > 1 << 23)) ||
+      P.K > 1 << 23)
+    return GDN_ERR_UNSUPPORTED;
+  if (P.M == 0) return GDN_OK;
+  if (P.x == nullptr || P.x_scale == nullptr || P.w == nullptr || P.w_scale == nullptr || P.y == nullptr)
+    return GDN_ERR_NULL_POINTER;
+  if (reinterpret_cast<uintptr_t>(P.x) % 16 != 0 || (P.M > 1 && P.x_stride % 16 != 0) ||
+      reinterpret_cast<uintptr_t>(P.w) % 16 != 0 || (P.N > 1 && P.w_stride % 16 != 0) ||
+      reinterpret_cast<uintptr_t>(P.y) % 16 != 0)
+    return GDN_ERR_MISALIGNED;
+  if (!grid_fits(tiles_of(P.N, P.M, 128, 64), 256)) return GDN_ERR_BAD_SHAPE;
+  LArgs a = {};
+  a.x = static_cast<const uint8_t*>(P.x);
+  a.xs = P.x_scale;
+  a.w = static_cast<const uint8_t*>(P.w);
+  a.ws = P.w_scale;
+  a.y = P.y;
+  a.xld = P.M > 1 ? P.x_stride : P.K;
+  a.wld = P.N > 1 ? P.w_stride : P.K;
+  a.M = P.M;
+  a.N = P.N;
+  a.K = P.K;
+  a.wsld = P.K / 128;
+  a.xsld = P.group != 0 ? P.K / 128 : 1;
+  a.xstep = P.group != 0 ? 1 : 0;
+  a.y_dtype = P.y_dtype;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (P.y_dtype == GDN_DTYPE_F32) launch_linear<true>(a, s);
+  else launch_linear<false>(a, s);
+  return (int)hipGetLastError();
+}
+
+}  // extern "C"

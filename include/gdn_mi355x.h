@@ -607,6 +607,53 @@ typedef struct GdnFp8LinearParams {
 
 int gdn_fp8_linear_launch(const GdnFp8LinearParams* params, void* stream);
 
+/* A key and value cache in e4m3: k_cache, v_cache [B,S,Hk,D] bytes with a scale
+ * for each row and head, k_scale, v_scale [B,S,Hk] fp32; scale = max|x| / 448 over
+ * the row's D columns and bytes x / scale (in fp32, by the scale that is stored)
+ * rounded to the nearest; a row of zeros has scale 0.
+ *   - write: the T rows k, v [B,T,Hk,D] (dtype) of sequence b become rows
+ *     cache_seqlens[b] - T .. cache_seqlens[b] - 1; those that would lie before
+ *     row 0 are dropped.  Other rows are not touched.
+ *   - read: all S rows into k, v [B,S,Hk,D] (dtype), byte times scale rounded once.
+ *   - decode: q, o [B,T,Hq,D] (fp16 or bf16), T in 1..16; as
+ *     gdn_attn_decode_launch over k_cache k_scale and v_cache v_scale.  P times
+ *     v_scale is rounded to dtype before its product.
+ *   - D in {64, 128}, contiguous; every pointer and (b, row, h) stride but the
+ *     scales' gives 16-byte aligned rows; the scales' strides are any.
+ *     cache_seqlens: device int32, clamped to [0, S] by the kernels; rows from
+ *     there on are never read.  The workspace is the decode's, 256-byte aligned. */
+typedef struct GdnCache8Params {
+  const void* k;            /* write: new rows; read: outputs */
+  const void* v;
+  const void* q;            /* decode only, like o */
+  void* o;
+  void* k_cache;
+  void* v_cache;
+  float* k_scale;
+  float* v_scale;
+  const int32_t* cache_seqlens;
+  void* workspace;          /* gdn_cache8_decode_workspace_size() bytes */
+  int64_t workspace_bytes;
+  int64_t k_stride[3];      /* (b, row, h), in elements */
+  int64_t v_stride[3];
+  int64_t q_stride[3];
+  int64_t o_stride[3];
+  int64_t kc_stride[3];
+  int64_t vc_stride[3];
+  int64_t ks_stride[3];
+  int64_t vs_stride[3];
+  int32_t B, T, S;
+  int32_t Hq, Hk, D;
+  int32_t window, sinks;
+  float scale;
+  int32_t dtype;
+} GdnCache8Params;
+
+int gdn_cache8_write_launch(const GdnCache8Params* params, void* stream);
+int gdn_cache8_read_launch(const GdnCache8Params* params, void* stream);
+int64_t gdn_cache8_decode_workspace_size(const GdnCache8Params* params);
+int gdn_cache8_decode_launch(const GdnCache8Params* params, void* stream);
+
 /* Human-readable text for a status code. */
 const char* gdn_fwd_status_string(int status);
 

@@ -20,6 +20,7 @@ from .ops import (gdn_fwd, gdn_chunk_fwd, auto_block_v, gdn_prep, l2norm,  # noq
 from .scan import gated_scan, gated_scan_bwd  # noqa: F401
 from .attn import window_attn, window_attn_bwd, window_attn_decode  # noqa: F401
 from .norm import add_rms_norm, add_rms_norm_bwd, add_rms_norm_fp8  # noqa: F401
+from .cache import cache_read_fp8, cache_write_fp8, window_attn_decode_fp8  # noqa: F401
 from .linear import fp8_linear, quantize_fp8, quantize_fp8_weight  # noqa: F401
 from .loss import linear_xent, linear_xent_bwd  # noqa: F401
 
@@ -28,4 +29,5 @@ _sys.modules.setdefault("v100_attention_lab_amd", _sys.modules[__name__])
 __all__ = ["gdn_fwd", "gdn_chunk_fwd", "chunk_gated_delta_rule", "gdn_prep", "l2norm",
            "gdn_bwd", "auto_block_v", "gated_scan", "gated_scan_bwd", "add_rms_norm", "add_rms_norm_bwd",
            "add_rms_norm_fp8", "window_attn", "window_attn_bwd", "window_attn_decode",
-           "linear_xent", "linear_xent_bwd", "fp8_linear", "quantize_fp8", "quantize_fp8_weight", "load_library", "status_string"]
+           "linear_xent", "linear_xent_bwd", "fp8_linear", "quantize_fp8", "quantize_fp8_weight",
+           "cache_write_fp8", "cache_read_fp8", "window_attn_decode_fp8", "load_library", "status_string"]

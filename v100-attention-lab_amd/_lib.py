@@ -70,6 +70,10 @@ EXPORTED_SYMBOLS = (
     "gdn_xent_bwd_launch",
     "gdn_fp8_quant_launch",
     "gdn_fp8_linear_launch",
+    "gdn_cache8_write_launch",
+    "gdn_cache8_read_launch",
+    "gdn_cache8_decode_workspace_size",
+    "gdn_cache8_decode_launch",
 )
 
 _I64x2 = ctypes.c_int64 * 2
@@ -244,6 +248,18 @@ class GdnFp8LinearParams(ctypes.Structure):
         ("M N K group y_dtype", ctypes.c_int32))
 
 
+class GdnCache8Params(ctypes.Structure):
+    """Mirror of ``GdnCache8Params`` in include/gdn_mi355x.h."""
+
+    _fields_ = _fields(
+        ("k v q o k_cache v_cache k_scale v_scale cache_seqlens workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
+        ("k_stride v_stride q_stride o_stride kc_stride vc_stride ks_stride vs_stride", _I64x3),
+        ("B T S Hq Hk D window sinks", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("dtype", ctypes.c_int32))
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -289,7 +305,8 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
                              ("norm_bwd", GdnNormParams), ("attn", GdnAttnParams), ("attn_bwd", GdnAttnParams),
                              ("attn_decode", GdnAttnDecodeParams), ("xent", GdnXentParams),
                              ("xent_bwd", GdnXentParams), ("fp8_quant", GdnFp8QuantParams),
-                             ("fp8_linear", GdnFp8LinearParams)):
+                             ("fp8_linear", GdnFp8LinearParams), ("cache8_write", GdnCache8Params),
+                             ("cache8_read", GdnCache8Params), ("cache8_decode", GdnCache8Params)):
             if f"gdn_{name}_workspace_size" in EXPORTED_SYMBOLS:
                 size = getattr(lib, f"gdn_{name}_workspace_size")
                 size.argtypes, size.restype = [ctypes.POINTER(struct)], ctypes.c_int64

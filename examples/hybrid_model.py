@@ -7,13 +7,17 @@ with the residual stream in fp32 between them.
 trains it on synthetic text (a noisy cycle of symbols) and then answers token by
 token, the states and caches going from step to step.
 
-Training runs gated_scan, window_attn, add_rms_norm and chunk_gated_delta_rule
-through autograd; answering runs gated_scan and chunk_gated_delta_rule on one row
-with their states, window_attn_decode over a cache, and, with fp8=True,
-add_rms_norm_fp8 before the projections.
+Training runs gated_scan, window_attn, add_rms_norm, chunk_gated_delta_rule and
+linear_xent (the head and its loss, without the logits) through autograd;
+answering runs gated_scan and chunk_gated_delta_rule on one row with their states,
+window_attn_decode over a cache, and, with fp8=True, add_rms_norm_fp8 before the
+projections.  to_8_bits(model) gives a copy that answers in 8 bits throughout: the
+norms hand e4m3 rows to fp8_linear, what the mixers leave is quantised on the way,
+and the attention's cache is 8-bit (prompts are written and read back in pieces).
 """
 
 import argparse
+import copy
 import importlib
 import os
 import sys
@@ -26,6 +30,21 @@ sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 gdn = importlib.import_module("v100-attention-lab_amd")
 
 DTYPE = torch.bfloat16
+
+
+class Linear8(nn.Module):
+    """A bias-free nn.Linear in e4m3; takes 16-bit rows or (bytes, scales)."""
+
+    def __init__(self, linear):
+        super().__init__()
+        w, s = gdn.quantize_fp8_weight(linear.weight.detach())
+        self.register_buffer("weight", w)
+        self.register_buffer("scale", s)
+        self.in_features, self.out_features = linear.in_features, linear.out_features
+
+    def forward(self, y):
+        x, s = y if isinstance(y, tuple) else gdn.quantize_fp8(y)
+        return gdn.fp8_linear(x, s, self.weight, self.scale, out_dtype=DTYPE)
 
 
 class DeltaRule(nn.Module):
@@ -41,9 +60,10 @@ class DeltaRule(nn.Module):
         return torch.zeros(batch, self.heads, self.dim, self.dim, device=device)
 
     def forward(self, y, state=None, length=None):
-        B, T, _ = y.shape
         n, d = self.heads, self.dim
-        q, k, v, b, g = self.inp(y).split([n * d, n * d, n * d, n, n], -1)
+        qkvbg = self.inp(y)
+        B, T, _ = qkvbg.shape
+        q, k, v, b, g = qkvbg.split([n * d, n * d, n * d, n, n], -1)
         q, k = (F.normalize(x.view(B, T, n, d), dim=-1) for x in (q, k))
         o, state = gdn.chunk_gated_delta_rule(
             q=q, k=k, v=v.reshape(B, T, n, d), g=F.logsigmoid(g.float() + 4), beta=torch.sigmoid(b.float()),
@@ -77,17 +97,32 @@ class WindowAttention(nn.Module):
         self.heads, self.key_heads, self.dim, self.window, self.sinks = heads, key_heads, dim, window, sinks
         self.inp = nn.Linear(width, (heads + 2 * key_heads) * dim, bias=False, dtype=DTYPE)
         self.out = nn.Linear(heads * dim, width, bias=False, dtype=DTYPE)
+        self.eight = False
 
     def start(self, batch, length, device):
+        if self.eight:
+            cache = torch.zeros(2, batch, length, self.key_heads, self.dim, device=device).to(torch.float8_e4m3fn)
+            scales = torch.zeros(2, batch, length, self.key_heads, device=device)
+            return cache[0], cache[1], scales[0], scales[1], torch.zeros(batch, dtype=torch.int32, device=device)
         cache = torch.zeros(2, batch, length, self.key_heads, self.dim, dtype=DTYPE, device=device)
         return cache[0], cache[1], torch.zeros(batch, dtype=torch.int32, device=device)
 
     def forward(self, y, state=None, length=None):
-        B, T, _ = y.shape
-        qkv = self.inp(y).view(B, T, -1, self.dim)
+        qkv = self.inp(y)
+        B, T, _ = qkv.shape
+        qkv = qkv.view(B, T, -1, self.dim)
         q, k, v = qkv.split([self.heads, self.key_heads, self.key_heads], 2)
         if state is None:
             o = gdn.window_attn(q, k, v, self.window, self.sinks)
+        elif self.eight:
+            *cache, n = state
+            n += T
+            gdn.cache_write_fp8(k, v, *cache, n)
+            if T > 16:       # a piece of a prompt: `length` rows with it, the same for all sequences
+                keys, values = gdn.cache_read_fp8(*(c[:, :length] for c in cache))
+                o = gdn.window_attn(q, keys, values, self.window, self.sinks)
+            else:
+                o = gdn.window_attn_decode_fp8(q, *cache, n, self.window, self.sinks)
         else:
             kc, vc, n = state
             rows = n[:, None].long() + torch.arange(T, device=y.device)
@@ -115,20 +150,32 @@ class HybridModel(nn.Module):
     def _norm(self, x, i, r, fp8):
         if not fp8:
             return gdn.add_rms_norm(x, self.norms[i], r)
+        if isinstance(self.head, Linear8):
+            y, scale, r = gdn.add_rms_norm_fp8(x, self.norms[i].detach(), r, group=128)
+            return (y, scale), r
         y, scale, r = gdn.add_rms_norm_fp8(x, self.norms[i].detach(), r)
-        return (y.float() * scale).to(DTYPE), r      # (an 8-bit product would take y and scale)
+        return (y.float() * scale).to(DTYPE), r      # (16-bit products behind 8-bit norms)
 
-    def forward(self, tokens, states=None, fp8=False):
-        """Logits of [B, T] tokens; with states (see start) they are continued in place."""
+    def rows(self, tokens, states=None, fp8=False, length=None):
+        """What the head takes of [B, T] tokens; with states (see start) they are
+        continued in place, to `length` tokens."""
         r = self.embed(tokens)
         x = torch.zeros_like(r, dtype=DTYPE)
         for i, mixer in enumerate(self.mixers):
             y, r = self._norm(x, i, r, fp8)
-            x, state = mixer(y, None if states is None else states[i])
+            x, state = mixer(y, None if states is None else states[i], length)
             if states is not None:
                 states[i] = state
-        y, _ = self._norm(x, len(self.mixers), r, fp8)
-        return self.head(y).float()
+        return self._norm(x, len(self.mixers), r, fp8)[0]
+
+    def forward(self, tokens, states=None, fp8=False, length=None):
+        """Logits of [B, T] tokens (see rows)."""
+        return self.head(self.rows(tokens, states, fp8, length)).float()
+
+    def loss(self, tokens, targets):
+        """Mean cross entropy over the targets that are not negative."""
+        losses = gdn.linear_xent(self.rows(tokens), self.head.weight, targets)
+        return losses.sum() / (targets >= 0).sum()
 
 
 def text(batch, length, vocab, seed, device):
@@ -146,7 +193,7 @@ def train(model, steps, batch=8, length=256, device="cuda", log=None):
     losses = []
     for i in range(steps):
         t = text(batch, length + 1, model.embed.num_embeddings, i, device)
-        loss = F.cross_entropy(model(t[:, :-1]).flatten(0, 1), t[:, 1:].flatten())
+        loss = model.loss(t[:, :-1], t[:, 1:])
         opt.zero_grad()
         loss.backward()
         opt.step()
@@ -170,6 +217,33 @@ def answer(model, tokens, new, fp8=False):
     return torch.cat(out, 1), torch.cat(logits, 1)
 
 
+def to_8_bits(model):
+    """A copy of the model for answering in 8 bits (answer_8_bits)."""
+    model = copy.deepcopy(model).requires_grad_(False)
+    model.head = Linear8(model.head)
+    for m in model.mixers:
+        m.inp, m.out = Linear8(m.inp), Linear8(m.out)
+        if isinstance(m, WindowAttention):
+            m.eight = True
+    return model
+
+
+@torch.no_grad()
+def answer_8_bits(model, tokens, new, piece=64):
+    """As answer, of a model in 8 bits; the prompt is read in pieces."""
+    B, T = tokens.shape
+    states = model.start(B, T + new, tokens.device)
+    out, logits = [tokens], []
+    at = 0
+    while at < T + new - 1:
+        n = min(piece, T - at) if at < T else 1
+        logits.append(model(torch.cat(out, 1)[:, at:at + n], states, True, at + n))
+        at += n
+        if at >= T:
+            out.append(logits[-1][:, -1:].argmax(-1))
+    return torch.cat(out, 1), torch.cat(logits, 1)
+
+
 def main():
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     ap.add_argument("--steps", type=int, default=30)
@@ -180,6 +254,9 @@ def main():
     tokens, _ = answer(model, text(2, 40, 64, 999, "cuda"), 12)
     for row in tokens.tolist():
         print(" ".join(map(str, row[:40])), "->", " ".join(map(str, row[40:])))
+    tokens, _ = answer_8_bits(to_8_bits(model), text(2, 40, 64, 999, "cuda"), 12)
+    for row in tokens.tolist():
+        print("in 8 bits ->", " ".join(map(str, row[40:])))
 
 
 if __name__ == "__main__":

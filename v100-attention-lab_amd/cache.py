@@ -172,7 +172,8 @@ def cache_read_fp8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.
         raise NotImplementedError("cache_read_fp8 has no gradient")
     params = _call("read", (k_cache, v_cache, k_scale, v_scale), dtype,
                    lambda: _read_plan(k_cache, v_cache, k_scale, v_scale, dtype))
-    k, v = (torch.empty(k_cache.shape, dtype=dtype, device=k_cache.device) for _ in range(2))
+    k = torch.empty(k_cache.shape, dtype=dtype, device=k_cache.device)
+    v = torch.empty_like(k)
     P = _bind(params, k_cache, v_cache, k_scale, v_scale)
     P.k, P.v = k.data_ptr(), v.data_ptr()
     status = _launch(_lib.load_library().gdn_cache8_read_launch, P, k_cache.device)

@@ -417,9 +417,10 @@ struct DxPlan {
 };
 DxPlan dx_plan(const GdnXentParams& P) {
   DxPlan d;
-  d.kind = kind_of(P.D, P.N, false);
+  const int rows = std::max(P.N, 1);
+  d.kind = kind_of(P.D, rows, false);
   const int b = d.kind == kBig ? 256 : 128;
-  d.tiles = tiles_of(P.D, P.N, b, b);
+  d.tiles = tiles_of(P.D, rows, b, b);
   const int64_t slabs = piece_of(P) / 64, places = d.kind == kBig ? 256 : 512;
   d.splits = (int)std::max<int64_t>(1, std::min(places / d.tiles, slabs / 8));
   const bool kept = d.splits > 1 || piece_of(P) < P.V;

@@ -16,6 +16,7 @@ BLOCK = 128
 _MAX_STRIDE = 1 << 23
 
 _PLANS = {}
+_QUANT_PLANS = {}
 
 
 def _flat(t):
@@ -34,9 +35,7 @@ def _check_rows(t, name):
         raise ValueError(f"{name}: rows must be 16-byte aligned (data_ptr and stride {t.stride(0)}); call .contiguous()")
 
 
-def _quantize(x, mode, scale_shape, name):
-    if _needs_grad(x):
-        raise NotImplementedError(f"{name} has no gradient")
+def _quant_plan(x, mode, name):
     if not isinstance(x, torch.Tensor) or x.dim() < 1:
         raise ValueError("x must be [..., D]")
     _code(x, "x")
@@ -47,13 +46,37 @@ def _quantize(x, mode, scale_shape, name):
         raise ValueError(f"{name} runs on a ROCm GPU (got {x.device}); there is no CPU path")
     x2 = _flat(x)
     _check_rows(x2, "x")
+    lead = tuple(x.shape[:-1])
+    scale = {_lib.FP8_ROWS: (*lead, 1), _lib.FP8_GROUPS: (*lead, D // BLOCK)}.get(mode)
+    if scale is None:
+        scale = (-(-lead[0] // BLOCK), D // BLOCK)
+    P = _lib.GdnFp8QuantParams()
+    P.x_stride, P.rows, P.D = x2.stride(0), x2.shape[0], D
+    P.x_dtype, P.mode = _DTYPE_CODE[x.dtype], mode
+    return bytes(P), scale
+
+
+def _quantize(x, mode, name):
+    if _needs_grad(x):
+        raise NotImplementedError(f"{name} has no gradient")
+    try:
+        key = (_sig(x), mode, x.data_ptr() & 15)
+        plan = _QUANT_PLANS.get(key)
+    except (AttributeError, TypeError):     # not a tensor: _quant_plan says so
+        key, plan = None, None
+    if plan is None:
+        plan = _quant_plan(x, mode, name)
+        if key is not None:
+            if len(_QUANT_PLANS) >= _PLANS_MAX:
+                _QUANT_PLANS.clear()
+            _QUANT_PLANS[key] = plan
+    params, shape = plan
     q = torch.empty(x.shape, dtype=FP8, device=x.device)
-    scale = torch.empty(scale_shape(x), dtype=torch.float32, device=x.device)
+    scale = torch.empty(shape, dtype=torch.float32, device=x.device)
     if q.numel() > 0:
-        P = _lib.GdnFp8QuantParams()
+        x2 = _flat(x)
+        P = _lib.GdnFp8QuantParams.from_buffer_copy(params)
         P.x, P.q, P.scale = x2.data_ptr(), q.data_ptr(), scale.data_ptr()
-        P.x_stride, P.rows, P.D = x2.stride(0), x2.shape[0], D
-        P.x_dtype, P.mode = _DTYPE_CODE[x.dtype], mode
         status = _launch(_lib.load_library().gdn_fp8_quant_launch, P, x.device)
         if status != 0:
             raise _failed("gdn_fp8_quant_launch", status)
@@ -72,8 +95,7 @@ def quantize_fp8(x: torch.Tensor, *, group: Optional[int] = BLOCK):
     """
     if group not in (None, BLOCK):
         raise ValueError(f"group must be None or {BLOCK}, got {group}")
-    mode = _lib.FP8_ROWS if group is None else _lib.FP8_GROUPS
-    return _quantize(x, mode, lambda t: (*t.shape[:-1], 1 if group is None else t.shape[-1] // BLOCK), "quantize_fp8")
+    return _quantize(x, _lib.FP8_ROWS if group is None else _lib.FP8_GROUPS, "quantize_fp8")
 
 
 def quantize_fp8_weight(weight: torch.Tensor):
@@ -82,8 +104,7 @@ def quantize_fp8_weight(weight: torch.Tensor):
     [ceil(N / 128), K / 128])``."""
     if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
         raise ValueError("weight must be [N, K]")
-    return _quantize(weight, _lib.FP8_BLOCKS, lambda t: (-(-t.shape[0] // BLOCK), t.shape[1] // BLOCK),
-                     "quantize_fp8_weight")
+    return _quantize(weight, _lib.FP8_BLOCKS, "quantize_fp8_weight")
 
 
 def _plan(x, x_scale, weight, weight_scale, out_dtype, lead):

@@ -50,19 +50,21 @@ def _validate(x, weight, target):
     _check_devices(x, weight, target)
 
 
-def _params(x, weight):
-    P = _lib.GdnXentParams()
-    P.N, P.D, P.V = x.shape[0], x.shape[1], weight.shape[0]
-    P.x_stride, P.w_stride = x.stride(0), weight.stride(0)
-    P.dtype = _DTYPE_CODE[x.dtype]
-    return P
-
-
-def _plan(x, weight, backward):
+def _plan(x, weight, target, lse, dloss, backward):
+    _validate(x, weight, target)
+    if backward:
+        for name, t in (("lse", lse), ("dloss", dloss)):
+            if not isinstance(t, torch.Tensor) or t.shape != target.shape or t.dtype != torch.float32:
+                raise ValueError(f"{name} must be float32 {tuple(target.shape)}")
+        _check_devices(x, lse, dloss)
+    x2 = _flat(x)
     if x.numel() > 0:
-        _check_rows(x, "x")
+        _check_rows(x2, "x")
     _check_rows(weight, "weight")
-    P = _params(x, weight)
+    P = _lib.GdnXentParams()
+    P.N, P.D, P.V = x2.shape[0], x2.shape[1], weight.shape[0]
+    P.x_stride, P.w_stride = x2.stride(0), weight.stride(0)
+    P.dtype = _DTYPE_CODE[x.dtype]
     lib = _lib.load_library()
     ws = (lib.gdn_xent_bwd_workspace_size if backward else lib.gdn_xent_workspace_size)(ctypes.byref(P))
     if ws < 0:
@@ -70,35 +72,39 @@ def _plan(x, weight, backward):
     return bytes(P), int(ws)
 
 
-def _cached(plans, key, make):
-    plan = plans.get(key)
+def _planned(plans, x, weight, target, lse=None, dloss=None):
+    """The plan of a signature seen before, or a new one.  (The alignment is of
+    this call's pointers: part of the signature.)"""
+    try:
+        key = (_sig(x), _sig(weight), _sig(target), _sig(lse), _sig(dloss), (x.data_ptr() | weight.data_ptr()) & 15)
+        plan = plans.get(key)
+    except (AttributeError, TypeError):     # not tensors: the checks say which
+        key, plan = None, None
     if plan is None:
-        plan = make()
-        if len(plans) >= _PLANS_MAX:
-            plans.clear()
-        plans[key] = plan
+        plan = _plan(x, weight, target, lse, dloss, plans is _BWD_PLANS)
+        if key is not None:
+            if len(plans) >= _PLANS_MAX:
+                plans.clear()
+            plans[key] = plan
     return plan
 
 
 def _targets(target):
-    return target.to(torch.int64).contiguous().reshape(-1)
+    """As the kernels read them: contiguous int64."""
+    return target if target.dtype == torch.int64 and target.is_contiguous() else target.to(torch.int64).contiguous()
 
 
 def _run(x, weight, target):
-    _validate(x, weight, target)
-    x2 = _flat(x)
-    # (the alignment is of this call's pointers)
-    key = (_sig(x2), _sig(weight), (x2.data_ptr() | weight.data_ptr()) & 15)
-    params, ws_bytes = _cached(_FWD_PLANS, key, lambda: _plan(x2, weight, False))
+    params, ws_bytes = _planned(_FWD_PLANS, x, weight, target)
+    x2, t = _flat(x), _targets(target)
     loss = torch.empty(target.shape, dtype=torch.float32, device=x.device)
     lse = torch.empty_like(loss)
-    ws = x.new_empty(ws_bytes, dtype=torch.uint8)
-    t = _targets(target)
-    P = _lib.GdnXentParams.from_buffer_copy(params)
-    P.x, P.w, P.target = x2.data_ptr(), weight.data_ptr(), t.data_ptr()
-    P.loss, P.lse = loss.data_ptr(), lse.data_ptr()
-    P.workspace, P.workspace_bytes = ws.data_ptr(), ws_bytes
-    if loss.numel() > 0:
+    if t.numel() > 0:
+        ws = x.new_empty(ws_bytes, dtype=torch.uint8)
+        P = _lib.GdnXentParams.from_buffer_copy(params)
+        P.x, P.w, P.target = x2.data_ptr(), weight.data_ptr(), t.data_ptr()
+        P.loss, P.lse = loss.data_ptr(), lse.data_ptr()
+        P.workspace, P.workspace_bytes = ws.data_ptr(), ws_bytes
         status = _launch(_lib.load_library().gdn_xent_launch, P, x.device)
         if status != 0:
             raise _failed("gdn_xent_launch", status)
@@ -133,26 +139,19 @@ def linear_xent(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, *, 
 
 
 def _run_bwd(x, weight, target, lse, dloss):
-    _validate(x, weight, target)
-    for name, t in (("lse", lse), ("dloss", dloss)):
-        if not isinstance(t, torch.Tensor) or t.shape != target.shape or t.dtype != torch.float32:
-            raise ValueError(f"{name} must be float32 {tuple(target.shape)}")
-    _check_devices(x, lse, dloss)
+    params, ws_bytes = _planned(_BWD_PLANS, x, weight, target, lse, dloss)
     dx, dw = _like(x), _like(weight)
     if target.numel() == 0:
         return dx, dw.zero_()
-    x2 = _flat(x)
+    x2, t, l = _flat(x), _targets(target), lse.contiguous()
     # one value for all rows, as a sum or mean hands it over, is read with a stride of 0
-    d = dloss.reshape(-1) if all(s == 0 for s, n in zip(dloss.stride(), dloss.shape) if n > 1) else \
-        dloss.contiguous().reshape(-1)
-    step = 0 if d.numel() == 1 else d.stride(0)
-    key = (_sig(x2), _sig(weight), (x2.data_ptr() | weight.data_ptr()) & 15)
-    params, ws_bytes = _cached(_BWD_PLANS, key, lambda: _plan(x2, weight, True))
-    t, l = _targets(target), lse.contiguous()
+    step = 0
+    if any(s != 0 for s, n in zip(dloss.stride(), dloss.shape) if n > 1):
+        dloss, step = dloss.contiguous(), 1
     ws = x.new_empty(ws_bytes, dtype=torch.uint8)
     P = _lib.GdnXentParams.from_buffer_copy(params)
     P.x, P.w, P.target = x2.data_ptr(), weight.data_ptr(), t.data_ptr()
-    P.lse, P.dloss, P.dloss_stride = l.data_ptr(), d.data_ptr(), step
+    P.lse, P.dloss, P.dloss_stride = l.data_ptr(), dloss.data_ptr(), step
     P.dx, P.dw = dx.data_ptr(), dw.data_ptr()
     P.workspace, P.workspace_bytes = ws.data_ptr(), ws_bytes
     status = _launch(_lib.load_library().gdn_xent_bwd_launch, P, x.device)

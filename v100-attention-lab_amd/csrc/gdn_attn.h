@@ -111,6 +111,7 @@ __device__ __forceinline__ int acc_row(int r, int half) { return 8 * (r >> 2) + 
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+typedef __attribute__((address_space(3))) float lds_f32;
 
 // LDS byte address of a shared array.
 __device__ __forceinline__ uint32_t lds_addr(const void* p) { return (uint32_t)(uintptr_t)(lds_void*)p; }
@@ -128,6 +129,11 @@ __device__ __forceinline__ void dma16(const void* src, uint32_t at) {
 __device__ __forceinline__ void dma16(const void* base, uint32_t ofs, uint32_t at) {
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(ofs), "s"(base), "s"(at)
                : "memory", "m0");
+}
+// 4 bytes per lane from global memory to LDS at `at` + 4 * lane (dma16's rules).
+__device__ __forceinline__ void dma4(const void* src, uint32_t at) {
+  at = __builtin_amdgcn_readfirstlane(at);
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(at) : "memory", "m0");
 }
 // Every load of this wave so far, from memory and from LDS, is done.
 __device__ __forceinline__ void dma_wait() {

@@ -210,12 +210,6 @@ __device__ __forceinline__ int64_t own_part(const BArgs& a, int unit, const Seq&
   return first + seq * a.sink_blocks + block;
 }
 
-// 4 bytes per lane from global memory to LDS at `at` + 4 * lane.
-__device__ __forceinline__ void dma4(const void* src, uint32_t at) {
-  at = __builtin_amdgcn_readfirstlane(at);
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(at) : "memory", "m0");
-}
-
 template <typename T, int D, int QH>
 __global__ __launch_bounds__(256 * QH, D == 64 && QH == 1 ? 3 : 2) void kv_kernel(const BArgs a) {
   constexpr int kQT = 32 * QH, kKVT = 256 * QH;     // query rows a tile, threads

@@ -129,13 +129,7 @@ constexpr int kMaxSplits = 64;
 
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
-typedef __attribute__((address_space(3))) float lds_f32;
 typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
-
-// 4 bytes per lane from global memory to LDS at `at` + 4 * lane (dma16's rules).
-__device__ __forceinline__ void dma4(const void* src, uint32_t at) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(at) : "memory", "m0");
-}
 
 // 4 bytes of e4m3 as two pairs of the operands' type.
 template <typename T>

@@ -170,32 +170,40 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(const LArgs a) {
 // tiles
 // ---------------------------------------------------------------------------
 
-// MT x NT products of 16 x 16 a wave, WM x WN waves.
+// MT x NT products of 16 x 16 a wave, WM x WN waves.  A stage holds the slabs of
+// both operands, a scale for each of the BN rows and one for each 128 outputs.
 template <int MT_, int NT_, int WM_, int WN_>
 struct Shape8 {
   static constexpr int MT = MT_, NT = NT_, WM = WM_, WN = WN_;
   static constexpr int BM = 16 * MT * WM, BN = 16 * NT * WN, kWaves = WM * WN, kThreads = 64 * kWaves;
-  static constexpr uint32_t kA = kSlab * BM, kB = kSlab * BN, kStage = kA + kB, kLds = 2 * kStage;
+  static constexpr uint32_t kA = kSlab * BM, kB = kSlab * BN, kScales = 4 * BN + 256;
+  static constexpr uint32_t kStage = kA + kB + kScales, kLds = 2 * kStage;
+  static_assert(MT % 4 == 0 && BN / 64 < kWaves, "4 operands in turn; a wave for each 64 rows' scales and one more");
 };
 typedef Shape8<8, 4, 2, 4> Big8;     // 256 outputs x 256 rows, one workgroup a CU
 typedef Shape8<4, 4, 2, 2> Mid8;     // 128 x 128, two
 typedef Shape8<4, 2, 2, 2> Low8;     // 128 x 64, three
 
-// Operand of a block: row 16 i + l % 16 from the wave's first, 32 bytes that lane
-// part l / 16 of both operands agrees on.
+// Operand of a block: row 16 i + l % 16 from the wave's first, and of it the pieces
+// l / 16 and l / 16 + 4 (any two, as long as both operands have the same; these leave
+// the banks free of conflicts, pieces 2 (l / 16) and 2 (l / 16) + 1 took twice as long).
 struct Read8 {
   uint32_t ofs;
   __device__ __forceinline__ Read8(int lane, int first) {
     const int r = lane & 15;      // (first: a multiple of 16)
-    ofs = (uint32_t)(first + r) * kSlab + 16 * ((2 * (lane >> 4)) ^ ((r >> 1) & 7));
+    ofs = (uint32_t)(first + r) * kSlab + 16 * ((lane >> 4) ^ ((r >> 1) & 7));
   }
   __device__ __forceinline__ i32x8 operator()(uint32_t tile, int i) const {
     const u32x4 a = *(const lds_u32x4*)(tile + ofs + 16 * kSlab * i);
-    const u32x4 b = *(const lds_u32x4*)(tile + (ofs ^ 16) + 16 * kSlab * i);
+    const u32x4 b = *(const lds_u32x4*)(tile + (ofs ^ 64) + 16 * kSlab * i);
     return i32x8{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
   }
 };
 
+// The operands of 4 rows of products are in registers at a time, read up to 3 rows
+// ahead.  The barrier of a slab stands before its last two rows, which go column by
+// column: the next slab's operands are read beside them, each column's over the one
+// that has just been used.
 template <typename S, bool EXACT>
 __global__ __launch_bounds__(S::kThreads) void tile_kernel(const LArgs a) {
   __shared__ __attribute__((aligned(1024))) uint8_t mem[S::kLds];
@@ -207,80 +215,76 @@ __global__ __launch_bounds__(S::kThreads) void tile_kernel(const LArgs a) {
   const PlainCopy<S::BM, S::kWaves> ca(a.w, a.wld, t.m * S::BM, a.N, a.K);
   const PlainCopy<S::BN, S::kWaves> cb(a.x, a.xld, t.n * S::BN, a.M, a.K);
   const Read8 ra(lane, 16 * MT * wm), rb(lane, 16 * NT * wn);
+  // wave w < BN / 64 brings the scales of rows 64 w .., the next one those of the outputs
+  const bool rows = wv < S::BN / 64;
+  const float* sp = rows ? a.xs + (int64_t)min(t.n * S::BN + 64 * wv + lane, a.M - 1) * a.xsld
+                         : a.ws + (int64_t)min(t.m * S::BM / 128 + lane, (a.N - 1) / 128) * a.wsld;
+  const int step = rows ? a.xstep : 1;
   auto copy = [&](int k, uint32_t at) {
+    if (wv <= S::BN / 64) dma4(sp + k * step, at + S::kA + S::kB + 256 * wv);
     ca.copy(k, at);
     cb.copy(k, at + S::kA);
   };
-  // scales: the lane's rows, and (the same for the wave) its 128 outputs
-  const auto* xs = (const __attribute__((address_space(1))) float*)(uintptr_t)uniform64(
-      (int64_t)(uintptr_t)(a.xs + (int64_t)t.n * S::BN * a.xsld));
-  uint32_t xofs[NT];
-#pragma unroll
-  for (int j = 0; j < NT; ++j)
-    xofs[j] = (uint32_t)min(16 * (NT * wn + j) + l16, a.M - 1 - t.n * S::BN) * (uint32_t)a.xsld;
-  const auto* ws = (const __attribute__((address_space(4))) float*)(uintptr_t)uniform64(
-      (int64_t)(uintptr_t)(a.ws + (int64_t)min((t.m * S::BM + 16 * MT * wm) / 128, (a.N - 1) / 128) * a.wsld));
+  const uint32_t sx = S::kA + S::kB + 4 * (16 * NT * wn + l16), sw = S::kA + S::kB + 4 * S::BN + 4 * (16 * MT * wm / 128);
   const int slabs = a.K / 128;
   f32x4 acc[MT][NT] = {};
-  float sx[NT], nx[NT], sw = ws[0], nw = 0.f;
-#pragma unroll
-  for (int j = 0; j < NT; ++j) sx[j] = xs[xofs[j]];
   copy(0, lds);
   dma_wait();
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
-  auto next_scales = [&](int k) {
-    const int b = min(k, slabs - 1);
-    nw = ws[b];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) nx[j] = (xs + b * a.xstep)[xofs[j]];
-  };
-  next_scales(1);
   if (slabs > 1) copy(1, lds + S::kStage);
-  i32x8 fb[NT], fa[2];
+  i32x8 fb[NT], fa[4];
+  float f[NT], x[NT], w;
+  auto scales = [&](uint32_t stage) {
+    w = *(const lds_f32*)(stage + sw);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) x[j] = *(const lds_f32*)(stage + sx + 64 * j);
+  };
+  scales(lds);
 #pragma unroll
   for (int j = 0; j < NT; ++j) fb[j] = rb(lds + S::kA, j);
   fa[0] = ra(lds, 0);
+  fa[1] = ra(lds, 1);
   for (int k = 0; k < slabs; ++k) {
     const uint32_t here = lds + (k & 1) * S::kStage, other = lds + ((k & 1) ^ 1) * S::kStage;
-    float f[NT];
 #pragma unroll
-    for (int j = 0; j < NT; ++j) f[j] = sx[j] * sw;
-    // a product enters its sum right before the next one of its column starts
-    f32x4 p[NT];
-    auto add = [&](int i, int j) {
+    for (int j = 0; j < NT; ++j) f[j] = x[j] * w;
+    // a product enters its sum when the fourth one behind it starts (or with the
+    // slab's last)
+    f32x4 p[4];
+    auto row = [](int e) { return e < (MT - 2) * NT ? e / NT : MT - 2 + ((e - (MT - 2) * NT) & 1); };
+    auto col = [](int e) { return e < (MT - 2) * NT ? e % NT : (e - (MT - 2) * NT) >> 1; };
+    auto add = [&](int e) {
+      const int i = row(e), j = col(e);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(p[j][r], f[j], acc[i][j][r]);
+      for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(p[e & 3][r], f[j], acc[i][j][r]);
       asm volatile("" : "+v"(acc[i][j]));     // (here, not at the slab's end with all products kept)
     };
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      if (i + 1 < MT) fa[(i + 1) & 1] = ra(here, i + 1);
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        if (i > 0) add(i - 1, j);
-        p[j] = mfma128<EXACT>(fa[i & 1], fb[j]);
-        __builtin_amdgcn_sched_barrier(0);
+    for (int e = 0; e < MT * NT; ++e) {
+      const int i = row(e), j = col(e);
+      if (e == (MT - 2) * NT) {
+        // every operand of this slab is in registers, and the next slab in LDS
+        dma_wait();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (k + 2 < slabs) copy(k + 2, here);
       }
+      if (e >= 4) add(e - 4);
+      p[e & 3] = mfma128<EXACT>(fa[i & 3], fb[j]);
+      if (i < MT - 2) {
+        if (e == 0) fa[2] = ra(here, 2);
+        if (j == (e < NT ? NT - 1 : 0) && i + 3 < MT) fa[(i + 3) & 3] = ra(here, i + 3);
+      } else if (i == MT - 1) {
+        // (behind the last slab from the other stage, for nobody)
+        fb[j] = rb(other + S::kA, j);
+        if (j == 0) scales(other);
+        if (j < 2) fa[j] = ra(other, j);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
-    // every operand of this slab is in registers, and the next slab in LDS
-    dma_wait();
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
 #pragma unroll
-    for (int j = 0; j < NT; ++j) sx[j] = nx[j];
-    sw = nw;
-#pragma unroll
-    for (int j = 0; j < NT; ++j) asm volatile("" : "+v"(sx[j]));
-    next_scales(k + 2);
-    if (k + 2 < slabs) copy(k + 2, here);
-    // (behind the last slab from the other stage, for nobody)
-#pragma unroll
-    for (int j = 0; j < NT; ++j) fb[j] = rb(other + S::kA, j);
-    fa[0] = ra(other, 0);
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int j = 0; j < NT; ++j) add(MT - 1, j);
+    for (int e = MT * NT - 4; e < MT * NT; ++e) add(e);
   }
 #pragma unroll
   for (int j = 0; j < NT; ++j) {

@@ -21,10 +21,12 @@ namespace gdn {
 namespace gemm {
 
 using attn::dma16;
+using attn::dma4;
 using attn::dma_wait;
 using attn::f32x16;
 using attn::lds_addr;
 using attn::lds_s16x4;
+using attn::lds_f32;
 using attn::lds_u32x4;
 using attn::s16x4;
 using attn::u32x4;

@@ -145,38 +145,38 @@ __global__ __launch_bounds__(S::kThreads) void fwd_kernel(const Args a) {
   a.part[(int64_t)t.m * a.N + n] = make_float2(m, s);
 }
 
-// lse and loss: 16 rows a workgroup, 16 threads a row.
-constexpr int kJoin = 256;
+// (maximum, sum) pairs of parts of the vocabulary.
+__device__ __forceinline__ float2 join(float2 a, float2 b) {
+  const float top = fmaxf(a.x, b.x);
+  // (a sum is 0, or NaN, only where all logits are -inf or NaN)
+  if (top == -__builtin_inff()) return make_float2(top, a.y + b.y);
+  return make_float2(top, a.y * (a.x == top ? 1.f : exp2_fast(a.x - top)) + b.y * (b.x == top ? 1.f : exp2_fast(b.x - top)));
+}
+
+// lse and loss: 16 rows a workgroup, 64 threads a row (one of 4 in each wave).
+constexpr int kJoin = 1024;
 __global__ __launch_bounds__(kJoin) void join_kernel(const Args a) {
   const int c = threadIdx.x & 15, g = threadIdx.x >> 4;
   const int n = blockIdx.x * 16 + c;
-  float m = -__builtin_inff(), s = 0.f;
-  auto add = [&](float2 p) {
-    // a part's sum is 0 only where all its logits are -inf
-    const float top = fmaxf(m, p.x);
-    if (top == -__builtin_inff()) {
-      s += p.y;      // (0, or NaN)
-      return;
-    }
-    s = s * (m == top ? 1.f : exp2_fast(m - top)) + p.y * (p.x == top ? 1.f : exp2_fast(p.x - top));
-    m = top;
-  };
+  float2 p = make_float2(-__builtin_inff(), 0.f);
   if (n < a.N) {
 #pragma unroll 4
-    for (int t = g; t < a.tm; t += 16) add(a.part[(int64_t)t * a.N + n]);
+    for (int t = g; t < a.tm; t += kJoin / 16) p = join(p, a.part[(int64_t)t * a.N + n]);
   }
-  __shared__ float2 all[16][16];
-  all[g][c] = make_float2(m, s);
+#pragma unroll
+  for (int o = 16; o <= 32; o *= 2) p = join(p, make_float2(__shfl_xor(p.x, o, 64), __shfl_xor(p.y, o, 64)));
+  __shared__ float2 all[kJoin / 64][16];
+  if ((threadIdx.x & 63) < 16) all[threadIdx.x >> 6][c] = p;
   __syncthreads();
   if (g != 0 || n >= a.N) return;
 #pragma unroll
-  for (int k = 1; k < 16; ++k) add(all[k][c]);
+  for (int k = 1; k < kJoin / 64; ++k) p = join(p, all[k][c]);
   const int64_t t = a.target[n];
   const bool counts = t >= 0 && t < a.V;
-  const float lse = (m + __builtin_amdgcn_logf(s)) * kLn2;
+  const float lse = (p.x + __builtin_amdgcn_logf(p.y)) * kLn2;
   a.lse[n] = counts ? lse : 0.f;
+  a.loss[n] = 0.f;
   if (counts) a.loss[n] = lse - a.hit[n];
-  else a.loss[n] = 0.f;
 }
 
 // ---------------------------------------------------------------------------
@@ -190,25 +190,26 @@ __device__ __forceinline__ bool row_counts(const Args& a, int n) {
 
 // What the pieces need of each row, and the unit of G (every workgroup finds it
 // for itself).
+constexpr int kRowsNT = 256;
 template <bool UNIT>
-__global__ __launch_bounds__(kJoin) void rows_kernel(const Args a) {
+__global__ __launch_bounds__(kRowsNT) void rows_kernel(const Args a) {
   float unit = 1.f;
   if constexpr (UNIT) {
     float top = 0.f;
-    for (int n = threadIdx.x; n < a.N; n += kJoin)
+    for (int n = threadIdx.x; n < a.N; n += kRowsNT)
       if (row_counts(a, n)) top = fmaxf(top, fabsf(a.dloss[n * a.dloss_step]));
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-    __shared__ float tops[kJoin / 64];
+    __shared__ float tops[kRowsNT / 64];
     if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kJoin / 64; ++w) top = fmaxf(top, tops[w]);
+    for (int w = 0; w < kRowsNT / 64; ++w) top = fmaxf(top, tops[w]);
     if (top > 0.f && top < __builtin_inff()) unit = ldexpf(1.f, max(-100, min(100, 13 - ilogbf(top))));
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) *a.unit = 1.f / unit;
   const int all = (a.N + 255) / 256 * 256;
-  for (int n = blockIdx.x * kJoin + threadIdx.x; n < all; n += gridDim.x * kJoin) {
+  for (int n = blockIdx.x * kRowsNT + threadIdx.x; n < all; n += gridDim.x * kRowsNT) {
     const bool c = row_counts(a, n);
     Row r = {0.f, 0.f};
     if (c) r = Row{a.lse[n] * kLog2e, a.dloss[n * a.dloss_step] * unit};
@@ -494,8 +495,8 @@ int launch_bwd(Args a, const GdnXentParams& P, hipStream_t s) {
   const DxPlan d = dx_plan(P);
   const int piece = piece_of(P);
   a.ldg = piece;
-  const int blocks = std::min<int>((a.N + kJoin - 1) / kJoin, 256);
-  hipLaunchKernelGGL((rows_kernel<std::is_same<T, f16>::value>), dim3(blocks), dim3(kJoin), 0, s, a);
+  const int blocks = std::min<int>((a.N + kRowsNT - 1) / kRowsNT, 256);
+  hipLaunchKernelGGL((rows_kernel<std::is_same<T, f16>::value>), dim3(blocks), dim3(kRowsNT), 0, s, a);
   for (int v = 0; v < a.V; v += piece) {
     a.v0 = v;
     a.vn = std::min(piece, a.V - v);

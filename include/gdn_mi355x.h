@@ -539,8 +539,8 @@ int gdn_attn_decode_launch(const GdnAttnDecodeParams* params, void* stream);
  *     multiple of 8 (at least 8); strides at most 2^22 elements.  target: int64.
  *   - lse: written by the forward, read by the backward; dloss: fp32 with a
  *     stride (0: one value for all rows); dx, dw: dense, dtype.
- *   - N, V up to 2^28; workspaces of gdn_xent[_bwd]_workspace_size() bytes,
- *     256-byte aligned. */
+ *   - N below 2^26, V up to 2^28; workspaces of gdn_xent[_bwd]_workspace_size()
+ *     bytes, 256-byte aligned. */
 typedef struct GdnXentParams {
   const void* x;
   const void* w;
@@ -591,7 +591,8 @@ int gdn_fp8_quant_launch(const GdnFp8QuantParams* params, void* stream);
  *     apart, K a multiple of 128; y [M,N] dense, 16-byte aligned, any dtype.
  *   - x_scale dense [M, K / 128] (group 128) or [M] (group 0); w_scale dense
  *     [ceil(N / 128), K / 128].
- *   - M, N up to 2^28. */
+ *   - M, N up to 2^28; GDN_ERR_BAD_SHAPE from 2^32 threads a launch on: 512 for each
+ *     16 outputs of up to 32 rows, else 256 for each 128 outputs of 64 rows. */
 typedef struct GdnFp8LinearParams {
   const void* x;
   const float* x_scale;

@@ -58,8 +58,8 @@ def _xent(L, **kw):
 
 
 XENT = [(dict(x=None), 1001), (dict(w=None), 1001), (dict(target=None), 1001), (dict(lse=None), 1001),
-        (dict(N=-1), 1002), (dict(V=0), 1002), (dict(D=0), 1002), (dict(N=1 << 29), 1002), (dict(V=1 << 29), 1002),
-        (dict(N=1 << 28, V=1 << 28), 1002), (dict(D=12), 1003), (dict(x_stride=1 << 23), 1003), (dict(w_stride=-256), 1003),
+        (dict(N=-1), 1002), (dict(V=0), 1002), (dict(D=0), 1002), (dict(N=1 << 26), 1002), (dict(V=1 << 29), 1002),
+        (dict(N=(1 << 26) - 1, V=1 << 28), 1002), (dict(D=12), 1003), (dict(x_stride=1 << 23), 1003), (dict(w_stride=-256), 1003),
         (dict(dtype=0), 1005), (dict(x=FAKE + 8), 1004), (dict(w_stride=260), 1004),
         (dict(workspace=None), 1006), (dict(workspace=FAKE + 16), 1006), (dict(workspace_bytes=100), 1006)]
 
@@ -83,13 +83,14 @@ def test_xent_sizes(lib, pkg):
     assert lib.gdn_xent_launch(None, None) == 1001 and lib.gdn_xent_bwd_launch(None, None) == 1001
     # 8 bytes a row and at least 128 words; never the logits
     assert fwd(N=8192, V=128000) <= 8192 * (1000 * 8 + 4) + 1024
-    # G of a piece, and fp32 sums of dx in a part for each share of the card that is empty
+    # G of a piece, and fp32 sums of dx and of a piece of dw in a part for each share of
+    # the card that is empty
     for N, D, V in ((8192, 4096, 128000), (100, 64, 50), (1, 8, 1), (1 << 20, 2048, 32000), (65536, 64, 1000)):
         rows = -(-N // 256) * 256
         size = bwd(N=N, D=D, V=V, x_stride=D, w_stride=D)
         g = max(128 << 20, rows * 256 * 2)
         parts = 4 * (-(-N // 256) * 256) * (-(-D // 256) * 256)
-        assert 0 < size <= g + rows * 16 + 1024 + max(parts, 4 * 512 * 128 * 128)
+        assert 0 < size <= g + rows * 16 + 1024 + max(parts, 4 * 512 * 128 * 128) + 4 * 512 * 128 * 128
 
 
 def _quant(L, **kw):
@@ -111,7 +112,7 @@ def _linear(L, **kw):
 
 @pytest.mark.parametrize("kw,code", [
     (dict(x=None), 1001), (dict(x_scale=None), 1001), (dict(w=None), 1001), (dict(w_scale=None), 1001), (dict(y=None), 1001),
-    (dict(M=-1), 1002), (dict(N=0), 1002), (dict(K=0), 1002), (dict(M=1 << 29), 1002), (dict(M=1 << 28, N=1 << 28), 1002),
+    (dict(M=-1), 1002), (dict(N=0), 1002), (dict(K=0), 1002), (dict(M=1 << 29), 1002), (dict(M=1 << 28, N=1 << 28), 1002), (dict(M=1, N=1 << 28), 1002),
     (dict(K=200), 1003), (dict(group=64), 1003), (dict(x_stride=1 << 24), 1003), (dict(w_stride=-128), 1003),
     (dict(y_dtype=8), 1005), (dict(x=FAKE + 8), 1004), (dict(w_stride=264), 1004), (dict(y=FAKE + 8), 1004)])
 def test_linear_refusals(lib, pkg, kw, code):

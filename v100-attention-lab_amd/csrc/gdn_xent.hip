@@ -58,7 +58,7 @@ struct Args {
   uint64_t* live;          // a bit for each row that counts
   float* unit;             // 1 / unit of G
   uint16_t* g;             // [N up to 256][ldg]
-  float4* dxp;             // sums of dX, in the order of the accumulators
+  float4* sums;            // of dX, or of dW's parts, in the order of the accumulators
   int ldg;
   int v0, vn;              // the piece: first of V, how many
   int tm, tn, splits, first, last;
@@ -220,6 +220,36 @@ __global__ __launch_bounds__(kRowsNT) void rows_kernel(const Args a) {
   }
 }
 
+// Columns 32 j .. of a wave's tile, times f, as rows n0 .. of `out` (ld elements
+// apart, below `rows`), columns m0 .. (below `cols`, a multiple of 8).  A lane has 4
+// neighbouring M of one row: they go through the wave's own share of LDS, so that the
+// rows leave in whole lines (8-byte stores of 32 rows at a time: 2.5 times as long
+// where the sums are short).
+template <typename T, typename S>
+__device__ __forceinline__ void store_columns(const f32x16 (&acc)[S::MT][S::NT], int j, float f, uint8_t* lds, void* out,
+                                              int64_t ld, int n0, int rows, int m0, int cols) {
+  using O = Ops<T>;
+  constexpr int kRow = 64 * S::MT, kPitch = kRow + 16, kLanes = kRow / 16;      // bytes; lanes a row
+  static_assert(32 * kPitch * S::kWaves <= (int)S::kLds, "a share for every wave");
+  const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
+  uint8_t* mine = lds + (threadIdx.x >> 6) * 32 * kPitch;
+#pragma unroll
+  for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      *reinterpret_cast<uint2*>(mine + l32 * kPitch + 64 * i + 16 * q + 8 * half) =
+          make_uint2(O::pack(acc[i][j][4 * q] * f, acc[i][j][4 * q + 1] * f),
+                     O::pack(acc[i][j][4 * q + 2] * f, acc[i][j][4 * q + 3] * f));
+  const int col = m0 + lane % kLanes * 8;
+#pragma unroll
+  for (int i = 0; i < 32 * kLanes / 64; ++i) {
+    const int r = lane / kLanes + i * (64 / kLanes);
+    const uint4 v = *reinterpret_cast<const uint4*>(mine + r * kPitch + lane % kLanes * 16);
+    if (n0 + r < rows && col < cols)
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + (int64_t)(n0 + r) * ld + col) = v;
+  }
+}
+
 // G of a tile of the piece.
 template <typename T, typename S>
 __global__ __launch_bounds__(S::kThreads) void grad_kernel(const Args a) {
@@ -258,21 +288,8 @@ __global__ __launch_bounds__(S::kThreads) void grad_kernel(const Args a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[i][j][r] = 32 * i + attn::acc_row(r, half) < left ? acc[i][j][r] : 0.f;
     }
-    uint16_t* g = a.g + (int64_t)n * a.ldg + v0 + 4 * half;
-#pragma unroll
-    for (int i = 0; i < S::MT; ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<uint2*>(g + 32 * i + 8 * q) =
-            make_uint2(O::pack(acc[i][j][4 * q], acc[i][j][4 * q + 1]), O::pack(acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]));
+    store_columns<T, S>(acc, j, 1.f, lds, a.g, a.ldg, t.n * S::BN + 32 * (S::NT * wn + j), 1 << 30, v0, a.ldg);
   }
-}
-
-// 4 neighbouring columns from 4 sums.
-template <typename T>
-__device__ __forceinline__ void store4(uint16_t* row, int col, int cols, float4 v, float f) {
-  if (col < cols)      // (cols: a multiple of 8)
-    *reinterpret_cast<uint2*>(row + col) = make_uint2(Ops<T>::pack(v.x * f, v.y * f), Ops<T>::pack(v.z * f, v.w * f));
 }
 
 // dX += G W over the piece, M the columns of X.
@@ -281,7 +298,7 @@ __global__ __launch_bounds__(S::kThreads) void dx_kernel(const Args a) {
   __shared__ __attribute__((aligned(1024))) uint8_t lds[S::kLds];
   const uint32_t tiles = a.tm * a.tn, split = blockIdx.x / tiles;
   const TileAt t(blockIdx.x % tiles, a.tm, a.tn);
-  const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
+  const int lane = threadIdx.x & 63;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wv % S::WM, wn = wv / S::WM;
   const int slabs = (a.vn + 63) / 64, per = (slabs + a.splits - 1) / a.splits;
   const int s0 = min((int)split * per, slabs), s1 = min(s0 + per, slabs);
@@ -297,54 +314,66 @@ __global__ __launch_bounds__(S::kThreads) void dx_kernel(const Args a) {
     });
   }
   const bool whole = a.last && a.splits == 1;
-  const float f = whole ? *a.unit : 1.f;
-  float4* sums = a.dxp + (int64_t)(blockIdx.x / tiles * tiles + t.m * a.tn + t.n) * (S::BM * S::BN / 4) + threadIdx.x;
+  float4* sums = a.sums + (int64_t)(blockIdx.x / tiles * tiles + t.m * a.tn + t.n) * (S::BM * S::BN / 4) + threadIdx.x;
+  if (!a.first || !whole) {
 #pragma unroll
-  for (int j = 0; j < S::NT; ++j) {
-    const int n = t.n * S::BN + 32 * (S::NT * wn + j) + l32;
-    uint16_t* row = (uint16_t*)a.dx + (int64_t)n * a.D;
+    for (int j = 0; j < S::NT; ++j)
 #pragma unroll
-    for (int i = 0; i < S::MT; ++i)
+      for (int i = 0; i < S::MT; ++i)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        float4 v = make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
-        float4* at = sums + ((j * S::MT + i) * 4 + q) * S::kThreads;
-        if (!a.first) {
-          const float4 o = *at;
-          v = make_float4(v.x + o.x, v.y + o.y, v.z + o.z, v.w + o.w);
+        for (int q = 0; q < 4; ++q) {
+          float4* at = sums + ((j * S::MT + i) * 4 + q) * S::kThreads;
+          if (!a.first) {
+            const float4 o = *at;
+            acc[i][j][4 * q] += o.x;
+            acc[i][j][4 * q + 1] += o.y;
+            acc[i][j][4 * q + 2] += o.z;
+            acc[i][j][4 * q + 3] += o.w;
+          }
+          if (!whole)
+            *at = make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
         }
-        if (!whole) *at = v;
-        else if (n < a.N) store4<T>(row, t.m * S::BM + 32 * (S::MT * wm + i) + 8 * q + 4 * half, a.D, v, f);
-      }
+  }
+  if (whole) {
+#pragma unroll
+    for (int j = 0; j < S::NT; ++j)
+      store_columns<T, S>(acc, j, *a.unit, lds, a.dx, a.D, t.n * S::BN + 32 * (S::NT * wn + j), a.N,
+                          t.m * S::BM + 32 * S::MT * wm, a.D);
   }
 }
 
-// The parts of dX, added in order.
+// Parts of dX or of a piece of dW (`rows` rows of D), added in order.
 template <typename T, typename S>
-__global__ __launch_bounds__(S::kThreads) void dx_join_kernel(const Args a) {
+__global__ __launch_bounds__(S::kThreads) void parts_kernel(const Args a, uint16_t* out, int rows) {
   constexpr int kPer = S::MT * S::NT * 4;
   const uint32_t tile = blockIdx.x / kPer, e = blockIdx.x % kPer, tiles = a.tm * a.tn;
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, wm = wv % S::WM, wn = wv / S::WM;
   const int q = e % 4, i = e / 4 % S::MT, j = e / 4 / S::MT;
   const int m = tile / a.tn * S::BM + 32 * (S::MT * wm + i) + 8 * q + 4 * (lane >> 5);
   const int n = tile % a.tn * S::BN + 32 * (S::NT * wn + j) + (lane & 31);
-  const float4* p = a.dxp + ((int64_t)tile * kPer + e) * S::kThreads + threadIdx.x;
+  const float4* p = a.sums + ((int64_t)tile * kPer + e) * S::kThreads + threadIdx.x;
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
   for (int s = 0; s < a.splits; ++s) {
     const float4 o = p[(int64_t)s * tiles * kPer * S::kThreads];
     v = make_float4(v.x + o.x, v.y + o.y, v.z + o.z, v.w + o.w);
   }
-  if (n < a.N) store4<T>((uint16_t*)a.dx + (int64_t)n * a.D, m, a.D, v, *a.unit);
+  const float f = *a.unit;
+  if (n < rows && m < a.D)      // (D: a multiple of 8)
+    *reinterpret_cast<uint2*>(out + (int64_t)n * a.D + m) =
+        make_uint2(Ops<T>::pack(v.x * f, v.y * f), Ops<T>::pack(v.z * f, v.w * f));
 }
 
 // dW of the piece = G^T X, M the columns of X, N the vocabulary.
 template <typename T, typename S>
 __global__ __launch_bounds__(S::kThreads) void dw_kernel(const Args a) {
   __shared__ __attribute__((aligned(1024))) uint8_t lds[S::kLds];
-  const TileAt t(blockIdx.x, a.tm, a.tn);
-  const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
+  const uint32_t tiles = a.tm * a.tn, split = blockIdx.x / tiles;
+  const TileAt t(blockIdx.x % tiles, a.tm, a.tn);
+  const int lane = threadIdx.x & 63;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wv % S::WM, wn = wv / S::WM;
+  const int slabs = (a.N + 63) / 64, per = (slabs + a.splits - 1) / a.splits;
+  const int s0 = min((int)split * per, slabs), s1 = min(s0 + per, slabs);
   f32x16 acc[S::MT][S::NT] = {};
   {
     const TurnedCopy<S::BM, S::kWaves> ca(a.x, a.xld, t.m * S::BM, a.D);
@@ -353,28 +382,30 @@ __global__ __launch_bounds__(S::kThreads) void dw_kernel(const Args a) {
     const TurnedRead<S::BN> rb(lane, 32 * S::NT * wn);
     // a row that does not count may hold anything; which do is read a slab ahead
     const auto* live = (const __attribute__((address_space(4))) uint64_t*)(uintptr_t)uniform64((int64_t)(uintptr_t)a.live);
-    const int slabs = (a.N + 63) / 64;
-    uint64_t now = live[0];
-    product16<T, S>(acc, slabs, lds_addr(lds), ra, rb, [&](int k, uint32_t at) {
+    uint64_t now = live[min(s0, slabs - 1)];
+    product16<T, S>(acc, s1 - s0, lds_addr(lds), ra, rb, [&](int k, uint32_t at) {
       const uint64_t rows = now;
-      now = live[min(k + 1, slabs - 1)];
-      ca.copy(k, at, rows);
-      cb.copy(k, at + S::kA, ~0ull);
+      now = live[min(s0 + k + 1, slabs - 1)];
+      ca.copy(s0 + k, at, rows);
+      cb.copy(s0 + k, at + S::kA, ~0ull);
     });
   }
-  const float f = *a.unit;
+  if (a.splits > 1) {
+    float4* sums = a.sums + (int64_t)(blockIdx.x / tiles * tiles + t.m * a.tn + t.n) * (S::BM * S::BN / 4) + threadIdx.x;
 #pragma unroll
-  for (int j = 0; j < S::NT; ++j) {
-    const int v = t.n * S::BN + 32 * (S::NT * wn + j) + l32;
-    uint16_t* row = (uint16_t*)a.dw + (int64_t)(a.v0 + v) * a.D;
-    if (v < a.vn)
+    for (int j = 0; j < S::NT; ++j)
 #pragma unroll
       for (int i = 0; i < S::MT; ++i)
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-          store4<T>(row, t.m * S::BM + 32 * (S::MT * wm + i) + 8 * q + 4 * half, a.D,
-                    make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]), f);
+          sums[((j * S::MT + i) * 4 + q) * S::kThreads] =
+              make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
+    return;
   }
+#pragma unroll
+  for (int j = 0; j < S::NT; ++j)
+    store_columns<T, S>(acc, j, *a.unit, lds, (uint16_t*)a.dw + (int64_t)a.v0 * a.D, a.D,
+                        t.n * S::BN + 32 * (S::NT * wn + j), a.vn, t.m * S::BM + 32 * S::MT * wm, a.D);
 }
 
 // ---------------------------------------------------------------------------
@@ -392,7 +423,7 @@ int check(const GdnXentParams& P) {
   if ((P.N > 1 && (P.x_stride < 0 || P.x_stride > 1 << 22)) || (P.V > 1 && (P.w_stride < 0 || P.w_stride > 1 << 22)) ||
       P.D > 1 << 22)
     return GDN_ERR_UNSUPPORTED;
-  if (P.N > 1 << 28 || P.V > 1 << 28) return GDN_ERR_BAD_SHAPE;
+  if (P.N >= 1 << 26 || P.V > 1 << 28) return GDN_ERR_BAD_SHAPE;      // (the join has 64 threads a row)
   return GDN_OK;
 }
 
@@ -410,27 +441,30 @@ int piece_of(const GdnXentParams& P) {
   return (int)std::min(most, ceil_to(P.V, 256));
 }
 
-// Parts of a piece's vocabulary for dX.
-struct DxPlan {
+// A gradient's product of m columns and n rows over k: shape, parts of its
+// contraction where its tiles do not fill the card, and fp32 sums that it keeps.
+struct GradPlan {
   Kind kind;
   int splits;
   int64_t tiles, floats;
+  GradPlan(int64_t m, int64_t n, int64_t k, bool kept) {
+    kind = kind_of(m, n, false);
+    const int b = kind == kBig ? 256 : 128;
+    tiles = tiles_of(m, n, b, b);
+    const int64_t slabs = (k + 63) / 64, places = kind == kBig ? 256 : 512;
+    splits = (int)std::max<int64_t>(1, std::min(places / tiles, slabs / 8));
+    floats = kept || splits > 1 ? tiles * splits * b * b : 0;
+  }
 };
-DxPlan dx_plan(const GdnXentParams& P) {
-  DxPlan d;
-  const int rows = std::max(P.N, 1);
-  d.kind = kind_of(P.D, rows, false);
-  const int b = d.kind == kBig ? 256 : 128;
-  d.tiles = tiles_of(P.D, rows, b, b);
-  const int64_t slabs = piece_of(P) / 64, places = d.kind == kBig ? 256 : 512;
-  d.splits = (int)std::max<int64_t>(1, std::min(places / d.tiles, slabs / 8));
-  const bool kept = d.splits > 1 || piece_of(P) < P.V;
-  d.floats = kept ? d.tiles * d.splits * b * b : 0;
-  return d;
+// dX: rows of X, the contraction is the piece's vocabulary; kept from piece to piece.
+GradPlan dx_plan(const GdnXentParams& P) {
+  return GradPlan(P.D, std::max(P.N, 1), piece_of(P), piece_of(P) < P.V);
 }
+// dW of a piece: rows of its vocabulary, the contraction is X's rows.
+GradPlan dw_plan(const GdnXentParams& P, int vn) { return GradPlan(P.D, vn, std::max(P.N, 1), false); }
 
 struct BwdLayout {
-  int64_t rows, tgt, live, unit, g, dx, bytes;
+  int64_t rows, tgt, live, unit, g, dx, dw, bytes;
   explicit BwdLayout(const GdnXentParams& P) {
     const int64_t n = ceil_to(std::max(P.N, 1), 256);
     rows = 0;
@@ -439,7 +473,10 @@ struct BwdLayout {
     unit = ceil_to(live + n / 8, 256);
     g = unit + 256;
     dx = g + n * piece_of(P) * 2;
-    bytes = dx + dx_plan(P).floats * 4;
+    dw = dx + dx_plan(P).floats * 4;
+    // (the last piece may be cut into more parts than the others)
+    const int piece = piece_of(P), last = P.V - (P.V - 1) / piece * piece;
+    bytes = dw + 4 * std::max(dw_plan(P, std::min(piece, P.V)).floats, dw_plan(P, last).floats);
   }
 };
 
@@ -491,31 +528,40 @@ int launch_fwd(Args a, Kind kind, hipStream_t s) {
 }
 
 template <typename T>
-int launch_bwd(Args a, const GdnXentParams& P, hipStream_t s) {
-  const DxPlan d = dx_plan(P);
+int launch_bwd(Args a, const GdnXentParams& P, const BwdLayout& l, hipStream_t s) {
+  char* ws = static_cast<char*>(P.workspace);
+  const GradPlan dx = dx_plan(P);
   const int piece = piece_of(P);
   a.ldg = piece;
   const int blocks = std::min<int>((a.N + kRowsNT - 1) / kRowsNT, 256);
   hipLaunchKernelGGL((rows_kernel<std::is_same<T, f16>::value>), dim3(blocks), dim3(kRowsNT), 0, s, a);
-  for (int v = 0; v < a.V; v += piece) {
-    a.v0 = v;
-    a.vn = std::min(piece, a.V - v);
+  auto parts = [&](const GradPlan& p, void* out, int rows) {
+    const uint32_t grid = (uint32_t)(p.tiles * (p.kind == kBig ? 32 : 16));
+    if (p.kind == kBig) hipLaunchKernelGGL((parts_kernel<T, Big>), dim3(grid), dim3(Big::kThreads), 0, s, a, (uint16_t*)out, rows);
+    else hipLaunchKernelGGL((parts_kernel<T, Mid>), dim3(grid), dim3(Mid::kThreads), 0, s, a, (uint16_t*)out, rows);
+  };
+  for (int64_t v = 0; v < a.V; v += piece) {
+    a.v0 = (int)v;
+    a.vn = std::min(piece, a.V - a.v0);
     a.first = v == 0;
     a.last = v + piece >= a.V;
-    a.splits = 1;
     const Kind kl = kind_of(a.vn, a.N, true);
     set_tiles(a, kl, a.vn, a.N);
     const uint32_t grid = (uint32_t)a.tm * a.tn;
     if (kl == kNarrow) hipLaunchKernelGGL((grad_kernel<T, Narrow>), dim3(grid), dim3(Narrow::kThreads), 0, s, a);
     else GDN_XENT_BY_KIND(grad_kernel, T, kl, grid, s, a);
-    const Kind kw = kind_of(a.D, a.vn, false);
-    set_tiles(a, kw, a.D, a.vn);
-    GDN_XENT_BY_KIND(dw_kernel, T, kw, (uint32_t)a.tm * a.tn, s, a);
-    set_tiles(a, d.kind, a.D, a.N);
-    a.splits = d.splits;
-    GDN_XENT_BY_KIND(dx_kernel, T, d.kind, (uint32_t)(d.tiles * d.splits), s, a);
+    const GradPlan dw = dw_plan(P, a.vn);
+    set_tiles(a, dw.kind, a.D, a.vn);
+    a.splits = dw.splits;
+    a.sums = reinterpret_cast<float4*>(ws + l.dw);
+    GDN_XENT_BY_KIND(dw_kernel, T, dw.kind, (uint32_t)(dw.tiles * dw.splits), s, a);
+    if (dw.splits > 1) parts(dw, (uint16_t*)a.dw + v * a.D, a.vn);
+    set_tiles(a, dx.kind, a.D, a.N);
+    a.splits = dx.splits;
+    a.sums = reinterpret_cast<float4*>(ws + l.dx);
+    GDN_XENT_BY_KIND(dx_kernel, T, dx.kind, (uint32_t)(dx.tiles * dx.splits), s, a);
   }
-  if (d.splits > 1) GDN_XENT_BY_KIND(dx_join_kernel, T, d.kind, (uint32_t)(d.tiles * (d.kind == kBig ? 32 : 16)), s, a);
+  if (dx.splits > 1) parts(dx, a.dx, a.N);
   return (int)hipGetLastError();
 }
 
@@ -583,9 +629,8 @@ int gdn_xent_bwd_launch(const GdnXentParams* prm, void* stream) {
   a.live = reinterpret_cast<uint64_t*>(ws + l.live);
   a.unit = reinterpret_cast<float*>(ws + l.unit);
   a.g = reinterpret_cast<uint16_t*>(ws + l.g);
-  a.dxp = reinterpret_cast<float4*>(ws + l.dx);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  return P.dtype == GDN_DTYPE_F16 ? launch_bwd<f16>(a, P, s) : launch_bwd<bf16_t>(a, P, s);
+  return P.dtype == GDN_DTYPE_F16 ? launch_bwd<f16>(a, P, l, s) : launch_bwd<bf16_t>(a, P, l, s);
 }
 
 }  // extern "C"

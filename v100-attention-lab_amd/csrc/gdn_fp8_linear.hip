@@ -11,7 +11,7 @@
 // about 1.4e-5 of a result of normally distributed terms, under what 16-bit results
 // show and far under e4m3's own steps.  fp32 results are made of the same bytes as
 // fp16 operands instead, whose products are summed in fp32, at less than half the rate.
-//   - up to 64 rows: the weight is read once from memory straight into the
+//   - up to 32 rows: the weight is read once from memory straight into the
 //     operands' registers, the contraction dealt to the waves of a workgroup,
 //     whose sums are joined in LDS in order;
 //   - more: tiles through LDS (gdn_gemm.h), a slab being one block of 128.
@@ -94,35 +94,32 @@ __device__ __forceinline__ void store_y(const LArgs& a, int64_t m, int n, const 
 
 constexpr int kFewWaves = 8;
 
-// 16 NA outputs of up to 16 NB rows; wave w takes blocks w, w + 8, ...  Lane l
-// holds row l % 16 of an operand, bytes 32 (l / 16) .. + 31 of the block.
-template <int NA, int NB, bool EXACT>
+// 16 outputs of up to 16 NB rows; wave w takes blocks w, w + 8, ...  Lane l holds row
+// l % 16 of an operand, bytes 32 (l / 16) .. + 31 of the block.
+template <int NB, bool EXACT>
 __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(const LArgs a) {
   const int lane = threadIdx.x & 63, l16 = lane & 15, part = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int n0 = blockIdx.x * 16 * NA, m0 = blockIdx.y * 16 * NB;
-  const uint8_t *w[NA], *x[NB];
+  const int n0 = blockIdx.x * 16;
+  const uint8_t* w = a.w + (int64_t)min(n0 + l16, a.N - 1) * a.wld + 32 * part;
+  const uint8_t* x[NB];
   const float* xs[NB];
 #pragma unroll
-  for (int i = 0; i < NA; ++i) w[i] = a.w + (int64_t)min(n0 + 16 * i + l16, a.N - 1) * a.wld + 32 * part;
-#pragma unroll
   for (int j = 0; j < NB; ++j) {
-    const int64_t m = min(m0 + 16 * j + l16, a.M - 1);
+    const int64_t m = min(16 * j + l16, a.M - 1);
     x[j] = a.x + m * a.xld + 32 * part;
     xs[j] = a.xs + m * a.xsld;
   }
   const float* ws = a.ws + (int64_t)(n0 / 128) * a.wsld;
-  f32x4 acc[NA][NB] = {};
+  f32x4 acc[NB] = {};
   const int blocks = a.K / 128;
   struct Block {
-    uint4 w[NA][2], x[NB][2];
+    uint4 w[2], x[NB][2];
     float xs[NB], ws;
   };
   auto load = [&](Block& f, int b) {
 #pragma unroll
-    for (int i = 0; i < NA; ++i)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) f.w[i][h] = *reinterpret_cast<const uint4*>(w[i] + (int64_t)b * 128 + 16 * h);
+    for (int h = 0; h < 2; ++h) f.w[h] = *reinterpret_cast<const uint4*>(w + (int64_t)b * 128 + 16 * h);
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
 #pragma unroll
@@ -135,12 +132,9 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(const LArgs a) {
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
       const float s = f.xs[j] * f.ws;
+      const f32x4 p = mfma128<EXACT>(join16(f.w[0], f.w[1]), join16(f.x[j][0], f.x[j][1]));
 #pragma unroll
-      for (int i = 0; i < NA; ++i) {
-        const f32x4 p = mfma128<EXACT>(join16(f.w[i][0], f.w[i][1]), join16(f.x[j][0], f.x[j][1]));
-#pragma unroll
-        for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(p[r], s, acc[i][j][r]);
-      }
+      for (int r = 0; r < 4; ++r) acc[j][r] = __builtin_fmaf(p[r], s, acc[j][r]);
     }
   };
   for (int b = wv; b < blocks; b += 2 * kFewWaves) {
@@ -151,18 +145,16 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(const LArgs a) {
     use(f[0]);
     if (two) use(f[1]);
   }
-  __shared__ f32x4 sums[kFewWaves][NA * NB][64];
+  __shared__ f32x4 sums[kFewWaves][NB][64];
 #pragma unroll
-  for (int i = 0; i < NA; ++i)
-#pragma unroll
-    for (int j = 0; j < NB; ++j) sums[wv][i * NB + j][lane] = acc[i][j];
+  for (int j = 0; j < NB; ++j) sums[wv][j][lane] = acc[j];
   __syncthreads();
-  for (int e = wv; e < NA * NB; e += kFewWaves) {
-    f32x4 v = sums[0][e][lane];
+  for (int j = wv; j < NB; j += kFewWaves) {
+    f32x4 v = sums[0][j][lane];
 #pragma unroll
-    for (int k = 1; k < kFewWaves; ++k) v += sums[k][e][lane];
-    const int m = m0 + 16 * (e % NB) + l16;
-    if (m < a.M) store_y(a, m, n0 + 16 * (e / NB) + 4 * part, v);
+    for (int k = 1; k < kFewWaves; ++k) v += sums[k][j][lane];
+    const int m = 16 * j + l16;
+    if (m < a.M) store_y(a, m, n0 + 4 * part, v);
   }
 }
 
@@ -170,19 +162,24 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(const LArgs a) {
 // tiles
 // ---------------------------------------------------------------------------
 
-// MT x NT products of 16 x 16 a wave, WM x WN waves.  A stage holds the slabs of
-// both operands, a scale for each of the BN rows and one for each 128 outputs.
-template <int MT_, int NT_, int WM_, int WN_>
+// MT x NT products of 16 x 16 a wave, WM x WN waves, STAGES slabs in LDS; GROUPS of
+// such waves take every GROUPS-th slab each.  A stage holds the slabs of both operands
+// and a line of 64 scales from each wave: of 64 rows each, then of the tile's
+// 128-output blocks.
+template <int MT_, int NT_, int WM_, int WN_, int STAGES_, int GROUPS_ = 1>
 struct Shape8 {
-  static constexpr int MT = MT_, NT = NT_, WM = WM_, WN = WN_;
-  static constexpr int BM = 16 * MT * WM, BN = 16 * NT * WN, kWaves = WM * WN, kThreads = 64 * kWaves;
-  static constexpr uint32_t kA = kSlab * BM, kB = kSlab * BN, kScales = 4 * BN + 256;
-  static constexpr uint32_t kStage = kA + kB + kScales, kLds = 2 * kStage;
+  static constexpr int MT = MT_, NT = NT_, WM = WM_, WN = WN_, kStages = STAGES_, kGroups = GROUPS_;
+  static constexpr int BM = 16 * MT * WM, BN = 16 * NT * WN, kWaves = WM * WN, kThreads = 64 * kWaves * kGroups;
+  static constexpr uint32_t kA = kSlab * BM, kB = kSlab * BN, kStage = kA + kB + 256 * kWaves, kRing = kStages * kStage;
+  static constexpr uint32_t kLds = kGroups * kRing;
+  static constexpr int kCopies = (kA + kB) / 1024 / kWaves + 1;       // of a wave for a slab
   static_assert(MT % 4 == 0 && BN / 64 < kWaves, "4 operands in turn; a wave for each 64 rows' scales and one more");
 };
-typedef Shape8<8, 4, 2, 4> Big8;     // 256 outputs x 256 rows, one workgroup a CU
-typedef Shape8<4, 4, 2, 2> Mid8;     // 128 x 128, two
-typedef Shape8<4, 2, 2, 2> Low8;     // 128 x 64, three
+typedef Shape8<8, 4, 2, 4, 2> Big8;      // 256 outputs x 256 rows, one workgroup a CU
+typedef Shape8<4, 4, 2, 2, 2> Mid8;      // 128 x 128, two
+typedef Shape8<4, 2, 2, 2, 2> Low8;      // 128 x 64, three
+typedef Shape8<4, 2, 2, 2, 3, 2> Low8x2; // the same, one: two groups that share the contraction
+typedef Shape8<4, 1, 1, 4, 2, 4> Tiny8;  // 64 x 64, one: four groups
 
 // Operand of a block: row 16 i + l % 16 from the wave's first, and of it the pieces
 // l / 16 and l / 16 + 4 (any two, as long as both operands have the same; these leave
@@ -200,6 +197,42 @@ struct Read8 {
   }
 };
 
+// Rows m0 .. m0 + 15, columns n0 .. of a wave's tile (products 16 j .. + 15 of its
+// rows).  A lane has 4 neighbouring columns of one row: they go through the wave's own
+// share of LDS, so that rows leave in whole lines.
+template <typename E, typename S>
+__device__ __forceinline__ void store_rows(const f32x4 (&acc)[S::MT][S::NT], int j, const LArgs& a, uint8_t* mem, int m0,
+                                           int n0) {
+  constexpr int kCols = 16 * S::MT, kPitch = kCols * (int)sizeof(E) + 16, kPer = 16 / (int)sizeof(E);
+  static_assert(16 * kPitch * S::kWaves <= (int)S::kLds, "a share for every wave");
+  const int lane = threadIdx.x & 63;
+  uint8_t* mine = mem + (threadIdx.x >> 6) * 16 * kPitch;
+#pragma unroll
+  for (int i = 0; i < S::MT; ++i) {
+    Pack<E, 4> p;
+    const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+    p.set(v);
+    p.store(reinterpret_cast<E*>(mine + (lane & 15) * kPitch) + 16 * i + 4 * (lane >> 4));
+  }
+  E* y = static_cast<E*>(a.y) + (int64_t)m0 * a.N + n0;
+  const int rows = a.M - m0, cols = a.N - n0;
+  if (a.N % kPer == 0) {
+    constexpr int kLanes = kCols / kPer;      // a row
+#pragma unroll
+    for (int i = 0; i < 16 * kLanes / 64; ++i) {
+      const int r = lane / kLanes + i * (64 / kLanes), c = lane % kLanes * kPer;
+      const uint4 v = *reinterpret_cast<const uint4*>(mine + r * kPitch + c * (int)sizeof(E));
+      if (r < rows && c < cols) *reinterpret_cast<uint4*>(y + (int64_t)r * a.N + c) = v;
+    }
+  } else {
+    for (int e = lane; e < 16 * kCols; e += 64) {
+      const int r = e / kCols, c = e % kCols;
+      const E v = reinterpret_cast<const E*>(mine + r * kPitch)[c];
+      if (r < rows && c < cols) y[(int64_t)r * a.N + c] = v;
+    }
+  }
+}
+
 // The operands of 4 rows of products are in registers at a time, read up to 3 rows
 // ahead.  The barrier of a slab stands before its last two rows, which go column by
 // column: the next slab's operands are read beside them, each column's over the one
@@ -210,29 +243,33 @@ __global__ __launch_bounds__(S::kThreads) void tile_kernel(const LArgs a) {
   constexpr int MT = S::MT, NT = S::NT;
   const TileAt t(blockIdx.x, a.tm, a.tn);
   const int lane = threadIdx.x & 63, l16 = lane & 15;
-  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wv % S::WM, wn = wv / S::WM;
-  const uint32_t lds = lds_addr(mem);
+  const int group = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) / S::kWaves);
+  const int wv = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) % S::kWaves), wm = wv % S::WM, wn = wv / S::WM;
+  const uint32_t lds = lds_addr(mem) + group * S::kRing;
   const PlainCopy<S::BM, S::kWaves> ca(a.w, a.wld, t.m * S::BM, a.N, a.K);
   const PlainCopy<S::BN, S::kWaves> cb(a.x, a.xld, t.n * S::BN, a.M, a.K);
   const Read8 ra(lane, 16 * MT * wm), rb(lane, 16 * NT * wn);
-  // wave w < BN / 64 brings the scales of rows 64 w .., the next one those of the outputs
+  // wave w < BN / 64 brings the scales of rows 64 w .., the others those of the outputs
   const bool rows = wv < S::BN / 64;
   const float* sp = rows ? a.xs + (int64_t)min(t.n * S::BN + 64 * wv + lane, a.M - 1) * a.xsld
                          : a.ws + (int64_t)min(t.m * S::BM / 128 + lane, (a.N - 1) / 128) * a.wsld;
   const int step = rows ? a.xstep : 1;
+  // the group's k-th slab (the last ones again where the groups' shares differ)
+  const int all = a.K / 128, slabs = (all + S::kGroups - 1) / S::kGroups;
   auto copy = [&](int k, uint32_t at) {
-    if (wv <= S::BN / 64) dma4(sp + k * step, at + S::kA + S::kB + 256 * wv);
-    ca.copy(k, at);
-    cb.copy(k, at + S::kA);
+    const int b = min(k * S::kGroups + group, all - 1);
+    dma4(sp + b * step, at + S::kA + S::kB + 256 * wv);
+    ca.copy(b, at);
+    cb.copy(b, at + S::kA);
   };
   const uint32_t sx = S::kA + S::kB + 4 * (16 * NT * wn + l16), sw = S::kA + S::kB + 4 * S::BN + 4 * (16 * MT * wm / 128);
-  const int slabs = a.K / 128;
+  constexpr int ST = S::kStages;
   f32x4 acc[MT][NT] = {};
-  copy(0, lds);
-  dma_wait();
+  for (int k = 0; k < ST && k < slabs; ++k) copy(k, lds + k * S::kStage);
+  if (slabs >= ST) dma_wait_but<(ST - 1) * S::kCopies>();
+  else dma_wait();
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
-  if (slabs > 1) copy(1, lds + S::kStage);
   i32x8 fb[NT], fa[4];
   float f[NT], x[NT], w;
   auto scales = [&](uint32_t stage) {
@@ -245,10 +282,12 @@ __global__ __launch_bounds__(S::kThreads) void tile_kernel(const LArgs a) {
   for (int j = 0; j < NT; ++j) fb[j] = rb(lds + S::kA, j);
   fa[0] = ra(lds, 0);
   fa[1] = ra(lds, 1);
+  uint32_t here = lds;
   for (int k = 0; k < slabs; ++k) {
-    const uint32_t here = lds + (k & 1) * S::kStage, other = lds + ((k & 1) ^ 1) * S::kStage;
+    const uint32_t other = here + S::kStage < lds + S::kRing ? here + S::kStage : lds;
+    const bool ours = S::kGroups == 1 || k * S::kGroups + group < all;
 #pragma unroll
-    for (int j = 0; j < NT; ++j) f[j] = x[j] * w;
+    for (int j = 0; j < NT; ++j) f[j] = ours ? x[j] * w : 0.f;
     // a product enters its sum when the fourth one behind it starts (or with the
     // slab's last)
     f32x4 p[4];
@@ -265,10 +304,11 @@ __global__ __launch_bounds__(S::kThreads) void tile_kernel(const LArgs a) {
       const int i = row(e), j = col(e);
       if (e == (MT - 2) * NT) {
         // every operand of this slab is in registers, and the next slab in LDS
-        dma_wait();
+        if (k + ST <= slabs) dma_wait_but<(ST - 2) * S::kCopies>();
+        else dma_wait();
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (k + 2 < slabs) copy(k + 2, here);
+        if (k + ST < slabs) copy(k + ST, here);
       }
       if (e >= 4) add(e - 4);
       p[e & 3] = mfma128<EXACT>(fa[i & 3], fb[j]);
@@ -279,19 +319,43 @@ __global__ __launch_bounds__(S::kThreads) void tile_kernel(const LArgs a) {
         // (behind the last slab from the other stage, for nobody)
         fb[j] = rb(other + S::kA, j);
         if (j == 0) scales(other);
-        if (j < 2) fa[j] = ra(other, j);
+        if (j == 0) fa[0] = ra(other, 0);
+        if (j == std::min(1, NT - 1)) fa[1] = ra(other, 1);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
     for (int e = MT * NT - 4; e < MT * NT; ++e) add(e);
+    here = other;
+  }
+  __syncthreads();      // (LDS is free)
+  if constexpr (S::kGroups > 1) {
+    // the groups' sums, added in order (behind the places that the rows go through)
+    constexpr int kRows = S::kWaves * 16 * (64 * MT + 16);
+    static_assert(kRows + (S::kGroups - 1) * S::BM * S::BN * 4 <= (int)S::kLds, "room for both");
+    f32x4* sums = reinterpret_cast<f32x4*>(mem + kRows) + wv * 64 + lane;
+    if (group > 0) {
+#pragma unroll
+      for (int e = 0; e < MT * NT; ++e)
+        sums[((group - 1) * MT * NT + e) * S::kWaves * 64] = acc[e / NT][e % NT];
+    }
+    __syncthreads();
+    if (group > 0) return;
+#pragma unroll
+    for (int g = 1; g < S::kGroups; ++g)
+#pragma unroll
+      for (int e = 0; e < MT * NT; ++e) acc[e / NT][e % NT] += sums[((g - 1) * MT * NT + e) * S::kWaves * 64];
   }
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
-    const int m = t.n * S::BN + 16 * (NT * wn + j) + l16;
-    if (m < a.M)
-#pragma unroll
-      for (int i = 0; i < MT; ++i) store_y(a, m, t.m * S::BM + 16 * (MT * wm + i) + 4 * (lane >> 4), acc[i][j]);
+    const int m0 = t.n * S::BN + 16 * (NT * wn + j), n0 = t.m * S::BM + 16 * MT * wm;
+    if (a.y_dtype == GDN_DTYPE_F32) {
+      if constexpr (EXACT) store_rows<float, S>(acc, j, a, mem, m0, n0);
+    } else if (a.y_dtype == GDN_DTYPE_F16) {
+      store_rows<f16, S>(acc, j, a, mem, m0, n0);
+    } else {
+      store_rows<bf16_t, S>(acc, j, a, mem, m0, n0);
+    }
   }
 }
 
@@ -408,21 +472,31 @@ void launch_tiles(LArgs& a, hipStream_t s) {
   a.tn = (a.M + S::BN - 1) / S::BN;
   hipLaunchKernelGGL((tile_kernel<S, EXACT>), dim3((uint32_t)a.tm * a.tn), dim3(S::kThreads), 0, s, a);
 }
-template <int NA, int NB, bool EXACT>
+template <int NB, bool EXACT>
 void launch_few(const LArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL((few_kernel<NA, NB, EXACT>), dim3((a.N + 16 * NA - 1) / (16 * NA), (a.M + 16 * NB - 1) / (16 * NB)),
-                     dim3(64 * kFewWaves), 0, s, a);
+  hipLaunchKernelGGL((few_kernel<NB, EXACT>), dim3((a.N + 15) / 16), dim3(64 * kFewWaves), 0, s, a);
 }
 
+// Which kernel (us in a graph, rows x K x N, 16-bit results):
+//   - up to 32 rows the weight goes straight into registers (1 x 4096 x 11008 10.8, by
+//     tiles 12.8; 17 x 4096 x 8192 12.7 either way; 40 x 4096 x 8192 15.2 and 13.4);
+//   - up to 256 tiles of 64 x 64 (a CU each) four groups share the contraction
+//     (256 x 2048 x 2048 7.0, Low8x2 8.9), up to 256 tiles of 128 x 64 two (512 x 4096
+//     x 4096 16.5, Low8 22.3, Tiny8 24.4);
+//   - then larger tiles as they fill the card: 256 x 256 from 192 of them (3000 x 2048 x
+//     4096 34.5, Mid8 34.7; 4096 x 4096 x 4096 70.5 and 78.8), 128 x 128 from 256 (1024 x
+//     2048 x 6176 21.3, Low8 27.4) unless few outputs leave it to the reading of x
+//     (34486 x 2304 x 77 Low8 22.1, Mid8 25.3).
 template <bool EXACT>
 void launch_linear(LArgs& a, hipStream_t s) {
-  if (a.M <= 16) return launch_few<1, 1, EXACT>(a, s);
-  if (a.M <= 32) return launch_few<1, 2, EXACT>(a, s);
-  if (a.M <= 64) return launch_few<2, 4, EXACT>(a, s);
+  if (a.M <= 16) return launch_few<1, EXACT>(a, s);
+  if (a.M <= 32) return launch_few<2, EXACT>(a, s);
+  if (tiles_of(a.N, a.M, 64, 64) <= 256) return launch_tiles<Tiny8, EXACT>(a, s);
+  if (tiles_of(a.N, a.M, 128, 64) <= 256) return launch_tiles<Low8x2, EXACT>(a, s);
   if constexpr (!EXACT) {
     if (tiles_of(a.N, a.M, 256, 256) >= 192) return launch_tiles<Big8, EXACT>(a, s);
   }
-  if (tiles_of(a.N, a.M, 128, 128) >= 256) return launch_tiles<Mid8, EXACT>(a, s);
+  if (a.N > 128 && tiles_of(a.N, a.M, 128, 128) >= 256) return launch_tiles<Mid8, EXACT>(a, s);
   launch_tiles<Low8, EXACT>(a, s);
 }
 
@@ -490,7 +564,8 @@ int gdn_fp8_linear_launch(const GdnFp8LinearParams* prm, void* stream) {
       reinterpret_cast<uintptr_t>(P.w) % 16 != 0 || (P.N > 1 && P.w_stride % 16 != 0) ||
       reinterpret_cast<uintptr_t>(P.y) % 16 != 0)
     return GDN_ERR_MISALIGNED;
-  if (!grid_fits(tiles_of(P.N, P.M, 128, 64), 256)) return GDN_ERR_BAD_SHAPE;
+  if (!(P.M <= 32 ? grid_fits((P.N + 15) / 16, 64 * kFewWaves) : grid_fits(tiles_of(P.N, P.M, 128, 64), 256)))
+    return GDN_ERR_BAD_SHAPE;
   LArgs a = {};
   a.x = static_cast<const uint8_t*>(P.x);
   a.xs = P.x_scale;

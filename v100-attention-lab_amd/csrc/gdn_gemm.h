@@ -64,7 +64,7 @@ struct PlainCopy {
   uint32_t wave;
   __device__ __forceinline__ PlainCopy(const void* p, int64_t ld, int row0, int rows, int bytes_) : bytes(bytes_) {
     const int lane = threadIdx.x & 63;
-    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    wave = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) % WAVES);
     base = uniform_bytes((const uint8_t*)p + (int64_t)row0 * ld);
     const int r = (int)wave * 8 + lane / 8;
     piece = (lane % 8) ^ ((r >> 1) & 7);     // (8 WAVES rows further on: the same)
@@ -164,6 +164,14 @@ struct TurnedRead {
     return u.v;
   }
 };
+
+// All but the last N loads of this wave from memory, and all from LDS, are done.
+template <int N>
+__device__ __forceinline__ void dma_wait_but() {
+  static_assert(N < 64, "6 bits");
+  __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | ((N >> 4) << 14));
+  asm volatile("" ::: "memory");
+}
 
 // acc += A B^T over `slabs` slabs of 16-bit elements.  copy(slab, at): the
 // workgroup's copies of both operands of a slab to `at`; every thread of the

@@ -35,12 +35,13 @@ typedef __attribute__((address_space(3))) uint8_t lds_u8;
 
 constexpr int kSlab = 128;      // bytes of a row of a slab
 
-// MT x NT products of 32 x 32 a wave, WM x WN waves.
-template <int MT_, int NT_, int WM_, int WN_>
+// MT x NT products of 32 x 32 a wave, WM x WN waves, STAGES slabs in LDS.
+template <int MT_, int NT_, int WM_, int WN_, int STAGES_ = 2>
 struct Shape {
-  static constexpr int MT = MT_, NT = NT_, WM = WM_, WN = WN_;
+  static constexpr int MT = MT_, NT = NT_, WM = WM_, WN = WN_, kStages = STAGES_;
   static constexpr int BM = 32 * MT * WM, BN = 32 * NT * WN, kWaves = WM * WN, kThreads = 64 * kWaves;
-  static constexpr uint32_t kA = kSlab * BM, kB = kSlab * BN, kStage = kA + kB, kLds = 2 * kStage;
+  static constexpr uint32_t kA = kSlab * BM, kB = kSlab * BN, kStage = kA + kB, kLds = kStages * kStage;
+  static constexpr int kCopies = kStage / 1024 / kWaves;      // of a wave for a slab
 };
 
 // What copies read where an operand has no row or column: zeros.
@@ -180,7 +181,7 @@ template <typename T, typename S, typename ReadA, typename ReadB, typename Copy>
 __device__ __forceinline__ void product16(f32x16 (&acc)[S::MT][S::NT], int slabs, uint32_t lds, const ReadA& ra,
                                           const ReadB& rb, Copy copy) {
   using O = attn::Ops<T>;
-  constexpr int MT = S::MT, NT = S::NT, N = MT * NT, F = MT + NT;
+  constexpr int MT = S::MT, NT = S::NT, N = MT * NT, F = MT + NT, ST = S::kStages;
   if (slabs <= 0) return;
   uint4 f[2][F];        // operands of two steps: NT of B, MT of A
   auto read = [&](uint32_t stage, int s, int e) {
@@ -199,23 +200,26 @@ __device__ __forceinline__ void product16(f32x16 (&acc)[S::MT][S::NT], int slabs
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  copy(0, lds);
-  dma_wait();
+  for (int k = 0; k < ST && k < slabs; ++k) copy(k, lds + k * S::kStage);
+  if (slabs >= ST) dma_wait_but<(ST - 1) * S::kCopies>();
+  else dma_wait();
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
-  if (slabs > 1) copy(1, lds + S::kStage);
 #pragma unroll
   for (int e = 0; e < F; ++e) read(lds, 0, e);
+  uint32_t here = lds;
   for (int k = 0; k < slabs; ++k) {
-    const uint32_t here = lds + (k & 1) * S::kStage, other = lds + ((k & 1) ^ 1) * S::kStage;
+    const uint32_t other = here + S::kStage < lds + S::kLds ? here + S::kStage : lds;
 #pragma unroll
     for (int s = 0; s < 3; ++s) step(s, here, s + 1);
     // every operand of this slab is in registers, and the next slab in LDS
-    dma_wait();
+    if (k + ST <= slabs) dma_wait_but<(ST - 2) * S::kCopies>();
+    else dma_wait();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (k + 2 < slabs) copy(k + 2, here);
+    if (k + ST < slabs) copy(k + ST, here);
     step(3, other, 0);
+    here = other;
   }
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");

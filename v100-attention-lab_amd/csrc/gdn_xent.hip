@@ -30,9 +30,13 @@ using attn::max_halves;
 using attn::Ops;
 using attn::swap_halves;
 
-typedef Shape<4, 2, 2, 4> Big;      // 256 x 256, one workgroup a CU
-typedef Shape<2, 2, 2, 2> Mid;      // 128 x 128, two
-typedef Shape<2, 1, 2, 2> Narrow;   // 128 x 64 (vocabulary x rows)
+// Where there are few of them, a third slab on the way pays more than another
+// workgroup beside: 128 rows, 16000 words of 2048 32 -> 26 us (Wide for Mid), 48 rows,
+// 50257 words 56 -> 53 (Narrow with 3 slabs for 2; with 4 and one workgroup 58).
+typedef Shape<4, 2, 2, 4> Big;         // 256 x 256, one workgroup a CU
+typedef Shape<2, 2, 2, 2> Mid;         // 128 x 128, two
+typedef Shape<2, 2, 2, 2, 3> Wide;     // the same, one
+typedef Shape<2, 1, 2, 2, 3> Narrow;   // 128 x 64 (vocabulary x rows), two
 
 struct Row {
   float lse2, g;      // lse log2 e; dloss in the unit of G, 0 for rows that do not count
@@ -427,11 +431,14 @@ int check(const GdnXentParams& P) {
   return GDN_OK;
 }
 
-// Tiles of 256 x 256 where they fill the card, else smaller ones, two or more a CU.
-enum Kind { kBig, kMid, kNarrow };
-Kind kind_of(int64_t m, int64_t n, bool narrow) {
-  if (narrow && n <= 64) return kNarrow;
-  return tiles_of(m, n, 256, 256) >= 192 ? kBig : kMid;
+// Tiles of 256 x 256 where they fill the card, else smaller ones.
+enum Kind { kBig, kMid, kWide, kNarrow };
+Kind kind_of(int64_t m, int64_t n) { return tiles_of(m, n, 256, 256) >= 192 ? kBig : kMid; }
+// Of logits: vocabulary x rows.
+Kind logits_kind(int64_t v, int64_t rows) {
+  if (rows <= 64) return kNarrow;
+  const Kind k = kind_of(v, rows);
+  return k == kMid && tiles_of(v, rows, 128, 128) <= 256 ? kWide : k;
 }
 
 // Vocabulary of a piece: G takes about 128 MiB.
@@ -448,7 +455,7 @@ struct GradPlan {
   int splits;
   int64_t tiles, floats;
   GradPlan(int64_t m, int64_t n, int64_t k, bool kept) {
-    kind = kind_of(m, n, false);
+    kind = kind_of(m, n);
     const int b = kind == kBig ? 256 : 128;
     tiles = tiles_of(m, n, b, b);
     const int64_t slabs = (k + 63) / 64, places = kind == kBig ? 256 : 512;
@@ -480,7 +487,6 @@ struct BwdLayout {
   }
 };
 
-Kind fwd_kind(const GdnXentParams& P) { return kind_of(P.V, P.N, true); }
 int64_t fwd_tiles(const GdnXentParams& P) { return (P.V + 127) / 128; }
 
 Args args_of(const GdnXentParams& P) {
@@ -502,27 +508,34 @@ Args args_of(const GdnXentParams& P) {
   return a;
 }
 
-// K<T, S>(args, stream), S by kind.
-#define GDN_XENT_BY_KIND(kernel, T, kind, grid, s, a)                                                        \
+// kernel<T, S> by kind: of logits, of gradients.
+#define GDN_XENT_LOGITS(kernel, T, kind, grid, s, a)                                                         \
+  switch (kind) {                                                                                            \
+    case kBig: hipLaunchKernelGGL((kernel<T, Big>), dim3(grid), dim3(Big::kThreads), 0, s, a); break;        \
+    case kMid: hipLaunchKernelGGL((kernel<T, Mid>), dim3(grid), dim3(Mid::kThreads), 0, s, a); break;        \
+    case kWide: hipLaunchKernelGGL((kernel<T, Wide>), dim3(grid), dim3(Wide::kThreads), 0, s, a); break;     \
+    default: hipLaunchKernelGGL((kernel<T, Narrow>), dim3(grid), dim3(Narrow::kThreads), 0, s, a); break;    \
+  }
+#define GDN_XENT_GRADIENT(kernel, T, kind, grid, s, a)                                                        \
   switch (kind) {                                                                                            \
     case kBig: hipLaunchKernelGGL((kernel<T, Big>), dim3(grid), dim3(Big::kThreads), 0, s, a); break;        \
     default: hipLaunchKernelGGL((kernel<T, Mid>), dim3(grid), dim3(Mid::kThreads), 0, s, a); break;          \
   }
 
 void set_tiles(Args& a, Kind k, int64_t m, int64_t n) {
-  const int bm = k == kBig ? 256 : 128, bn = k == kBig ? 256 : k == kMid ? 128 : 64;
+  const int bm = k == kBig ? 256 : 128, bn = k == kBig ? 256 : k == kNarrow ? 64 : 128;
   a.tm = (int)((m + bm - 1) / bm);
   a.tn = (int)((n + bn - 1) / bn);
 }
 
 template <typename T>
-int launch_fwd(Args a, Kind kind, hipStream_t s) {
+int launch_fwd(Args a, hipStream_t s) {
+  const Kind kind = logits_kind(a.V, a.N);
   a.v0 = 0;
   a.vn = a.V;
   set_tiles(a, kind, a.V, a.N);
   const uint32_t grid = (uint32_t)a.tm * a.tn;
-  if (kind == kNarrow) hipLaunchKernelGGL((fwd_kernel<T, Narrow>), dim3(grid), dim3(Narrow::kThreads), 0, s, a);
-  else GDN_XENT_BY_KIND(fwd_kernel, T, kind, grid, s, a);
+  GDN_XENT_LOGITS(fwd_kernel, T, kind, grid, s, a);
   hipLaunchKernelGGL(join_kernel, dim3((a.N + 15) / 16), dim3(kJoin), 0, s, a);
   return (int)hipGetLastError();
 }
@@ -545,21 +558,20 @@ int launch_bwd(Args a, const GdnXentParams& P, const BwdLayout& l, hipStream_t s
     a.vn = std::min(piece, a.V - a.v0);
     a.first = v == 0;
     a.last = v + piece >= a.V;
-    const Kind kl = kind_of(a.vn, a.N, true);
+    const Kind kl = logits_kind(a.vn, a.N);
     set_tiles(a, kl, a.vn, a.N);
     const uint32_t grid = (uint32_t)a.tm * a.tn;
-    if (kl == kNarrow) hipLaunchKernelGGL((grad_kernel<T, Narrow>), dim3(grid), dim3(Narrow::kThreads), 0, s, a);
-    else GDN_XENT_BY_KIND(grad_kernel, T, kl, grid, s, a);
+    GDN_XENT_LOGITS(grad_kernel, T, kl, grid, s, a);
     const GradPlan dw = dw_plan(P, a.vn);
     set_tiles(a, dw.kind, a.D, a.vn);
     a.splits = dw.splits;
     a.sums = reinterpret_cast<float4*>(ws + l.dw);
-    GDN_XENT_BY_KIND(dw_kernel, T, dw.kind, (uint32_t)(dw.tiles * dw.splits), s, a);
+    GDN_XENT_GRADIENT(dw_kernel, T, dw.kind, (uint32_t)(dw.tiles * dw.splits), s, a);
     if (dw.splits > 1) parts(dw, (uint16_t*)a.dw + v * a.D, a.vn);
     set_tiles(a, dx.kind, a.D, a.N);
     a.splits = dx.splits;
     a.sums = reinterpret_cast<float4*>(ws + l.dx);
-    GDN_XENT_BY_KIND(dx_kernel, T, dx.kind, (uint32_t)(dx.tiles * dx.splits), s, a);
+    GDN_XENT_GRADIENT(dx_kernel, T, dx.kind, (uint32_t)(dx.tiles * dx.splits), s, a);
   }
   if (dx.splits > 1) parts(dx, a.dx, a.N);
   return (int)hipGetLastError();
@@ -611,7 +623,7 @@ int gdn_xent_launch(const GdnXentParams* prm, void* stream) {
   a.part = static_cast<float2*>(P.workspace);
   a.hit = reinterpret_cast<float*>(a.part + fwd_tiles(P) * P.N);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  return P.dtype == GDN_DTYPE_F16 ? launch_fwd<f16>(a, fwd_kind(P), s) : launch_fwd<bf16_t>(a, fwd_kind(P), s);
+  return P.dtype == GDN_DTYPE_F16 ? launch_fwd<f16>(a, s) : launch_fwd<bf16_t>(a, s);
 }
 
 int gdn_xent_bwd_launch(const GdnXentParams* prm, void* stream) {

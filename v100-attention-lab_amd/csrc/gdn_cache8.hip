@@ -28,7 +28,7 @@ using fp8::kFp8Max;
 using fp8::lanes_max;
 using fp8::nan_max;
 using fp8::Quant;
-using fp8::store_fp8;
+using fp8::pack_fp8;
 using rowio::Pack;
 
 struct Args {
@@ -58,30 +58,34 @@ __device__ __forceinline__ int64_t at3(const int64_t* st, int b, int t, int h) {
 
 constexpr int kRowNT = 256;
 
-// D / 8 lanes a row; blockIdx.y: keys, values.
+// D / 16 lanes a row; blockIdx.y: keys, values.
 template <typename E, int D>
 __global__ __launch_bounds__(kRowNT) void write_kernel(const Args a) {
-  constexpr int L = D / 8;
-  const uint32_t row = blockIdx.x * (kRowNT / L) + threadIdx.x / L, e0 = threadIdx.x % L * 8;
+  constexpr int L = D / 16;
+  const uint32_t row = blockIdx.x * (kRowNT / L) + threadIdx.x / L, e0 = threadIdx.x % L * 16;
   const uint32_t per = a.T * a.Hk;
   if (row >= a.B * per) return;       // (the row's lanes leave together)
   const int b = row / per, r = row - b * per, t = r / a.Hk, h = r - t * a.Hk;
   const int s = max(0, min(a.lens[b], a.S)) - a.T + t;
   if (s < 0) return;
   const bool v = blockIdx.y;
-  Pack<E, 8> x;
-  x.load((v ? static_cast<const E*>(a.v) + at3(a.vst, b, t, h) : static_cast<const E*>(a.k) + at3(a.kst, b, t, h)) + e0);
-  float f[8], m = 0.f;
+  const E* from = (v ? static_cast<const E*>(a.v) + at3(a.vst, b, t, h) : static_cast<const E*>(a.k) + at3(a.kst, b, t, h)) + e0;
+  Pack<E, 8> x[2];
+  x[0].load(from);
+  x[1].load(from + 8);
+  float f[16], m = 0.f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    f[e] = x.get(e);
+  for (int e = 0; e < 16; ++e) {
+    f[e] = x[e / 8].get(e % 8);
     m = nan_max(m, fabsf(f[e]));
   }
   m = lanes_max<L>(m) / kFp8Max;
   const Quant quant(m);
+  uint32_t q[4];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) f[e] = quant(f[e]);
-  store_fp8<8>((v ? a.vc + at3(a.vcst, b, s, h) : a.kc + at3(a.kcst, b, s, h)) + e0, f);
+  for (int i = 0; i < 4; ++i) q[i] = pack_fp8(quant(f[4 * i]), quant(f[4 * i + 1]), quant(f[4 * i + 2]), quant(f[4 * i + 3]));
+  *reinterpret_cast<uint4*>((v ? a.vc + at3(a.vcst, b, s, h) : a.kc + at3(a.kcst, b, s, h)) + e0) =
+      make_uint4(q[0], q[1], q[2], q[3]);
   if (e0 == 0) {
     if (v) a.vs[at3(a.vsst, b, s, h)] = m;
     else a.ks[at3(a.ksst, b, s, h)] = m;
@@ -550,7 +554,7 @@ Args args_of(const GdnCache8Params& P) {
 template <typename E>
 void launch_write(const Args& a, int D, hipStream_t s) {
   const int64_t rows = (int64_t)a.B * a.T * a.Hk;
-  const int per = kRowNT / (D / 8);
+  const int per = kRowNT / (D / 16);
   const dim3 grid((uint32_t)((rows + per - 1) / per), 2);
   if (D == 128) hipLaunchKernelGGL((write_kernel<E, 128>), grid, dim3(kRowNT), 0, s, a);
   else hipLaunchKernelGGL((write_kernel<E, 64>), grid, dim3(kRowNT), 0, s, a);
@@ -592,7 +596,7 @@ int gdn_cache8_write_launch(const GdnCache8Params* prm, void* stream) {
   if (!rows_ok(P.k, P.k_stride, P.B, P.T, P.Hk, es) || !rows_ok(P.v, P.v_stride, P.B, P.T, P.Hk, es) || !cache_ok(P))
     return GDN_ERR_MISALIGNED;
   // (two of these: keys and values)
-  if ((int64_t)P.T * P.Hk > 0x7fffffff || !grid_fits((int64_t)P.B * P.T * P.Hk, 2 * P.D / 8)) return GDN_ERR_BAD_SHAPE;
+  if ((int64_t)P.T * P.Hk > 0x7fffffff || !grid_fits((int64_t)P.B * P.T * P.Hk, 2 * P.D / 16)) return GDN_ERR_BAD_SHAPE;
   const Args a = args_of(P);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (P.dtype == GDN_DTYPE_F16) launch_write<f16>(a, P.D, s);

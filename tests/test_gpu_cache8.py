@@ -316,3 +316,22 @@ def test_fixed_order(pkg, cuda):
     q = _new(cuda, 2, 1, 8, 128, torch.float16, 8)
     runs = [_decode(pkg, q, kc, vc, ks, vs, [9000, 5000]) for _ in range(3)]
     assert torch.equal(runs[0], runs[1]) and torch.equal(runs[0], runs[2])
+
+
+def test_offsets_beyond_32_bits(pkg, cuda):
+    """Caches of more than 2^31 bytes: written, read back and attended at their end."""
+    B, S, Hk, D, Hq = 2, 33_000, 256, 128, 512
+    kc, vc = (torch.zeros(B, S, Hk, D, dtype=torch.uint8, device=cuda).view(FP8) for _ in range(2))
+    ks, vs = torch.zeros(B, S, Hk, device=cuda), torch.zeros(B, S, Hk, device=cuda)
+    lens = torch.tensor([S, S - 11], dtype=torch.int32, device=cuda)
+    k, v = _new(cuda, B, 40, Hk, D, torch.bfloat16, 1), _new(cuda, B, 40, Hk, D, torch.bfloat16, 2)
+    pkg.cache_write_fp8(k, v, kc, vc, ks, vs, lens)
+    q = _new(cuda, B, 1, Hq, D, torch.bfloat16, 3)
+    o = pkg.window_attn_decode_fp8(q, kc, vc, ks, vs, lens, 30)
+    tail = slice(S - 60, S)
+    _check_written(k, kc[:, tail], ks[:, tail], torch.zeros_like(kc[:, tail], dtype=torch.uint8).view(FP8),
+                   torch.zeros_like(ks[:, tail]), [60, 49])
+    assert (ks[:, :S - 60] == 0).all()
+    _close(o, oracle(q, kc[:, tail], vc[:, tail], ks[:, tail], vs[:, tail], [60, 49], 30, 0))
+    k16, _ = pkg.cache_read_fp8(kc, vc, ks, vs)
+    assert torch.equal(k16[:, tail], (kc[:, tail].float() * ks[:, tail, :, None]).bfloat16())

@@ -217,3 +217,28 @@ def test_captured_calls(pkg, cuda):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(got, run())
+
+
+@pytest.mark.parametrize("M,K,N", [(40_000, 128, 60_000), (17_000_000, 128, 24), (5, 128, 17_000_000)])
+def test_offsets_beyond_32_bits(pkg, cuda, M, K, N):
+    """Rows, weights or results of more than 2^31 bytes: the last ones against the formula."""
+    gen = torch.Generator(device=cuda).manual_seed(1)
+    bytes_ = lambda n: torch.randint(0, 0x70, (n, K), generator=gen, device=cuda, dtype=torch.uint8).view(FP8)
+    x, w = bytes_(M), bytes_(N)
+    xs, ws = torch.rand(M, 1, generator=gen, device=cuda), torch.rand(-(-N // 128), 1, generator=gen, device=cuda)
+    y = pkg.fp8_linear(x, xs, w, ws)
+    m, n = min(M, 300), min(N, 300) // 4 * 4
+    n0 = (N - n) // 128 * 128          # (whole blocks of outputs)
+    for r in (slice(0, m), slice(M - m, M)):
+        want, size = oracle(x[r], xs[r], w[n0:], ws[n0 // 128:])
+        _check(y[r, n0:], want, size, K)
+
+
+def test_quantize_beyond_32_bits(pkg, cuda):
+    x = torch.zeros(9_000_000, 256, dtype=torch.bfloat16, device=cuda)
+    x[-100:] = torch.randn(100, 256, device=cuda).bfloat16()
+    for group in (128, None):
+        q, s = pkg.quantize_fp8(x, group=group)
+        q2, s2 = pkg.quantize_fp8(x[-100:].clone(), group=group)
+        assert torch.equal(q[-100:].view(torch.uint8), q2.view(torch.uint8)) and torch.equal(s[-100:], s2)
+        assert (s[:-100] == 0).all()

@@ -295,3 +295,74 @@ def test_many_rows_of_few_columns(pkg, cuda, dtype, N, D, V):
     x, w, t, dloss = _inputs(cuda, N, D, V, dtype, N + V)
     t[torch.rand(N, device=cuda) < 0.2] = -100
     _check(pkg, x, w, t, dloss)
+
+
+def test_captured_autograd(pkg, cuda):
+    """Forward and backward through autograd in one graph, the leaves made in it, while
+    an eager graph of the same memory lives."""
+    x, w, t, _ = _inputs(cuda, 200, 128, 700, torch.bfloat16, 6)
+
+    def step():
+        xg, wg = x.detach().requires_grad_(), w.detach().requires_grad_()
+        loss = pkg.linear_xent(xg, wg, t).sum()
+        return (loss, *torch.autograd.grad(loss, (xg, wg)))
+    want = [r.detach().clone() for r in step()]
+    eager = pkg.linear_xent(x.detach().requires_grad_(), w, t).sum()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got[1:], want[1:])), i
+        step()
+    assert torch.isfinite(eager)
+
+
+def test_one_gradient_alone(pkg, cuda):
+    """x or the weight without a gradient, a weight that is expanded from one row."""
+    x, w, t, _ = _inputs(cuda, 60, 64, 100, torch.bfloat16, 6)
+    ones = torch.ones(60, device=cuda)
+    _, _, wx, ww, sizes = oracle(x, w, t, ones)
+    xg = x.clone().requires_grad_()
+    pkg.linear_xent(xg, w, t).sum().backward()
+    _close(xg.grad, wx, 1.5, sizes[0], "dx")
+    wg = w.clone().requires_grad_()
+    pkg.linear_xent(x, wg, t).sum().backward()
+    _close(wg.grad, ww, 1.5, sizes[1], "dw")
+    row = w[:1].clone().requires_grad_()
+    pkg.linear_xent(x, row.expand(100, 64), t).sum().backward()
+    # every word has the same logit: the gradient of their common weights is 0, of terms of this size
+    g = torch.full((60, 100), 0.01, device=cuda, dtype=torch.float64)
+    g[torch.arange(60, device=cuda), t] -= 1
+    size = (g.abs().T @ x.double().abs()).sum(0).norm()
+    assert row.grad.double().norm() <= 2 * 2.0 ** -8 * size
+
+
+def test_offsets_beyond_32_bits(pkg, cuda):
+    """A weight of more than 2^31 elements: the last words against the formulas."""
+    V, D, N = 530_000, 4096, 20
+    gen = torch.Generator(device=cuda).manual_seed(1)
+    w = torch.empty(V, D, dtype=torch.bfloat16, device=cuda)
+    for v in range(0, V, 100_000):
+        w[v:v + 100_000] = torch.randn(min(100_000, V - v), D, generator=gen, device=cuda) * (2.0 / 64)
+    x = torch.randn(N, D, generator=gen, device=cuda).bfloat16()
+    t = torch.randint(V - 3000, V, (N,), generator=gen, device=cuda)
+    dloss = torch.ones(N, device=cuda)
+    loss, lse = pkg.linear_xent(x, w, t, return_lse=True)
+    dx, dw = pkg.linear_xent_bwd(x, w, t, lse, dloss)
+    logits = torch.cat([x.double() @ w[v:v + 50_000].double().T for v in range(0, V, 50_000)], 1)
+    want_lse = torch.logsumexp(logits, 1)
+    _losses(loss, lse, want_lse - logits[torch.arange(N, device=cuda), t], want_lse)
+    p = torch.exp(logits - want_lse[:, None])
+    g = p.clone()
+    g[torch.arange(N, device=cuda), t] -= 1
+    for part in (slice(0, 2000), slice(V - 4000, V)):
+        _close(dw[part], g[:, part].T @ x.double(), 1.5, ((g[:, part].square().T @ x.double().square()).sum().sqrt().item(), 1e-3), "dw")
+    want = sum(g[:, v:v + 50_000] @ w[v:v + 50_000].double() for v in range(0, V, 50_000))
+    _close(dx, want, 1.5, (want.norm().item(), 0.0), "dx")

@@ -282,3 +282,20 @@ def test_scale_without_gradient_is_refused(pkg):
     s = torch.tensor(0.1, requires_grad=True)
     with pytest.raises(NotImplementedError, match="scale"):
         CALLS["window_attn_decode_fp8"](pkg, {**_operands(), "args": (None, 0, s)})
+
+
+def test_sizes_beyond_32_bits(pkg):
+    """Nothing is cut off on its way through the C boundary."""
+    from importlib import import_module
+    check = import_module("v100-attention-lab_amd.ops")._check_sizes
+    check(0, 2 ** 31 - 1)
+    with pytest.raises(ValueError, match="2\\^31"):
+        check(5, 2 ** 31)
+    L = import_module("v100-attention-lab_amd.loss")
+    with pytest.raises(ValueError, match="2\\^31"):      # (checks before it pass on meta tensors)
+        L._validate, keep = (lambda *a: None), L._validate
+        try:
+            L._plan(torch.empty(2 ** 31, 8, dtype=torch.float16, device="meta"), torch.empty(9, 8, dtype=torch.float16, device="meta"),
+                    None, None, None, False)
+        finally:
+            L._validate = keep

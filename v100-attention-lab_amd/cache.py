@@ -11,7 +11,7 @@ import torch
 
 from . import _lib
 from .attn import MAX_DECODE_T, SUPPORTED_D, _check_window, _number
-from .ops import _DTYPE_CODE, _PLANS_MAX, _check_devices, _code, _launch, _needs_grad
+from .ops import _DTYPE_CODE, _PLANS_MAX, _check_devices, _check_sizes, _code, _launch, _needs_grad
 from .scan import _failed, _like, _sig
 
 FP8 = torch.float8_e4m3fn
@@ -48,6 +48,7 @@ def _check_cache(k_cache, v_cache, k_scale, v_scale):
     if k_cache.device.type != "cuda":
         raise ValueError(f"the 8-bit cache lives on a ROCm GPU (got {k_cache.device}); there is no CPU path")
     _check_devices(k_cache, v_cache, k_scale, v_scale)
+    _check_sizes(*k_cache.shape)
     _check_rows(k_cache, "k_cache")
     _check_rows(v_cache, "v_cache")
     return B, S, Hk, D
@@ -74,14 +75,14 @@ def _params(k_cache, v_cache, k_scale, v_scale, B, S, Hk, D):
     return P
 
 
-def _call(what, tensors, options, make):
-    """The plan of a signature seen before, or make()'s.  (The alignment is of this
-    call's pointers: part of the signature.)"""
+def _call(what, rows, others, options, make):
+    """The plan of a signature seen before, or make()'s.  (The alignment of `rows` is
+    of this call's pointers: part of the signature.)"""
     try:
         bits = 0
-        for t in tensors:
+        for t in rows:
             bits |= t.data_ptr()
-        key = (what, *(_sig(t) for t in tensors), options, bits & 15)
+        key = (what, *(_sig(t) for t in rows), *(_sig(t) for t in others), options, bits & 15)
         plan = _PLANS.get(key)
     except (AttributeError, TypeError):     # not tensors: the checks say which
         key, plan = None, None
@@ -113,6 +114,7 @@ def _write_plan(k, v, k_cache, v_cache, k_scale, v_scale, lens):
     _check_devices(k_cache, k, v)
     _check_rows(k, "k")
     _check_rows(v, "v")
+    _check_sizes(k.shape[1])
     P = _params(k_cache, v_cache, k_scale, v_scale, B, S, Hk, D)
     P.T, P.dtype = k.shape[1], _DTYPE_CODE[k.dtype]
     P.k_stride[:], P.v_stride[:] = k.stride()[:3], v.stride()[:3]
@@ -140,7 +142,7 @@ def cache_write_fp8(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     """
     if _needs_grad(k, v):
         raise NotImplementedError("cache_write_fp8 has no gradient")
-    params = _call("write", (k, v, k_cache, v_cache, k_scale, v_scale, cache_seqlens), None,
+    params = _call("write", (k, v, k_cache, v_cache), (k_scale, v_scale, cache_seqlens), None,
                    lambda: _write_plan(k, v, k_cache, v_cache, k_scale, v_scale, cache_seqlens))
     if k.shape[1] == 0:
         return
@@ -170,7 +172,7 @@ def cache_read_fp8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.
     for the keys that a prefill continues."""
     if _needs_grad(k_scale, v_scale):
         raise NotImplementedError("cache_read_fp8 has no gradient")
-    params = _call("read", (k_cache, v_cache, k_scale, v_scale), dtype,
+    params = _call("read", (k_cache, v_cache), (k_scale, v_scale), dtype,
                    lambda: _read_plan(k_cache, v_cache, k_scale, v_scale, dtype))
     k = torch.empty(k_cache.shape, dtype=dtype, device=k_cache.device)
     v = torch.empty_like(k)
@@ -196,6 +198,7 @@ def _decode_plan(q, k_cache, v_cache, k_scale, v_scale, lens, window, sinks, sca
         raise ValueError(f"q must hold 1 to {MAX_DECODE_T} new tokens of each sequence, got {T}")
     _check_lens(lens, k_cache)
     _check_devices(k_cache, q)
+    _check_sizes(Hq)
     _check_rows(q, "q")
     P = _params(k_cache, v_cache, k_scale, v_scale, B, S, Hk, D)
     P.T, P.Hq, P.window, P.sinks = T, Hq, w, s
@@ -229,7 +232,7 @@ def window_attn_decode_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
         raise NotImplementedError("window_attn_decode_fp8 has no gradient: use window_attn in training")
     scale = _number(scale)
     params, ws_bytes = _call(
-        "decode", (q, k_cache, v_cache, k_scale, v_scale, cache_seqlens), (window, sinks, scale),
+        "decode", (q, k_cache, v_cache), (k_scale, v_scale, cache_seqlens), (window, sinks, scale),
         lambda: _decode_plan(q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, window, sinks, scale))
     lens = _lens32(cache_seqlens, k_cache.shape[1])
     o = _like(q)

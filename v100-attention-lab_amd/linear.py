@@ -8,7 +8,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .ops import _DTYPE_CODE, _PLANS_MAX, _check_devices, _code, _launch, _needs_grad
+from .ops import _DTYPE_CODE, _PLANS_MAX, _check_devices, _check_sizes, _code, _launch, _needs_grad
 from .scan import _failed, _sig
 
 FP8 = torch.float8_e4m3fn
@@ -50,6 +50,7 @@ def _quant_plan(x, mode, name):
     scale = {_lib.FP8_ROWS: (*lead, 1), _lib.FP8_GROUPS: (*lead, D // BLOCK)}.get(mode)
     if scale is None:
         scale = (-(-lead[0] // BLOCK), D // BLOCK)
+    _check_sizes(*x2.shape)
     P = _lib.GdnFp8QuantParams()
     P.x_stride, P.rows, P.D = x2.stride(0), x2.shape[0], D
     P.x_dtype, P.mode = _DTYPE_CODE[x.dtype], mode
@@ -133,6 +134,7 @@ def _plan(x, x_scale, weight, weight_scale, out_dtype, lead):
         _check_rows(t, name)
         if t.shape[0] > 1 and t.stride(0) > _MAX_STRIDE:
             raise ValueError(f"{name}: rows may be at most {_MAX_STRIDE} elements apart (stride {t.stride(0)})")
+    _check_sizes(*x.shape, N)
     P = _lib.GdnFp8LinearParams()
     P.M, P.N, P.K = x.shape[0], N, K
     P.x_stride, P.w_stride = x.stride(0), weight.stride(0)

@@ -8,7 +8,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import _DTYPE_CODE, _PLANS_MAX, _check_devices, _first_order, _launch, _needs_grad
+from .ops import _DTYPE_CODE, _PLANS_MAX, _check_devices, _check_sizes, _first_order, _launch, _needs_grad
 from .scan import _failed, _like, _sig
 
 _MAX_STRIDE = 1 << 22
@@ -61,6 +61,7 @@ def _plan(x, weight, target, lse, dloss, backward):
     if x.numel() > 0:
         _check_rows(x2, "x")
     _check_rows(weight, "weight")
+    _check_sizes(*x2.shape, weight.shape[0])
     P = _lib.GdnXentParams()
     P.N, P.D, P.V = x2.shape[0], x2.shape[1], weight.shape[0]
     P.x_stride, P.w_stride = x2.stride(0), weight.stride(0)

@@ -112,6 +112,12 @@ def _check_devices(q, *others):
         raise ValueError("all inputs must be on the same device")
 
 
+def _check_sizes(*sizes):
+    """Sizes cross the C boundary as 32-bit integers."""
+    if any(n >= 2 ** 31 for n in sizes):
+        raise ValueError(f"sizes of 2^31 or more are not supported: {sizes}")
+
+
 _KERNELS = {"auto": 0, "phased": _lib.FLAG_PHASED_KERNEL, "fused": _lib.FLAG_FUSED_KERNEL}
 
 # Launch plans keyed by everything but the data pointers: shapes, strides,

@@ -216,19 +216,15 @@ __global__ __launch_bounds__(kNT) void decode_kernel(const Args a) {
   using Vec = typename O::Vec;
   using TL = Tile8<D>;
   constexpr uint32_t kTile = TL::kBytes, kBuf = 2 * kTile + 256, kWave = 2 * kBuf;
-  constexpr int kRow = D + 3;
-  constexpr uint32_t kJoin = kDWaves * 32 * kRow * 4, kTiles = kDWaves * kWave;
+  constexpr int kRow = D + 3, kPitch = D + 4;
+  constexpr uint32_t kJoin = kDWaves * 32 * (kPitch + 3) * 4, kTiles = kDWaves * kWave;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[kJoin > kTiles ? kJoin : kTiles];
   const int split = blockIdx.x % a.splits, unit = blockIdx.x / a.splits;
   const int rt = unit % a.tiles_r, bh = unit / a.tiles_r, hk = bh % a.Hk, b = bh / a.Hk;
   const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int n = __builtin_amdgcn_readfirstlane(max(0, min(a.lens[b], a.S)));
+  const int len = a.lens[b];
   const QRow qr(a, hk, rt, l32);
-  const int p = n - a.T + qr.t;
-  const int r0 = rt * 32, rows = min(32, a.G * a.T - r0);
-  const int p0 = n - a.T + r0 / a.G, p1 = n - a.T + (r0 + rows - 1) / a.G;
-
   Vec qf[D / 16];      // elements 32 u + 16 half + 8 w of product 2 u + w
   {
     const uint16_t* q = a.q + at3(a.qst, b, qr.t, qr.h);
@@ -236,6 +232,11 @@ __global__ __launch_bounds__(kNT) void decode_kernel(const Args a) {
     for (int i = 0; i < D / 16; ++i)
       qf[i] = signed_vec<T>(*reinterpret_cast<const uint4*>(q + 32 * (i >> 1) + 16 * half + 8 * (i & 1)), a.flip);
   }
+  const int n = __builtin_amdgcn_readfirstlane(max(0, min(len, a.S)));
+  const int p = n - a.T + qr.t;
+  const int r0 = rt * 32, rows = min(32, a.G * a.T - r0);
+  const int p0 = n - a.T + r0 / a.G, p1 = n - a.T + (r0 + rows - 1) / a.G;
+
   // the tiles of any row; rows before the first key see none
   const KeyRange kr(max(p0, 0), p1, n, a.window, a.sinks, kDN);
   const int per = (kr.n + a.splits - 1) / a.splits;
@@ -371,7 +372,7 @@ __global__ __launch_bounds__(kNT) void decode_kernel(const Args a) {
 
   // the waves' parts, joined by all of them
   __syncthreads();
-  float* sm = reinterpret_cast<float*>(lds);        // [8][32] m, l, M, then [8][D][32] O
+  float* sm = reinterpret_cast<float*>(lds);        // [8][32] m, l, M, then [8][32][D + 4] O
   float* sl = sm + kDWaves * 32;
   float* sM = sl + kDWaves * 32;
   float* so = sM + kDWaves * 32;
@@ -384,46 +385,45 @@ __global__ __launch_bounds__(kNT) void decode_kernel(const Args a) {
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) so[(wv * D + 32 * dt + acc_row(r, half)) * 32 + l32] = acc[dt][r];
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<float4*>(so + (wv * 32 + l32) * kPitch + 32 * dt + 8 * g + 4 * half) =
+            make_float4(acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]);
   }
   __syncthreads();
-  // thread: row c = tid / 16, D / 16 columns from 16 neighbouring threads
-  constexpr int kCols = D / 16;
-  const int c = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * kCols;
-  if (c >= rows) return;
-  float top = sm[c], topM = sM[c];
+  // two columns of a row a thread
+  for (int e = threadIdx.x; e < rows * (D / 2); e += kNT) {
+    const int c = e / (D / 2), d = e % (D / 2) * 2;
+    float top = sm[c], topM = sM[c];
 #pragma unroll
-  for (int w = 1; w < kDWaves; ++w) {
-    top = fmaxf(top, sm[w * 32 + c]);
-    topM = fmaxf(topM, sM[w * 32 + c]);
-  }
-  float sum = 0.f, out[kCols] = {};
-#pragma unroll
-  for (int w = 0; w < kDWaves; ++w) {
-    sum += weight(sm[w * 32 + c], top) * sl[w * 32 + c];
-    const float f = weight(sM[w * 32 + c], topM);
-    // (a wave without a key holds zeros; one that saw NaN alone has no maximum and keeps it)
-#pragma unroll
-    for (int e = 0; e < kCols; ++e) out[e] += f * so[(w * D + d0 + e) * 32 + c];
-  }
-  // a NaN score leaves no maximum either, but its sum is NaN, and 0 NaN stays so
-  if (a.splits > 1) {
-    float* part = a.part + ((int64_t)unit * a.splits + split) * 32 * kRow;
-    if (d0 == 0) {
-      part[c] = top;
-      part[32 + c] = sum;
-      part[64 + c] = topM;
+    for (int w = 1; w < kDWaves; ++w) {
+      top = fmaxf(top, sm[w * 32 + c]);
+      topM = fmaxf(topM, sM[w * 32 + c]);
     }
+    // (a wave without a key holds zeros; one that saw NaN alone has no maximum and keeps
+    // it: 0 NaN is NaN, in the sum too)
+    float sum = 0.f, x = 0.f, y = 0.f;
 #pragma unroll
-    for (int e = 0; e < kCols; e += 4)
-      *reinterpret_cast<float4*>(part + 96 + c * D + d0 + e) = make_float4(out[e], out[e + 1], out[e + 2], out[e + 3]);
-    return;
+    for (int w = 0; w < kDWaves; ++w) {
+      sum += weight(sm[w * 32 + c], top) * sl[w * 32 + c];
+      const float f = weight(sM[w * 32 + c], topM);
+      const float2 o = *reinterpret_cast<const float2*>(so + (w * 32 + c) * kPitch + d);
+      x += f * o.x;
+      y += f * o.y;
+    }
+    if (a.splits > 1) {
+      float* part = a.part + ((int64_t)unit * a.splits + split) * 32 * kRow;
+      if (d == 0) {
+        part[c] = top;
+        part[32 + c] = sum;
+        part[64 + c] = topM;
+      }
+      *reinterpret_cast<float2*>(part + 96 + c * D + d) = make_float2(x, y);
+    } else {
+      const float f = result_factor<T>(top, sum, topM);
+      const QRow row(a, hk, rt, c);
+      *reinterpret_cast<uint32_t*>(a.o + at3(a.ost, b, row.t, row.h) + d) = O::pack(x * f, y * f);
+    }
   }
-  const float f = result_factor<T>(top, sum, topM);
-  const QRow row(a, hk, rt, c);
-  uint16_t* o = a.o + at3(a.ost, b, row.t, row.h) + d0;
-#pragma unroll
-  for (int e = 0; e < kCols; e += 2) *reinterpret_cast<uint32_t*>(o + e) = O::pack(out[e] * f, out[e + 1] * f);
 }
 
 // One workgroup a query row: every wave weighs the splits (one a lane), then

@@ -270,6 +270,8 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
     There is no fallback: without the library the GDN forward is unavailable.
     """
     global _lib
+    if _lib is not None:        # (set once, whole)
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib

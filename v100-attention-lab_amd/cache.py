@@ -79,10 +79,13 @@ def _call(what, rows, others, options, make):
     """The plan of a signature seen before, or make()'s.  (The alignment of `rows` is
     of this call's pointers: part of the signature.)"""
     try:
-        bits = 0
+        key, bits = [what, options], 0
         for t in rows:
             bits |= t.data_ptr()
-        key = (what, *(_sig(t) for t in rows), *(_sig(t) for t in others), options, bits & 15)
+            key.append(_sig(t))
+        for t in others:
+            key.append(_sig(t))
+        key = (*key, bits & 15)
         plan = _PLANS.get(key)
     except (AttributeError, TypeError):     # not tensors: the checks say which
         key, plan = None, None

@@ -9,7 +9,7 @@ import torch
 
 from . import _lib
 from .ops import _DTYPE_CODE, _PLANS_MAX, _check_devices, _check_sizes, _code, _launch, _needs_grad
-from .scan import _failed, _sig
+from .scan import _failed, _like, _sig
 
 FP8 = torch.float8_e4m3fn
 BLOCK = 128
@@ -54,7 +54,7 @@ def _quant_plan(x, mode, name):
     P = _lib.GdnFp8QuantParams()
     P.x_stride, P.rows, P.D = x2.stride(0), x2.shape[0], D
     P.x_dtype, P.mode = _DTYPE_CODE[x.dtype], mode
-    return bytes(P), scale
+    return bytes(P), scale, x.dim() == 2
 
 
 def _quantize(x, mode, name):
@@ -71,11 +71,11 @@ def _quantize(x, mode, name):
             if len(_QUANT_PLANS) >= _PLANS_MAX:
                 _QUANT_PLANS.clear()
             _QUANT_PLANS[key] = plan
-    params, shape = plan
-    q = torch.empty(x.shape, dtype=FP8, device=x.device)
-    scale = torch.empty(shape, dtype=torch.float32, device=x.device)
+    params, shape, rows = plan
+    q = _like(x, FP8)
+    scale = x.new_empty(shape, dtype=torch.float32)
     if q.numel() > 0:
-        x2 = _flat(x)
+        x2 = x if rows else _flat(x)
         P = _lib.GdnFp8QuantParams.from_buffer_copy(params)
         P.x, P.q, P.scale = x2.data_ptr(), q.data_ptr(), scale.data_ptr()
         status = _launch(_lib.load_library().gdn_fp8_quant_launch, P, x.device)
@@ -108,11 +108,11 @@ def quantize_fp8_weight(weight: torch.Tensor):
     return _quantize(weight, _lib.FP8_BLOCKS, "quantize_fp8_weight")
 
 
-def _plan(x, x_scale, weight, weight_scale, out_dtype, lead):
+def _plan(x, x_scale, weight, weight_scale, out_dtype):
     for name, t in (("x", x), ("weight", weight)):
         if not isinstance(t, torch.Tensor) or t.dtype != FP8 or t.dim() < 1:
             raise ValueError(f"{name} must be a float8_e4m3fn tensor, x [..., K] and weight [N, K]")
-    K = x.shape[-1]
+    lead, K = tuple(x.shape[:-1]), x.shape[-1]
     if weight.dim() != 2 or weight.shape[1] != K or weight.shape[0] < 1:
         raise ValueError(f"weight must be [N, K] with x's K={K}, got {tuple(weight.shape)}")
     if K < BLOCK or K % BLOCK != 0:
@@ -130,17 +130,18 @@ def _plan(x, x_scale, weight, weight_scale, out_dtype, lead):
     if x.device.type != "cuda":
         raise ValueError(f"fp8_linear runs on a ROCm GPU (got {x.device}); there is no CPU path")
     _check_devices(x, x_scale, weight, weight_scale)
-    for name, t in (("x", x), ("weight", weight)):
+    x2 = _flat(x)
+    for name, t in (("x", x2), ("weight", weight)):
         _check_rows(t, name)
         if t.shape[0] > 1 and t.stride(0) > _MAX_STRIDE:
             raise ValueError(f"{name}: rows may be at most {_MAX_STRIDE} elements apart (stride {t.stride(0)})")
-    _check_sizes(*x.shape, N)
+    _check_sizes(*x2.shape, N)
     P = _lib.GdnFp8LinearParams()
-    P.M, P.N, P.K = x.shape[0], N, K
-    P.x_stride, P.w_stride = x.stride(0), weight.stride(0)
+    P.M, P.N, P.K = x2.shape[0], N, K
+    P.x_stride, P.w_stride = x2.stride(0), weight.stride(0)
     P.group = BLOCK if x_scale.shape[-1] == K // BLOCK else 0
     P.y_dtype = _DTYPE_CODE[out_dtype]
-    return bytes(P), (*lead, N)
+    return bytes(P), (*lead, N), x.dim() == 2, x_scale.is_contiguous() and weight_scale.is_contiguous()
 
 
 def fp8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, *,
@@ -159,27 +160,26 @@ def fp8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, wei
     """
     if _needs_grad(x, x_scale, weight, weight_scale):
         raise NotImplementedError("fp8_linear has no gradient: multiply in 16 bits in training")
-    ok = isinstance(x, torch.Tensor) and x.dim() >= 1
-    lead = tuple(x.shape[:-1]) if ok else ()
-    x2 = _flat(x) if ok else x
     try:
-        key = (_sig(x2), _sig(x_scale), _sig(weight), _sig(weight_scale), out_dtype, lead,
-               (x2.data_ptr() | weight.data_ptr()) & 15)
+        key = (x.shape, x.stride(), x.dtype, x.device, _sig(x_scale), _sig(weight), _sig(weight_scale), out_dtype,
+               (x.data_ptr() | weight.data_ptr()) & 15)
         plan = _PLANS.get(key)
     except (AttributeError, TypeError):     # not tensors: _plan says which
         key, plan = None, None
     if plan is None:
-        plan = _plan(x2, x_scale, weight, weight_scale, out_dtype, lead)
+        plan = _plan(x, x_scale, weight, weight_scale, out_dtype)
         if key is not None:
             if len(_PLANS) >= _PLANS_MAX:
                 _PLANS.clear()
             _PLANS[key] = plan
-    params, shape = plan
-    y = torch.empty(shape, dtype=out_dtype, device=x.device)
+    params, shape, rows, dense = plan
+    x2 = x if rows else _flat(x)
+    if not dense:
+        x_scale, weight_scale = x_scale.contiguous(), weight_scale.contiguous()
+    y = x.new_empty(shape, dtype=out_dtype)
     if y.numel() > 0:
-        xs, ws = x_scale.contiguous(), weight_scale.contiguous()
         P = _lib.GdnFp8LinearParams.from_buffer_copy(params)
-        P.x, P.x_scale, P.w, P.w_scale = x2.data_ptr(), xs.data_ptr(), weight.data_ptr(), ws.data_ptr()
+        P.x, P.x_scale, P.w, P.w_scale = x2.data_ptr(), x_scale.data_ptr(), weight.data_ptr(), weight_scale.data_ptr()
         P.y = y.data_ptr()
         status = _launch(_lib.load_library().gdn_fp8_linear_launch, P, x.device)
         if status != 0:

@@ -760,5 +760,9 @@ def _needs_grad(*ts) -> bool:
     if forward_ad._current_level >= 0 and any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None
                                               for t in ts):
         raise NotImplementedError("forward mode (tangents of dual tensors) is not supported")
-    return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad
-                                           for t in ts)
+    if not torch.is_grad_enabled():
+        return False
+    for t in ts:        # (a generator takes twice as long)
+        if isinstance(t, torch.Tensor) and t.requires_grad:
+            return True
+    return False

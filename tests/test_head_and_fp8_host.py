@@ -254,6 +254,17 @@ def test_cache_refusals(pkg, as_if_on_gpu, name, kw, match):
         CALLS[name](pkg, {**_operands(), **kw})
 
 
+@pytest.mark.parametrize("i", range(4))
+def test_expanded_caches_are_not_written(pkg, as_if_on_gpu, i):
+    """Two sequences (or heads) would write the same rows."""
+    for dim in (0, 2):
+        o = _operands()
+        to = [o["kc"], o["kc"].clone(), o["ks"], o["ks"].clone()]
+        to[i] = to[i].narrow(dim, 0, 1).expand_as(to[i])
+        with pytest.raises(ValueError, match="expanded"):
+            pkg.cache_write_fp8(o["k"], o["k"], *to, o["lens"])
+
+
 @pytest.mark.parametrize("name,key", [("quantize_fp8", "y"), ("quantize_fp8_weight", "y"), ("fp8_linear", "xs"),
                                       ("fp8_linear", "ws"), ("cache_write_fp8", "k"), ("cache_read_fp8", "ks"),
                                       ("window_attn_decode_fp8", "k"), ("window_attn_decode_fp8", "ks")])

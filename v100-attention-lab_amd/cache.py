@@ -107,6 +107,9 @@ def _bind(params, k_cache, v_cache, k_scale, v_scale):
 
 def _write_plan(k, v, k_cache, v_cache, k_scale, v_scale, lens):
     B, S, Hk, D = _check_cache(k_cache, v_cache, k_scale, v_scale)
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache), ("k_scale", k_scale), ("v_scale", v_scale)):
+        if any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
+            raise ValueError(f"{name} is written to and must not be expanded (strides {t.stride()})")
     for name, t in (("k", k), ("v", v)):
         if not isinstance(t, torch.Tensor) or t.dim() != 4 or (t.shape[0], *t.shape[2:]) != (B, Hk, D):
             raise ValueError(f"{name} must be [B, T, Hk, D] with the cache's B={B}, Hk={Hk}, D={D}")

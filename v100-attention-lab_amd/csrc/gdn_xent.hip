@@ -432,13 +432,13 @@ int check(const GdnXentParams& P) {
 }
 
 // Tiles of 256 x 256 or of 128 x 128, by the rounds that they make of the card: 256 at
-// a time take about 7 parts of time, 512 small ones 4.  So small ones up to 512, and
-// where the big ones leave much of their last round idle: logits of 1024 rows of 2048
+// a time take about 13 parts of time, 512 small ones 8.  So small ones up to 512, and
+// where the big ones leave much of their second round idle: logits of 1024 rows of 2048
 // in us, small and big, 8000 words 40 and 51, 10240 59 and 51, 17408 88 and 104,
-// 26624 118 and 107, 34816 149 and 159, 65536 279 and 237.
+// 26624 118 and 107, 65536 279 and 237 (40960 words, 640 big tiles, 167 and 160).
 enum Kind { kBig, kMid, kWide, kNarrow };
 Kind kind_of(int64_t m, int64_t n) {
-  return 7 * ((tiles_of(m, n, 256, 256) + 255) / 256) <= 4 * ((tiles_of(m, n, 128, 128) + 511) / 512) ? kBig : kMid;
+  return 13 * ((tiles_of(m, n, 256, 256) + 255) / 256) <= 8 * ((tiles_of(m, n, 128, 128) + 511) / 512) ? kBig : kMid;
 }
 // Of logits: vocabulary x rows.
 Kind logits_kind(int64_t v, int64_t rows) {

@@ -225,14 +225,16 @@ __device__ __forceinline__ void product16(f32x16 (&acc)[S::MT][S::NT], int slabs
   asm volatile("" ::: "memory");
 }
 
-// Tile of a workgroup, tm x tn of them.  Workgroups go round the 8 dies one by
-// one: each die gets neighbouring tiles, 8 of N at a time, that share rows in
-// its L2.
+// Tile of a workgroup, tm x tn of them for each part of the contraction.  Workgroups
+// go round the 8 dies one by one: each die gets neighbouring tiles of as few parts as
+// may be, 8 of N at a time, that share rows in its L2.
 struct TileAt {
-  int m, n;
-  __device__ __forceinline__ TileAt(uint32_t id, uint32_t tm, uint32_t tn) {
-    const uint32_t total = tm * tn, per = total / 8, left = total % 8, die = id % 8;
-    const uint32_t at = die * per + min(die, left) + id / 8;
+  int m, n, split;
+  __device__ __forceinline__ TileAt(uint32_t id, uint32_t tm, uint32_t tn, uint32_t splits = 1) {
+    const uint32_t tiles = tm * tn, total = tiles * splits, per = total / 8, left = total % 8, die = id % 8;
+    uint32_t at = die * per + min(die, left) + id / 8;
+    split = (int)(at / tiles);
+    at %= tiles;
     const uint32_t group = at / (8 * tm), in = at % (8 * tm), width = min(8u, tn - 8 * group);
     n = (int)(8 * group + in % width);
     m = (int)(in / width);

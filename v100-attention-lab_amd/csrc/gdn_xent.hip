@@ -300,12 +300,11 @@ __global__ __launch_bounds__(S::kThreads) void grad_kernel(const Args a) {
 template <typename T, typename S>
 __global__ __launch_bounds__(S::kThreads) void dx_kernel(const Args a) {
   __shared__ __attribute__((aligned(1024))) uint8_t lds[S::kLds];
-  const uint32_t tiles = a.tm * a.tn, split = blockIdx.x / tiles;
-  const TileAt t(blockIdx.x % tiles, a.tm, a.tn);
+  const TileAt t(blockIdx.x, a.tm, a.tn, a.splits);
   const int lane = threadIdx.x & 63;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wv % S::WM, wn = wv / S::WM;
   const int slabs = (a.vn + 63) / 64, per = (slabs + a.splits - 1) / a.splits;
-  const int s0 = min((int)split * per, slabs), s1 = min(s0 + per, slabs);
+  const int s0 = min(t.split * per, slabs), s1 = min(s0 + per, slabs);
   f32x16 acc[S::MT][S::NT] = {};
   {
     const TurnedCopy<S::BM, S::kWaves> ca((const uint8_t*)a.w + (int64_t)a.v0 * a.wld, a.wld, t.m * S::BM, a.D);
@@ -318,7 +317,7 @@ __global__ __launch_bounds__(S::kThreads) void dx_kernel(const Args a) {
     });
   }
   const bool whole = a.last && a.splits == 1;
-  float4* sums = a.sums + (int64_t)(blockIdx.x / tiles * tiles + t.m * a.tn + t.n) * (S::BM * S::BN / 4) + threadIdx.x;
+  float4* sums = a.sums + ((int64_t)(t.split * a.tm + t.m) * a.tn + t.n) * (S::BM * S::BN / 4) + threadIdx.x;
   if (!a.first || !whole) {
 #pragma unroll
     for (int j = 0; j < S::NT; ++j)
@@ -372,12 +371,11 @@ __global__ __launch_bounds__(S::kThreads) void parts_kernel(const Args a, uint16
 template <typename T, typename S>
 __global__ __launch_bounds__(S::kThreads) void dw_kernel(const Args a) {
   __shared__ __attribute__((aligned(1024))) uint8_t lds[S::kLds];
-  const uint32_t tiles = a.tm * a.tn, split = blockIdx.x / tiles;
-  const TileAt t(blockIdx.x % tiles, a.tm, a.tn);
+  const TileAt t(blockIdx.x, a.tm, a.tn, a.splits);
   const int lane = threadIdx.x & 63;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wv % S::WM, wn = wv / S::WM;
   const int slabs = (a.N + 63) / 64, per = (slabs + a.splits - 1) / a.splits;
-  const int s0 = min((int)split * per, slabs), s1 = min(s0 + per, slabs);
+  const int s0 = min(t.split * per, slabs), s1 = min(s0 + per, slabs);
   f32x16 acc[S::MT][S::NT] = {};
   {
     const TurnedCopy<S::BM, S::kWaves> ca(a.x, a.xld, t.m * S::BM, a.D);
@@ -395,7 +393,7 @@ __global__ __launch_bounds__(S::kThreads) void dw_kernel(const Args a) {
     });
   }
   if (a.splits > 1) {
-    float4* sums = a.sums + (int64_t)(blockIdx.x / tiles * tiles + t.m * a.tn + t.n) * (S::BM * S::BN / 4) + threadIdx.x;
+    float4* sums = a.sums + ((int64_t)(t.split * a.tm + t.m) * a.tn + t.n) * (S::BM * S::BN / 4) + threadIdx.x;
 #pragma unroll
     for (int j = 0; j < S::NT; ++j)
 #pragma unroll

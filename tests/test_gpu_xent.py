@@ -366,3 +366,31 @@ def test_offsets_beyond_32_bits(pkg, cuda):
         _close(dw[part], g[:, part].T @ x.double(), 1.5, ((g[:, part].square().T @ x.double().square()).sum().sqrt().item(), 1e-3), "dw")
     want = sum(g[:, v:v + 50_000] @ w[v:v + 50_000].double() for v in range(0, V, 50_000))
     _close(dx, want, 1.5, (want.norm().item(), 0.0), "dx")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("form", ["expanded", "rows", "padded"])
+def test_a_mean_adds_no_error_of_its_own(pkg, cuda, dtype, form):
+    """1 / 511 lies half a step of bf16 from its neighbours: G's largest terms, -dloss of
+    every row, are not to be off by that.  Logits of 0 and 4096 words: p = 2^-12 within
+    2^-11.8 of itself, and 1 - p is rounded to 1 in either type (2^-12 off at most); so an
+    element of dx is off by the rounding of p (2^-11 of it, in fp16) over all words, by
+    the target's 2^-12 and by its own half step."""
+    N, D, V = 511, 64, 4096
+    gen = torch.Generator(device=cuda).manual_seed(2)
+    w = torch.randn(V, D, generator=gen, device=cuda).to(dtype)
+    x = torch.zeros(N, D, device=cuda, dtype=dtype)
+    t = torch.randint(0, V, (N,), generator=gen, device=cuda)
+    dloss = torch.full((1,), 1 / 511, device=cuda).expand(N)
+    if form != "expanded":
+        dloss = dloss.contiguous()
+    if form == "padded":
+        t[::7], dloss[::7] = -100, 100.0
+    _, lse = pkg.linear_xent(x, w, t, return_lse=True)
+    dx, _ = pkg.linear_xent_bwd(x, w, t, lse, dloss)
+    counts = (t >= 0)[:, None]
+    W, Wt = w.double(), w.double()[t.clamp(min=0)]
+    want = torch.where(counts, (W.mean(0) - Wt) * dloss.double()[:, None], 0.0)
+    off = (Wt.abs() * (2.0 ** -12 + 2.0 ** -20) + W.abs().mean(0) * (2.0 ** -11 + 2.0 ** -11.8)) / 511
+    bound = UNIT[dtype] * (want.abs() + off) + off + 2.0 ** -25
+    assert ((dx.double() - want).abs() <= torch.where(counts, bound, 0.0)).all()

@@ -4,11 +4,18 @@
 //
 // A workgroup takes a tile of BM x BN outputs, M being the dimension that lies
 // contiguous in the result, and goes over the contraction in slabs of 128 bytes
-// of each row (64 elements of 16 bits, 128 of 8).  Two slabs of both operands
-// lie in LDS; slab k + 2 is copied (LDS-DMA) over slab k once every wave has its
-// last operands of k in registers, so a copy has as long as the products of a
-// whole slab, and there is one barrier a slab.  Operands of a step are read
-// from LDS while the step before it is in the matrix unit.
+// of each row (64 elements of 16 bits, 128 of 8).  A ring of S slabs of both
+// operands lies in LDS, 2 or 3; slab k + S is copied (LDS-DMA) over slab k once
+// every wave has its last operands of k in registers, so a copy has as long as the
+// products of S - 1 slabs, and there is one barrier a slab.  Operands of a step are
+// read from LDS while the step before it is in the matrix unit.
+//
+// Large tiles are 256 x 256, 8 waves of 128 x 64: 64 KB a slab for 4 times the
+// products of a 128 x 128 tile at twice its reading.  8192 x 4096 x 32000 in bf16: 1.27
+// PFLOP/s, the card at about 2.0 of its 2.4 GHz, its matrix units busy for 67 % of the
+// cycles.  Tried: slabs of 64 bytes in a ring of 4 (5 % slower: twice the barriers), 4
+// waves of 128 x 128 (17 %: one wave a SIMD, with spills), copies spread between the
+// products (no change).
 //
 // An operand is `Plain` where its rows are contiguous along the contraction and
 // `Turned` where they are contiguous along M or N (16 bits only: the transposing

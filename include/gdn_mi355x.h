@@ -533,7 +533,7 @@ int gdn_attn_decode_launch(const GdnAttnDecodeParams* params, void* stream);
  *     lse_n = log sum_v e^{l_nv},   loss_n = lse_n - l_{n, target_n}
  *     G = dloss_n (e^{l - lse} - [v = target_n]),  dx = G w,  dw = G^T x
  * A row whose target is outside [0, V) does not count: loss and lse 0, dx 0,
- * nothing in dw, whatever the row holds.  G is rounded once to dtype (fp16: in a
+ * nothing in dw, whatever the row holds.  G is rounded once to dtype (in a
  * unit from the largest |dloss|); sums are fp32, in a fixed order.
  *   - x [N,D], w [V,D]: fp16 or bf16, rows contiguous and 16-byte aligned, D a
  *     multiple of 8 (at least 8); strides at most 2^22 elements.  target: int64.

@@ -5,7 +5,9 @@ gdn_triton.py:113-140) as a hand-written gfx950 HIP kernel behind a C ABI
 (``include/gdn_mi355x.h``), called from PyTorch-ROCm through ctypes, and the
 operators that a hybrid model runs beside it: ``gated_scan`` (an elementwise
 gated recurrence), ``window_attn`` (softmax attention with a sliding window and
-sinks) and ``add_rms_norm``, with their backward and single-token forms.
+sinks) and ``add_rms_norm``, with their backward and single-token forms; the
+head's loss ``linear_xent``; and for serving ``fp8_linear`` and an 8-bit key and
+value cache (``cache_write_fp8``, ``window_attn_decode_fp8``).
 
 The directory name is not a Python identifier; import it with
 ``importlib.import_module("v100-attention-lab_amd")`` -- it also registers

@@ -539,8 +539,10 @@ int gdn_attn_decode_launch(const GdnAttnDecodeParams* params, void* stream);
  *     multiple of 8 (at least 8); strides at most 2^22 elements.  target: int64.
  *   - lse: written by the forward, read by the backward; dloss: fp32 with a
  *     stride (0: one value for all rows); dx, dw: dense, dtype.
- *   - N below 2^26, V up to 2^28; workspaces of gdn_xent[_bwd]_workspace_size()
- *     bytes, 256-byte aligned. */
+ *   - N below 2^26, V up to 2^28; GDN_ERR_BAD_SHAPE (and a workspace size of -1) from
+ *     2^32 threads a launch on: 512 for each 256 x 256 of N x V (N V of about 5.5e11),
+ *     256 for each 128 x 128 of D x N and of D x V.  Workspaces of
+ *     gdn_xent[_bwd]_workspace_size() bytes, 256-byte aligned. */
 typedef struct GdnXentParams {
   const void* x;
   const void* w;

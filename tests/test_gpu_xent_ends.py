@@ -1,5 +1,5 @@
 """GPU tests of linear_xent at the ends of its range: sure predictions, logits of
-thousands.
+thousands, more logits than 2^37.
 
 Where logits have to be exact, rows are unit vectors: the logits of row n are
 column n % 64 of the weight, without a rounding."""
@@ -8,7 +8,7 @@ import math
 
 import pytest
 import torch
-from test_gpu_xent import DTYPES, _close, oracle
+from test_gpu_xent import DTYPES, _close, _losses, oracle
 
 pytestmark = pytest.mark.gpu
 
@@ -97,3 +97,27 @@ def test_logits_of_thousands(pkg, cuda, dtype):
     offs = ((off.square() @ w.double().square()).sum().sqrt().item(), (off.square().T @ x.double().square()).sum().sqrt().item())
     _close(dx, wx, 1.5, (sizes[0][0], offs[0]), "dx")
     _close(dw, ww, 1.5, (sizes[1][0], offs[1]), "dw")
+
+
+def test_a_million_rows_of_a_large_vocabulary(pkg, cuda):
+    """More logits than the smallest tiles' launch would hold: forward and backward,
+    some rows (the last among them) and some words against the formulas."""
+    N, V, K = 1_000_000, 151_936, 8
+    gen = torch.Generator(device=cuda).manual_seed(2)
+    x = torch.randn(N, K, generator=gen, device=cuda).bfloat16()
+    w = torch.randn(V, K, generator=gen, device=cuda).bfloat16()
+    t = torch.randint(-1000, V, (N,), generator=gen, device=cuda)
+    loss, lse = pkg.linear_xent(x, w, t, return_lse=True)
+    some = torch.cat([torch.randint(0, N, (100,), generator=gen, device=cuda), torch.arange(N - 100, N, device=cuda)])
+    ones = torch.ones(1, device=cuda).expand(N)
+    want, want_lse, wx, _, sizes = oracle(x[some], w, t[some], ones[some])
+    _losses(loss[some], lse[some], want, want_lse)
+    dx, dw = pkg.linear_xent_bwd(x, w, t, lse, ones)
+    _close(dx[some], wx, 1.5, sizes[0], "dx")
+    words = torch.cat([torch.arange(20, device=cuda), torch.arange(V - 20, V, device=cuda)])
+    counts = (t >= 0)[:, None]
+    g = torch.where(counts, torch.exp(x.double() @ w[words].double().T - lse.double()[:, None]), 0.0)
+    off = g * 2.0 ** -15 * (1 + lse.abs())[:, None]
+    g -= (t[:, None] == words).double()
+    sq = lambda z: (z.square().T @ x.double().square()).sum().sqrt().item()
+    _close(dw[words], g.T @ x.double(), 1.5, (sq(g), sq(off)), "dw")

@@ -1,0 +1,27 @@
+"""CPU tests of the sizes that linear_xent, the 8-bit product and the 8-bit cache take,
+at their ends (nothing is enqueued: what is in order but for its workspace is told so)."""
+
+import ctypes
+
+import pytest
+import torch
+from test_head_and_fp8_host import _xent, lib  # noqa: F401
+
+
+@pytest.mark.parametrize("name", ["gdn_xent", "gdn_xent_bwd"])
+@pytest.mark.parametrize("kw,ok", [
+    (dict(N=1_000_000, V=151_936), True), (dict(N=4_000_000, V=128_000), True), (dict(N=(1 << 26) - 1, V=7900), True), (dict(N=(1 << 26) - 1, V=8000), False),
+    (dict(N=40, V=1 << 28), True), (dict(N=5_000_000, V=128_000), False), (dict(N=1 << 20, V=1 << 20), False)])
+def test_xent_takes_what_a_launch_holds(lib, pkg, name, kw, ok):  # noqa: F811
+    P = lambda **more: ctypes.byref(_xent(pkg._lib, **kw, **more))
+    assert getattr(lib, name + "_launch")(P(workspace=None), None) == (1006 if ok else 1002)
+    assert (getattr(lib, name + "_workspace_size")(P()) > 0) == ok
+
+
+def test_too_many_logits_is_a_value_error(pkg, monkeypatch):
+    from importlib import import_module
+    L = import_module("v100-attention-lab_amd.loss")
+    monkeypatch.setattr(L, "_validate", lambda *a: None)
+    x, w = (torch.empty(1, 64, dtype=torch.float16).expand(n, 64) for n in (1 << 20, 1 << 20))
+    with pytest.raises(ValueError, match="does not support"):
+        L._plan(x, w, None, None, None, False)

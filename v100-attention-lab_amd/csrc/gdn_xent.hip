@@ -47,6 +47,7 @@ using attn::swap_halves;
 // workgroup beside: 128 rows, 16000 words of 2048 32 -> 26 us (Wide for Mid), 48 rows,
 // 50257 words 56 -> 53 (Narrow with 3 slabs for 2; with 4 and one workgroup 58).
 typedef Shape<4, 2, 2, 4> Big;         // 256 x 256, one workgroup a CU
+static_assert(Big::BM == 256 && Big::BN == 256 && Big::kThreads == 512, "as check() counts them");
 typedef Shape<2, 2, 2, 2> Mid;         // 128 x 128, two
 typedef Shape<2, 2, 2, 2, 3> Wide;     // the same, one
 typedef Shape<2, 1, 2, 2, 3> Narrow;   // 128 x 64 (vocabulary x rows), two
@@ -446,18 +447,6 @@ __global__ __launch_bounds__(S::kThreads) void dw_kernel(const Args a) {
 inline int64_t ceil_to(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 inline int64_t tiles_of(int64_t m, int64_t n, int bm, int bn) { return (m + bm - 1) / bm * ((n + bn - 1) / bn); }
 
-int check(const GdnXentParams& P) {
-  if (P.N < 0 || P.D < 8 || P.V < 1) return GDN_ERR_BAD_SHAPE;
-  if (P.D % 8 != 0) return GDN_ERR_UNSUPPORTED;
-  if (P.dtype != GDN_DTYPE_F16 && P.dtype != GDN_DTYPE_BF16) return GDN_ERR_BAD_DTYPE;
-  // rows of a tile lie within 31 bits
-  if ((P.N > 1 && (P.x_stride < 0 || P.x_stride > 1 << 22)) || (P.V > 1 && (P.w_stride < 0 || P.w_stride > 1 << 22)) ||
-      P.D > 1 << 22)
-    return GDN_ERR_UNSUPPORTED;
-  if (P.N >= 1 << 26 || P.V > 1 << 28) return GDN_ERR_BAD_SHAPE;      // (the join has 64 threads a row)
-  return GDN_OK;
-}
-
 // Tiles of 256 x 256 or of 128 x 128, by the rounds that they make of the card: 256 at
 // a time take about 13 parts of time, 512 small ones 8.  So small ones up to 512, and
 // where the big ones leave much of their second round idle: logits of 1024 rows of 2048
@@ -472,6 +461,24 @@ Kind logits_kind(int64_t v, int64_t rows) {
   if (rows <= 64) return kNarrow;
   const Kind k = kind_of(v, rows);
   return k == kMid && tiles_of(v, rows, 128, 128) <= 256 ? kWide : k;
+}
+
+int check(const GdnXentParams& P) {
+  if (P.N < 0 || P.D < 8 || P.V < 1) return GDN_ERR_BAD_SHAPE;
+  if (P.D % 8 != 0) return GDN_ERR_UNSUPPORTED;
+  if (P.dtype != GDN_DTYPE_F16 && P.dtype != GDN_DTYPE_BF16) return GDN_ERR_BAD_DTYPE;
+  // rows of a tile lie within 31 bits
+  if ((P.N > 1 && (P.x_stride < 0 || P.x_stride > 1 << 22)) || (P.V > 1 && (P.w_stride < 0 || P.w_stride > 1 << 22)) ||
+      P.D > 1 << 22)
+    return GDN_ERR_UNSUPPORTED;
+  if (P.N >= 1 << 26 || P.V > 1 << 28) return GDN_ERR_BAD_SHAPE;      // (the join has 64 threads a row)
+  // one launch each: the logits in the tiles that they are made in (512 threads for
+  // 256 x 256, the smaller ones are chosen for few alone), the gradients in the smallest
+  const bool big = logits_kind(P.V, P.N) == kBig;
+  if (!(big ? grid_fits(tiles_of(P.V, P.N, 256, 256), 512) : grid_fits(tiles_of(P.V, P.N, 128, 64), 256)) ||
+      !grid_fits(tiles_of(P.D, std::max(P.N, P.V), 128, 128), 256))
+    return GDN_ERR_BAD_SHAPE;
+  return GDN_OK;
 }
 
 // Vocabulary of a piece: G takes about 128 MiB.
@@ -637,9 +644,6 @@ static int check_call(const GdnXentParams& P, int64_t need) {
   if (st != GDN_OK) return st;
   if ((P.N > 0 && (P.x == nullptr || P.target == nullptr || P.lse == nullptr)) || P.w == nullptr) return GDN_ERR_NULL_POINTER;
   if (!rows_ok(P.x, P.x_stride, P.N) || !rows_ok(P.w, P.w_stride, P.V)) return GDN_ERR_MISALIGNED;
-  // workgroups of the smallest tiles
-  if (!grid_fits(tiles_of(P.V, P.N, 128, 64), 256) || !grid_fits(tiles_of(P.D, std::max(P.N, P.V), 128, 128), 256))
-    return GDN_ERR_BAD_SHAPE;
   if (need > 0 && (P.workspace == nullptr || P.workspace_bytes < need ||
                    reinterpret_cast<uintptr_t>(P.workspace) % 256 != 0))
     return GDN_ERR_WORKSPACE;

@@ -25,3 +25,13 @@ def test_too_many_logits_is_a_value_error(pkg, monkeypatch):
     x, w = (torch.empty(1, 64, dtype=torch.float16).expand(n, 64) for n in (1 << 20, 1 << 20))
     with pytest.raises(ValueError, match="does not support"):
         L._plan(x, w, None, None, None, False)
+
+
+def test_xent_workspace_is_what_the_tiles_leave(lib, pkg):  # noqa: F811
+    """A pair (8 bytes) for a row and tile of the vocabulary, 256 words in the large
+    tiles and 128 in the others, and a row's target logit."""
+    size = lambda **kw: lib.gdn_xent_workspace_size(ctypes.byref(_xent(pkg._lib, **kw)))
+    assert size(N=1_000_000, V=128_000) == 1_000_000 * (500 * 8 + 4)
+    assert size(N=8192, V=32_001) == 8192 * (126 * 8 + 4)
+    assert size(N=64, V=50_257) == 64 * (393 * 8 + 4)
+    assert size(N=1000, V=500) == 1000 * (4 * 8 + 4)

@@ -527,7 +527,11 @@ struct BwdLayout {
   }
 };
 
-int64_t fwd_tiles(const GdnXentParams& P) { return (P.V + 127) / 128; }
+// Pairs that the forward leaves for a row: one a tile.
+int64_t fwd_tiles(const GdnXentParams& P) {
+  const int bm = logits_kind(P.V, P.N) == kBig ? 256 : 128;
+  return (P.V + bm - 1) / bm;
+}
 
 Args args_of(const GdnXentParams& P) {
   Args a = {};

@@ -534,7 +534,7 @@ int gdn_attn_decode_launch(const GdnAttnDecodeParams* params, void* stream);
  *     G = dloss_n (e^{l - lse} - [v = target_n]),  dx = G w,  dw = G^T x
  * A row whose target is outside [0, V) does not count: loss and lse 0, dx 0,
  * nothing in dw, whatever the row holds.  G is rounded once to dtype (in a
- * unit from the largest |dloss|); sums are fp32, in a fixed order.
+ * unit from the largest finite |dloss|); sums are fp32, in a fixed order.
  *   - x [N,D], w [V,D]: fp16 or bf16, rows contiguous and 16-byte aligned, D a
  *     multiple of 8 (at least 8); strides at most 2^22 elements.  target: int64.
  *   - lse: written by the forward, read by the backward; dloss: fp32 with a

@@ -1,5 +1,5 @@
 """GPU tests of linear_xent at the ends of its range: sure predictions, logits of
-thousands, more logits than 2^37.
+thousands, dloss that is not finite, more logits than 2^37.
 
 Where logits have to be exact, rows are unit vectors: the logits of row n are
 column n % 64 of the weight, without a rounding."""
@@ -8,7 +8,7 @@ import math
 
 import pytest
 import torch
-from test_gpu_xent import DTYPES, _close, _losses, oracle
+from test_gpu_xent import DTYPES, _close, _inputs, _losses, oracle
 
 pytestmark = pytest.mark.gpu
 
@@ -97,6 +97,21 @@ def test_logits_of_thousands(pkg, cuda, dtype):
     offs = ((off.square() @ w.double().square()).sum().sqrt().item(), (off.square().T @ x.double().square()).sum().sqrt().item())
     _close(dx, wx, 1.5, (sizes[0][0], offs[0]), "dx")
     _close(dw, ww, 1.5, (sizes[1][0], offs[1]), "dw")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_dloss_that_is_not_finite_stays_its_rows(pkg, cuda, dtype, bad):
+    """The other rows' gradients as without it, though G has one unit for all."""
+    x, w, t, dloss = _inputs(cuda, 200, 64, 1500, dtype, 4)
+    w, x, dloss = (w.float() * 2 ** 12).to(dtype), (x.float() / 2 ** 12).to(dtype), dloss / 2 ** 10
+    lse = pkg.linear_xent(x, w, t, return_lse=True)[1]
+    keep = torch.arange(200, device=cuda) != 7
+    wx, sizes = oracle(x, w, t, dloss)[2::2]
+    dloss[7] = bad
+    dx, dw = pkg.linear_xent_bwd(x, w, t, lse, dloss)
+    _close(dx[keep], wx[keep], 1.5, sizes[0], "dx")
+    assert not torch.isfinite(dx[7]).any() and not torch.isfinite(dw[t[7]]).any()
 
 
 def test_a_million_rows_of_a_large_vocabulary(pkg, cuda):

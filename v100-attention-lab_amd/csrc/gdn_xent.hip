@@ -22,7 +22,7 @@
 // ms, dX with its fp32 sums read and written.  48 rows of 2048 against 50257 words are
 // bound by reading the weight, 32 us at 6.4 TB/s where the last-level cache holds it.
 //
-// G is kept in a unit that makes the largest |dloss| a power of 2.  A mean gives all
+// G is kept in a unit that makes the largest finite |dloss| a power of 2.  A mean gives all
 // rows the same dloss, and the target's G, close to -dloss, outweighs the others: it
 // is then rounded not at all where the target is improbable, and else by the row and
 // not for all alike (511 x 1024 x 4000, dloss 1/511, bf16: dX 0.0024 -> 0.0017 off).  In fp16 the
@@ -226,7 +226,8 @@ __global__ __launch_bounds__(kRowsNT) void rows_kernel(const Args a) {
         d[i] = fabsf(a.dloss[n * a.dloss_step]);
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) top = t[i] >= 0 && t[i] < a.V ? fmaxf(top, d[i]) : top;
+      for (int i = 0; i < 4; ++i)      // (of the finite ones: one that is not is its row's alone)
+        top = t[i] >= 0 && t[i] < a.V && d[i] < __builtin_inff() ? fmaxf(top, d[i]) : top;
     }
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));

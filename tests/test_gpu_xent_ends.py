@@ -1,5 +1,5 @@
 """GPU tests of linear_xent at the ends of its range: sure predictions, logits of
-thousands, dloss that is not finite, more logits than 2^37.
+thousands, dloss of every size and not finite, more logits than 2^37.
 
 Where logits have to be exact, rows are unit vectors: the logits of row n are
 column n % 64 of the weight, without a rounding."""
@@ -97,6 +97,33 @@ def test_logits_of_thousands(pkg, cuda, dtype):
     offs = ((off.square() @ w.double().square()).sum().sqrt().item(), (off.square().T @ x.double().square()).sum().sqrt().item())
     _close(dx, wx, 1.5, (sizes[0][0], offs[0]), "dx")
     _close(dw, ww, 1.5, (sizes[1][0], offs[1]), "dw")
+
+
+# dloss, and the size of the operand that brings the gradient into fp16's range
+SIZES = [(2.0 ** -30, 2.0 ** 13), (2.0 ** -16, 2.0 ** 8), (1.0, 1.0), (2.0 ** 16, 2.0 ** -8)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("f,c", SIZES)
+@pytest.mark.parametrize("which", ["dx", "dw"])
+def test_dloss_of_every_size(pkg, cuda, dtype, f, c, which):
+    """The unit of G follows dloss: a mean over many rows, a loss scale.  One operand is
+    as large as makes its gradient a number of fp16, the other as small as keeps the
+    logits."""
+    gen = torch.Generator(device=cuda).manual_seed(6)
+    N, V = 1100, 1100
+    x, w = torch.randn(N, D, generator=gen, device=cuda), torch.randn(V, D, generator=gen, device=cuda)
+    a, b = (0.25 / c, c) if which == "dx" else (c, 0.25 / c)
+    x, w = (x * a).to(dtype), (w * b).to(dtype)
+    t = torch.randint(0, V, (N,), generator=gen, device=cuda)
+    dloss = f * (0.5 + torch.rand(N, generator=gen, device=cuda))
+    lse = pkg.linear_xent(x, w, t, return_lse=True)[1]
+    got = pkg.linear_xent_bwd(x, w, t, lse, dloss)
+    _, _, wx, ww, sizes = oracle(x, w, t, dloss)
+    i = 0 if which == "dx" else 1
+    want = (wx, ww)[i]
+    assert want.norm() > 100 * 2.0 ** -25 * want.numel() ** 0.5       # (more than fp16's steps near zero)
+    _close(got[i], want, 1.5, sizes[i], which)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

@@ -403,13 +403,15 @@ __global__ __launch_bounds__(kQ) void quant_groups_kernel(const QArgs a) {
   store_fp8<8>(a.q + (int64_t)row * a.D + c, v);
 }
 
-// A whole row, read twice: a workgroup.
+// A whole row, read twice: a workgroup.  (Columns are counted past the last one, which
+// 31 bits need not hold.)
 template <typename T>
 __global__ __launch_bounds__(kQ) void quant_rows_kernel(const QArgs a) {
   const int64_t row = blockIdx.x;
+  const uint32_t D = a.D;
   const T* x = static_cast<const T*>(a.x) + row * a.ld;
   float m = 0.f;
-  for (int c = threadIdx.x * 8; c < a.D; c += kQ * 8) {
+  for (uint32_t c = threadIdx.x * 8; c < D; c += kQ * 8) {
     Pack<T, 8> p;
     p.load(x + c);
 #pragma unroll
@@ -424,7 +426,7 @@ __global__ __launch_bounds__(kQ) void quant_rows_kernel(const QArgs a) {
   m = m / kFp8Max;
   if (threadIdx.x == 0) a.scale[row] = m;
   const Quant quant(m);
-  for (int c = threadIdx.x * 8; c < a.D; c += kQ * 8) {
+  for (uint32_t c = threadIdx.x * 8; c < D; c += kQ * 8) {
     Pack<T, 8> p;
     p.load(x + c);
     float v[8];

@@ -570,8 +570,8 @@ int gdn_xent_bwd_launch(const GdnXentParams* params, void* stream);
  * that is stored) rounded to the nearest; a group of zeros has scale 0, one with a
  * NaN is NaN.  A group is 128 columns of a row (scale [rows, D / 128]), a row
  * ([rows]) or a block of 128 x 128 ([ceil(rows / 128), D / 128]).
- *   - x: any dtype, rows contiguous and 16-byte aligned, D a multiple of 128;
- *     q [rows, D] and scale dense. */
+ *   - x: any dtype, rows contiguous and 16-byte aligned, D a multiple of 128, any
+ *     rows (below 2^38 elements); q [rows, D] and scale dense. */
 enum GdnFp8Mode { GDN_FP8_GROUPS = 0, GDN_FP8_ROWS = 1, GDN_FP8_BLOCKS = 2 };
 
 typedef struct GdnFp8QuantParams {

@@ -376,6 +376,7 @@ struct QArgs {
   int64_t ld;        // elements between rows
   int rows, D;
   uint32_t groups;   // of all rows
+  uint32_t first;    // workgroup of a launch
 };
 
 constexpr int kQ = 256;
@@ -383,7 +384,7 @@ constexpr int kQ = 256;
 // A group of 128 columns: 16 lanes.
 template <typename T>
 __global__ __launch_bounds__(kQ) void quant_groups_kernel(const QArgs a) {
-  const uint32_t g = blockIdx.x * (kQ / 16) + threadIdx.x / 16, per = a.D / 128;
+  const uint32_t g = (a.first + blockIdx.x) * (kQ / 16) + threadIdx.x / 16, per = a.D / 128;
   const bool ok = g < a.groups;
   const uint32_t row = ok ? g / per : 0, c = (ok ? g - row * per : 0) * 128 + threadIdx.x % 16 * 8;
   Pack<T, 8> x;
@@ -407,7 +408,7 @@ __global__ __launch_bounds__(kQ) void quant_groups_kernel(const QArgs a) {
 // 31 bits need not hold.)
 template <typename T>
 __global__ __launch_bounds__(kQ) void quant_rows_kernel(const QArgs a) {
-  const int64_t row = blockIdx.x;
+  const int64_t row = a.first + blockIdx.x;
   const uint32_t D = a.D;
   const T* x = static_cast<const T*>(a.x) + row * a.ld;
   float m = 0.f;
@@ -439,7 +440,7 @@ __global__ __launch_bounds__(kQ) void quant_rows_kernel(const QArgs a) {
 // A block of 128 x 128 of a weight: 16 lanes a row, 8 rows a thread.
 template <typename T>
 __global__ __launch_bounds__(kQ) void quant_blocks_kernel(const QArgs a) {
-  const uint32_t per = a.D / 128, br = blockIdx.x / per, bc = blockIdx.x - br * per;
+  const uint32_t block = a.first + blockIdx.x, per = a.D / 128, br = block / per, bc = block - br * per;
   const int c = bc * 128 + threadIdx.x % 16 * 8, r0 = br * 128 + threadIdx.x / 16;
   Pack<T, 8> x[8];
   float m = 0.f;
@@ -457,7 +458,7 @@ __global__ __launch_bounds__(kQ) void quant_blocks_kernel(const QArgs a) {
 #pragma unroll
   for (int w = 0; w < kQ / 64; ++w) m = nan_max(m, slots[w]);
   m = m / kFp8Max;
-  if (threadIdx.x == 0) a.scale[blockIdx.x] = m;
+  if (threadIdx.x == 0) a.scale[block] = m;
   const Quant quant(m);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -508,14 +509,22 @@ void launch_linear(LArgs& a, hipStream_t s) {
   launch_tiles<Low8, EXACT>(a, s);
 }
 
+// As many launches as the workgroups take (see grid_fits).
 template <typename T>
-void launch_quant(const QArgs& a, int mode, hipStream_t s) {
-  if (mode == GDN_FP8_GROUPS)
-    hipLaunchKernelGGL((quant_groups_kernel<T>), dim3((a.groups + kQ / 16 - 1) / (kQ / 16)), dim3(kQ), 0, s, a);
-  else if (mode == GDN_FP8_ROWS)
-    hipLaunchKernelGGL((quant_rows_kernel<T>), dim3(a.rows), dim3(kQ), 0, s, a);
-  else
-    hipLaunchKernelGGL((quant_blocks_kernel<T>), dim3((uint32_t)((a.rows + 127) / 128) * (a.D / 128)), dim3(kQ), 0, s, a);
+int launch_quant(QArgs a, int mode, hipStream_t s) {
+  constexpr uint32_t kMost = 1 << 23;
+  static_assert(kMost <= 0xffffffffu / kQ, "one launch holds them");
+  const uint32_t all = mode == GDN_FP8_GROUPS ? (a.groups + kQ / 16 - 1) / (kQ / 16)
+                       : mode == GDN_FP8_ROWS ? (uint32_t)a.rows
+                                              : ((uint32_t)a.rows + 127) / 128 * (a.D / 128);
+  for (; a.first < all; a.first += kMost) {
+    const dim3 grid(std::min(kMost, all - a.first));
+    if (mode == GDN_FP8_GROUPS) hipLaunchKernelGGL((quant_groups_kernel<T>), grid, dim3(kQ), 0, s, a);
+    else if (mode == GDN_FP8_ROWS) hipLaunchKernelGGL((quant_rows_kernel<T>), grid, dim3(kQ), 0, s, a);
+    else hipLaunchKernelGGL((quant_blocks_kernel<T>), grid, dim3(kQ), 0, s, a);
+    if (const int st = (int)hipGetLastError()) return st;
+  }
+  return GDN_OK;
 }
 
 }  // namespace fp8
@@ -538,7 +547,7 @@ int gdn_fp8_quant_launch(const GdnFp8QuantParams* prm, void* stream) {
       reinterpret_cast<uintptr_t>(P.q) % 8 != 0)
     return GDN_ERR_MISALIGNED;
   const int64_t groups = (int64_t)P.rows * (P.D / 128);
-  if (!grid_fits(groups, 16) || !grid_fits(P.rows, kQ)) return GDN_ERR_BAD_SHAPE;
+  if (groups > 0x7fffffff) return GDN_ERR_BAD_SHAPE;      // they are counted in 32 bits
   QArgs a = {};
   a.x = P.x;
   a.q = static_cast<uint8_t*>(P.q);
@@ -548,10 +557,9 @@ int gdn_fp8_quant_launch(const GdnFp8QuantParams* prm, void* stream) {
   a.D = P.D;
   a.groups = (uint32_t)groups;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (P.x_dtype == GDN_DTYPE_F16) launch_quant<f16>(a, P.mode, s);
-  else if (P.x_dtype == GDN_DTYPE_BF16) launch_quant<bf16_t>(a, P.mode, s);
-  else launch_quant<float>(a, P.mode, s);
-  return (int)hipGetLastError();
+  if (P.x_dtype == GDN_DTYPE_F16) return launch_quant<f16>(a, P.mode, s);
+  if (P.x_dtype == GDN_DTYPE_BF16) return launch_quant<bf16_t>(a, P.mode, s);
+  return launch_quant<float>(a, P.mode, s);
 }
 
 int gdn_fp8_linear_launch(const GdnFp8LinearParams* prm, void* stream) {

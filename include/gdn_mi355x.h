@@ -618,6 +618,7 @@ int gdn_fp8_linear_launch(const GdnFp8LinearParams* params, void* stream);
  *     cache_seqlens[b] - T .. cache_seqlens[b] - 1; those that would lie before
  *     row 0 are dropped.  Other rows are not touched.
  *   - read: all S rows into k, v [B,S,Hk,D] (dtype), byte times scale rounded once.
+ *     Write and read take B T Hk and B S Hk below 2^31.
  *   - decode: q, o [B,T,Hq,D] (fp16 or bf16), T in 1..16; as
  *     gdn_attn_decode_launch over k_cache k_scale and v_cache v_scale.  P times
  *     v_scale is rounded to dtype before its product.

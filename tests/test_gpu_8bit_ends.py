@@ -1,9 +1,11 @@
-"""GPU tests of the quantisers at their largest sizes."""
+"""GPU tests of the quantisers and of the 8-bit cache at their largest sizes."""
 
 import pytest
 import torch
 
 pytestmark = pytest.mark.gpu
+
+FP8 = torch.float8_e4m3fn
 
 
 @pytest.mark.parametrize("group", [128, None])
@@ -33,3 +35,35 @@ def test_the_longest_row(pkg, cuda, form):
     assert torch.equal(q.view(torch.uint8)[:, -384:], q2.view(torch.uint8)) and torch.equal(s[:, -s2.shape[1]:], s2)
     assert int((q.view(torch.uint8)[:, :-300] != 0).any()) == 0
     assert int((s != 0).sum()) == s2.shape[1]
+
+
+def _all_rows_are(t, row):
+    """t [rows, n bytes] holds `row` everywhere."""
+    words, row = t.view(torch.int64), row.view(torch.int64)
+    for i in range(0, len(words), 2 ** 25):
+        assert bool((words[i:i + 2 ** 25] == row).all()), i
+
+
+def test_a_prompt_of_more_rows_than_a_launch_holds(pkg, cuda):
+    """2^28 rows and more are 2^32 threads for keys and values; the rows behind are left."""
+    T, D = 2 ** 28 + 7, 128
+    gen = torch.Generator(device=cuda).manual_seed(1)
+    k, v = torch.randn(2, 1, 1, 1, D, generator=gen, device=cuda).bfloat16().unbind()
+    kc, vc = (torch.zeros(1, T + 9, 1, D, dtype=torch.uint8, device=cuda).view(FP8) for _ in range(2))
+    ks, vs = torch.zeros(1, T + 9, 1, device=cuda), torch.zeros(1, T + 9, 1, device=cuda)
+    lens = torch.tensor([T], dtype=torch.int32, device=cuda)
+    pkg.cache_write_fp8(k.expand(1, T, 1, D), v.expand(1, T, 1, D), kc, vc, ks, vs, lens)
+    for x, c, s in ((k, kc, ks), (v, vc, vs)):
+        q, scale = pkg.quantize_fp8(x.view(1, D), group=None)
+        _all_rows_are(c.view(torch.uint8)[0, :T, 0], q.view(torch.uint8))
+        assert bool((s[0, :T] == scale).all()) and not s[0, T:].any() and not c.view(torch.uint8)[0, T:].any()
+
+
+def test_a_cache_of_more_rows_than_a_launch_holds(pkg, cuda):
+    S, D = 2 ** 28 + 7, 128
+    gen = torch.Generator(device=cuda).manual_seed(1)
+    q = torch.randn(2, D, generator=gen, device=cuda).to(FP8).view(torch.uint8)
+    kc, vc = q.view(FP8).view(2, 1, 1, 1, D).expand(2, 1, S, 1, D).unbind()
+    ks, vs = torch.tensor([0.5, 2.0], device=cuda).view(2, 1, 1, 1).expand(2, 1, S, 1).unbind()
+    for x, row, f in zip(pkg.cache_read_fp8(kc, vc, ks, vs), q.view(FP8), (0.5, 2.0)):
+        _all_rows_are(x.view(S, D), (row.float() * f).bfloat16())

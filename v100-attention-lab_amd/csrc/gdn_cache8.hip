@@ -50,6 +50,7 @@ struct Args {
   float* part;          // [units][splits][32][D + 3]
   int64_t kst[3], vst[3], qst[3], ost[3], kcst[3], vcst[3], ksst[3], vsst[3];
   int B, T, S, Hk, G, tiles_r, splits, window, sinks;
+  uint32_t first;       // workgroup of a launch (write, read)
   float scale_log2;
   uint32_t flip;
 };
@@ -68,7 +69,7 @@ constexpr int kRowNT = 256;
 template <typename E, int D>
 __global__ __launch_bounds__(kRowNT) void write_kernel(const Args a) {
   constexpr int L = D / 16;
-  const uint32_t row = blockIdx.x * (kRowNT / L) + threadIdx.x / L, e0 = threadIdx.x % L * 16;
+  const uint32_t row = (a.first + blockIdx.x) * (kRowNT / L) + threadIdx.x / L, e0 = threadIdx.x % L * 16;
   const uint32_t per = a.T * a.Hk;
   if (row >= a.B * per) return;       // (the row's lanes leave together)
   const int b = row / per, r = row - b * per, t = r / a.Hk, h = r - t * a.Hk;
@@ -102,7 +103,7 @@ __global__ __launch_bounds__(kRowNT) void write_kernel(const Args a) {
 template <typename E, int D>
 __global__ __launch_bounds__(kRowNT) void read_kernel(const Args a) {
   constexpr int L = D / 16;
-  const uint32_t row = blockIdx.x * (kRowNT / L) + threadIdx.x / L, e0 = threadIdx.x % L * 16;
+  const uint32_t row = (a.first + blockIdx.x) * (kRowNT / L) + threadIdx.x / L, e0 = threadIdx.x % L * 16;
   const uint32_t per = a.S * a.Hk;
   if (row >= a.B * per) return;
   const int b = row / per, r = row - b * per, s = r / a.Hk, h = r - s * a.Hk;
@@ -559,21 +560,33 @@ Args args_of(const GdnCache8Params& P) {
   return a;
 }
 
-template <typename E>
-void launch_write(const Args& a, int D, hipStream_t s) {
-  const int64_t rows = (int64_t)a.B * a.T * a.Hk;
-  const int per = kRowNT / (D / 16);
-  const dim3 grid((uint32_t)((rows + per - 1) / per), 2);
-  if (D == 128) hipLaunchKernelGGL((write_kernel<E, 128>), grid, dim3(kRowNT), 0, s, a);
-  else hipLaunchKernelGGL((write_kernel<E, 64>), grid, dim3(kRowNT), 0, s, a);
+// launch(args, grid) for keys and values of all rows, as many launches as they take
+// (see grid_fits).
+template <typename F>
+int by_rows(Args a, int64_t rows, int D, F launch) {
+  constexpr uint32_t kMost = 1 << 22;
+  static_assert(2 * kMost <= 0xffffffffu / kRowNT, "one launch holds them");
+  const int64_t per = kRowNT / (D / 16);
+  const uint32_t all = (uint32_t)((rows + per - 1) / per);
+  for (; a.first < all; a.first += kMost) {
+    launch(a, dim3(std::min(kMost, all - a.first), 2));
+    if (const int st = (int)hipGetLastError()) return st;
+  }
+  return GDN_OK;
 }
 template <typename E>
-void launch_read(const Args& a, int D, hipStream_t s) {
-  const int64_t rows = (int64_t)a.B * a.S * a.Hk;
-  const int per = kRowNT / (D / 16);
-  const dim3 grid((uint32_t)((rows + per - 1) / per), 2);
-  if (D == 128) hipLaunchKernelGGL((read_kernel<E, 128>), grid, dim3(kRowNT), 0, s, a);
-  else hipLaunchKernelGGL((read_kernel<E, 64>), grid, dim3(kRowNT), 0, s, a);
+int launch_write(const Args& a, int D, hipStream_t s) {
+  return by_rows(a, (int64_t)a.B * a.T * a.Hk, D, [&](const Args& b, dim3 grid) {
+    if (D == 128) hipLaunchKernelGGL((write_kernel<E, 128>), grid, dim3(kRowNT), 0, s, b);
+    else hipLaunchKernelGGL((write_kernel<E, 64>), grid, dim3(kRowNT), 0, s, b);
+  });
+}
+template <typename E>
+int launch_read(const Args& a, int D, hipStream_t s) {
+  return by_rows(a, (int64_t)a.B * a.S * a.Hk, D, [&](const Args& b, dim3 grid) {
+    if (D == 128) hipLaunchKernelGGL((read_kernel<E, 128>), grid, dim3(kRowNT), 0, s, b);
+    else hipLaunchKernelGGL((read_kernel<E, 64>), grid, dim3(kRowNT), 0, s, b);
+  });
 }
 template <typename T, int D>
 void launch_decode(const Args& a, hipStream_t s) {
@@ -603,14 +616,12 @@ int gdn_cache8_write_launch(const GdnCache8Params* prm, void* stream) {
   const int es = dtype_bytes(P.dtype);
   if (!rows_ok(P.k, P.k_stride, P.B, P.T, P.Hk, es) || !rows_ok(P.v, P.v_stride, P.B, P.T, P.Hk, es) || !cache_ok(P))
     return GDN_ERR_MISALIGNED;
-  // (two of these: keys and values)
-  if ((int64_t)P.T * P.Hk > 0x7fffffff || !grid_fits((int64_t)P.B * P.T * P.Hk, 2 * P.D / 16)) return GDN_ERR_BAD_SHAPE;
+  if ((int64_t)P.T * P.Hk > 0x7fffffff / P.B) return GDN_ERR_BAD_SHAPE;      // rows are 32-bit
   const Args a = args_of(P);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (P.dtype == GDN_DTYPE_F16) launch_write<f16>(a, P.D, s);
-  else if (P.dtype == GDN_DTYPE_BF16) launch_write<bf16_t>(a, P.D, s);
-  else launch_write<float>(a, P.D, s);
-  return (int)hipGetLastError();
+  if (P.dtype == GDN_DTYPE_F16) return launch_write<f16>(a, P.D, s);
+  if (P.dtype == GDN_DTYPE_BF16) return launch_write<bf16_t>(a, P.D, s);
+  return launch_write<float>(a, P.D, s);
 }
 
 int gdn_cache8_read_launch(const GdnCache8Params* prm, void* stream) {
@@ -624,13 +635,12 @@ int gdn_cache8_read_launch(const GdnCache8Params* prm, void* stream) {
   const int es = dtype_bytes(P.dtype);
   if (!rows_ok(P.k, P.k_stride, P.B, P.S, P.Hk, es) || !rows_ok(P.v, P.v_stride, P.B, P.S, P.Hk, es) || !cache_ok(P))
     return GDN_ERR_MISALIGNED;
-  if ((int64_t)P.S * P.Hk > 0x7fffffff || !grid_fits((int64_t)P.B * P.S * P.Hk, 2 * P.D / 16)) return GDN_ERR_BAD_SHAPE;
+  if ((int64_t)P.S * P.Hk > 0x7fffffff / P.B) return GDN_ERR_BAD_SHAPE;      // rows are 32-bit
   const Args a = args_of(P);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (P.dtype == GDN_DTYPE_F16) launch_read<f16>(a, P.D, s);
-  else if (P.dtype == GDN_DTYPE_BF16) launch_read<bf16_t>(a, P.D, s);
-  else launch_read<float>(a, P.D, s);
-  return (int)hipGetLastError();
+  if (P.dtype == GDN_DTYPE_F16) return launch_read<f16>(a, P.D, s);
+  if (P.dtype == GDN_DTYPE_BF16) return launch_read<bf16_t>(a, P.D, s);
+  return launch_read<float>(a, P.D, s);
 }
 
 int64_t gdn_cache8_decode_workspace_size(const GdnCache8Params* prm) {

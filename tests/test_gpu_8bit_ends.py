@@ -1,11 +1,11 @@
-"""GPU tests of the quantisers and of the 8-bit cache at their largest sizes."""
+"""GPU tests of the quantisers and of the 8-bit cache at their largest sizes and
+of the cache at the smallest values."""
 
 import pytest
 import torch
+from test_gpu_cache8 import FP8, _decode, _new, oracle
 
 pytestmark = pytest.mark.gpu
-
-FP8 = torch.float8_e4m3fn
 
 
 @pytest.mark.parametrize("group", [128, None])
@@ -67,3 +67,20 @@ def test_a_cache_of_more_rows_than_a_launch_holds(pkg, cuda):
     ks, vs = torch.tensor([0.5, 2.0], device=cuda).view(2, 1, 1, 1).expand(2, 1, S, 1).unbind()
     for x, row, f in zip(pkg.cache_read_fp8(kc, vc, ks, vs), q.view(FP8), (0.5, 2.0)):
         _all_rows_are(x.view(S, D), (row.float() * f).bfloat16())
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("S", [100, 3000])
+def test_values_near_the_smallest_numbers(pkg, cuda, D, S):
+    """Values of 2^-121, whose scale is no normal number any more: the output is of the
+    values' own size and off by the roundings of P vs and of itself, 1.5 units, alone
+    (log2 of the scale, about 128, by 2^-17)."""
+    k, v = _new(cuda, 1, S, 2, D, torch.bfloat16, 1), _new(cuda, 1, S, 2, D, torch.bfloat16, 2) * 2.0 ** -121
+    kc, vc = (torch.zeros(1, S, 2, D, device=cuda).to(FP8) for _ in range(2))
+    ks, vs = torch.zeros(1, S, 2, device=cuda), torch.zeros(1, S, 2, device=cuda)
+    pkg.cache_write_fp8(k, v, kc, vc, ks, vs, torch.tensor([S], dtype=torch.int32, device=cuda))
+    q = _new(cuda, 1, 1, 4, D, torch.bfloat16, 3) * 4
+    o = _decode(pkg, q, kc, vc, ks, vs, [S]).double() * 2.0 ** 121
+    want = oracle(q, kc, vc, ks, vs, [S], None, 0) * 2.0 ** 121
+    assert 0 < vs.max().item() < 2.0 ** -126
+    assert ((o - want).norm() / want.norm()).item() <= 1.5 * 2.0 ** -8

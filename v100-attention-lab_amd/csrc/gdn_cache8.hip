@@ -206,12 +206,25 @@ struct QRow {
 // The factor of a part with maximum m under the common one.
 __device__ __forceinline__ float weight(float m, float top) { return m == -__builtin_inff() ? 0.f : exp2_fast(m - top); }
 
-// The result's factor: 2^(M - m) / l (0 where no key was seen, NaN where l is).
-template <typename T>
-__device__ __forceinline__ float result_factor(float m, float l, float M) {
-  if (l == 0.f) return 0.f;
-  return M == -__builtin_inff() ? (l != l ? l : 0.f) : exp2_fast(M - m - Ops<T>::kShift) / l;
+// log2 of a value's scale, of the smallest ones too (the instruction takes those below
+// 2^-126 for 0).
+__device__ __forceinline__ float log2_scale(float x) {
+  return x < 0x1p-126f ? __builtin_amdgcn_logf(x * 0x1p32f) - 32.f : __builtin_amdgcn_logf(x);
 }
+
+// What O becomes the result by: 2^(M - m) / l (0 where no key was seen, NaN where l is),
+// in two factors where the power is no normal number.
+template <typename T>
+struct Result {
+  float f, down;
+  __device__ __forceinline__ Result(float m, float l, float M) {
+    const float e = M - m - Ops<T>::kShift;
+    const bool small = e < -64.f;
+    down = small ? 0x1p-64f : 1.f;
+    f = l == 0.f ? 0.f : M == -__builtin_inff() ? (l != l ? l : 0.f) : exp2_fast(small ? e + 64.f : e) / l;
+  }
+  __device__ __forceinline__ float operator()(float o) const { return o * f * down; }
+};
 
 constexpr uint32_t kNan = 0x7f7f7f7fu;       // e4m3: all ones but the sign
 // Bits 0x80 of the bytes that are NaN.
@@ -277,7 +290,7 @@ __global__ __launch_bounds__(kNT) void decode_kernel(const Args a) {
     {
       lds_f32* at = (lds_f32*)(st + 4 * lane);
       const float x = *at;
-      *at = half == 0 ? x * a.scale_log2 : __builtin_amdgcn_logf(x);
+      *at = half == 0 ? x * a.scale_log2 : log2_scale(x);
     }
     const Mask seen(p, kr.tile(t) * kDN, kDN, half, n, p0, p1, a.window, a.sinks);
     f32x16 s[1] = {};
@@ -426,9 +439,9 @@ __global__ __launch_bounds__(kNT) void decode_kernel(const Args a) {
       }
       *reinterpret_cast<float2*>(part + 96 + c * D + d) = make_float2(x, y);
     } else {
-      const float f = result_factor<T>(top, sum, topM);
+      const Result<T> result(top, sum, topM);
       const QRow row(a, hk, rt, c);
-      *reinterpret_cast<uint32_t*>(a.o + at3(a.ost, b, row.t, row.h) + d) = O::pack(x * f, y * f);
+      *reinterpret_cast<uint32_t*>(a.o + at3(a.ost, b, row.t, row.h) + d) = O::pack(result(x), result(y));
     }
   }
 }
@@ -484,10 +497,10 @@ __global__ __launch_bounds__(kJT) void join_kernel(const Args a) {
     o.z += x.z;
     o.w += x.w;
   }
-  const float e = result_factor<T>(top, l, topM);
+  const Result<T> result(top, l, topM);
   const QRow w(a, hk, r / 32, c);
   *reinterpret_cast<uint2*>(a.o + at3(a.ost, b, w.t, w.h) + 4 * d) =
-      make_uint2(Ops<T>::pack(o.x * e, o.y * e), Ops<T>::pack(o.z * e, o.w * e));
+      make_uint2(Ops<T>::pack(result(o.x), result(o.y)), Ops<T>::pack(result(o.z), result(o.w)));
 }
 
 // ---------------------------------------------------------------------------

@@ -5,7 +5,7 @@ import ctypes
 
 import pytest
 import torch
-from test_head_and_fp8_host import _xent, lib  # noqa: F401
+from test_head_and_fp8_host import _operands, _xent, lib  # noqa: F401
 
 
 @pytest.mark.parametrize("name", ["gdn_xent", "gdn_xent_bwd"])
@@ -35,3 +35,16 @@ def test_xent_workspace_is_what_the_tiles_leave(lib, pkg):  # noqa: F811
     assert size(N=8192, V=32_001) == 8192 * (126 * 8 + 4)
     assert size(N=64, V=50_257) == 64 * (393 * 8 + 4)
     assert size(N=1000, V=500) == 1000 * (4 * 8 + 4)
+
+
+@pytest.mark.parametrize("i", [0, 1])
+def test_scales_with_a_gradient_are_not_written(pkg, i):
+    """They would change under the graph that holds them."""
+    o = _operands()
+    scales = [o["ks"].clone(), o["ks"].clone()]
+    scales[i].requires_grad_()
+    write = lambda: pkg.cache_write_fp8(o["k"], o["k"], o["kc"], o["kc"], *scales, o["lens"])
+    with pytest.raises(NotImplementedError, match="no gradient"):
+        write()
+    with torch.no_grad(), pytest.raises(ValueError, match="GPU"):
+        write()

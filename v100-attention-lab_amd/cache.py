@@ -146,7 +146,7 @@ def cache_write_fp8(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
 
     Not differentiable.
     """
-    if _needs_grad(k, v):
+    if _needs_grad(k, v, k_scale, v_scale):
         raise NotImplementedError("cache_write_fp8 has no gradient")
     params = _call("write", (k, v, k_cache, v_cache), (k_scale, v_scale, cache_seqlens), None,
                    lambda: _write_plan(k, v, k_cache, v_cache, k_scale, v_scale, cache_seqlens))

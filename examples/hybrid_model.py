@@ -116,6 +116,8 @@ class WindowAttention(nn.Module):
             o = gdn.window_attn(q, k, v, self.window, self.sinks)
         elif self.eight:
             *cache, n = state
+            if T > 16 and length is None:
+                raise ValueError(f"a piece of {T} tokens needs length, the tokens of a sequence with it")
             n += T
             gdn.cache_write_fp8(k, v, *cache, n)
             if T > 16:       # a piece of a prompt: `length` rows with it, the same for all sequences
@@ -158,7 +160,8 @@ class HybridModel(nn.Module):
 
     def rows(self, tokens, states=None, fp8=False, length=None):
         """What the head takes of [B, T] tokens; with states (see start) they are
-        continued in place, to `length` tokens."""
+        continued in place, to `length` tokens (asked for from 17 new ones on in 8
+        bits)."""
         r = self.embed(tokens)
         x = torch.zeros_like(r, dtype=DTYPE)
         for i, mixer in enumerate(self.mixers):

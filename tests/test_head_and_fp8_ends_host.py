@@ -1,7 +1,10 @@
 """CPU tests of the sizes that linear_xent, the 8-bit product and the 8-bit cache take,
-at their ends (nothing is enqueued: what is in order but for its workspace is told so)."""
+at their ends (nothing is enqueued: what is in order but for its workspace is told so),
+and of further refusals."""
 
 import ctypes
+import importlib.util
+import os
 
 import pytest
 import torch
@@ -48,3 +51,18 @@ def test_scales_with_a_gradient_are_not_written(pkg, i):
         write()
     with torch.no_grad(), pytest.raises(ValueError, match="GPU"):
         write()
+
+
+def test_a_piece_without_its_length_is_refused(pkg):
+    """The hybrid model in 8 bits reads back as many rows as it is told; nothing is
+    counted up before."""
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "hybrid_model.py")
+    spec = importlib.util.spec_from_file_location("hybrid_model", path)
+    hybrid = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(hybrid)
+    m = hybrid.WindowAttention(256, 4, 2, 64, 48, 4)
+    m.eight = True
+    state = m.start(1, 40, "cpu")
+    with torch.no_grad(), pytest.raises(ValueError, match="length"):
+        m(torch.zeros(1, 17, 256, dtype=torch.bfloat16), state)
+    assert state[-1].tolist() == [0]

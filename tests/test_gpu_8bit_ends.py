@@ -1,5 +1,5 @@
-"""GPU tests of the quantisers and of the 8-bit cache at their largest sizes and
-of the cache at the smallest values."""
+"""GPU tests of the quantisers and of the 8-bit cache at their largest sizes, of the
+cache at the smallest values and of the 8-bit product where its terms cancel."""
 
 import pytest
 import torch
@@ -84,3 +84,26 @@ def test_values_near_the_smallest_numbers(pkg, cuda, D, S):
     want = oracle(q, kc, vc, ks, vs, [S], None, 0) * 2.0 ** 121
     assert 0 < vs.max().item() < 2.0 ** -126
     assert ((o - want).norm() / want.norm()).item() <= 1.5 * 2.0 ** -8
+
+
+@pytest.mark.parametrize("M", [1, 40, 700])
+@pytest.mark.parametrize("out", [torch.float32, torch.float16, torch.bfloat16])
+def test_terms_that_cancel(pkg, cuda, M, out):
+    """448 and -448 side by side, small numbers between them: fp32 sums are off by
+    (K + K / 128) 2^-24 of the terms' sizes at most, 16-bit results come from products
+    cut at 2^-13 of the largest of 8, 2^-10 of the terms' sizes, and are rounded."""
+    K, N = 512, 300
+    gen = torch.Generator(device=cuda).manual_seed(M)
+    x = torch.randn(M, K, generator=gen, device=cuda)
+    x[:, 0::4], x[:, 1::4] = 448.0, -448.0
+    x, w = x.to(FP8), torch.randn(N, K, generator=gen, device=cuda)
+    w[:, 1::4] = w[:, 0::4]
+    w = w.to(FP8)
+    xs, ws = torch.full((M, K // 128), 0.25, device=cuda), torch.full((-(-N // 128), K // 128), 0.5, device=cuda)
+    y = pkg.fp8_linear(x, xs, w, ws, out_dtype=out)
+    a, b = x.double() / 4, w.double() / 2
+    want, size = a @ b.T, a.abs() @ b.abs().T
+    assert (want.abs().mean() < 2.0 ** -8 * size.mean()).item()
+    half = torch.finfo(out).eps / 2
+    bound = size * ((K + K // 128) * 2.0 ** -24 + (0.0 if out == torch.float32 else 2.0 ** -10)) * (1 + half) + half * want.abs()
+    assert ((y.double() - want).abs() / bound).max().item() <= 1

@@ -154,7 +154,12 @@ def fp8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, wei
         (as ``quantize_fp8`` and ``add_rms_norm_fp8`` give them).
       weight: ``[N, K]`` float8_e4m3fn; weight_scale: float32
         ``[ceil(N / 128), K / 128]`` (as ``quantize_fp8_weight`` gives them).
-      out_dtype: of the result, rounded once from fp32 sums.
+      out_dtype: float32 comes from fp32 sums.  float16 and bfloat16 come from
+        the 8-bit matrix unit, at more than twice the rate, which cuts each
+        product at 2^-13 of the largest of its group of 8: off by up to 2^-10 of
+        the sum of the terms' sizes beside the one rounding (about 1.4e-5 of the
+        result where the terms are normally distributed; more than its rounding
+        where they cancel).
 
     Returns ``y [..., N]``.  Not differentiable.
     """

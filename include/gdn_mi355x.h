@@ -530,7 +530,7 @@ int gdn_attn_decode_launch(const GdnAttnDecodeParams* params, void* stream);
 
 /* Softmax cross entropy of a linear head, N rows of D against V weights, the
  * logits l = x w^T (in fp32) made in pieces of the vocabulary and never kept:
- *     lse_n = log sum_v e^{l_nv},   loss_n = lse_n - l_{n, target_n}
+ *     lse_n = log sum_v e^{l_nv},   loss_n = lse_n - l_{n, target_n} (0 or more)
  *     G = dloss_n (e^{l - lse} - [v = target_n]),  dx = G w,  dw = G^T x
  * A row whose target is outside [0, V) does not count: loss and lse 0, dx 0,
  * nothing in dw, whatever the row holds.  G is rounded once to dtype (in a

@@ -16,7 +16,7 @@
 //
 // Bound by reading 2 D + 8 bytes of each visible key and head: 32 sequences of up to
 // 16384 keys, 4 heads of 128 in a window of 4096, 27 us at 4.8 TB/s, the rate of a copy;
-// one sequence of 65536 keys 17.3 us at 3.7 TB/s (4 tiles a wave, of which the first two
+// one sequence of 65536 keys 17.3 to 18 us at 3.6 TB/s (4 tiles a wave, of which the first two
 // wait for the length, the query and memory alone), its join 5 us.  Two tiles on
 // the way before the first is used changed nothing.
 // Writing 8 x 2048 rows of 4 heads from bf16: 12.5 us, 4 TB/s; reading 8 x 4096 back:

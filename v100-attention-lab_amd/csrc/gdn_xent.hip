@@ -17,10 +17,10 @@
 //
 // Bound by the products: 2 N D V forward, 6 N D V backward (the logits a second time;
 // keeping them would take 2 N V bytes and their reading).  bf16 on a card whose large
-// matrix product reaches 1.41 PFLOP/s: 8192 x 4096, 128000 words forward 6.6 ms (1.30
-// PFLOP/s), backward 21.3 ms (1.21); a piece of 8192 words G 0.44, dW 0.44 and dX 0.46
+// matrix product reaches 1.41 PFLOP/s: 8192 x 4096, 128000 words forward 6.7 ms (1.28
+// PFLOP/s), backward 21 ms (1.23); a piece of 8192 words G 0.44, dW 0.44 and dX 0.47
 // ms, dX with its fp32 sums read and written.  48 rows of 2048 against 50257 words are
-// bound by reading the weight, 32 us at 6.4 TB/s where the last-level cache holds it.
+// bound by reading the weight, 32 us at 6.5 TB/s where the last-level cache holds it.
 //
 // G is kept in a unit that makes the largest finite |dloss| a power of 2.  A mean gives all
 // rows the same dloss, and the target's G, close to -dloss, outweighs the others: it
@@ -482,7 +482,10 @@ int check(const GdnXentParams& P) {
   return GDN_OK;
 }
 
-// Vocabulary of a piece: G takes about 128 MiB.
+// Vocabulary of a piece: G takes about 128 MiB.  (Larger pieces gave 0 to 1.6 % at 8192
+// rows.  More rows make a piece of fewer words, and dX's sums are read and written for
+// each: rows of 4096 against 128000 words backward, in 6 N D V operations, 1.24 PFLOP/s
+// at 8192 rows, 1.04 at 32768, 0.87 at 65536.)
 int piece_of(const GdnXentParams& P) {
   const int64_t rows = ceil_to(std::max(P.N, 1), 256);
   const int64_t most = std::max<int64_t>((128ll << 20) / (2 * rows) / 256 * 256, 256);

@@ -473,8 +473,9 @@ int check(const GdnXentParams& P) {
       P.D > 1 << 22)
     return GDN_ERR_UNSUPPORTED;
   if (P.N >= 1 << 26 || P.V > 1 << 28) return GDN_ERR_BAD_SHAPE;      // (the join has 64 threads a row)
-  // one launch each: the logits in the tiles that they are made in (512 threads for
-  // 256 x 256, the smaller ones are chosen for few alone), the gradients in the smallest
+  // one launch each: the logits in the tiles that they are made in (512 threads for 256 x
+  // 256; else 256 for 128 x 64 at the least, which only sizes that fit take: with more
+  // than 384 rows and words the rule comes to the large ones), the gradients in 128 x 128
   const bool big = logits_kind(P.V, P.N) == kBig;
   if (!(big ? grid_fits(tiles_of(P.V, P.N, 256, 256), 512) : grid_fits(tiles_of(P.V, P.N, 128, 64), 256)) ||
       !grid_fits(tiles_of(P.D, std::max(P.N, P.V), 128, 128), 256))
